@@ -80,6 +80,9 @@ static const DataLayout I8 = INFINIOP_DT(1, 1, 1, 7, 0), I16 = INFINIOP_DT(1, 1,
                         U32 = INFINIOP_DT(1, 0, 4, 32, 0), U64 = INFINIOP_DT(1, 0, 8, 64, 0),
                         F16 = INFINIOP_DT(1, 1, 2, 10, 5), BF16 = INFINIOP_DT(1, 1, 2, 7, 8),
                         F32 = INFINIOP_DT(1, 1, 4, 23, 8), F64 = INFINIOP_DT(1, 1, 8, 52, 11);
+/* 8-bit floating point e4m3 (largest value 448, no infinities, NaN 0x7F / 0xFF): the paged KV cache below.  NO
+ * counterpart in the reference. */
+static const DataLayout F8E4M3 = INFINIOP_DT(1, 1, 1, 3, 4);
 
 /* ---- tensor descriptor: include/tensor.h:7-18 ----------------------------- *
  * Layout is visible to callers (the Python wrapper mirrors it field by field).
@@ -271,6 +274,139 @@ INFINIOP_API infiniopStatus_t infiniopAttention(infiniopAttentionDescriptor_t de
                                                 uint64_t workspace_size, void *out, void const *q, void const *k,
                                                 void const *v, void *k_cache, void *v_cache, void *stream);
 INFINIOP_API infiniopStatus_t infiniopDestroyAttentionDescriptor(infiniopAttentionDescriptor_t desc);
+
+/* ---- paged KV cache in 8 bits (NO counterpart in the reference) ------------ *
+ * infiniopAttention keeps one sequence's cache in fp16 and its position in the
+ * descriptor.  The four operators below serve many sequences per call out of a
+ * pool of pages, at half the cache bytes; lengths and page ids live on the
+ * device, so a captured graph can be replayed while the sequences grow.
+ *
+ * The cache of one layer, shared by the four operators:
+ *   k_pages, v_pages   F8E4M3 [num_pages, n_kv_head, page_size, dh], unit
+ *                      innermost stride, positive outer strides in any order
+ *                      ([num_pages, page_size, n_kv_head, dh] storage is a
+ *                      view of this shape)
+ *   k_scales, v_scales F32 [num_pages, n_kv_head], positive: a cached element
+ *                      is code * scale of its page and head
+ *   block_table        I32 [batch, columns], unit inner stride: entry (b, i)
+ *                      is the page that holds tokens i * page_size .. of b
+ *   seq_lens           I32 [batch]: tokens of each sequence WITH the new ones
+ *   q_offsets          I32 [batch + 1]: the new tokens of sequence b are rows
+ *                      q_offsets[b] .. q_offsets[b + 1] of k, v, q and out, at
+ *                      positions seq_lens[b] - n .. seq_lens[b] - 1 of b.  May
+ *                      be NULL where every sequence has one new token (rows ==
+ *                      batch).  Rows behind the last sequence's are left alone.
+ * dh <= 256; columns * page_size < 2^31.  Table entries behind a sequence's
+ * last page are never read.  Values that lead nowhere do no harm: a page id
+ * outside the pool is a page whose tokens are masked (attention) or dropped
+ * (append, copy, compact), offsets outside the rows are clamped, tokens beyond
+ * the table's columns are dropped, a length <= 0 is an empty sequence.
+ * Pointers must be aligned to their element.  The workspace must hold the
+ * reported size, else STATUS_MEMORY_NOT_ALLOCATED; calls that may overlap on
+ * the GPU (two streams, two captured graphs) need a workspace each.
+ * Roundings are to nearest, ties to even (there is no reference counterpart
+ * whose truncation would have to be followed). */
+
+/* Appends the new tokens' k, v (F16 or BF16 [rows, n_kv_head, dh], unit
+ * innermost stride) to the pages.  The scale of a page and head becomes
+ *   s = max(old scale if the page keeps earlier tokens, 2^x, 2^-40),
+ * x the smallest integer with max|new finite elements| <= 448 * 2^x; kept
+ * codes are re-encoded when it grows (a power of two: exact but for codes that
+ * become subnormal), new ones are e4m3(x / s), infinities saturate at 448 * s,
+ * NaN stays NaN.  A page that is written must belong to one sequence only
+ * (infiniopPagedCacheCopy gives a forked sequence its own copy).  Appending the
+ * same tokens at the same positions again changes nothing. */
+typedef struct PagedCacheAppendDescriptor {
+    Device device;
+} PagedCacheAppendDescriptor;
+typedef PagedCacheAppendDescriptor *infiniopPagedCacheAppendDescriptor_t;
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheAppendDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheAppendDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_desc,
+    infiniopTensorDescriptor_t v_desc, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc, infiniopTensorDescriptor_t block_table_desc,
+    infiniopTensorDescriptor_t seq_lens_desc, infiniopTensorDescriptor_t q_offsets_desc);
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheAppendWorkspaceSize(infiniopPagedCacheAppendDescriptor_t desc,
+                                                                       uint64_t *size);
+INFINIOP_API infiniopStatus_t infiniopPagedCacheAppend(infiniopPagedCacheAppendDescriptor_t desc, void *workspace,
+                                                       uint64_t workspace_size, void const *k, void const *v,
+                                                       void *k_pages, void *v_pages, void *k_scales, void *v_scales,
+                                                       void const *block_table, void const *seq_lens,
+                                                       void const *q_offsets, void *stream);
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheAppendDescriptor(infiniopPagedCacheAppendDescriptor_t desc);
+
+/* out[t, h, :] = softmax_j(scale * q[t, h, :] . k_j) . v_j over the cached
+ * tokens j <= position of t of its sequence, kv head h / (n_q_head / n_kv_head).
+ * q, out F16 or BF16 [rows, n_q_head, dh], unit innermost stride, free positive
+ * outer strides; `scale` finite.  The new tokens' own k and v are read from the
+ * pages: append them first.  A token without visible keys gets zeros.  What the
+ * pages hold behind a sequence's last token is not used, NaN included. */
+typedef struct PagedAttentionDescriptor {
+    Device device;
+} PagedAttentionDescriptor;
+typedef PagedAttentionDescriptor *infiniopPagedAttentionDescriptor_t;
+INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
+    infiniopHandle_t handle, infiniopPagedAttentionDescriptor_t *desc_ptr, infiniopTensorDescriptor_t out_desc,
+    infiniopTensorDescriptor_t q_desc, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc, infiniopTensorDescriptor_t block_table_desc,
+    infiniopTensorDescriptor_t seq_lens_desc, infiniopTensorDescriptor_t q_offsets_desc, float scale);
+INFINIOP_API infiniopStatus_t infiniopGetPagedAttentionWorkspaceSize(infiniopPagedAttentionDescriptor_t desc,
+                                                                     uint64_t *size);
+INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescriptor_t desc, void *workspace,
+                                                     uint64_t workspace_size, void *out, void const *q,
+                                                     void const *k_pages, void const *v_pages, void const *k_scales,
+                                                     void const *v_scales, void const *block_table,
+                                                     void const *seq_lens, void const *q_offsets, void *stream);
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedAttentionDescriptor(infiniopPagedAttentionDescriptor_t desc);
+
+/* Copies whole pages, K, V and their scales: pairs I32 [n, 2] on the device,
+ * row i = (source page, destination page); rows with an id outside the pool are
+ * skipped (padding).  One source may serve many destinations; a destination
+ * must appear once and not be a source of the same call. */
+typedef struct PagedCacheCopyDescriptor {
+    Device device;
+} PagedCacheCopyDescriptor;
+typedef PagedCacheCopyDescriptor *infiniopPagedCacheCopyDescriptor_t;
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheCopyDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheCopyDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc, infiniopTensorDescriptor_t pairs_desc);
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheCopyWorkspaceSize(infiniopPagedCacheCopyDescriptor_t desc,
+                                                                     uint64_t *size);
+INFINIOP_API infiniopStatus_t infiniopPagedCacheCopy(infiniopPagedCacheCopyDescriptor_t desc, void *workspace,
+                                                     uint64_t workspace_size, void *k_pages, void *v_pages,
+                                                     void *k_scales, void *v_scales, void const *pairs, void *stream);
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheCopyDescriptor(infiniopPagedCacheCopyDescriptor_t desc);
+
+/* Frees and compacts: a page is live when a table row names it within the
+ * row's length (a sequence is freed by setting its length to 0); the L live
+ * pages are brought to pages 0 .. L - 1.  Live pages below L stay; those at or
+ * above L move, in ascending order, to the free pages below L, in ascending
+ * order.  Pages L .. are free afterwards.
+ *   new_table  I32 [batch, columns]: block_table with the live entries
+ *              renamed, all others copied; may be block_table itself
+ *   page_map   I32 [num_pages]: each live page's new id, -1 for the others
+ *   live       I32 [1]: L
+ * A page that several rows name moves once.  Needs at most 2^27 pages. */
+typedef struct PagedCacheCompactDescriptor {
+    Device device;
+} PagedCacheCompactDescriptor;
+typedef PagedCacheCompactDescriptor *infiniopPagedCacheCompactDescriptor_t;
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheCompactDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheCompactDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc, infiniopTensorDescriptor_t new_table_desc,
+    infiniopTensorDescriptor_t block_table_desc, infiniopTensorDescriptor_t seq_lens_desc,
+    infiniopTensorDescriptor_t page_map_desc, infiniopTensorDescriptor_t live_desc);
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheCompactWorkspaceSize(infiniopPagedCacheCompactDescriptor_t desc,
+                                                                        uint64_t *size);
+INFINIOP_API infiniopStatus_t infiniopPagedCacheCompact(infiniopPagedCacheCompactDescriptor_t desc, void *workspace,
+                                                        uint64_t workspace_size, void *k_pages, void *v_pages,
+                                                        void *k_scales, void *v_scales, void *new_table,
+                                                        void const *block_table, void const *seq_lens, void *page_map,
+                                                        void *live, void *stream);
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheCompactDescriptor(infiniopPagedCacheCompactDescriptor_t desc);
 
 /* ---- matmul: include/ops/matmul/matmul.h:7-32 ------------------------------ *
  * c = alpha * a b + beta * c on 2-D [m,k] x [k,n] or batched 3-D matrices,

@@ -1,0 +1,661 @@
+// The paged 8-bit KV cache: appending tokens, copying pages, freeing and compacting.  Attention over it is in
+// paged_attention.cu.  No counterpart in the reference, whose cache is one fp16 tensor per sequence that its attention
+// composite writes with rearrange (src/ops/attention/operator.cc:87-91).
+//
+// Append.  A block (page x kv head, K and V apart) has one scale s, a power of two:
+//     s = max(s_old if rows of the page are kept, 2^x, 2^-40),  x = min { x : max|x_new| <= 448 * 2^x }
+//     code = e4m3(x_new / s),  kept codes: e4m3(code * s_old / s)
+// e4m3 carries its own exponent, so a power of two costs no precision against an exact 448 / max (the step relative to
+// the value is the same in every binade), division by it is exact, and when the scale of a half-filled page grows the
+// kept codes only move in their exponent: nothing is lost but bits of codes that become subnormal, however often it
+// happens.  One CTA owns a block: it reads the new rows once into registers, takes the maximum, and writes codes.
+//
+// Copy and compact move whole pages; compact first finds the live pages (one cluster, a bitmap in the workspace).
+#include "paged_cache.cuh"
+
+#include <new>
+
+using namespace b200;
+using namespace b200::paged;
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------- append --
+
+struct AppendParams {
+    const uint16_t *k, *v;
+    int64_t k_st, k_sh, v_st, v_sh;// strides of token and head
+    uint8_t *kp, *vp;
+    float *ks, *vs;
+    const int32_t *table, *lens, *offs;
+    int32_t rows;
+    CacheShape c;
+    TableShape t;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kHeld = 4;// vectors of new elements that a thread keeps between the maximum and the encoding
+
+// Exclusive sum over the CTA; `total` = sum over all threads.  `slot`: 33 words of shared memory.
+__device__ __forceinline__ int32_t cta_exclusive_sum(int32_t v, int32_t *slot, int32_t &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();
+    if (lane == 31) slot[warp] = incl;
+    __syncthreads();
+    int32_t before = 0, all = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += slot[w];
+        all += slot[w];
+    }
+    total = all;
+    return before + incl - v;
+}
+
+// VEC new elements of one row at a time: 8 (16-byte loads, 8-byte stores of codes) or 1.
+template<bool BF, int VEC>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+    __shared__ int32_t slot[33], found[2];
+    __shared__ uint32_t wmax[kAppendThreads / 32];
+    const int32_t item = (int32_t) blockIdx.x, head = (int32_t) blockIdx.y;
+    const bool is_v = blockIdx.z != 0;
+    const int32_t P = p.c.page, D = p.c.dh;
+
+    // the item-th touched page of the call: sequence b, its k-th page
+    int32_t b, nth;
+    if (p.offs == nullptr) {
+        b = item, nth = 0;// one token, one page per sequence
+        if (b >= p.t.batch) return;
+    } else {
+        int32_t base = 0;
+        bool hit = false;
+        for (int32_t b0 = 0; b0 < p.t.batch && !hit; b0 += (int32_t) blockDim.x) {
+            const int32_t mine = b0 + (int32_t) threadIdx.x;
+            int32_t count = 0;
+            if (mine < p.t.batch) {
+                int32_t lo, hi;
+                written(seq_of(p.lens, p.offs, p.rows, mine), p.t.cap, lo, hi);
+                count = pages_touched(lo, hi, P);
+            }
+            int32_t total;
+            const int32_t before = base + cta_exclusive_sum(count, slot, total);
+            if (item >= before && item - before < count) found[0] = mine, found[1] = item - before;
+            base += total;
+            hit = item < base;// the same in every thread
+        }
+        if (!hit) return;
+        __syncthreads();
+        b = found[0], nth = found[1];
+    }
+    const Seq s = seq_of(p.lens, p.offs, p.rows, b);
+    int32_t lo, hi;
+    written(s, p.t.cap, lo, hi);
+    if (hi <= lo) return;
+    const int32_t col = lo / P + nth, page0 = col * P;
+    const int32_t p0 = lo > page0 ? lo : page0, p1 = hi - page0 < P ? hi : page0 + P;
+    const int32_t page = p.table[(int64_t) b * p.t.stride + col];
+    if (page < 0 || page >= p.c.pages) return;
+    const int32_t kept = p0 - page0, m = p1 - p0;
+
+    const PoolStrides st = is_v ? p.c.v : p.c.k;
+    const int64_t x_st = is_v ? p.v_st : p.k_st;
+    const uint16_t *x = (is_v ? p.v + (int64_t) head * p.v_sh : p.k + (int64_t) head * p.k_sh) + (int64_t) (s.first + (p0 - (s.len - s.n))) * x_st;
+    uint8_t *codes = (is_v ? p.vp : p.kp) + (int64_t) page * st.sn + (int64_t) head * st.sh;
+    float *scale = (is_v ? p.vs : p.ks) + (int64_t) page * st.cn + (int64_t) head * st.ch;
+    const float old = kept > 0 ? *scale : 0.f;
+
+    // the new rows: into registers, and their largest finite magnitude
+    const int32_t per_row = D / VEC;
+    const int64_t nv = (int64_t) m * per_row;
+    uint4 held_v[kHeld];
+    uint32_t top = 0;
+    auto load = [&](int64_t i) -> uint4 {
+        const int64_t r = i / per_row;
+        const uint16_t *src = x + r * x_st + (i - r * per_row) * VEC;
+        if (VEC == 8) return *reinterpret_cast<const uint4 *>(src);
+        return make_uint4(*src, 0u, 0u, 0u);
+    };
+    auto grow = [&](uint4 w) {
+        top = __vmaxu2(top, finite_abs2<BF>(w.x));
+        if (VEC == 8) top = __vmaxu2(__vmaxu2(top, finite_abs2<BF>(w.y)), __vmaxu2(finite_abs2<BF>(w.z), finite_abs2<BF>(w.w)));
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int64_t i = threadIdx.x + (int64_t) j * blockDim.x;
+        held_v[j] = i < nv ? load(i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) grow(held_v[j]);
+    for (int64_t i = threadIdx.x + (int64_t) kHeld * blockDim.x; i < nv; i += blockDim.x) grow(load(i));
+    top = __vmaxu2(top, top >> 16) & 0xFFFFu;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (uint32_t w = 0; w < blockDim.x / 32; ++w) top = max(top, wmax[w]);
+    const float amax = BF ? __uint_as_float(top << 16) : f16_to_f32((uint16_t) top);
+    const int32_t e = scale_exponent(__float_as_uint(amax));
+    const float fresh = __uint_as_float(pow2_bits(e)), now = fmaxf(old, fresh);
+    // 1 / now: exact for powers of two (an old scale that is none is divided by as it stands)
+    const bool pow2 = (__float_as_uint(now) & 0x7FFFFFu) == 0;
+    const float inv = 1.f / now;
+    auto code2 = [&](float2 f) -> uint32_t { return pow2 ? f32x2_to_e4m3x2(f.x * inv, f.y * inv) : f32x2_to_e4m3x2(f.x / now, f.y / now); };
+
+    // rows that stay, where the scale has grown
+    if (kept > 0 && now != old) {
+        const float ratio = old / now;
+        const int32_t n = kept * per_row;
+        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
+            const int32_t r = i / per_row;
+            uint8_t *at = codes + (int64_t) r * st.sp + (i - r * per_row) * VEC;
+            if (VEC == 8) {
+                uint2 w = *reinterpret_cast<uint2 *>(at);
+                uint32_t out[2] = {w.x, w.y};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) out[j])), c = unpack2(e4m3x2_to_f16x2((uint16_t) (out[j] >> 16)));
+                    out[j] = (uint32_t) f32x2_to_e4m3x2(a.x * ratio, a.y * ratio) | ((uint32_t) f32x2_to_e4m3x2(c.x * ratio, c.y * ratio) << 16);
+                }
+                *reinterpret_cast<uint2 *>(at) = make_uint2(out[0], out[1]);
+            } else {
+                const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) *at));
+                *at = (uint8_t) f32x2_to_e4m3x2(a.x * ratio, 0.f);
+            }
+        }
+    }
+    // the new rows
+    auto store = [&](int64_t i, uint4 w) {
+        const int64_t r = i / per_row;
+        uint8_t *at = codes + (kept + r) * st.sp + (i - r * per_row) * VEC;
+        if (VEC == 8) {
+            *reinterpret_cast<uint2 *>(at) = make_uint2(code2(f16or_bf16x2<BF>(w.x)) | (code2(f16or_bf16x2<BF>(w.y)) << 16),
+                                                        code2(f16or_bf16x2<BF>(w.z)) | (code2(f16or_bf16x2<BF>(w.w)) << 16));
+        } else {
+            *at = (uint8_t) code2(f16or_bf16x2<BF>(w.x));
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int64_t i = threadIdx.x + (int64_t) j * blockDim.x;
+        if (i < nv) store(i, held_v[j]);
+    }
+    for (int64_t i = threadIdx.x + (int64_t) kHeld * blockDim.x; i < nv; i += blockDim.x) store(i, load(i));
+    if (threadIdx.x == 0) *scale = now;// (every read of the old scale lies before the barrier)
+}
+
+struct AppendDesc {
+    Device device;
+    int device_id;
+    CacheShape c;
+    TableShape t;
+    int32_t rows;
+    bool bf16;
+    int64_t k_st, k_sh, v_st, v_sh;
+};
+
+// ------------------------------------------------------------------------------------------------ copying pages --
+
+// A page of one pool as runs of consecutive bytes: `runs` = n0 x n1 of them, `len` bytes each.
+struct PageRuns {
+    int64_t page, s0, s1, cn, ch;// strides: page, runs (n1 fastest), scales
+    int32_t n0, n1, len;
+};
+struct MoveParams {
+    uint8_t *kp, *vp;
+    float *ks, *vs;
+    PageRuns k, v;
+    int32_t pages, heads;
+};
+
+constexpr int kMoveThreads = 256;
+
+PageRuns page_runs(const CacheShape &c, const PoolStrides &s) {
+    PageRuns r{s.sn, s.sh, s.sp, s.cn, s.ch, c.heads, c.page, c.dh};
+    if (r.n0 > 1 && r.n1 > 1 && r.s0 < r.s1) std::swap(r.s0, r.s1), std::swap(r.n0, r.n1);// the smaller stride inside
+    if (r.n1 == 1) std::swap(r.s0, r.s1), std::swap(r.n0, r.n1);
+    for (int i = 0; i < 2 && r.n1 > 1 && r.s1 == r.len && (int64_t) r.n1 * r.len < ((int64_t) 1 << 31); ++i) {
+        r.len *= r.n1;// the runs of the inner dimension follow each other
+        r.n1 = r.n0, r.s1 = r.s0, r.n0 = 1, r.s0 = 0;
+    }
+    return r;
+}
+// Widest unit (bytes) that every run can be moved in.
+int run_unit(const PageRuns &r, const void *base) {
+    uint64_t all = (uint64_t) (uintptr_t) base | (uint64_t) r.len | 16u;
+    if (r.n0 > 1) all |= (uint64_t) r.s0;
+    if (r.n1 > 1) all |= (uint64_t) r.s1;
+    all |= (uint64_t) r.page;
+    return (all & 15u) == 0 ? 16 : (all & 3u) == 0 ? 4 : 1;
+}
+
+// Units [begin, begin + 4 * threads) of one page of one pool, and with the first of them the page's scales.
+template<typename U>
+__device__ __forceinline__ void move_piece(uint8_t *pool, float *scales, const PageRuns &r, int32_t heads, int64_t src, int64_t dst, int64_t begin) {
+    const int64_t per_run = r.len / (int32_t) sizeof(U), units = per_run * r.n1 * r.n0;
+    const uint8_t *from = pool + src * r.page;
+    uint8_t *to = pool + dst * r.page;
+    U v[4];
+    int64_t at[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t u = begin + threadIdx.x + (int64_t) j * kMoveThreads;
+        at[j] = -1;
+        if (u < units) {
+            const int64_t run = u / per_run;
+            at[j] = (run / r.n1) * r.s0 + (run % r.n1) * r.s1 + (u - run * per_run) * (int64_t) sizeof(U);
+            v[j] = *reinterpret_cast<const U *>(from + at[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (at[j] >= 0) *reinterpret_cast<U *>(to + at[j]) = v[j];
+    }
+    if (begin == 0) {
+        for (int32_t h = threadIdx.x; h < heads; h += kMoveThreads) scales[dst * r.cn + h * r.ch] = scales[src * r.cn + h * r.ch];
+    }
+}
+template<typename U>
+int64_t pieces_of(const PageRuns &r) {
+    const int64_t units = (int64_t) (r.len / (int32_t) sizeof(U)) * r.n1 * r.n0;
+    return (units + 4 * kMoveThreads - 1) / (4 * kMoveThreads);
+}
+
+template<typename U>
+__global__ void __launch_bounds__(kMoveThreads) copy_pairs_kernel(const MoveParams p, const int32_t *pairs, int64_t stride, int64_t count, int64_t pieces) {
+    // work: (pair, pool, piece), piece fastest
+    for (int64_t w = blockIdx.x; w < count * 2 * pieces; w += gridDim.x) {
+        const int64_t i = w / (2 * pieces), rest = w - i * 2 * pieces;
+        const bool is_v = rest >= pieces;
+        const int32_t src = pairs[i * stride], dst = pairs[i * stride + 1];
+        if (src < 0 || src >= p.pages || dst < 0 || dst >= p.pages || src == dst) continue;
+        const int64_t begin = (is_v ? rest - pieces : rest) * 4 * kMoveThreads;
+        if (is_v) move_piece<U>(p.vp, p.vs, p.v, p.heads, src, dst, begin);
+        else move_piece<U>(p.kp, p.ks, p.k, p.heads, src, dst, begin);
+    }
+}
+
+struct CopyDesc {
+    Device device;
+    int device_id, sm_count;
+    CacheShape c;
+    int64_t count, stride;
+};
+
+MoveParams move_params(const CacheShape &c, void *kp, void *vp, void *ks, void *vs) {
+    return MoveParams{reinterpret_cast<uint8_t *>(kp), reinterpret_cast<uint8_t *>(vp), reinterpret_cast<float *>(ks),
+                      reinterpret_cast<float *>(vs), page_runs(c, c.k), page_runs(c, c.v), c.pages, c.heads};
+}
+
+// ---------------------------------------------------------------------------------------------------- compacting --
+
+constexpr uint32_t kPlanCtas = 8, kPlanThreads = 1024;
+
+// Workspace: header, bitmap of live pages, sources and destinations of the moves.
+struct PlanHeader {
+    int32_t live, moves, pad[2];
+};
+struct PlanView {
+    PlanHeader *head;
+    uint32_t *bits;
+    int32_t *src, *dst;
+};
+uint64_t plan_words(uint64_t pages) { return (pages + 31) / 32; }
+uint64_t plan_bytes(uint64_t pages) { return sizeof(PlanHeader) + 4 * ((plan_words(pages) + 3) / 4 * 4) + 8 * (pages / 2 + 1); }
+PlanView plan_view(void *ws, uint64_t pages) {
+    PlanView v;
+    v.head = reinterpret_cast<PlanHeader *>(ws);
+    v.bits = reinterpret_cast<uint32_t *>(v.head + 1);
+    v.src = reinterpret_cast<int32_t *>(v.bits + (plan_words(pages) + 3) / 4 * 4);
+    v.dst = v.src + (pages / 2 + 1);
+    return v;
+}
+
+struct CompactParams {
+    const int32_t *table, *lens;
+    int32_t *new_table, *page_map, *live;
+    int64_t new_stride;
+    TableShape t;
+    int32_t pages, page;
+    PlanView plan;
+};
+
+// One cluster finds the live pages and the moves.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactParams p) {
+    __shared__ int32_t slot[33];
+    __shared__ int32_t below;// live pages below the count
+    const int32_t words = (p.pages + 31) / 32;
+    const uint32_t rank = cluster_rank(), gtid = rank * kPlanThreads + threadIdx.x;
+    for (int32_t w = (int32_t) gtid; w < words; w += (int32_t) (kPlanCtas * kPlanThreads)) p.plan.bits[w] = 0;
+    cluster_sync_all();
+    // marks: the warps of the cluster share out the rows, several warps to a row where rows are few
+    {
+        const int32_t warps = kPlanCtas * kPlanThreads / 32, warp = (int32_t) (gtid / 32), lane = (int32_t) (gtid & 31);
+        const int32_t per_row = p.t.batch >= warps ? 1 : warps / (p.t.batch > 0 ? p.t.batch : 1);
+        for (int64_t u = warp; u < (int64_t) p.t.batch * per_row; u += warps) {
+            const int32_t b = (int32_t) (u / per_row), part = (int32_t) (u % per_row);
+            const int32_t len = held(p.lens[b] > 0 ? p.lens[b] : 0, p.t.cap), used = len > 0 ? (len - 1) / p.page + 1 : 0;
+            const int32_t *row = p.table + (int64_t) b * p.t.stride;
+            for (int64_t i = (int64_t) part * 32 + lane; i < used; i += (int64_t) per_row * 32) {
+                const int32_t id = row[i];
+                if (id >= 0 && id < p.pages) atomicOr(&p.plan.bits[id >> 5], 1u << (id & 31));
+            }
+        }
+    }
+    cluster_sync_all();
+    if (rank != 0) return;
+    // ranks of live pages and holes: a stretch of words per thread
+    const int32_t each = (words + (int32_t) kPlanThreads - 1) / (int32_t) kPlanThreads;
+    const int32_t w0 = min((int32_t) threadIdx.x * each, words), w1 = min(w0 + each, words);
+    int32_t mine = 0;
+    for (int32_t w = w0; w < w1; ++w) mine += __popc(p.plan.bits[w]);
+    int32_t live;
+    const int32_t before = cta_exclusive_sum(mine, slot, live);
+    if (threadIdx.x == 0) below = 0;
+    __syncthreads();
+    int32_t seen = before;
+    for (int32_t w = w0; w < w1; ++w) {
+        const uint32_t bits = p.plan.bits[w];
+        if (live / 32 == w) below = seen + __popc(bits & ((1u << (live & 31)) - 1u));
+        seen += __popc(bits);
+    }
+    if (threadIdx.x == 0 && live / 32 >= words) below = live;// every page is live and the last word is full
+    __syncthreads();
+    seen = before;
+    for (int32_t w = w0; w < w1; ++w) {
+        const uint32_t bits = p.plan.bits[w];
+        // holes: dead pages below `live`; the j-th of them has j dead ones before it
+        uint32_t holes = ~bits;
+        if ((w + 1) * 32 > live) holes &= live > w * 32 ? (1u << (live - w * 32)) - 1u : 0u;
+        while (holes != 0) {
+            const int32_t i = __ffs((int) holes) - 1;
+            holes &= holes - 1;
+            p.plan.dst[w * 32 + i - (seen + __popc(bits & ((1u << i) - 1u)))] = w * 32 + i;
+        }
+        uint32_t movers = bits;
+        if (w * 32 < live) movers &= live - w * 32 >= 32 ? 0u : ~((1u << (live - w * 32)) - 1u);
+        while (movers != 0) {
+            const int32_t i = __ffs((int) movers) - 1;
+            movers &= movers - 1;
+            p.plan.src[seen + __popc(bits & ((1u << i) - 1u)) - below] = w * 32 + i;
+        }
+        seen += __popc(bits);
+    }
+    __syncthreads();
+    const int32_t moves = live - below;
+    for (int32_t j = (int32_t) threadIdx.x; j < moves; j += (int32_t) kPlanThreads) p.page_map[p.plan.src[j]] = p.plan.dst[j];
+    if (threadIdx.x == 0) {
+        p.plan.head->live = live, p.plan.head->moves = moves;
+        *p.live = live;
+    }
+}
+
+// Renames the table's entries, fills the map and moves the pages.  Sources lie at or above the live count,
+// destinations below it, so no page is both.
+template<typename U>
+__global__ void __launch_bounds__(kMoveThreads) compact_apply_kernel(const CompactParams p, const MoveParams m, int64_t pieces) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t live = p.plan.head->live;
+    const int64_t moves = p.plan.head->moves;
+    const int64_t gtid = (int64_t) blockIdx.x * kMoveThreads + threadIdx.x, threads = (int64_t) gridDim.x * kMoveThreads;
+    for (int64_t i = gtid; i < p.pages; i += threads) {
+        const bool is_live = (p.plan.bits[i >> 5] >> (i & 31)) & 1u;
+        if (!is_live) p.page_map[i] = -1;
+        else if (i < live) p.page_map[i] = (int32_t) i;
+    }
+    for (int64_t i = gtid; i < (int64_t) p.t.batch * p.t.cols; i += threads) {
+        const int32_t b = (int32_t) (i / p.t.cols), col = (int32_t) (i - (int64_t) b * p.t.cols);
+        const int32_t len = held(p.lens[b] > 0 ? p.lens[b] : 0, p.t.cap);
+        int32_t id = p.table[(int64_t) b * p.t.stride + col];
+        if ((int64_t) col * p.page < len && id >= live && id < p.pages) id = p.page_map[id];// a mover: written by the plan
+        p.new_table[(int64_t) b * p.new_stride + col] = id;
+    }
+    for (int64_t w = blockIdx.x; w < moves * 2 * pieces; w += gridDim.x) {
+        const int64_t i = w / (2 * pieces), rest = w - i * 2 * pieces;
+        const bool is_v = rest >= pieces;
+        const int64_t begin = (is_v ? rest - pieces : rest) * 4 * kMoveThreads;
+        if (is_v) move_piece<U>(m.vp, m.vs, m.v, m.heads, p.plan.src[i], p.plan.dst[i], begin);
+        else move_piece<U>(m.kp, m.ks, m.k, m.heads, p.plan.src[i], p.plan.dst[i], begin);
+    }
+}
+
+struct CompactDesc {
+    Device device;
+    int device_id, sm_count;
+    CacheShape c;
+    TableShape t;
+    int64_t new_stride;
+};
+
+}// namespace
+
+// ------------------------------------------------------------------------------------------------- entry points --
+
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheAppendDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheAppendDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_desc,
+    infiniopTensorDescriptor_t v_desc, infiniopTensorDescriptor_t k_pages_desc, infiniopTensorDescriptor_t v_pages_desc,
+    infiniopTensorDescriptor_t k_scales_desc, infiniopTensorDescriptor_t v_scales_desc,
+    infiniopTensorDescriptor_t block_table_desc, infiniopTensorDescriptor_t seq_lens_desc,
+    infiniopTensorDescriptor_t q_offsets_desc) {
+    if (handle == nullptr || handle->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (desc_ptr == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    if (k_desc == nullptr || v_desc == nullptr) return STATUS_BAD_PARAM;
+    AppendDesc d{};
+    infiniopStatus_t st = check_cache(k_pages_desc, v_pages_desc, k_scales_desc, v_scales_desc, d.c);
+    if (st != STATUS_SUCCESS) return st;
+    st = check_tables(block_table_desc, seq_lens_desc, q_offsets_desc, d.c.page, d.t);
+    if (st != STATUS_SUCCESS) return st;
+    if (k_desc->ndim != 3) return STATUS_BAD_TENSOR_SHAPE;
+    const uint64_t rows = k_desc->shape[0];
+    for (auto *x : {k_desc, v_desc}) {
+        st = check_rows(x, rows, (uint64_t) d.c.heads, (uint64_t) d.c.dh, k_desc->dt);
+        if (st != STATUS_SUCCESS) return st;
+    }
+    if (!d.t.offsets && rows != (uint64_t) d.t.batch) return STATUS_BAD_TENSOR_SHAPE;
+    auto *h = reinterpret_cast<Handle *>(handle);
+    d.device = DevNvGpu, d.device_id = h->device_id, d.rows = (int32_t) rows, d.bf16 = dt_eq(k_desc->dt, BF16);
+    d.k_st = k_desc->strides[0], d.k_sh = k_desc->strides[1], d.v_st = v_desc->strides[0], d.v_sh = v_desc->strides[1];
+    auto *r = new (std::nothrow) AppendDesc(d);
+    if (r == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    *desc_ptr = reinterpret_cast<infiniopPagedCacheAppendDescriptor_t>(r);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheAppendWorkspaceSize(infiniopPagedCacheAppendDescriptor_t desc, uint64_t *size) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (size == nullptr) return STATUS_BAD_PARAM;
+    *size = 0;
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopPagedCacheAppend(infiniopPagedCacheAppendDescriptor_t desc, void *workspace,
+                                                       uint64_t workspace_size, void const *k, void const *v, void *k_pages,
+                                                       void *v_pages, void *k_scales, void *v_scales,
+                                                       void const *block_table, void const *seq_lens, void const *q_offsets,
+                                                       void *stream) {
+    (void) workspace;
+    (void) workspace_size;
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    auto *d = reinterpret_cast<AppendDesc *>(desc);
+    if (d->rows == 0 || d->t.batch == 0 || d->t.cols == 0 || d->c.pages == 0) return STATUS_SUCCESS;
+    if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr ||
+        block_table == nullptr || seq_lens == nullptr || d->t.offsets != (q_offsets != nullptr)) {
+        return STATUS_BAD_PARAM;
+    }
+    DeviceGuard guard(d->device_id);
+    AppendParams p{reinterpret_cast<const uint16_t *>(k), reinterpret_cast<const uint16_t *>(v), d->k_st, d->k_sh, d->v_st, d->v_sh,
+                   reinterpret_cast<uint8_t *>(k_pages), reinterpret_cast<uint8_t *>(v_pages), reinterpret_cast<float *>(k_scales),
+                   reinterpret_cast<float *>(v_scales), reinterpret_cast<const int32_t *>(block_table),
+                   reinterpret_cast<const int32_t *>(seq_lens), reinterpret_cast<const int32_t *>(q_offsets), d->rows, d->c, d->t};
+    // 8 elements at a time where every row of the new tokens starts on 16 bytes and every row of codes on 8
+    bool vec = d->c.dh % 8 == 0 && aligned16(k) && aligned16(v) && ((uintptr_t) k_pages | (uintptr_t) v_pages) % 8 == 0;
+    for (int64_t s : {d->k_st, d->k_sh, d->v_st, d->v_sh, d->c.k.sn, d->c.k.sh, d->c.k.sp, d->c.v.sn, d->c.v.sh, d->c.v.sp}) vec = vec && s % 8 == 0;
+    const int64_t items = d->t.offsets ? pages_bound(d->rows, d->t.batch, d->c.page) : d->rows;
+    const dim3 grid((unsigned) items, (unsigned) d->c.heads, 2);
+    // one token per sequence is 16 vectors of 8: a small block leaves the SM to more of them
+    const unsigned threads = d->t.offsets ? kAppendThreads : 128;
+    auto st = reinterpret_cast<cudaStream_t>(stream);
+    if (d->bf16) {
+        if (vec) append_kernel<true, 8><<<grid, threads, 0, st>>>(p);
+        else append_kernel<true, 1><<<grid, threads, 0, st>>>(p);
+    } else {
+        if (vec) append_kernel<false, 8><<<grid, threads, 0, st>>>(p);
+        else append_kernel<false, 1><<<grid, threads, 0, st>>>(p);
+    }
+    return check_launch("paged cache append");
+}
+
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheAppendDescriptor(infiniopPagedCacheAppendDescriptor_t desc) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    delete reinterpret_cast<AppendDesc *>(desc);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheCopyDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheCopyDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc, infiniopTensorDescriptor_t v_scales_desc,
+    infiniopTensorDescriptor_t pairs_desc) {
+    if (handle == nullptr || handle->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (desc_ptr == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    if (pairs_desc == nullptr) return STATUS_BAD_PARAM;
+    CopyDesc d{};
+    const infiniopStatus_t st = check_cache(k_pages_desc, v_pages_desc, k_scales_desc, v_scales_desc, d.c);
+    if (st != STATUS_SUCCESS) return st;
+    if (pairs_desc->ndim != 2 || pairs_desc->shape[1] != 2 || pairs_desc->shape[0] > 0x7FFFFFFFull) return STATUS_BAD_TENSOR_SHAPE;
+    if (!dt_eq(pairs_desc->dt, I32)) return STATUS_BAD_TENSOR_DTYPE;
+    if (!unit_rows(pairs_desc)) return STATUS_BAD_TENSOR_STRIDES;
+    auto *h = reinterpret_cast<Handle *>(handle);
+    d.device = DevNvGpu, d.device_id = h->device_id, d.sm_count = h->sm_count;
+    d.count = (int64_t) pairs_desc->shape[0], d.stride = pairs_desc->strides[0];
+    auto *r = new (std::nothrow) CopyDesc(d);
+    if (r == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    *desc_ptr = reinterpret_cast<infiniopPagedCacheCopyDescriptor_t>(r);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheCopyWorkspaceSize(infiniopPagedCacheCopyDescriptor_t desc, uint64_t *size) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (size == nullptr) return STATUS_BAD_PARAM;
+    *size = 0;
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopPagedCacheCopy(infiniopPagedCacheCopyDescriptor_t desc, void *workspace, uint64_t workspace_size,
+                                                     void *k_pages, void *v_pages, void *k_scales, void *v_scales,
+                                                     void const *pairs, void *stream) {
+    (void) workspace;
+    (void) workspace_size;
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    auto *d = reinterpret_cast<CopyDesc *>(desc);
+    if (d->count == 0 || d->c.pages == 0) return STATUS_SUCCESS;
+    if (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || pairs == nullptr) return STATUS_BAD_PARAM;
+    DeviceGuard guard(d->device_id);
+    const MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
+    const int unit = std::min(run_unit(m.k, k_pages), run_unit(m.v, v_pages));
+    auto st = reinterpret_cast<cudaStream_t>(stream);
+    const auto *list = reinterpret_cast<const int32_t *>(pairs);
+    auto run = [&](auto u, auto *kernel) {
+        using U = decltype(u);
+        const int64_t pieces = std::max(pieces_of<U>(m.k), pieces_of<U>(m.v)), work = d->count * 2 * pieces;
+        kernel<<<(unsigned) std::min<int64_t>(work, 0x7FFFFFFF), kMoveThreads, 0, st>>>(m, list, d->stride, d->count, pieces);
+    };
+    if (unit == 16) run(uint4{}, copy_pairs_kernel<uint4>);
+    else if (unit == 4) run(uint32_t{}, copy_pairs_kernel<uint32_t>);
+    else run(uint8_t{}, copy_pairs_kernel<uint8_t>);
+    return check_launch("paged cache copy");
+}
+
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheCopyDescriptor(infiniopPagedCacheCopyDescriptor_t desc) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    delete reinterpret_cast<CopyDesc *>(desc);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopCreatePagedCacheCompactDescriptor(
+    infiniopHandle_t handle, infiniopPagedCacheCompactDescriptor_t *desc_ptr, infiniopTensorDescriptor_t k_pages_desc,
+    infiniopTensorDescriptor_t v_pages_desc, infiniopTensorDescriptor_t k_scales_desc, infiniopTensorDescriptor_t v_scales_desc,
+    infiniopTensorDescriptor_t new_table_desc, infiniopTensorDescriptor_t block_table_desc, infiniopTensorDescriptor_t seq_lens_desc,
+    infiniopTensorDescriptor_t page_map_desc, infiniopTensorDescriptor_t live_desc) {
+    if (handle == nullptr || handle->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (desc_ptr == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    if (new_table_desc == nullptr || page_map_desc == nullptr || live_desc == nullptr) return STATUS_BAD_PARAM;
+    CompactDesc d{};
+    infiniopStatus_t st = check_cache(k_pages_desc, v_pages_desc, k_scales_desc, v_scales_desc, d.c);
+    if (st != STATUS_SUCCESS) return st;
+    st = check_tables(block_table_desc, seq_lens_desc, nullptr, d.c.page, d.t);
+    if (st != STATUS_SUCCESS) return st;
+    if (new_table_desc->ndim != 2 || page_map_desc->ndim != 1 || live_desc->ndim != 1) return STATUS_BAD_TENSOR_SHAPE;
+    if (new_table_desc->shape[0] != (uint64_t) d.t.batch || new_table_desc->shape[1] != (uint64_t) d.t.cols ||
+        page_map_desc->shape[0] != (uint64_t) d.c.pages || live_desc->shape[0] != 1 || d.c.pages > (1 << 27)) {
+        return STATUS_BAD_TENSOR_SHAPE;
+    }
+    for (auto *x : {new_table_desc, page_map_desc, live_desc}) {
+        if (!dt_eq(x->dt, I32)) return STATUS_BAD_TENSOR_DTYPE;
+    }
+    for (auto *x : {new_table_desc, page_map_desc, live_desc}) {
+        if (!unit_rows(x) || !disjoint(x)) return STATUS_BAD_TENSOR_STRIDES;
+    }
+    auto *h = reinterpret_cast<Handle *>(handle);
+    d.device = DevNvGpu, d.device_id = h->device_id, d.sm_count = h->sm_count, d.new_stride = new_table_desc->strides[0];
+    auto *r = new (std::nothrow) CompactDesc(d);
+    if (r == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
+    *desc_ptr = reinterpret_cast<infiniopPagedCacheCompactDescriptor_t>(r);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopGetPagedCacheCompactWorkspaceSize(infiniopPagedCacheCompactDescriptor_t desc, uint64_t *size) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    if (size == nullptr) return STATUS_BAD_PARAM;
+    *size = plan_bytes((uint64_t) reinterpret_cast<CompactDesc *>(desc)->c.pages);
+    return STATUS_SUCCESS;
+}
+
+INFINIOP_API infiniopStatus_t infiniopPagedCacheCompact(infiniopPagedCacheCompactDescriptor_t desc, void *workspace,
+                                                        uint64_t workspace_size, void *k_pages, void *v_pages, void *k_scales,
+                                                        void *v_scales, void *new_table, void const *block_table,
+                                                        void const *seq_lens, void *page_map, void *live, void *stream) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    auto *d = reinterpret_cast<CompactDesc *>(desc);
+    const bool no_pages = d->c.pages == 0, no_rows = d->t.batch == 0 || d->t.cols == 0;
+    if (live == nullptr) return STATUS_BAD_PARAM;
+    if (!no_pages && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || page_map == nullptr)) return STATUS_BAD_PARAM;
+    if (!no_rows && (new_table == nullptr || block_table == nullptr || seq_lens == nullptr)) return STATUS_BAD_PARAM;
+    if (workspace == nullptr || workspace_size < plan_bytes((uint64_t) d->c.pages)) return STATUS_MEMORY_NOT_ALLOCATED;
+    DeviceGuard guard(d->device_id);
+    auto st = reinterpret_cast<cudaStream_t>(stream);
+    CompactParams p{};
+    p.table = reinterpret_cast<const int32_t *>(block_table), p.lens = reinterpret_cast<const int32_t *>(seq_lens);
+    p.new_table = reinterpret_cast<int32_t *>(new_table), p.page_map = reinterpret_cast<int32_t *>(page_map);
+    p.live = reinterpret_cast<int32_t *>(live);
+    p.new_stride = d->new_stride, p.t = d->t, p.pages = d->c.pages, p.page = d->c.page;
+    if (no_rows) p.t.batch = 0;
+    p.plan = plan_view(workspace, (uint64_t) d->c.pages);
+    if (launch_cluster(compact_plan_kernel, kPlanCtas, kPlanThreads, kPlanCtas, st, p) != cudaSuccess) return check_launch("paged cache compact (plan)");
+    const MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
+    const int unit = std::min(run_unit(m.k, k_pages), run_unit(m.v, v_pages));
+    auto run = [&](auto u, auto *kernel) {
+        using U = decltype(u);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned) d->sm_count * 8);
+        cfg.blockDim = dim3(kMoveThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr, cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, p, m, std::max(pieces_of<U>(m.k), pieces_of<U>(m.v)));
+    };
+    const cudaError_t e = unit == 16 ? run(uint4{}, compact_apply_kernel<uint4>) : unit == 4 ? run(uint32_t{}, compact_apply_kernel<uint32_t>)
+                                                                                             : run(uint8_t{}, compact_apply_kernel<uint8_t>);
+    (void) e;// reported by the check below
+    return check_launch("paged cache compact");
+}
+
+INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheCompactDescriptor(infiniopPagedCacheCompactDescriptor_t desc) {
+    if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
+    delete reinterpret_cast<CompactDesc *>(desc);
+    return STATUS_SUCCESS;
+}

@@ -30,3 +30,5 @@ I8, I16, I32, I64 = _dl(1, 1, 1, 7, 0), _dl(1, 1, 2, 15, 0), _dl(1, 1, 4, 31, 0)
 U8, U16, U32, U64 = _dl(1, 0, 1, 8, 0), _dl(1, 0, 2, 16, 0), _dl(1, 0, 4, 32, 0), _dl(1, 0, 8, 64, 0)
 F16, BF16 = _dl(1, 1, 2, 10, 5), _dl(1, 1, 2, 7, 8)
 F32, F64 = _dl(1, 1, 4, 23, 8), _dl(1, 1, 8, 52, 11)
+# e4m3 (additive, see include/infiniop.h): the codes of the paged KV cache
+F8E4M3 = _dl(1, 1, 1, 3, 4)

@@ -13,7 +13,7 @@ from ctypes import POINTER, c_float, c_int, c_int64, c_uint64, c_void_p
 
 from .data_layout import U64
 from .liboperators import infiniopHandle_t, infiniopTensorDescriptor_t
-from .utils import check_error, create_workspace, destroy_tensor_descriptor, to_tensor
+from .utils import check_error, create_scratch, create_workspace, destroy_tensor_descriptor, to_tensor
 
 _desc_t = c_void_p  # operator descriptors are opaque to Python
 
@@ -61,6 +61,22 @@ def _declare(lib):
         "infiniopGetAddRMSNormWorkspaceSize": [D, POINTER(c_uint64)],
         "infiniopAddRMSNorm": [D, c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
         "infiniopDestroyAddRMSNormDescriptor": [D],
+        "infiniopCreatePagedCacheAppendDescriptor": [H, POINTER(D)] + [T] * 9,
+        "infiniopGetPagedCacheAppendWorkspaceSize": [D, POINTER(c_uint64)],
+        "infiniopPagedCacheAppend": [D, c_void_p, c_uint64] + [c_void_p] * 10,
+        "infiniopDestroyPagedCacheAppendDescriptor": [D],
+        "infiniopCreatePagedAttentionDescriptor": [H, POINTER(D)] + [T] * 9 + [c_float],
+        "infiniopGetPagedAttentionWorkspaceSize": [D, POINTER(c_uint64)],
+        "infiniopPagedAttention": [D, c_void_p, c_uint64] + [c_void_p] * 10,
+        "infiniopDestroyPagedAttentionDescriptor": [D],
+        "infiniopCreatePagedCacheCopyDescriptor": [H, POINTER(D)] + [T] * 5,
+        "infiniopGetPagedCacheCopyWorkspaceSize": [D, POINTER(c_uint64)],
+        "infiniopPagedCacheCopy": [D, c_void_p, c_uint64] + [c_void_p] * 6,
+        "infiniopDestroyPagedCacheCopyDescriptor": [D],
+        "infiniopCreatePagedCacheCompactDescriptor": [H, POINTER(D)] + [T] * 9,
+        "infiniopGetPagedCacheCompactWorkspaceSize": [D, POINTER(c_uint64)],
+        "infiniopPagedCacheCompact": [D, c_void_p, c_uint64] + [c_void_p] * 10,
+        "infiniopDestroyPagedCacheCompactDescriptor": [D],
         "infiniopCreateCausalSoftmaxDescriptor": [H, POINTER(D), T],
         "infiniopGetCausalSoftmaxWorkspaceSize": [D, POINTER(c_uint64)],
         "infiniopCausalSoftmax": [D, c_void_p, c_uint64, c_void_p, c_void_p],
@@ -260,6 +276,108 @@ class AttentionOp(_Op):
                                                v_cache.data_ptr(), _stream_ptr(stream)))
 
 
+def _data(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+class _PagedOp(_Op):
+    """The operators of the paged cache write every byte of their workspace that they read."""
+
+    def _make_workspace(self, device):
+        size = c_uint64(0)
+        check_error(getattr(self.lib, self._wsize)(self.desc, ctypes.byref(size)))
+        self.workspace_size = size.value
+        self.workspace = create_scratch(size.value, device)
+
+    def release_after(self, stream):
+        """For the one-shot forms: the workspace goes back to torch's allocator when `stream` is done with it."""
+        if self.workspace is not None and stream is not None:
+            import torch
+
+            self.workspace.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream))
+
+
+class PagedCacheAppendOp(_PagedOp):
+    """Writes the new tokens' k, v[rows, n_kv_head, dh] (fp16 or bf16) into the pages of an e4m3 KV cache with one
+    scale per page and kv head (an addition of this library; the cache is described in include/infiniop.h):
+    k_pages, v_pages float8_e4m3fn [num_pages, n_kv_head, page_size, dh], k_scales, v_scales fp32
+    [num_pages, n_kv_head], block_table int32 [batch, columns], seq_lens int32 [batch] with the new tokens counted,
+    q_offsets int32 [batch + 1] or None for one new token per sequence."""
+    _destroy, _wsize = "infiniopDestroyPagedCacheAppendDescriptor", "infiniopGetPagedCacheAppendWorkspaceSize"
+
+    def __init__(self, lib, handle, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None):
+        super().__init__(lib, handle)
+        ts = [self._t(x).descriptor for x in (k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens)]
+        ts.append(None if q_offsets is None else self._t(q_offsets).descriptor)
+        check_error(lib.infiniopCreatePagedCacheAppendDescriptor(handle, ctypes.byref(self.desc), *ts))
+        self._make_workspace(k.device)
+
+    def __call__(self, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None, stream=None):
+        check_error(self.lib.infiniopPagedCacheAppend(
+            self.desc, self._ws_ptr(), self.workspace_size, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            _data(q_offsets), _stream_ptr(stream)))
+
+
+class PagedAttentionOp(_PagedOp):
+    """out[rows, n_q_head, dh] = causal attention of the new tokens q[rows, n_q_head, dh] over their sequences' pages,
+    scores times `scale` (an addition of this library; see PagedCacheAppendOp for the cache).  The new tokens' own k
+    and v must have been appended."""
+    _destroy, _wsize = "infiniopDestroyPagedAttentionDescriptor", "infiniopGetPagedAttentionWorkspaceSize"
+
+    def __init__(self, lib, handle, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
+                 scale=None):
+        super().__init__(lib, handle)
+        ts = [self._t(x).descriptor for x in (out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens)]
+        ts.append(None if q_offsets is None else self._t(q_offsets).descriptor)
+        check_error(lib.infiniopCreatePagedAttentionDescriptor(handle, ctypes.byref(self.desc), *ts,
+                                                               q.shape[-1] ** -0.5 if scale is None else scale))
+        self._make_workspace(q.device)
+
+    def __call__(self, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None, stream=None):
+        check_error(self.lib.infiniopPagedAttention(
+            self.desc, self._ws_ptr(), self.workspace_size, out.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            _data(q_offsets), _stream_ptr(stream)))
+
+
+class PagedCacheCopyOp(_PagedOp):
+    """Copies whole pages (K, V and scales): pairs int32 [n, 2] of (source, destination) on the device; rows with an
+    id outside the pool are skipped."""
+    _destroy, _wsize = "infiniopDestroyPagedCacheCopyDescriptor", "infiniopGetPagedCacheCopyWorkspaceSize"
+
+    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, pairs):
+        super().__init__(lib, handle)
+        ts = [self._t(x).descriptor for x in (k_pages, v_pages, k_scales, v_scales, pairs)]
+        check_error(lib.infiniopCreatePagedCacheCopyDescriptor(handle, ctypes.byref(self.desc), *ts))
+        self._make_workspace(k_pages.device)
+
+    def __call__(self, k_pages, v_pages, k_scales, v_scales, pairs, stream=None):
+        check_error(self.lib.infiniopPagedCacheCopy(
+            self.desc, self._ws_ptr(), self.workspace_size, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+            v_scales.data_ptr(), pairs.data_ptr(), _stream_ptr(stream)))
+
+
+class PagedCacheCompactOp(_PagedOp):
+    """Brings the pages that block_table names within seq_lens to the front of the pool: new_table int32 like
+    block_table (or block_table itself), page_map int32 [num_pages] (new id of each live page, -1 for free ones), live
+    int32 [1] (their number).  A sequence is freed by setting its length to 0."""
+    _destroy, _wsize = "infiniopDestroyPagedCacheCompactDescriptor", "infiniopGetPagedCacheCompactWorkspaceSize"
+
+    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live):
+        super().__init__(lib, handle)
+        ts = [self._t(x).descriptor for x in (k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens,
+                                              page_map, live)]
+        check_error(lib.infiniopCreatePagedCacheCompactDescriptor(handle, ctypes.byref(self.desc), *ts))
+        self._make_workspace(k_pages.device)
+
+    def __call__(self, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live, stream=None):
+        check_error(self.lib.infiniopPagedCacheCompact(
+            self.desc, self._ws_ptr(), self.workspace_size, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+            v_scales.data_ptr(), new_table.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), page_map.data_ptr(),
+            live.data_ptr(), _stream_ptr(stream)))
+
+
 class MatmulOp(_Op):
     """c = alpha * a @ b + beta * c on 2-D or batched 3-D tensors (reference operatorspy/tests/matmul.py)."""
     _destroy, _wsize = "infiniopDestroyMatmulDescriptor", "infiniopGetMatmulWorkspaceSize"
@@ -424,6 +542,37 @@ class RandomSampleOp(_Op):
 def attention(lib, handle, out, q, k, v, k_cache, v_cache, pos, stream=None):
     with AttentionOp(lib, handle, out, q, k, v, k_cache, v_cache, pos) as op:
         op(out, q, k, v, k_cache, v_cache, stream)
+
+
+def paged_cache_append(lib, handle, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
+                       stream=None):
+    args = (k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets)
+    with PagedCacheAppendOp(lib, handle, *args) as op:
+        op(*args, stream)
+        op.release_after(stream)
+
+
+def paged_attention(lib, handle, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
+                    scale=None, stream=None):
+    args = (out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets)
+    with PagedAttentionOp(lib, handle, *args, scale) as op:
+        op(*args, stream)
+        op.release_after(stream)
+
+
+def paged_cache_copy(lib, handle, k_pages, v_pages, k_scales, v_scales, pairs, stream=None):
+    args = (k_pages, v_pages, k_scales, v_scales, pairs)
+    with PagedCacheCopyOp(lib, handle, *args) as op:
+        op(*args, stream)
+        op.release_after(stream)
+
+
+def paged_cache_compact(lib, handle, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map,
+                        live, stream=None):
+    args = (k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live)
+    with PagedCacheCompactOp(lib, handle, *args) as op:
+        op(*args, stream)
+        op.release_after(stream)
 
 
 def matmul(lib, handle, c, a, b, alpha=1.0, beta=0.0, stream=None):

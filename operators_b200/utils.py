@@ -2,7 +2,7 @@
 reference's (reference operatorspy/utils.py:6-108)."""
 import ctypes
 
-from .data_layout import BF16, F16, F32, F64, I8, I16, I32, I64, U8, U16, U32, U64
+from .data_layout import BF16, F8E4M3, F16, F32, F64, I8, I16, I32, I64, U8, U16, U32, U64
 from .liboperators import CTensor, infiniopHandle_t, infiniopTensorDescriptor_t
 
 STATUS_NAMES = {
@@ -34,7 +34,7 @@ def _layout_of(dtype):
 
     table = {
         torch.int8: I8, torch.int16: I16, torch.int32: I32, torch.int64: I64, torch.uint8: U8,
-        torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64,
+        torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64, torch.float8_e4m3fn: F8E4M3,
     }
     for name, dl in (("uint16", U16), ("uint32", U32), ("uint64", U64)):
         if hasattr(torch, name):
@@ -70,6 +70,14 @@ def create_workspace(size, torch_device):
     import torch
 
     return torch.zeros(size=(size,), dtype=torch.uint8, device=torch_device)
+
+
+def create_scratch(size, torch_device):
+    """A workspace whose contents do not matter: no fill is queued on the current stream, so the operator may be
+    launched on another one right away."""
+    import torch
+
+    return torch.empty(size, dtype=torch.uint8, device=torch_device) if size else None
 
 
 def create_handle(lib, device, id=0):

@@ -1,9 +1,30 @@
-// Attention over the paged 8-bit KV cache (no counterpart in the reference, whose attention composite reads one fp16
-// cache per call, src/ops/attention/operator.cc:30-305):
-//     out[t, h, :] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q[t, h, :] . k_j - max),   j <= position of t
+// Attention over the paged 8-bit KV cache for few new tokens per sequence (no counterpart in the reference, whose
+// attention composite reads one fp16 cache per call, src/ops/attention/operator.cc:30-305):
+//     out[t, h, :] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(log2e * scale * q[t, h, :] . k_j - m),   j <= position of t
 // with k_j, v_j = code * scale of the page and kv head.
+//
+// What bounds it: one read of the codes, 2 * dh bytes per cached token and kv head, whatever the number of q heads that
+// share the kv head.  So a warp owns up to 8 or 16 query rows (the q heads of a group x the new tokens) and a tile of
+// 32 cached tokens at a time, and everything else is arranged around keeping loads in flight:
+//  * Work is a list of units = tiles of 32 tokens, ordered by sequence, kv head, block of query rows, tile.  Every
+//    CTA takes an equal stretch of the list, whatever the lengths (they are read on the device, so a captured graph
+//    follows the growing sequences); a stretch may end inside a sequence, and then the parts are joined by a second,
+//    small kernel in the order of the list.  No CTA waits for another.
+//  * A warp loads its own tiles with cp.async into a ring of its own in shared memory: no barrier in the loop.
+//  * Products run on mma.m16n8k16 (fp16 in, fp32 accumulation) with 16 cached tokens (q . k) or 16 head elements
+//    (p . v) as its rows and the query rows as its 8 columns: the contraction is far below a tcgen05 tile.  Codes
+//    become fp16 exactly in registers.  The contraction index is only a label, so every lane reads 16 consecutive
+//    bytes of a row; for p . v the bytes of two tokens are paired with one byte permutation per 4 elements.
+//  * q in fp16 too: each row is multiplied by a power of two that brings its largest element to [2^14, 2^15), which
+//    holds every bf16 element that is not 2^-29 of the largest exactly, and is undone in the score's factor.
+//  * The running maximum m of a row moves only when a score exceeds it by more than a factor 2, so most tiles rescale
+//    nothing.  The weight of a value is w_j = p_j * (scale of v_j): its own reference M keeps fp16 weights
+//    between 2^15 and what is 2^-28 of the largest (2^-39 with subnormals), however the pages' scales differ.  Sums
+//    of p and the output stay in fp32.
 #include "paged_cache.cuh"
+#include "paged_attention.cuh"
 
+#include <atomic>
 #include <cmath>
 #include <new>
 
@@ -12,87 +33,631 @@ using namespace b200::paged;
 
 namespace {
 
-struct AttendParams {
-    uint16_t *out;
-    const uint16_t *q;
-    int64_t o_st, o_sh, q_st, q_sh;// strides of token and head
-    const uint8_t *kp, *vp;
-    const float *ks, *vs;
-    const int32_t *table, *lens, *offs;
-    int32_t rows, q_heads, group;
-    float scale;
-    CacheShape c;
-    TableShape t;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kTile = 32;      // cached tokens per warp and step
+constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
+constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
+constexpr float kLift = 14.f;  // weights are stored times 2^14: at most 2^(14 + slack) < 65504
+
+__host__ __device__ constexpr int stages_of(int dhc) { return dhc == 64 ? 4 : 3; }
+// One stage of a warp's ring: K rows, V rows, their scales, the mask of valid tokens.
+__host__ __device__ constexpr int stage_bytes(int dhc) { return 2 * kTile * dhc + 2 * kTile * 4 + 16; }
+__host__ __device__ constexpr int smem_bytes(int dhc) { return kWarps * stages_of(dhc) * stage_bytes(dhc); }
+__host__ __device__ constexpr int ctas_per_sm(int dhc) { return dhc <= 128 ? 2 : 1; }
+
+// A part of an item (one block of query rows of one kv head of one sequence) that a CTA worked on: its rows' reference
+// and sum, the weights' reference, and the unnormalised output.
+struct PartHead {
+    float m, l, w, pad;
+};
+struct CtaMeta {
+    int32_t b, kvh, rb;// the item that begins in this CTA's stretch and goes on behind it; b < 0: none
+    int32_t head;      // the stretch begins inside an item: 1 = that item ends in it, 2 = goes on behind it; else 0
 };
 
-constexpr int kThreads = 128;
-
-template<bool BF>
-__device__ __forceinline__ uint16_t round16(float v) {
-    if (BF) {
-        uint16_t r;
-        asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
-        return r;
-    }
-    return __half_as_ushort(__float2half_rn(v));
+// Byte position of 16-byte chunk c of row r in a tile of rows of DHC bytes.  Chosen so that the lanes of a quarter warp
+// hit different banks in both access patterns: 4 chunks of each of 2 neighbouring rows (q . k) and 2 chunks of each of
+// 4 rows that are 2 apart (p . v).
+template<int DHC>
+__device__ __forceinline__ uint32_t chunk_at(uint32_t r, uint32_t c) {
+    if (DHC == 128) return r * 128 + ((c ^ (r & 7u)) << 4);
+    if (DHC == 64) return (r >> 1) * 128 + (((((r & 1u) << 2) | c) ^ ((r >> 1 & 3u) << 1)) << 4);
+    return r * 256 + ((c ^ ((r >> 1 & 1u) | (((r ^ (r >> 2)) & 1u) << 2))) << 4);
 }
-__device__ __forceinline__ float e4m3_to_f32(uint8_t c) { return unpack2(e4m3x2_to_f16x2(c)).x; }
+// The chunk that lane t (of 4) of a row reads as its h-th in q . k.
+template<int DHC>
+__device__ __forceinline__ uint32_t key_chunk(uint32_t t, uint32_t h) {
+    return DHC == 128 ? 2 * t + h : t + 4 * h;
+}
 
-// One CTA per new token and q head; a warp per cached token, a lane per 32nd element.
-template<bool BF>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendParams p) {
-    __shared__ float part[4][256], stats[4][2];
-    __shared__ int32_t owner;
-    const int32_t row = (int32_t) blockIdx.x, head = (int32_t) blockIdx.y, kvh = head / p.group;
-    if (threadIdx.x == 0) owner = -1;
-    __syncthreads();
-    for (int32_t b = threadIdx.x; b < p.t.batch; b += kThreads) {
-        const Seq s = seq_of(p.lens, p.offs, p.rows, b);
-        if (row >= s.first && row - s.first < s.n) owner = b;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template<int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t lo_f16x2(uint32_t w) { return e4m3x2_to_f16x2((uint16_t) w); }
+__device__ __forceinline__ uint32_t hi_f16x2(uint32_t w) { return e4m3x2_to_f16x2((uint16_t) (w >> 16)); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+
+
+// Sum over the CTA of a 64-bit value and the sum over the threads before; `slot`: kWarps words.
+__device__ __forceinline__ int64_t cta_exclusive_sum64(int64_t v, int64_t *slot, int64_t &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
     }
     __syncthreads();
-    if (owner < 0) return;
-    const int32_t b = owner;
-    const Seq s = seq_of(p.lens, p.offs, p.rows, b);
-    const int32_t pos = s.len - s.n + (row - s.first);
-    const int32_t keys = pos < 0 ? 0 : held(pos + 1, p.t.cap), D = p.c.dh;
-    const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float q[8], acc[8], m = -INFINITY, l = 0.f;
-    for (int i = 0; i < 8; ++i) {
-        const int32_t d = lane + 32 * i;
-        q[i] = d < D ? f16or_bf16x2<BF>(p.q[(int64_t) row * p.q_st + (int64_t) head * p.q_sh + d]).x : 0.f;
-        acc[i] = 0.f;
+    if (lane == 31) slot[warp] = incl;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += slot[w];
+        total += slot[w];
     }
-    for (int32_t j = warp; j < keys; j += 4) {
-        const int32_t page = p.table[(int64_t) b * p.t.stride + j / p.c.page], at = j % p.c.page;
-        if (page < 0 || page >= p.c.pages) continue;
-        const uint8_t *k = p.kp + page * p.c.k.sn + kvh * p.c.k.sh + at * p.c.k.sp, *v = p.vp + page * p.c.v.sn + kvh * p.c.v.sh + at * p.c.v.sp;
-        float x = 0.f;
-        for (int i = 0; i < 8; ++i) {
-            if (lane + 32 * i < D) x = fmaf(q[i], e4m3_to_f32(k[lane + 32 * i]), x);
+    return before + incl - v;
+}
+
+struct DecodeParams {
+    AttendParams a;
+    PartHead *heads;// [cta][2][rows]
+    float *parts;   // [cta][2][rows][DHC]
+    CtaMeta *meta;  // [cta]
+};
+
+// Blocks of query rows and tiles of a sequence; its units are blocks x kv heads x tiles.
+template<int ROWS>
+__device__ __forceinline__ void extent_of(const AttendParams &p, const Seq &s, int32_t &blocks, int32_t &tiles) {
+    blocks = (int32_t) (((int64_t) s.n * p.group + ROWS - 1) / ROWS);
+    const int32_t keys = held(s.len, p.t.cap);
+    tiles = keys > 0 ? (keys - 1) / kTile + 1 : 1;// a sequence without keys still writes zeros
+}
+
+// The state of a warp's ring while it walks tiles first, first + kWarps, .. of one item.
+struct Walk {
+    int32_t b, keys;
+    const uint8_t *k, *v;// this kv head's pages
+    const float *ks, *vs;
+};
+
+// DHC: head size rounded up to 64, 128 or 256; NT: 8 * NT query rows.
+template<int DHC, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(const DecodeParams dp) {
+    constexpr int kRows = 8 * NT, kStages = stages_of(DHC), kStage = stage_bytes(DHC), kChunks = DHC / 16;
+    constexpr int kHalf = DHC / 64;  // chunks per lane and row in q . k
+    constexpr int kSteps = DHC / 16; // mma steps of q . k, and m-tiles of p . v
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int64_t slot[kWarps], found_base;
+    __shared__ int32_t found_b;
+    const AttendParams &p = dp.a;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t ring = (uint32_t) __cvta_generic_to_shared(smem) + warp * kStages * kStage;
+
+    // ---- this CTA's stretch of the units
+    auto units_of = [&](int32_t b) -> int64_t {
+        int32_t blocks, tiles;
+        extent_of<kRows>(p, seq_of(p.lens, p.offs, p.rows, b), blocks, tiles);
+        return (int64_t) blocks * tiles * p.c.heads;
+    };
+    int64_t mine = 0, total;
+    for (int32_t b = (int32_t) threadIdx.x; b < p.t.batch; b += kThreads) mine += units_of(b);
+    cta_exclusive_sum64(mine, slot, total);
+    int64_t each = (total + gridDim.x - 1) / gridDim.x;
+    if (each < kMinUnits) each = kMinUnits;
+    int64_t u = each * blockIdx.x;
+    const int64_t u_end = u + each < total ? u + each : total;
+    if (u >= u_end) {
+        if (threadIdx.x == 0) dp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
+        asm volatile("griddepcontrol.launch_dependents;");
+        return;
+    }
+    {
+        int64_t base = 0;
+        for (int32_t b0 = 0; b0 < p.t.batch && base <= u; b0 += kThreads) {
+            const int32_t b = b0 + (int32_t) threadIdx.x;
+            const int64_t n = b < p.t.batch ? units_of(b) : 0;
+            int64_t sum;
+            const int64_t before = base + cta_exclusive_sum64(n, slot, sum);
+            if (u >= before && u - before < n) found_b = b, found_base = before;
+            base += sum;
         }
-        x = warp_sum(x) * p.ks[page * p.c.k.cn + kvh * p.c.k.ch] * p.scale;
-        const float m_new = fmaxf(m, x), shrink = m == -INFINITY ? 0.f : expf(m - m_new), w = m_new == -INFINITY ? 0.f : expf(x - m_new);
-        const float wv = w * p.vs[page * p.c.v.cn + kvh * p.c.v.ch];
-        l = l * shrink + w, m = m_new;
-        for (int i = 0; i < 8; ++i) {
-            if (lane + 32 * i < D) acc[i] = acc[i] * shrink + wv * e4m3_to_f32(v[lane + 32 * i]);
+    }
+    // head elements beyond dh: zeros in every stage, never written again
+    if (p.c.dh < DHC) {
+        for (uint32_t i = lane * 16; i < (uint32_t) (kStages * kStage); i += 512) {
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(ring + i), "r"(0) : "memory");
         }
     }
-    for (int i = 0; i < 8; ++i) part[warp][lane + 32 * i] = acc[i];
-    if (lane == 0) stats[warp][0] = m, stats[warp][1] = l;
     __syncthreads();
-    float top = -INFINITY, sum = 0.f, w[4];
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, stats[i][0]);
-    for (int i = 0; i < 4; ++i) {
-        w[i] = stats[i][0] == -INFINITY ? 0.f : expf(stats[i][0] - top);
-        sum += w[i] * stats[i][1];
+    int32_t b = found_b;
+    int64_t base = found_base;
+    CtaMeta meta{-1, 0, 0, 0};
+    const bool one_page = p.c.page % kTile == 0;// a tile lies in one page
+
+    while (u < u_end) {
+        Seq s = seq_of(p.lens, p.offs, p.rows, b);
+        int32_t blocks, tiles;
+        extent_of<kRows>(p, s, blocks, tiles);
+        const int64_t units = (int64_t) blocks * tiles * p.c.heads;
+        if (units == 0 || u - base >= units) {// on to the next sequence (u < total: there is one)
+            base += units, ++b;
+            continue;
+        }
+        const int64_t item = (u - base) / tiles;
+        const int32_t t0 = (int32_t) (u - base - item * tiles);
+        const int32_t t1 = u_end - u < tiles - t0 ? t0 + (int32_t) (u_end - u) : tiles;
+        const int32_t kvh = (int32_t) (item / blocks), rb = (int32_t) (item - (int64_t) kvh * blocks);
+        u += t1 - t0;
+
+        Walk w;
+        w.b = b, w.keys = held(s.len, p.t.cap);
+        w.k = p.kp + (int64_t) kvh * p.c.k.sh, w.v = p.vp + (int64_t) kvh * p.c.v.sh;
+        w.ks = p.ks + (int64_t) kvh * p.c.k.ch, w.vs = p.vs + (int64_t) kvh * p.c.v.ch;
+        const int32_t *row_table = p.table + (int64_t) b * p.t.stride;
+
+        // page of this lane's token of a tile (-1: none), read one step ahead of its use
+        auto page_of = [&](int32_t tile) -> int32_t {
+            const int32_t tok = tile * kTile + (int32_t) lane;
+            if (tile >= t1 || tok >= w.keys) return -1;
+            const int32_t id = row_table[tok / p.c.page];
+            return id >= 0 && id < p.c.pages ? id : -1;
+        };
+        // loads of one tile into a stage
+        auto fetch = [&](uint32_t st, int32_t tile, int32_t page) {
+            const uint32_t at = ring + st * kStage, kat = at, vat = at + kTile * DHC, sat = vat + kTile * DHC;
+            const int32_t tok = tile * kTile + (int32_t) lane, in_page = tok % p.c.page;
+            const bool valid = page >= 0;
+            const int64_t koff = valid ? (int64_t) page * p.c.k.sn + (int64_t) in_page * p.c.k.sp : 0;
+            const int64_t voff = valid ? (int64_t) page * p.c.v.sn + (int64_t) in_page * p.c.v.sp : 0;
+            cp_async4(sat + lane * 4, valid ? w.ks + (int64_t) page * p.c.k.cn : w.ks, valid);
+            cp_async4(sat + 128 + lane * 4, valid ? w.vs + (int64_t) page * p.c.v.cn : w.vs, valid);
+            const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+            if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sat + 256), "r"(mask) : "memory");
+            if (p.vec) {
+                constexpr int kPer = kChunks, kRowsAtOnce = 32 / kPer;// lanes per row; DHC 256: 16 lanes, 2 rows
+                const uint32_t c = lane % kPer, r0 = lane / kPer;
+                const bool has = (int32_t) c * 16 < p.c.dh;
+                if (one_page) {
+                    // one page: rows follow each other at the token stride
+                    const int64_t k0 = shfl64(koff, 0) + (int64_t) r0 * p.c.k.sp + c * 16, v0 = shfl64(voff, 0) + (int64_t) r0 * p.c.v.sp + c * 16;
+#pragma unroll
+                    for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+                        const uint32_t r = r0 + i * kRowsAtOnce, to = chunk_at<DHC>(r, c);
+                        const bool ok = (mask >> r) & 1u;
+                        if (has) {
+                            cp_async16(kat + to, ok ? w.k + (k0 + (int64_t) (i * kRowsAtOnce) * p.c.k.sp) : w.k, ok);
+                            cp_async16(vat + to, ok ? w.v + (v0 + (int64_t) (i * kRowsAtOnce) * p.c.v.sp) : w.v, ok);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+                        const uint32_t r = r0 + i * kRowsAtOnce, to = chunk_at<DHC>(r, c);
+                        const int64_t kr = shfl64(koff, (int) r) + c * 16, vr = shfl64(voff, (int) r) + c * 16;
+                        const bool ok = (mask >> r) & 1u;
+                        if (has) {
+                            cp_async16(kat + to, ok ? w.k + kr : w.k, ok);
+                            cp_async16(vat + to, ok ? w.v + vr : w.v, ok);
+                        }
+                    }
+                }
+            } else {
+                // rows that are no whole aligned vectors: a lane copies its token's bytes one by one
+                for (int32_t d = 0; d < p.c.dh; ++d) {
+                    const uint32_t to = chunk_at<DHC>(lane, (uint32_t) d >> 4) + (d & 15);
+                    const uint32_t kb = valid ? w.k[koff + d] : 0u, vb = valid ? w.v[voff + d] : 0u;
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(kat + to), "r"(kb) : "memory");
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(vat + to), "r"(vb) : "memory");
+                }
+            }
+        };
+
+        // ---- start the ring, then read q
+        int32_t ahead = t0 + (int32_t) warp, page = page_of(ahead);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) {
+            const int32_t next = page_of(ahead + kWarps);
+            if (ahead < t1) fetch((uint32_t) i, ahead, page);
+            cp_async_commit();
+            page = next, ahead += kWarps;
+        }
+
+        // q: lane (g, t) holds the elements of row g that its chunks of a key row meet.  Row r of the block is new token
+        // (rb * kRows + r) / group, q head kvh * group + (..) % group.
+        uint32_t qf[NT][kSteps][2];
+        float factor[NT];
+        const int32_t n_rows = (int32_t) min((int64_t) kRows, (int64_t) s.n * p.group - (int64_t) rb * kRows);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int32_t r = nt * 8 + (int32_t) g;
+            const bool have = r < n_rows;
+            const int64_t rr = (int64_t) rb * kRows + r;
+            const int32_t tok = have ? (int32_t) (rr / p.group) : 0, hd = have ? (int32_t) (rr - (int64_t) tok * p.group) : 0;
+            const uint16_t *q = p.q + (int64_t) (s.first + tok) * p.q_st + (int64_t) (kvh * p.group + hd) * p.q_sh;
+            uint32_t top = 0;
+#pragma unroll
+            for (int h = 0; h < kHalf; ++h) {
+                const int32_t d0 = (int32_t) key_chunk<DHC>(t, (uint32_t) h) * 16;
+                uint32_t x[8];
+                if (have && p.q_vec && d0 + 16 <= p.c.dh) {
+                    const uint4 lo = *reinterpret_cast<const uint4 *>(q + d0), hi = *reinterpret_cast<const uint4 *>(q + d0 + 8);
+                    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int32_t d = d0 + 2 * i;
+                        const uint32_t a = have && d < p.c.dh ? q[d] : 0u, c = have && d + 1 < p.c.dh ? q[d + 1] : 0u;
+                        x[i] = a | (c << 16);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    qf[nt][h * 4 + i / 2][i % 2] = x[i];
+                    top = __vmaxu2(top, x[i] & 0x7FFF7FFFu);
+                }
+            }
+            top = __vmaxu2(top, top >> 16) & 0xFFFFu;
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int32_t shift = query_shift(p.bf16, top);
+            const float up = __uint_as_float(pow2_bits(shift));
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 f = p.bf16 ? unpack2_t<kBF16>(qf[nt][i][j]) : unpack2(qf[nt][i][j]);
+                    const __half2 v = __floats2half2_rn(f.x * up, f.y * up);
+                    qf[nt][i][j] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+            }
+            factor[nt] = __uint_as_float(pow2_bits(-shift)) * p.scale_log2;
+        }
+        // scores come as (token g, rows 2t and 2t + 1): the factors and limits of those rows
+        float rf[NT][2];
+        int32_t limit[NT][2], least = w.keys;// keys that a row sees
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int32_t r = nt * 8 + (int32_t) (2 * t) + i;
+                rf[nt][i] = __shfl_sync(0xffffffffu, factor[nt], (int) (2 * t + i) * 4);
+                const int64_t rr = (int64_t) rb * kRows + r;
+                const int32_t pos = s.len - s.n + (int32_t) (rr / p.group);
+                limit[nt][i] = r < n_rows ? max(0, min(pos + 1, w.keys)) : 0;
+                if (r < n_rows) least = min(least, limit[nt][i]);
+            }
+        }
+        least = __reduce_min_sync(0xffffffffu, least);
+
+        // ---- the loop over this warp's tiles
+        float o[NT][kSteps][4], m[NT][2], wm[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = wm[nt][0] = wm[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        }
+        uint32_t st = 0, st_ahead = kStages - 1;
+        for (int32_t tile = t0 + (int32_t) warp; tile < t1; tile += kWarps) {
+            const int32_t next = page_of(ahead + kWarps);
+            cp_async_wait<kStages - 2>();
+            __syncwarp();// every lane's copies have landed, and every lane is done with the stage that is filled next
+            if (ahead < t1) fetch(st_ahead, ahead, page);
+            cp_async_commit();
+            page = next, ahead += kWarps;
+            if (++st_ahead == kStages) st_ahead = 0;
+
+            const uint32_t kat = ring + st * kStage, vat = kat + kTile * DHC, sat = vat + kTile * DHC;
+            if (++st == kStages) st = 0;
+            // q . k
+            float x[2][NT][4];
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) x[sub][nt][0] = x[sub][nt][1] = x[sub][nt][2] = x[sub][nt][3] = 0.f;
+            }
+#pragma unroll
+            for (int h = 0; h < kHalf; ++h) {
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    const uint32_t c = key_chunk<DHC>(t, (uint32_t) h);
+                    const uint4 lo = lds128(kat + chunk_at<DHC>(sub * 16 + g, c)), hi = lds128(kat + chunk_at<DHC>(sub * 16 + 8 + g, c));
+                    const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, e[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a0 = lo_f16x2(a[i]), a2 = hi_f16x2(a[i]), a1 = lo_f16x2(e[i]), a3 = hi_f16x2(e[i]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_f16(x[sub][nt], a0, a1, a2, a3, qf[nt][h * 4 + i][0], qf[nt][h * 4 + i][1]);
+                    }
+                }
+            }
+            // scores in powers of two, masked
+            float lv[4];// log2 of the values' scales: tokens g, g + 8, g + 16, g + 24
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float ks = lds_f32(sat + (i * 8 + g) * 4);
+                lv[i] = lds_f32(sat + 128 + (i * 8 + g) * 4);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    x[i >> 1][nt][(i & 1) * 2] *= ks * rf[nt][0];
+                    x[i >> 1][nt][(i & 1) * 2 + 1] *= ks * rf[nt][1];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lv[i] = log2f(lv[i]);
+            const uint32_t mask = lds_u32(sat + 256);
+            if (mask != 0xFFFFFFFFu || tile * kTile + kTile > least) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int32_t tok = tile * kTile + i * 8 + (int32_t) g;
+                    const bool ok = (mask >> (i * 8 + g)) & 1u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (!ok || tok >= limit[nt][0]) x[i >> 1][nt][(i & 1) * 2] = -INFINITY;
+                        if (!ok || tok >= limit[nt][1]) x[i >> 1][nt][(i & 1) * 2 + 1] = -INFINITY;
+                    }
+                    if (!ok) lv[i] = 0.f;
+                }
+            }
+            // references: moved when a score or a weight exceeds its own by more than the slack
+            bool over = false;
+            float top[NT][2], wtop[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float a0 = x[0][nt][i], a1 = x[0][nt][2 + i], a2 = x[1][nt][i], a3 = x[1][nt][2 + i];
+                    top[nt][i] = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
+                    wtop[nt][i] = fmaxf(fmaxf(a0 + lv[0], a1 + lv[1]), fmaxf(a2 + lv[2], a3 + lv[3]));
+                    over = over || top[nt][i] > m[nt][i] + kSlack || wtop[nt][i] > wm[nt][i] + kSlack;
+                }
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) {
+                            top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
+                            wtop[nt][i] = fmaxf(wtop[nt][i], __shfl_xor_sync(0xffffffffu, wtop[nt][i], d));
+                        }
+                        if (top[nt][i] > m[nt][i] + kSlack) {
+                            l[nt][i] *= fast_exp2(m[nt][i] - top[nt][i]);// from -inf: 0
+                            m[nt][i] = top[nt][i];
+                        }
+                        if (wtop[nt][i] > wm[nt][i] + kSlack) {
+                            const float f = fast_exp2(wm[nt][i] - wtop[nt][i]);
+#pragma unroll
+                            for (int j = 0; j < kSteps; ++j) o[nt][j][i] *= f, o[nt][j][2 + i] *= f;
+                            wm[nt][i] = wtop[nt][i];
+                        }
+                    }
+                }
+            }
+            // p to its sum, w in fp16 as operand B of p . v
+            uint32_t bw[2][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                // rows that have seen nothing yet: their scores are all -inf, any finite reference gives 0
+                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+                const float w0 = wm[nt][0] == -INFINITY ? 0.f : wm[nt][0] - kLift, w1 = wm[nt][1] == -INFINITY ? 0.f : wm[nt][1] - kLift;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[i >> 1][nt][(i & 1) * 2], c = x[i >> 1][nt][(i & 1) * 2 + 1];
+                    l[nt][0] += fast_exp2(a - m0), l[nt][1] += fast_exp2(c - m1);
+                    const __half2 h = __floats2half2_rn(fast_exp2(a - w0 + lv[i]), fast_exp2(c - w1 + lv[i]));
+                    bw[i >> 1][nt][i & 1] = transpose8x8(*reinterpret_cast<const uint32_t *>(&h));
+                }
+            }
+            // p . v: lane (g, t) holds DHC / 8 consecutive head elements of tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                constexpr int kWords = DHC / 32;
+                uint32_t v[4][kWords];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t r = sub * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+                    if (DHC == 64) {
+                        const uint2 a = lds64(vat + chunk_at<DHC>(r, g >> 1) + (g & 1) * 8);
+                        v[i][0] = a.x, v[i][1] = a.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kWords / 4; ++c) {
+                            const uint4 a = lds128(vat + chunk_at<DHC>(r, g * (kWords / 4) + c));
+                            v[i][c * 4] = a.x, v[i][c * 4 + 1] = a.y, v[i][c * 4 + 2] = a.z, v[i][c * 4 + 3] = a.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    // bytes of two tokens side by side: (a0 b0 a1 b1) and (a2 b2 a3 b3)
+                    const uint32_t e0 = __byte_perm(v[0][i], v[1][i], 0x5140), e1 = __byte_perm(v[0][i], v[1][i], 0x7362);
+                    const uint32_t f0 = __byte_perm(v[2][i], v[3][i], 0x5140), f1 = __byte_perm(v[2][i], v[3][i], 0x7362);
+                    const uint32_t a0 = lo_f16x2(e0), a1 = hi_f16x2(e0), a2 = lo_f16x2(f0), a3 = hi_f16x2(f0);
+                    const uint32_t c0 = lo_f16x2(e1), c1 = hi_f16x2(e1), c2 = lo_f16x2(f1), c3 = hi_f16x2(f1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_f16(o[nt][2 * i], a0, a1, a2, a3, bw[sub][nt][0], bw[sub][nt][1]);
+                        mma_f16(o[nt][2 * i + 1], c0, c1, c2, c3, bw[sub][nt][0], bw[sub][nt][1]);
+                    }
+                }
+            }
+        }
+
+        // ---- the warps' results meet in shared memory: [warp][row][DHC] and the rows' references
+        cp_async_wait<0>();
+        __syncthreads();
+        float *so = reinterpret_cast<float *>(smem);
+        PartHead *sh = reinterpret_cast<PartHead *>(so + kWarps * kRows * DHC);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = nt * 8 + 2 * (int) t + i;
+                float sum = l[nt][i];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (g == 0) sh[warp * kRows + r] = PartHead{m[nt][i], sum, wm[nt][i], 0.f};
+                // elements g * DHC / 8 .. of this row; 16-byte groups rotated by the row, so that the four rows of a
+                // store spread over the banks
+                float *dst = so + (warp * kRows + r) * DHC;
+#pragma unroll
+                for (int j = 0; j < kSteps; j += 2) {
+                    const uint32_t grp = g * (DHC / 32) + j / 2;
+                    *reinterpret_cast<float4 *>(dst + ((grp ^ (uint32_t) (r & 7)) << 2)) = make_float4(o[nt][j][i], o[nt][j][2 + i], o[nt][j + 1][i], o[nt][j + 1][2 + i]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == tiles;
+        const int part = t0 > 0 ? 0 : 1;
+        const int64_t slot0 = ((int64_t) blockIdx.x * 2 + part) * kRows;
+        for (int r = (int) warp; r < n_rows; r += kWarps) {
+            float mr = -INFINITY, wr = -INFINITY, lr = 0.f, f[kWarps];
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) mr = fmaxf(mr, sh[i * kRows + r].m), wr = fmaxf(wr, sh[i * kRows + r].w);
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                const PartHead h = sh[i * kRows + r];
+                lr += h.m == -INFINITY ? 0.f : h.l * fast_exp2(h.m - mr);
+                f[i] = h.w == -INFINITY ? 0.f : fast_exp2(h.w - wr);
+            }
+            const int64_t rr = (int64_t) rb * kRows + r;
+            const int32_t tok = (int32_t) (rr / p.group), hd = (int32_t) (rr - (int64_t) tok * p.group);
+            uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (kvh * p.group + hd) * p.o_sh;
+            if (!whole && lane == 0) dp.heads[slot0 + r] = PartHead{mr, lr, wr, 0.f};
+#pragma unroll
+            for (int j = 0; j < (DHC + 127) / 128; ++j) {
+                const uint32_t grp = lane + 32 * j;
+                if (DHC == 64 && grp >= 16) break;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) {
+                    const float4 a = *reinterpret_cast<const float4 *>(so + (i * kRows + r) * DHC + ((grp ^ (uint32_t) (r & 7)) << 2));
+                    if (f[i] != 0.f) y.x += f[i] * a.x, y.y += f[i] * a.y, y.z += f[i] * a.z, y.w += f[i] * a.w;
+                }
+                if (whole) store_out(p, out, (int32_t) grp * 4, y, lr, wr - kLift - mr);
+                else *reinterpret_cast<float4 *>(dp.parts + (slot0 + r) * DHC + grp * 4) = y;
+            }
+        }
+        if (!whole) {
+            if (part == 0) meta.head = t1 == tiles ? 1 : 2;
+            else meta.b = b, meta.kvh = kvh, meta.rb = rb;
+        }
+        if (u < u_end) {
+            __syncthreads();// the ring is loaded again
+            if (p.c.dh < DHC) {// .. and the zeros beyond dh were written over
+                for (uint32_t i = lane * 16; i < (uint32_t) (kStages * kStage); i += 512) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(ring + i), "r"(0) : "memory");
+                }
+                __syncwarp();
+            }
+        }
     }
-    for (int32_t d = threadIdx.x; d < D; d += kThreads) {
-        float y = 0.f;
-        for (int i = 0; i < 4; ++i) y += w[i] * part[i][d];
-        p.out[(int64_t) row * p.o_st + (int64_t) head * p.o_sh + d] = round16<BF>(sum == 0.f ? 0.f : y / sum);
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) dp.meta[blockIdx.x] = meta;
+}
+
+// Joins the parts of the item that begins in stretch blockIdx.x and goes on behind it: one block per row, 8 groups of
+// threads take every eighth part, the groups' sums are added in order.
+constexpr int kJoinGroups = 8;
+template<int DHC, int NT>
+__global__ void __launch_bounds__(kJoinGroups * DHC / 4) join_kernel(const DecodeParams dp, int32_t ctas) {
+    constexpr int kRows = 8 * NT, kLanes = DHC / 4;
+    __shared__ float4 acc[kJoinGroups][kLanes];
+    __shared__ float stat[kJoinGroups][3];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const AttendParams &p = dp.a;
+    const CtaMeta first = dp.meta[blockIdx.x];
+    if (first.b < 0) return;
+    const int r = (int) blockIdx.y;
+    const Seq s = seq_of(p.lens, p.offs, p.rows, first.b);
+    const int64_t rr = (int64_t) first.rb * kRows + r;
+    if (rr >= (int64_t) s.n * p.group) return;
+    int32_t last = (int32_t) blockIdx.x + 1;// the stretch that holds the item's end
+    while (last + 1 < ctas && dp.meta[last].head == 2) ++last;
+    const int grp = (int) threadIdx.x / kLanes, ln = (int) threadIdx.x % kLanes;
+    float m = -INFINITY, l = 0.f, w = -INFINITY;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int32_t c = (int32_t) blockIdx.x + grp; c <= last; c += kJoinGroups) {
+        const int64_t at = ((int64_t) c * 2 + (c == (int32_t) blockIdx.x ? 1 : 0)) * kRows + r;
+        const PartHead h = dp.heads[at];
+        const float4 v = *reinterpret_cast<const float4 *>(dp.parts + at * DHC + ln * 4);
+        if (h.m != -INFINITY) {
+            const float n = fmaxf(m, h.m);
+            l = l * fast_exp2(m - n) + h.l * fast_exp2(h.m - n);
+            m = n;
+        }
+        if (h.w != -INFINITY) {
+            const float n = fmaxf(w, h.w), f0 = fast_exp2(w - n), f1 = fast_exp2(h.w - n);
+            y.x = y.x * f0 + v.x * f1, y.y = y.y * f0 + v.y * f1, y.z = y.z * f0 + v.z * f1, y.w = y.w * f0 + v.w * f1;
+            w = n;
+        }
     }
+    acc[grp][ln] = y;
+    if (ln == 0) stat[grp][0] = m, stat[grp][1] = l, stat[grp][2] = w;
+    __syncthreads();
+    if (grp != 0) return;
+    m = w = -INFINITY, l = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kJoinGroups; ++i) m = fmaxf(m, stat[i][0]), w = fmaxf(w, stat[i][2]);
+#pragma unroll
+    for (int i = 0; i < kJoinGroups; ++i) {
+        if (stat[i][0] != -INFINITY) l += stat[i][1] * fast_exp2(stat[i][0] - m);
+        if (stat[i][2] != -INFINITY) {
+            const float f = fast_exp2(stat[i][2] - w);
+            const float4 v = acc[i][ln];
+            y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+        }
+    }
+    const int32_t tok = (int32_t) (rr / p.group), hd = (int32_t) (rr - (int64_t) tok * p.group);
+    uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (first.kvh * p.group + hd) * p.o_sh;
+    store_out(p, out, ln * 4, y, l, w - kLift - m);
 }
 
 struct AttendDesc {
@@ -104,7 +669,48 @@ struct AttendDesc {
     bool bf16;
     int64_t o_st, o_sh, q_st, q_sh;
     float scale;
+    int dhc, nt;
+    uint32_t ctas;
 };
+
+uint64_t workspace_of(const AttendDesc &d) {
+    const uint64_t slots = (uint64_t) d.ctas * 2 * 8 * d.nt;
+    return slots * (sizeof(PartHead) + (uint64_t) d.dhc * 4) + d.ctas * sizeof(CtaMeta);
+}
+
+template<int DHC, int NT>
+cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
+    constexpr int kSmem = smem_bytes(DHC);
+    static_assert(kWarps * 8 * NT * DHC * 4 + kWarps * 8 * NT * (int) sizeof(PartHead) <= kSmem, "the warps' results fit their rings");
+    static_assert(stage_bytes(DHC) % 16 == 0, "stages start on 16 bytes");
+    DecodeParams dp{};
+    dp.a = a;
+    const uint64_t slots = (uint64_t) d.ctas * 2 * 8 * NT;
+    dp.parts = reinterpret_cast<float *>(workspace);
+    dp.heads = reinterpret_cast<PartHead *>(dp.parts + slots * DHC);
+    dp.meta = reinterpret_cast<CtaMeta *>(dp.heads + slots);
+    // more shared memory than the default: asked for once per device (again, where two threads come first)
+    static std::atomic<uint64_t> ready{0};
+    const uint64_t bit = d.device_id < 64 ? 1ull << d.device_id : 0;
+    cudaError_t e = cudaSuccess;
+    if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+        e = cudaFuncSetAttribute(decode_kernel<DHC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    decode_kernel<DHC, NT><<<d.ctas, kThreads, kSmem, st>>>(dp);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || d.ctas == 1) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(d.ctas - 1, 8 * NT);
+    cfg.blockDim = dim3(kJoinGroups * DHC / 4);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<DHC, NT>, dp, (int32_t) d.ctas);
+}
 
 }// namespace
 
@@ -135,6 +741,18 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     d.device = DevNvGpu, d.device_id = h->device_id, d.sm_count = h->sm_count;
     d.rows = (int32_t) rows, d.q_heads = (int32_t) heads, d.bf16 = dt_eq(q_desc->dt, BF16), d.scale = scale;
     d.o_st = out_desc->strides[0], d.o_sh = out_desc->strides[1], d.q_st = q_desc->strides[0], d.q_sh = q_desc->strides[1];
+    d.dhc = d.c.dh <= 64 ? 64 : d.c.dh <= 128 ? 128 : 256;
+    // query rows per sequence on average (the device knows each one's): more than 8 share a read of the cache in 16s
+    const int64_t group = d.q_heads / d.c.heads, rows_each = d.t.batch > 0 ? (int64_t) d.rows * group / d.t.batch : 0;
+    d.nt = rows_each > 8 ? 2 : 1;
+    // every CTA that fits the GPU at once, but no more than there can be units for
+    const int64_t blocks = ((int64_t) d.rows * group + 8 * d.nt - 1) / (8 * d.nt) + d.t.batch;
+    const int64_t tiles = std::max<int64_t>(1, ((int64_t) d.t.cap + kTile - 1) / kTile);
+    const int64_t places = (int64_t) d.sm_count * ctas_per_sm(d.dhc);
+    d.ctas = (uint32_t) places;
+    if (blocks * d.c.heads < places * kMinUnits) {
+        d.ctas = (uint32_t) std::max<int64_t>(1, std::min(places, (blocks * d.c.heads * tiles + kMinUnits - 1) / kMinUnits));
+    }
     auto *r = new (std::nothrow) AttendDesc(d);
     if (r == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
     *desc_ptr = reinterpret_cast<infiniopPagedAttentionDescriptor_t>(r);
@@ -144,7 +762,7 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
 INFINIOP_API infiniopStatus_t infiniopGetPagedAttentionWorkspaceSize(infiniopPagedAttentionDescriptor_t desc, uint64_t *size) {
     if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
     if (size == nullptr) return STATUS_BAD_PARAM;
-    *size = 0;
+    *size = workspace_of(*reinterpret_cast<AttendDesc *>(desc));
     return STATUS_SUCCESS;
 }
 
@@ -153,8 +771,6 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
                                                      void const *v_pages, void const *k_scales, void const *v_scales,
                                                      void const *block_table, void const *seq_lens, void const *q_offsets,
                                                      void *stream) {
-    (void) workspace;
-    (void) workspace_size;
     if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
     auto *d = reinterpret_cast<AttendDesc *>(desc);
     if (d->rows == 0 || d->t.batch == 0) return STATUS_SUCCESS;
@@ -162,17 +778,39 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     // a table without columns or a pool without pages has no keys: every token gets zeros
     const bool empty = d->t.cols == 0 || d->c.pages == 0;
     if (!empty && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || block_table == nullptr)) return STATUS_BAD_PARAM;
+    if (workspace == nullptr || workspace_size < workspace_of(*d)) return STATUS_MEMORY_NOT_ALLOCATED;
     DeviceGuard guard(d->device_id);
-    AttendParams p{reinterpret_cast<uint16_t *>(out), reinterpret_cast<const uint16_t *>(q), d->o_st, d->o_sh, d->q_st, d->q_sh,
-                   reinterpret_cast<const uint8_t *>(k_pages), reinterpret_cast<const uint8_t *>(v_pages),
-                   reinterpret_cast<const float *>(k_scales), reinterpret_cast<const float *>(v_scales),
-                   reinterpret_cast<const int32_t *>(block_table), reinterpret_cast<const int32_t *>(seq_lens),
-                   reinterpret_cast<const int32_t *>(q_offsets), d->rows, d->q_heads, d->q_heads / d->c.heads, d->scale, d->c, d->t};
+    AttendParams p{};
+    p.out = reinterpret_cast<uint16_t *>(out), p.q = reinterpret_cast<const uint16_t *>(q);
+    p.o_st = d->o_st, p.o_sh = d->o_sh, p.q_st = d->q_st, p.q_sh = d->q_sh;
+    p.kp = reinterpret_cast<const uint8_t *>(k_pages), p.vp = reinterpret_cast<const uint8_t *>(v_pages);
+    p.ks = reinterpret_cast<const float *>(k_scales), p.vs = reinterpret_cast<const float *>(v_scales);
+    p.table = reinterpret_cast<const int32_t *>(block_table), p.lens = reinterpret_cast<const int32_t *>(seq_lens);
+    p.offs = reinterpret_cast<const int32_t *>(q_offsets);
+    p.rows = d->rows, p.group = d->q_heads / d->c.heads;
+    p.scale_log2 = (float) ((double) d->scale * 1.4426950408889634);
+    p.c = d->c, p.t = d->t, p.bf16 = d->bf16;
     if (empty) p.t.cap = 0;
+    // whole 16-byte vectors: rows of codes, rows of q; 8-byte pieces of out's rows
+    p.vec = d->c.dh % 16 == 0 && aligned16(k_pages) && aligned16(v_pages);
+    for (int64_t s : {d->c.k.sn, d->c.k.sh, d->c.k.sp, d->c.v.sn, d->c.v.sh, d->c.v.sp}) p.vec = p.vec && s % 16 == 0;
+    p.q_vec = aligned16(q) && d->q_st % 8 == 0 && d->q_sh % 8 == 0;
+    p.o_vec = (uintptr_t) out % 8 == 0 && d->o_st % 4 == 0 && d->o_sh % 4 == 0 && d->c.dh % 4 == 0;
     auto st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned) d->rows, (unsigned) d->q_heads);
-    if (d->bf16) attend_kernel<true><<<grid, kThreads, 0, st>>>(p);
-    else attend_kernel<false><<<grid, kThreads, 0, st>>>(p);
+    cudaError_t e;
+    switch (d->dhc * 4 + d->nt) {
+        case 64 * 4 + 1: e = launch_decode<64, 1>(*d, p, workspace, st); break;
+        case 64 * 4 + 2: e = launch_decode<64, 2>(*d, p, workspace, st); break;
+        case 128 * 4 + 1: e = launch_decode<128, 1>(*d, p, workspace, st); break;
+        case 128 * 4 + 2: e = launch_decode<128, 2>(*d, p, workspace, st); break;
+        case 256 * 4 + 1: e = launch_decode<256, 1>(*d, p, workspace, st); break;
+        default: e = launch_decode<256, 2>(*d, p, workspace, st); break;
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        fprintf(stderr, "infiniop[b200]: paged attention launch failed: %s\n", cudaGetErrorString(e));
+        return STATUS_EXECUTION_FAILED;
+    }
     return check_launch("paged attention");
 }
 

@@ -39,11 +39,13 @@ constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
 constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
 constexpr float kLift = 14.f;  // weights are stored times 2^14: at most 2^(14 + slack) < 65504
 
-__host__ __device__ constexpr int stages_of(int dhc) { return dhc == 64 ? 4 : 3; }
+// Resident CTAs per SM and stages of a warp's ring.  8 rows of a head size up to 128 leave registers for 12 to 16 warps
+// per SM, which hide each other's latency better than deeper rings of fewer warps do.
+__host__ __device__ constexpr int ctas_per_sm(int dhc, int nt) { return dhc == 256 ? 1 : dhc == 128 ? (nt == 1 ? 3 : 2) : (nt == 1 ? 4 : 3); }
+__host__ __device__ constexpr int stages_of(int dhc, int nt) { return dhc == 128 && nt == 1 ? 2 : 3; }
 // One stage of a warp's ring: K rows, V rows, their scales, the mask of valid tokens.
 __host__ __device__ constexpr int stage_bytes(int dhc) { return 2 * kTile * dhc + 2 * kTile * 4 + 16; }
-__host__ __device__ constexpr int smem_bytes(int dhc) { return kWarps * stages_of(dhc) * stage_bytes(dhc); }
-__host__ __device__ constexpr int ctas_per_sm(int dhc) { return dhc <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int smem_bytes(int dhc, int nt) { return kWarps * stages_of(dhc, nt) * stage_bytes(dhc); }
 
 // A part of an item (one block of query rows of one kv head of one sequence) that a CTA worked on: its rows' reference
 // and sum, the weights' reference, and the unnormalised output.
@@ -155,6 +157,13 @@ __device__ __forceinline__ void extent_of(const AttendParams &p, const Seq &s, i
     tiles = keys > 0 ? (keys - 1) / kTile + 1 : 1;// a sequence without keys still writes zeros
 }
 
+// log2 of a scale; exact and cheap for the powers of two that append writes.  Zero gives -inf.
+__device__ __forceinline__ float log2_of(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if (__any_sync(0xffffffffu, (u & 0x807FFFFFu) != 0 || u == 0)) return log2f(v);
+    return (float) ((int32_t) (u >> 23) - 127);
+}
+
 // The state of a warp's ring while it walks tiles first, first + kWarps, .. of one item.
 struct Walk {
     int32_t b, keys;
@@ -162,10 +171,11 @@ struct Walk {
     const float *ks, *vs;
 };
 
-// DHC: head size rounded up to 64, 128 or 256; NT: 8 * NT query rows.
-template<int DHC, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(const DecodeParams dp) {
-    constexpr int kRows = 8 * NT, kStages = stages_of(DHC), kStage = stage_bytes(DHC), kChunks = DHC / 16;
+// DHC: head size rounded up to 64, 128 or 256; NT: 8 * NT query rows; ONE: a tile lies in one page (the page size is a
+// multiple of 32) and its rows are whole aligned vectors, so one page id, two scales and a count describe it.
+template<int DHC, int NT, bool ONE>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(const DecodeParams dp) {
+    constexpr int kRows = 8 * NT, kStages = stages_of(DHC, NT), kStage = stage_bytes(DHC), kChunks = DHC / 16;
     constexpr int kHalf = DHC / 64;  // chunks per lane and row in q . k
     constexpr int kSteps = DHC / 16; // mma steps of q . k, and m-tiles of p . v
     extern __shared__ __align__(128) unsigned char smem[];
@@ -214,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
     int32_t b = found_b;
     int64_t base = found_base;
     CtaMeta meta{-1, 0, 0, 0};
-    const bool one_page = p.c.page % kTile == 0;// a tile lies in one page
 
     while (u < u_end) {
         Seq s = seq_of(p.lens, p.offs, p.rows, b);
@@ -239,57 +248,78 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
 
         // page of this lane's token of a tile (-1: none), read one step ahead of its use
         auto page_of = [&](int32_t tile) -> int32_t {
-            const int32_t tok = tile * kTile + (int32_t) lane;
+            const int32_t tok = tile * kTile + (ONE ? 0 : (int32_t) lane);
             if (tile >= t1 || tok >= w.keys) return -1;
-            const int32_t id = row_table[tok / p.c.page];
+            const int32_t id = row_table[p.page_div.div((uint32_t) tok)];
             return id >= 0 && id < p.c.pages ? id : -1;
         };
-        // loads of one tile into a stage
+        // loads of one tile into a stage.  Tokens without a page become zeros; their addresses stay inside the pool.
         auto fetch = [&](uint32_t st, int32_t tile, int32_t page) {
             const uint32_t at = ring + st * kStage, kat = at, vat = at + kTile * DHC, sat = vat + kTile * DHC;
-            const int32_t tok = tile * kTile + (int32_t) lane, in_page = tok % p.c.page;
-            const bool valid = page >= 0;
-            const int64_t koff = valid ? (int64_t) page * p.c.k.sn + (int64_t) in_page * p.c.k.sp : 0;
-            const int64_t voff = valid ? (int64_t) page * p.c.v.sn + (int64_t) in_page * p.c.v.sp : 0;
-            cp_async4(sat + lane * 4, valid ? w.ks + (int64_t) page * p.c.k.cn : w.ks, valid);
-            cp_async4(sat + 128 + lane * 4, valid ? w.vs + (int64_t) page * p.c.v.cn : w.vs, valid);
-            const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-            if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sat + 256), "r"(mask) : "memory");
-            if (p.vec) {
-                constexpr int kPer = kChunks, kRowsAtOnce = 32 / kPer;// lanes per row; DHC 256: 16 lanes, 2 rows
-                const uint32_t c = lane % kPer, r0 = lane / kPer;
-                const bool has = (int32_t) c * 16 < p.c.dh;
-                if (one_page) {
-                    // one page: rows follow each other at the token stride
-                    const int64_t k0 = shfl64(koff, 0) + (int64_t) r0 * p.c.k.sp + c * 16, v0 = shfl64(voff, 0) + (int64_t) r0 * p.c.v.sp + c * 16;
+            constexpr int kAtOnce = 32 / kChunks;// rows that the lanes load at a time, 16 bytes each
+            const uint32_t c = lane % kChunks, r0 = lane / kChunks;
+            const int32_t id = max(page, 0);
+            if (ONE) {
+                const int32_t first = tile * kTile, in_page = first - (int32_t) p.page_div.div((uint32_t) first) * p.c.page;
+                const int32_t count = page < 0 ? 0 : min(kTile, w.keys - first);
+                const uint8_t *k = w.k + (int64_t) id * p.c.k.sn + (int64_t) (in_page + (int32_t) r0) * p.c.k.sp + c * 16;
+                const uint8_t *v = w.v + (int64_t) id * p.c.v.sn + (int64_t) (in_page + (int32_t) r0) * p.c.v.sp + c * 16;
+                if (lane < 2) {
+                    const float *s = lane == 0 ? w.ks + (int64_t) id * p.c.k.cn : w.vs + (int64_t) id * p.c.v.cn;
+                    cp_async4(sat + lane * 4, s, page >= 0);// no page: scales of 0, log2 -inf
+                }
+                if (lane == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sat + 8), "r"(count) : "memory");
+                if ((int32_t) c * 16 < p.c.dh) {
+                    if (count == kTile) {
 #pragma unroll
-                    for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-                        const uint32_t r = r0 + i * kRowsAtOnce, to = chunk_at<DHC>(r, c);
-                        const bool ok = (mask >> r) & 1u;
-                        if (has) {
-                            cp_async16(kat + to, ok ? w.k + (k0 + (int64_t) (i * kRowsAtOnce) * p.c.k.sp) : w.k, ok);
-                            cp_async16(vat + to, ok ? w.v + (v0 + (int64_t) (i * kRowsAtOnce) * p.c.v.sp) : w.v, ok);
+                        for (int i = 0; i < kTile / kAtOnce; ++i) {
+                            const uint32_t to = chunk_at<DHC>(r0 + i * kAtOnce, c);
+                            cp_async16(kat + to, k, true);
+                            cp_async16(vat + to, v, true);
+                            k += kAtOnce * p.c.k.sp, v += kAtOnce * p.c.v.sp;
                         }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-                        const uint32_t r = r0 + i * kRowsAtOnce, to = chunk_at<DHC>(r, c);
-                        const int64_t kr = shfl64(koff, (int) r) + c * 16, vr = shfl64(voff, (int) r) + c * 16;
-                        const bool ok = (mask >> r) & 1u;
-                        if (has) {
-                            cp_async16(kat + to, ok ? w.k + kr : w.k, ok);
-                            cp_async16(vat + to, ok ? w.v + vr : w.v, ok);
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < kTile / kAtOnce; ++i) {
+                            const uint32_t to = chunk_at<DHC>(r0 + i * kAtOnce, c);
+                            const bool ok = (int32_t) r0 + i * kAtOnce < count;
+                            cp_async16(kat + to, k, ok);
+                            cp_async16(vat + to, v, ok);
+                            k += kAtOnce * p.c.k.sp, v += kAtOnce * p.c.v.sp;
                         }
                     }
                 }
             } else {
-                // rows that are no whole aligned vectors: a lane copies its token's bytes one by one
-                for (int32_t d = 0; d < p.c.dh; ++d) {
-                    const uint32_t to = chunk_at<DHC>(lane, (uint32_t) d >> 4) + (d & 15);
-                    const uint32_t kb = valid ? w.k[koff + d] : 0u, vb = valid ? w.v[voff + d] : 0u;
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(kat + to), "r"(kb) : "memory");
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(vat + to), "r"(vb) : "memory");
+                const int32_t tok = tile * kTile + (int32_t) lane;
+                const bool valid = page >= 0;
+                const int32_t in_page = valid ? tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page : 0;
+                const int64_t koff = (int64_t) id * p.c.k.sn + (int64_t) in_page * p.c.k.sp;
+                const int64_t voff = (int64_t) id * p.c.v.sn + (int64_t) in_page * p.c.v.sp;
+                cp_async4(sat + lane * 4, w.ks + (int64_t) id * p.c.k.cn, valid);
+                cp_async4(sat + 128 + lane * 4, w.vs + (int64_t) id * p.c.v.cn, valid);
+                const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+                if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sat + 256), "r"(mask) : "memory");
+                if (p.vec) {
+                    const bool has = (int32_t) c * 16 < p.c.dh;
+#pragma unroll 4
+                    for (int i = 0; i < kTile / kAtOnce; ++i) {
+                        const uint32_t r = r0 + i * kAtOnce, to = chunk_at<DHC>(r, c);
+                        const int64_t kr = shfl64(koff, (int) r) + c * 16, vr = shfl64(voff, (int) r) + c * 16;
+                        const bool ok = (mask >> r) & 1u;
+                        if (has) {
+                            cp_async16(kat + to, w.k + kr, ok);
+                            cp_async16(vat + to, w.v + vr, ok);
+                        }
+                    }
+                } else {
+                    // rows that are no whole aligned vectors: a lane copies its token's bytes one by one
+#pragma unroll 1
+                    for (int32_t d = 0; d < p.c.dh; ++d) {
+                        const uint32_t to = chunk_at<DHC>(lane, (uint32_t) d >> 4) + (d & 15);
+                        const uint32_t kb = valid ? w.k[koff + d] : 0u, vb = valid ? w.v[voff + d] : 0u;
+                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(kat + to), "r"(kb) : "memory");
+                        asm volatile("st.shared.u8 [%0], %1;" ::"r"(vat + to), "r"(vb) : "memory");
+                    }
                 }
             }
         };
@@ -297,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
         // ---- start the ring, then read q
         int32_t ahead = t0 + (int32_t) warp, page = page_of(ahead);
         __syncwarp();
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kStages - 1; ++i) {
             const int32_t next = page_of(ahead + kWarps);
             if (ahead < t1) fetch((uint32_t) i, ahead, page);
@@ -415,21 +445,33 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
                     }
                 }
             }
-            // scores in powers of two, masked
-            float lv[4];// log2 of the values' scales: tokens g, g + 8, g + 16, g + 24
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float ks = lds_f32(sat + (i * 8 + g) * 4);
-                lv[i] = lds_f32(sat + 128 + (i * 8 + g) * 4);
+            // scores in powers of two, masked; lv: log2 of the values' scales of tokens g, g + 8, g + 16, g + 24
+            float lv[4];
+            uint32_t mask;
+            if (ONE) {
+                const float ks = lds_f32(sat);
+                lv[0] = lv[1] = lv[2] = lv[3] = log2_of(lds_f32(sat + 4));
+                const uint32_t count = lds_u32(sat + 8);
+                mask = count >= 32 ? 0xFFFFFFFFu : (1u << count) - 1u;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    x[i >> 1][nt][(i & 1) * 2] *= ks * rf[nt][0];
-                    x[i >> 1][nt][(i & 1) * 2 + 1] *= ks * rf[nt][1];
+                    const float f0 = ks * rf[nt][0], f1 = ks * rf[nt][1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i >> 1][nt][(i & 1) * 2] *= f0, x[i >> 1][nt][(i & 1) * 2 + 1] *= f1;
+                }
+            } else {
+                mask = lds_u32(sat + 256);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float ks = lds_f32(sat + (i * 8 + g) * 4);
+                    lv[i] = log2_of(lds_f32(sat + 128 + (i * 8 + g) * 4));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        x[i >> 1][nt][(i & 1) * 2] *= ks * rf[nt][0];
+                        x[i >> 1][nt][(i & 1) * 2 + 1] *= ks * rf[nt][1];
+                    }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) lv[i] = log2f(lv[i]);
-            const uint32_t mask = lds_u32(sat + 256);
             if (mask != 0xFFFFFFFFu || tile * kTile + kTile > least) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -440,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
                         if (!ok || tok >= limit[nt][0]) x[i >> 1][nt][(i & 1) * 2] = -INFINITY;
                         if (!ok || tok >= limit[nt][1]) x[i >> 1][nt][(i & 1) * 2 + 1] = -INFINITY;
                     }
-                    if (!ok) lv[i] = 0.f;
+                    if (!ONE && !ok) lv[i] = 0.f;
                 }
             }
             // references: moved when a score or a weight exceeds its own by more than the slack
@@ -452,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
                 for (int i = 0; i < 2; ++i) {
                     const float a0 = x[0][nt][i], a1 = x[0][nt][2 + i], a2 = x[1][nt][i], a3 = x[1][nt][2 + i];
                     top[nt][i] = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-                    wtop[nt][i] = fmaxf(fmaxf(a0 + lv[0], a1 + lv[1]), fmaxf(a2 + lv[2], a3 + lv[3]));
+                    wtop[nt][i] = ONE ? top[nt][i] + lv[0] : fmaxf(fmaxf(a0 + lv[0], a1 + lv[1]), fmaxf(a2 + lv[2], a3 + lv[3]));
                     over = over || top[nt][i] > m[nt][i] + kSlack || wtop[nt][i] > wm[nt][i] + kSlack;
                 }
             }
@@ -464,8 +506,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) {
                             top[nt][i] = fmaxf(top[nt][i], __shfl_xor_sync(0xffffffffu, top[nt][i], d));
-                            wtop[nt][i] = fmaxf(wtop[nt][i], __shfl_xor_sync(0xffffffffu, wtop[nt][i], d));
+                            if (!ONE) wtop[nt][i] = fmaxf(wtop[nt][i], __shfl_xor_sync(0xffffffffu, wtop[nt][i], d));
                         }
+                        if (ONE) wtop[nt][i] = top[nt][i] + lv[0];
                         if (top[nt][i] > m[nt][i] + kSlack) {
                             l[nt][i] *= fast_exp2(m[nt][i] - top[nt][i]);// from -inf: 0
                             m[nt][i] = top[nt][i];
@@ -485,12 +528,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC)) decode_kernel(cons
             for (int nt = 0; nt < NT; ++nt) {
                 // rows that have seen nothing yet: their scores are all -inf, any finite reference gives 0
                 const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                const float w0 = wm[nt][0] == -INFINITY ? 0.f : wm[nt][0] - kLift, w1 = wm[nt][1] == -INFINITY ? 0.f : wm[nt][1] - kLift;
+                float w0 = wm[nt][0] == -INFINITY ? 0.f : wm[nt][0] - kLift, w1 = wm[nt][1] == -INFINITY ? 0.f : wm[nt][1] - kLift;
+                if (ONE) w0 -= lv[0], w1 -= lv[0];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float a = x[i >> 1][nt][(i & 1) * 2], c = x[i >> 1][nt][(i & 1) * 2 + 1];
                     l[nt][0] += fast_exp2(a - m0), l[nt][1] += fast_exp2(c - m1);
-                    const __half2 h = __floats2half2_rn(fast_exp2(a - w0 + lv[i]), fast_exp2(c - w1 + lv[i]));
+                    const __half2 h = ONE ? __floats2half2_rn(fast_exp2(a - w0), fast_exp2(c - w1)) : __floats2half2_rn(fast_exp2(a - w0 + lv[i]), fast_exp2(c - w1 + lv[i]));
                     bw[i >> 1][nt][i & 1] = transpose8x8(*reinterpret_cast<const uint32_t *>(&h));
                 }
             }
@@ -678,9 +722,9 @@ uint64_t workspace_of(const AttendDesc &d) {
     return slots * (sizeof(PartHead) + (uint64_t) d.dhc * 4) + d.ctas * sizeof(CtaMeta);
 }
 
-template<int DHC, int NT>
-cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
-    constexpr int kSmem = smem_bytes(DHC);
+template<int DHC, int NT, bool ONE>
+cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
+    constexpr int kSmem = smem_bytes(DHC, NT);
     static_assert(kWarps * 8 * NT * DHC * 4 + kWarps * 8 * NT * (int) sizeof(PartHead) <= kSmem, "the warps' results fit their rings");
     static_assert(stage_bytes(DHC) % 16 == 0, "stages start on 16 bytes");
     DecodeParams dp{};
@@ -694,11 +738,11 @@ cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *work
     const uint64_t bit = d.device_id < 64 ? 1ull << d.device_id : 0;
     cudaError_t e = cudaSuccess;
     if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-        e = cudaFuncSetAttribute(decode_kernel<DHC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        e = cudaFuncSetAttribute(decode_kernel<DHC, NT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    decode_kernel<DHC, NT><<<d.ctas, kThreads, kSmem, st>>>(dp);
+    decode_kernel<DHC, NT, ONE><<<d.ctas, kThreads, kSmem, st>>>(dp);
     e = cudaGetLastError();
     if (e != cudaSuccess || d.ctas == 1) return e;
     cudaLaunchConfig_t cfg = {};
@@ -710,6 +754,10 @@ cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *work
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, join_kernel<DHC, NT>, dp, (int32_t) d.ctas);
+}
+template<int DHC, int NT>
+cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
+    return a.vec && a.c.page % kTile == 0 ? launch_decode_as<DHC, NT, true>(d, a, workspace, st) : launch_decode_as<DHC, NT, false>(d, a, workspace, st);
 }
 
 }// namespace
@@ -748,7 +796,7 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     // every CTA that fits the GPU at once, but no more than there can be units for
     const int64_t blocks = ((int64_t) d.rows * group + 8 * d.nt - 1) / (8 * d.nt) + d.t.batch;
     const int64_t tiles = std::max<int64_t>(1, ((int64_t) d.t.cap + kTile - 1) / kTile);
-    const int64_t places = (int64_t) d.sm_count * ctas_per_sm(d.dhc);
+    const int64_t places = (int64_t) d.sm_count * ctas_per_sm(d.dhc, d.nt);
     d.ctas = (uint32_t) places;
     if (blocks * d.c.heads < places * kMinUnits) {
         d.ctas = (uint32_t) std::max<int64_t>(1, std::min(places, (blocks * d.c.heads * tiles + kMinUnits - 1) / kMinUnits));
@@ -789,6 +837,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     p.offs = reinterpret_cast<const int32_t *>(q_offsets);
     p.rows = d->rows, p.group = d->q_heads / d->c.heads;
     p.scale_log2 = (float) ((double) d->scale * 1.4426950408889634);
+    p.page_div = FastDiv((uint32_t) d->c.page);
     p.c = d->c, p.t = d->t, p.bf16 = d->bf16;
     if (empty) p.t.cap = 0;
     // whole 16-byte vectors: rows of codes, rows of q; 8-byte pieces of out's rows

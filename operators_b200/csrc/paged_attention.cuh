@@ -16,6 +16,7 @@ struct AttendParams {
     int32_t rows, group;
     float scale_log2;// scale * log2(e)
     bool bf16, vec, q_vec, o_vec;
+    FastDiv page_div;// by the page size
     CacheShape c;
     TableShape t;
 };

@@ -36,6 +36,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;      // cached tokens per warp and step
 constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
+constexpr int kPrefillRows = 32;// query rows per sequence from which on the tcgen05 kernel takes the call
 constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
 constexpr float kLift = 14.f;  // weights are stored times 2^14: at most 2^(14 + slack) < 65504
 
@@ -46,16 +47,6 @@ __host__ __device__ constexpr int stages_of(int dhc, int nt) { return dhc == 128
 // One stage of a warp's ring: K rows, V rows, their scales, the mask of valid tokens.
 __host__ __device__ constexpr int stage_bytes(int dhc) { return 2 * kTile * dhc + 2 * kTile * 4 + 16; }
 __host__ __device__ constexpr int smem_bytes(int dhc, int nt) { return kWarps * stages_of(dhc, nt) * stage_bytes(dhc); }
-
-// A part of an item (one block of query rows of one kv head of one sequence) that a CTA worked on: its rows' reference
-// and sum, the weights' reference, and the unnormalised output.
-struct PartHead {
-    float m, l, w, pad;
-};
-struct CtaMeta {
-    int32_t b, kvh, rb;// the item that begins in this CTA's stretch and goes on behind it; b < 0: none
-    int32_t head;      // the stretch begins inside an item: 1 = that item ends in it, 2 = goes on behind it; else 0
-};
 
 // Byte position of 16-byte chunk c of row r in a tile of rows of DHC bytes.  Chosen so that the lanes of a quarter warp
 // hit different banks in both access patterns: 4 chunks of each of 2 neighbouring rows (q . k) and 2 chunks of each of
@@ -120,39 +111,10 @@ __device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
 __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
 
 
-// Sum over the CTA of a 64-bit value and the sum over the threads before; `slot`: kWarps words.
-__device__ __forceinline__ int64_t cta_exclusive_sum64(int64_t v, int64_t *slot, int64_t &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t incl = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
-    }
-    __syncthreads();
-    if (lane == 31) slot[warp] = incl;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += slot[w];
-        total += slot[w];
-    }
-    return before + incl - v;
-}
-
-struct DecodeParams {
-    AttendParams a;
-    PartHead *heads;// [cta][2][rows]
-    float *parts;   // [cta][2][rows][DHC]
-    CtaMeta *meta;  // [cta]
-};
-
 // Blocks of query rows and tiles of a sequence; its units are blocks x kv heads x tiles.
 template<int ROWS>
 __device__ __forceinline__ void extent_of(const AttendParams &p, const Seq &s, int32_t &blocks, int32_t &tiles) {
-    blocks = (int32_t) (((int64_t) s.n * p.group + ROWS - 1) / ROWS);
+    blocks = (int32_t) (((uint32_t) s.n * (uint32_t) p.group + ROWS - 1) / ROWS);// (rows x group < 2^31)
     const int32_t keys = held(s.len, p.t.cap);
     tiles = keys > 0 ? (keys - 1) / kTile + 1 : 1;// a sequence without keys still writes zeros
 }
@@ -174,7 +136,7 @@ struct Walk {
 // DHC: head size rounded up to 64, 128 or 256; NT: 8 * NT query rows; ONE: a tile lies in one page (the page size is a
 // multiple of 32) and its rows are whole aligned vectors, so one page id, two scales and a count describe it.
 template<int DHC, int NT, bool ONE>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(const DecodeParams dp) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(const SplitParams dp) {
     constexpr int kRows = 8 * NT, kStages = stages_of(DHC, NT), kStage = stage_bytes(DHC), kChunks = DHC / 16;
     constexpr int kHalf = DHC / 64;  // chunks per lane and row in q . k
     constexpr int kSteps = DHC / 16; // mma steps of q . k, and m-tiles of p . v
@@ -193,9 +155,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
     };
     int64_t mine = 0, total;
     for (int32_t b = (int32_t) threadIdx.x; b < p.t.batch; b += kThreads) mine += units_of(b);
-    cta_exclusive_sum64(mine, slot, total);
-    int64_t each = (total + gridDim.x - 1) / gridDim.x;
-    if (each < kMinUnits) each = kMinUnits;
+    cta_exclusive_sum64<kWarps>(mine, slot, total);
+    const int64_t each = stretch_of(total, kMinUnits);
     int64_t u = each * blockIdx.x;
     const int64_t u_end = u + each < total ? u + each : total;
     if (u >= u_end) {
@@ -209,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             const int32_t b = b0 + (int32_t) threadIdx.x;
             const int64_t n = b < p.t.batch ? units_of(b) : 0;
             int64_t sum;
-            const int64_t before = base + cta_exclusive_sum64(n, slot, sum);
+            const int64_t before = base + cta_exclusive_sum64<kWarps>(n, slot, sum);
             if (u >= before && u - before < n) found_b = b, found_base = before;
             base += sum;
         }
@@ -223,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
     __syncthreads();
     int32_t b = found_b;
     int64_t base = found_base;
-    CtaMeta meta{-1, 0, 0, 0};
+    CtaMeta meta{-1, 0, 0, 0};// joined by the second kernel
 
     while (u < u_end) {
         Seq s = seq_of(p.lens, p.offs, p.rows, b);
@@ -234,10 +195,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             base += units, ++b;
             continue;
         }
-        const int64_t item = (u - base) / tiles;
+        const int64_t item = divide(u - base, tiles);
         const int32_t t0 = (int32_t) (u - base - item * tiles);
         const int32_t t1 = u_end - u < tiles - t0 ? t0 + (int32_t) (u_end - u) : tiles;
-        const int32_t kvh = (int32_t) (item / blocks), rb = (int32_t) (item - (int64_t) kvh * blocks);
+        const int32_t kvh = (int32_t) divide(item, blocks), rb = (int32_t) (item - (int64_t) kvh * blocks);
         u += t1 - t0;
 
         Walk w;
@@ -339,13 +300,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
         // (rb * kRows + r) / group, q head kvh * group + (..) % group.
         uint32_t qf[NT][kSteps][2];
         float factor[NT];
-        const int32_t n_rows = (int32_t) min((int64_t) kRows, (int64_t) s.n * p.group - (int64_t) rb * kRows);
+        const int32_t n_rows = min(kRows, s.n * p.group - rb * kRows);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int32_t r = nt * 8 + (int32_t) g;
             const bool have = r < n_rows;
-            const int64_t rr = (int64_t) rb * kRows + r;
-            const int32_t tok = have ? (int32_t) (rr / p.group) : 0, hd = have ? (int32_t) (rr - (int64_t) tok * p.group) : 0;
+            const uint32_t rr = (uint32_t) rb * kRows + (uint32_t) r;
+            const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0, hd = have ? (int32_t) rr - tok * p.group : 0;
             const uint16_t *q = p.q + (int64_t) (s.first + tok) * p.q_st + (int64_t) (kvh * p.group + hd) * p.q_sh;
             uint32_t top = 0;
 #pragma unroll
@@ -394,8 +355,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             for (int i = 0; i < 2; ++i) {
                 const int32_t r = nt * 8 + (int32_t) (2 * t) + i;
                 rf[nt][i] = __shfl_sync(0xffffffffu, factor[nt], (int) (2 * t + i) * 4);
-                const int64_t rr = (int64_t) rb * kRows + r;
-                const int32_t pos = s.len - s.n + (int32_t) (rr / p.group);
+                const int32_t pos = s.len - s.n + (int32_t) p.group_div.div((uint32_t) rb * kRows + (uint32_t) r);
                 limit[nt][i] = r < n_rows ? max(0, min(pos + 1, w.keys)) : 0;
                 if (r < n_rows) least = min(least, limit[nt][i]);
             }
@@ -611,10 +571,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 lr += h.m == -INFINITY ? 0.f : h.l * fast_exp2(h.m - mr);
                 f[i] = h.w == -INFINITY ? 0.f : fast_exp2(h.w - wr);
             }
-            const int64_t rr = (int64_t) rb * kRows + r;
-            const int32_t tok = (int32_t) (rr / p.group), hd = (int32_t) (rr - (int64_t) tok * p.group);
-            uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (kvh * p.group + hd) * p.o_sh;
-            if (!whole && lane == 0) dp.heads[slot0 + r] = PartHead{mr, lr, wr, 0.f};
+            uint16_t *out = row_of_out(p, s, kvh, (uint32_t) rb * kRows + (uint32_t) r);
+            if (!whole && lane == 0) dp.heads[slot0 + r] = PartHead{mr, lr, wr - kLift, 0.f};
 #pragma unroll
             for (int j = 0; j < (DHC + 127) / 128; ++j) {
                 const uint32_t grp = lane + 32 * j;
@@ -629,9 +587,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 else *reinterpret_cast<float4 *>(dp.parts + (slot0 + r) * DHC + grp * 4) = y;
             }
         }
-        if (!whole) {
-            if (part == 0) meta.head = t1 == tiles ? 1 : 2;
-            else meta.b = b, meta.kvh = kvh, meta.rb = rb;
+        if (!whole && part == 1) {
+            meta.b = b, meta.kvh = kvh, meta.rb = rb;
+            meta.last = (int32_t) divide(base + (item + 1) * tiles - 1, each);
         }
         if (u < u_end) {
             __syncthreads();// the ring is loaded again
@@ -647,63 +605,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
     if (threadIdx.x == 0) dp.meta[blockIdx.x] = meta;
 }
 
-// Joins the parts of the item that begins in stretch blockIdx.x and goes on behind it: one block per row, 8 groups of
-// threads take every eighth part, the groups' sums are added in order.
-constexpr int kJoinGroups = 8;
-template<int DHC, int NT>
-__global__ void __launch_bounds__(kJoinGroups * DHC / 4) join_kernel(const DecodeParams dp, int32_t ctas) {
-    constexpr int kRows = 8 * NT, kLanes = DHC / 4;
-    __shared__ float4 acc[kJoinGroups][kLanes];
-    __shared__ float stat[kJoinGroups][3];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const AttendParams &p = dp.a;
-    const CtaMeta first = dp.meta[blockIdx.x];
-    if (first.b < 0) return;
-    const int r = (int) blockIdx.y;
-    const Seq s = seq_of(p.lens, p.offs, p.rows, first.b);
-    const int64_t rr = (int64_t) first.rb * kRows + r;
-    if (rr >= (int64_t) s.n * p.group) return;
-    int32_t last = (int32_t) blockIdx.x + 1;// the stretch that holds the item's end
-    while (last + 1 < ctas && dp.meta[last].head == 2) ++last;
-    const int grp = (int) threadIdx.x / kLanes, ln = (int) threadIdx.x % kLanes;
-    float m = -INFINITY, l = 0.f, w = -INFINITY;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int32_t c = (int32_t) blockIdx.x + grp; c <= last; c += kJoinGroups) {
-        const int64_t at = ((int64_t) c * 2 + (c == (int32_t) blockIdx.x ? 1 : 0)) * kRows + r;
-        const PartHead h = dp.heads[at];
-        const float4 v = *reinterpret_cast<const float4 *>(dp.parts + at * DHC + ln * 4);
-        if (h.m != -INFINITY) {
-            const float n = fmaxf(m, h.m);
-            l = l * fast_exp2(m - n) + h.l * fast_exp2(h.m - n);
-            m = n;
-        }
-        if (h.w != -INFINITY) {
-            const float n = fmaxf(w, h.w), f0 = fast_exp2(w - n), f1 = fast_exp2(h.w - n);
-            y.x = y.x * f0 + v.x * f1, y.y = y.y * f0 + v.y * f1, y.z = y.z * f0 + v.z * f1, y.w = y.w * f0 + v.w * f1;
-            w = n;
-        }
-    }
-    acc[grp][ln] = y;
-    if (ln == 0) stat[grp][0] = m, stat[grp][1] = l, stat[grp][2] = w;
-    __syncthreads();
-    if (grp != 0) return;
-    m = w = -INFINITY, l = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < kJoinGroups; ++i) m = fmaxf(m, stat[i][0]), w = fmaxf(w, stat[i][2]);
-#pragma unroll
-    for (int i = 0; i < kJoinGroups; ++i) {
-        if (stat[i][0] != -INFINITY) l += stat[i][1] * fast_exp2(stat[i][0] - m);
-        if (stat[i][2] != -INFINITY) {
-            const float f = fast_exp2(stat[i][2] - w);
-            const float4 v = acc[i][ln];
-            y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
-        }
-    }
-    const int32_t tok = (int32_t) (rr / p.group), hd = (int32_t) (rr - (int64_t) tok * p.group);
-    uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (first.kvh * p.group + hd) * p.o_sh;
-    store_out(p, out, ln * 4, y, l, w - kLift - m);
-}
-
 struct AttendDesc {
     Device device;
     int device_id, sm_count;
@@ -713,26 +614,19 @@ struct AttendDesc {
     bool bf16;
     int64_t o_st, o_sh, q_st, q_sh;
     float scale;
-    int dhc, nt;
+    int dhc;      // head size rounded up to 64, 128 or 256
+    int block;    // query rows per block: 8 or 16 (mma.sync), 128 (tcgen05)
     uint32_t ctas;
 };
 
-uint64_t workspace_of(const AttendDesc &d) {
-    const uint64_t slots = (uint64_t) d.ctas * 2 * 8 * d.nt;
-    return slots * (sizeof(PartHead) + (uint64_t) d.dhc * 4) + d.ctas * sizeof(CtaMeta);
-}
+uint64_t workspace_of_desc(const AttendDesc &d) { return split_bytes(d.ctas, (uint64_t) d.block, (uint64_t) d.dhc); }
 
 template<int DHC, int NT, bool ONE>
 cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
     constexpr int kSmem = smem_bytes(DHC, NT);
     static_assert(kWarps * 8 * NT * DHC * 4 + kWarps * 8 * NT * (int) sizeof(PartHead) <= kSmem, "the warps' results fit their rings");
     static_assert(stage_bytes(DHC) % 16 == 0, "stages start on 16 bytes");
-    DecodeParams dp{};
-    dp.a = a;
-    const uint64_t slots = (uint64_t) d.ctas * 2 * 8 * NT;
-    dp.parts = reinterpret_cast<float *>(workspace);
-    dp.heads = reinterpret_cast<PartHead *>(dp.parts + slots * DHC);
-    dp.meta = reinterpret_cast<CtaMeta *>(dp.heads + slots);
+    const SplitParams dp = split_params(a, workspace, d.ctas, 8 * NT, DHC);
     // more shared memory than the default: asked for once per device (again, where two threads come first)
     static std::atomic<uint64_t> ready{0};
     const uint64_t bit = d.device_id < 64 ? 1ull << d.device_id : 0;
@@ -745,15 +639,7 @@ cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *w
     decode_kernel<DHC, NT, ONE><<<d.ctas, kThreads, kSmem, st>>>(dp);
     e = cudaGetLastError();
     if (e != cudaSuccess || d.ctas == 1) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(d.ctas - 1, 8 * NT);
-    cfg.blockDim = dim3(kJoinGroups * DHC / 4);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<DHC, NT>, dp, (int32_t) d.ctas);
+    return launch_join<DHC, 8 * NT>(dp, d.ctas, st);
 }
 template<int DHC, int NT>
 cudaError_t launch_decode(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
@@ -790,13 +676,15 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     d.rows = (int32_t) rows, d.q_heads = (int32_t) heads, d.bf16 = dt_eq(q_desc->dt, BF16), d.scale = scale;
     d.o_st = out_desc->strides[0], d.o_sh = out_desc->strides[1], d.q_st = q_desc->strides[0], d.q_sh = q_desc->strides[1];
     d.dhc = d.c.dh <= 64 ? 64 : d.c.dh <= 128 ? 128 : 256;
-    // query rows per sequence on average (the device knows each one's): more than 8 share a read of the cache in 16s
-    const int64_t group = d.q_heads / d.c.heads, rows_each = d.t.batch > 0 ? (int64_t) d.rows * group / d.t.batch : 0;
-    d.nt = rows_each > 8 ? 2 : 1;
+    const int64_t group = d.q_heads / d.c.heads;
+    if ((int64_t) d.rows * group > 0x7FFFFFFF) return STATUS_BAD_TENSOR_SHAPE;
+    // query rows per sequence on average (only the device knows each one's)
+    const int64_t rows_each = d.t.batch > 0 ? (int64_t) d.rows * group / d.t.batch : 0;
+    d.block = rows_each > kPrefillRows && d.t.batch <= kPrefillMaxBatch ? 128 : rows_each > 8 ? 16 : 8;
     // every CTA that fits the GPU at once, but no more than there can be units for
-    const int64_t blocks = ((int64_t) d.rows * group + 8 * d.nt - 1) / (8 * d.nt) + d.t.batch;
-    const int64_t tiles = std::max<int64_t>(1, ((int64_t) d.t.cap + kTile - 1) / kTile);
-    const int64_t places = (int64_t) d.sm_count * ctas_per_sm(d.dhc, d.nt);
+    const int64_t blocks = ((int64_t) d.rows * group + d.block - 1) / d.block + d.t.batch, keys = d.block == 128 ? kPrefillKeys : kTile;
+    const int64_t tiles = std::max<int64_t>(1, ((int64_t) d.t.cap + keys - 1) / keys);
+    const int64_t places = (int64_t) d.sm_count * (d.block == 128 ? (d.dhc == 256 ? 1 : 2) : ctas_per_sm(d.dhc, d.block / 8));
     d.ctas = (uint32_t) places;
     if (blocks * d.c.heads < places * kMinUnits) {
         d.ctas = (uint32_t) std::max<int64_t>(1, std::min(places, (blocks * d.c.heads * tiles + kMinUnits - 1) / kMinUnits));
@@ -810,7 +698,7 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
 INFINIOP_API infiniopStatus_t infiniopGetPagedAttentionWorkspaceSize(infiniopPagedAttentionDescriptor_t desc, uint64_t *size) {
     if (desc == nullptr || desc->device != DevNvGpu) return STATUS_BAD_DEVICE;
     if (size == nullptr) return STATUS_BAD_PARAM;
-    *size = workspace_of(*reinterpret_cast<AttendDesc *>(desc));
+    *size = workspace_of_desc(*reinterpret_cast<AttendDesc *>(desc));
     return STATUS_SUCCESS;
 }
 
@@ -826,7 +714,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     // a table without columns or a pool without pages has no keys: every token gets zeros
     const bool empty = d->t.cols == 0 || d->c.pages == 0;
     if (!empty && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || block_table == nullptr)) return STATUS_BAD_PARAM;
-    if (workspace == nullptr || workspace_size < workspace_of(*d)) return STATUS_MEMORY_NOT_ALLOCATED;
+    if (workspace == nullptr || workspace_size < workspace_of_desc(*d)) return STATUS_MEMORY_NOT_ALLOCATED;
     DeviceGuard guard(d->device_id);
     AttendParams p{};
     p.out = reinterpret_cast<uint16_t *>(out), p.q = reinterpret_cast<const uint16_t *>(q);
@@ -837,7 +725,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     p.offs = reinterpret_cast<const int32_t *>(q_offsets);
     p.rows = d->rows, p.group = d->q_heads / d->c.heads;
     p.scale_log2 = (float) ((double) d->scale * 1.4426950408889634);
-    p.page_div = FastDiv((uint32_t) d->c.page);
+    p.page_div = FastDiv((uint32_t) d->c.page), p.group_div = FastDiv((uint32_t) p.group);
     p.c = d->c, p.t = d->t, p.bf16 = d->bf16;
     if (empty) p.t.cap = 0;
     // whole 16-byte vectors: rows of codes, rows of q; 8-byte pieces of out's rows
@@ -847,13 +735,13 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     p.o_vec = (uintptr_t) out % 8 == 0 && d->o_st % 4 == 0 && d->o_sh % 4 == 0 && d->c.dh % 4 == 0;
     auto st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e;
-    switch (d->dhc * 4 + d->nt) {
-        case 64 * 4 + 1: e = launch_decode<64, 1>(*d, p, workspace, st); break;
-        case 64 * 4 + 2: e = launch_decode<64, 2>(*d, p, workspace, st); break;
-        case 128 * 4 + 1: e = launch_decode<128, 1>(*d, p, workspace, st); break;
-        case 128 * 4 + 2: e = launch_decode<128, 2>(*d, p, workspace, st); break;
-        case 256 * 4 + 1: e = launch_decode<256, 1>(*d, p, workspace, st); break;
-        default: e = launch_decode<256, 2>(*d, p, workspace, st); break;
+    if (d->block == 128) {
+        e = launch_prefill(p, workspace, d->dhc, d->ctas, d->device_id, st);
+    } else {
+        const bool few = d->block == 8;
+        if (d->dhc == 64) e = few ? launch_decode<64, 1>(*d, p, workspace, st) : launch_decode<64, 2>(*d, p, workspace, st);
+        else if (d->dhc == 128) e = few ? launch_decode<128, 1>(*d, p, workspace, st) : launch_decode<128, 2>(*d, p, workspace, st);
+        else e = few ? launch_decode<256, 1>(*d, p, workspace, st) : launch_decode<256, 2>(*d, p, workspace, st);
     }
     if (e != cudaSuccess) {
         cudaGetLastError();

@@ -16,7 +16,7 @@ struct AttendParams {
     int32_t rows, group;
     float scale_log2;// scale * log2(e)
     bool bf16, vec, q_vec, o_vec;
-    FastDiv page_div;// by the page size
+    FastDiv page_div, group_div;// by the page size and by the q heads per kv head
     CacheShape c;
     TableShape t;
 };
@@ -56,6 +56,171 @@ __device__ __forceinline__ void store_out(const AttendParams &p, uint16_t *out, 
     if (d + 2 < p.c.dh) out[d + 2] = (uint16_t) hi;
     if (d + 3 < p.c.dh) out[d + 3] = (uint16_t) (hi >> 16);
 }
+
+// Row of out of the rr-th query row (new token x q head of the group) of a sequence and kv head.
+__device__ __forceinline__ uint16_t *row_of_out(const AttendParams &p, const Seq &s, int32_t kvh, uint32_t rr) {
+    const int32_t tok = (int32_t) p.group_div.div(rr), hd = (int32_t) rr - tok * p.group;
+    return p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (kvh * p.group + hd) * p.o_sh;
+}
+
+// ---- equal stretches of work ------------------------------------------------------------------------------------
+// The work of a call is a list of units, tiles of cached tokens, ordered by sequence, kv head, block of query rows,
+// tile; CTA c takes units [c * each, (c + 1) * each).  An item (sequence, kv head, block of rows) that lies in one
+// stretch is finished there; of any other, each CTA stores its part (unnormalised output and the rows' references) and
+// join_kernel adds the parts in the order of the list.
+
+// a / b of values that mostly fit 32 bits (a 64-bit division takes a few hundred cycles)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t) ((uint32_t) a / (uint32_t) b) : a / b;
+}
+__device__ __forceinline__ int64_t stretch_of(int64_t total, int64_t least) {
+    const int64_t each = divide(total + gridDim.x - 1, gridDim.x);
+    return each < least ? least : each;
+}
+
+// Sum over the CTA of a 64-bit value and the sum over the threads before; `slot`: WARPS words.
+template<int WARPS>
+__device__ __forceinline__ int64_t cta_exclusive_sum64(int64_t v, int64_t *slot, int64_t &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();
+    if (lane == 31) slot[warp] = incl;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += slot[w];
+        total += slot[w];
+    }
+    return before + incl - v;
+}
+
+// log2 of a scale; exact and cheap for the powers of two that append writes.  Zero gives -inf.  All lanes call it.
+__device__ __forceinline__ float log2_of(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if (__any_sync(0xffffffffu, (u & 0x807FFFFFu) != 0 || u == 0)) return log2f(v);
+    return (float) ((int32_t) (u >> 23) - 127);
+}
+
+// A row's part: sum over its keys of 2^(score - m) = l, and of 2^(score - w) * scale of the value * code = the output
+struct PartHead {
+    float m, l, w, pad;
+};
+struct CtaMeta {
+    int32_t b, kvh, rb;// the item that begins in this CTA's stretch and goes on behind it; b < 0: none
+    int32_t last;      // the CTA whose stretch holds its end
+};
+struct SplitParams {
+    AttendParams a;
+    float *parts;   // [cta][2][rows][DHC]: the part of an item that began before the stretch, and of one that goes on
+    PartHead *heads;// [cta][2][rows]
+    CtaMeta *meta;  // [cta]
+};
+static inline uint64_t split_bytes(uint64_t ctas, uint64_t rows, uint64_t dhc) {
+    return ctas * (2 * rows * (sizeof(PartHead) + dhc * 4) + sizeof(CtaMeta));
+}
+static inline SplitParams split_params(const AttendParams &a, void *workspace, uint64_t ctas, uint64_t rows, uint64_t dhc) {
+    SplitParams s{};
+    s.a = a;
+    s.parts = reinterpret_cast<float *>(workspace);
+    s.heads = reinterpret_cast<PartHead *>(s.parts + ctas * 2 * rows * dhc);
+    s.meta = reinterpret_cast<CtaMeta *>(s.heads + ctas * 2 * rows);
+    return s;
+}
+
+// Joins the parts of the item that begins in stretch blockIdx.x and goes on behind it.  A block takes two rows; for each,
+// four groups of threads add every fourth part (kBatch of them loaded at a time: the loads' latency is all there is to
+// this kernel), and the groups' sums are added in order.
+constexpr int kJoinRows = 2, kJoinGroups = 4, kBatch = 7;
+template<int DHC, int ROWS>
+__global__ void __launch_bounds__(kJoinRows * kJoinGroups * DHC / 4) join_kernel(const SplitParams dp) {
+    constexpr int kLanes = DHC / 4;
+    __shared__ float4 acc[kJoinRows][kJoinGroups][kLanes];
+    __shared__ float stat[kJoinRows][kJoinGroups][3];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const AttendParams &p = dp.a;
+    const CtaMeta item = dp.meta[blockIdx.x];
+    if (item.b < 0) return;
+    const int ln = (int) threadIdx.x % kLanes, grp = (int) threadIdx.x / kLanes % kJoinGroups, sub = (int) threadIdx.x / (kLanes * kJoinGroups);
+    const int r = (int) blockIdx.y * kJoinRows + sub, first = (int) blockIdx.x;
+    const Seq s = seq_of(p.lens, p.offs, p.rows, item.b);
+    const uint32_t rr = (uint32_t) item.rb * ROWS + (uint32_t) r;
+    const bool have = rr < (uint32_t) s.n * (uint32_t) p.group;
+    float m = -INFINITY, l = 0.f, w = -INFINITY;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int32_t c0 = first + grp; have && c0 <= item.last; c0 += kJoinGroups * kBatch) {
+        PartHead h[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int32_t c = c0 + i * kJoinGroups;
+            const int64_t at = ((int64_t) c * 2 + (c == first ? 1 : 0)) * ROWS + r;
+            h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0.f};
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c <= item.last) h[i] = dp.heads[at], v[i] = *reinterpret_cast<const float4 *>(dp.parts + at * DHC + ln * 4);
+        }
+        float m1 = m, w1 = w;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) m1 = fmaxf(m1, h[i].m), w1 = fmaxf(w1, h[i].w);
+        if (m1 != -INFINITY) {
+            l *= fast_exp2(m - m1);// (from -inf: 0)
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) l += h[i].l * fast_exp2(h[i].m - m1);
+            m = m1;
+        }
+        if (w1 != -INFINITY) {
+            const float f0 = fast_exp2(w - w1);
+            y.x *= f0, y.y *= f0, y.z *= f0, y.w *= f0;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const float f = fast_exp2(h[i].w - w1);
+                y.x += v[i].x * f, y.y += v[i].y * f, y.z += v[i].z * f, y.w += v[i].w * f;
+            }
+            w = w1;
+        }
+    }
+    acc[sub][grp][ln] = y;
+    if (ln == 0) stat[sub][grp][0] = m, stat[sub][grp][1] = l, stat[sub][grp][2] = w;
+    __syncthreads();
+    if (grp != 0 || !have) return;
+    m = w = -INFINITY, l = 0.f, y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kJoinGroups; ++i) m = fmaxf(m, stat[sub][i][0]), w = fmaxf(w, stat[sub][i][2]);
+#pragma unroll
+    for (int i = 0; i < kJoinGroups; ++i) {
+        if (stat[sub][i][0] != -INFINITY) l += stat[sub][i][1] * fast_exp2(stat[sub][i][0] - m);
+        if (stat[sub][i][2] != -INFINITY) {
+            const float f = fast_exp2(stat[sub][i][2] - w);
+            const float4 v = acc[sub][i][ln];
+            y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+        }
+    }
+    store_out(p, row_of_out(p, s, item.kvh, rr), ln * 4, y, l, w - m);
+}
+
+template<int DHC, int ROWS>
+static inline cudaError_t launch_join(const SplitParams &sp, uint32_t ctas, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas - 1, ROWS / kJoinRows);
+    cfg.blockDim = dim3(kJoinRows * kJoinGroups * DHC / 4);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<DHC, ROWS>, sp);
+}
+
+// Prompts and chunks (paged_prefill.cu): 128 query rows x 64 cached tokens per tile.
+constexpr int kPrefillKeys = 64;
+constexpr int64_t kPrefillMaxBatch = 4096;// sequences whose unit counts fit the kernel's shared memory
+cudaError_t launch_prefill(const AttendParams &a, void *workspace, int dhc, uint32_t ctas, int device_id, cudaStream_t st);
 
 }// namespace paged
 }// namespace b200

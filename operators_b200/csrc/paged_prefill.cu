@@ -1,0 +1,643 @@
+// Attention over the paged 8-bit KV cache for prompts, chunks of prompts and long drafts: tcgen05.
+//
+// A block is 128 query rows (new tokens x the q heads that share a kv head, row = token * group + head), one TMEM lane
+// each; a tile is 64 cached tokens.  Per tile: S = q k^T into TMEM, weights in fp16 back into TMEM over S (operand A of
+// the second product), O += W v in TMEM.  The operands of kind::f16 are fp16: q is scaled per row by a power of two
+// (see paged_attention.cu), the codes become fp16 exactly on their way into shared memory, once per block of 128 rows.
+//
+// Softmax in one pass: score 2^(s f - m) with f the row's and the page's factor and m the row's running reference,
+// which moves only when a score exceeds it by 2^8, so that O (which then has to be read, multiplied and written
+// back) almost never moves after the first tiles.  The weight of a value is w = p * 2^c with
+// 2^c = 2^(m - M + 7) * (scale of the values' page) and M the weights' own reference, so fp16 holds weights between
+// 2^15 and 2^-21 of the reference (2^-32 with subnormals) however the pages' scales differ, and one exponential gives
+// w; the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way,
+// and their sum must not underflow.
+//
+// What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x
+// dh multiply-adds (512 cycles at dh 128), so two CTAs share an SM and one's exponentials run beside the other's
+// products.
+//
+// Roles (288 threads): warps 0-3 softmax and epilogue, a thread per row; warps 4-7 convert codes (their loads run a
+// tile ahead in registers); warp 8 allocates TMEM, one lane issues the products.  Shared memory: q, two tiles of K, two
+// of V (128-byte swizzled rows as TMA would lay them).  S is double-buffered: S of tile j + 1 is issued before W v of
+// tile j.  Work is divided into equal stretches of tiles as in paged_attention.cu (row blocks stop where their last row's
+// mask begins), and all roles walk the stretch's items by themselves.
+// A product's completion is waited for only where O is touched, so it has a barrier for even and one for odd tiles: a row
+// that has seen S of tile n knows that W v of tile n - 2 (issued before it) is done, not that of tile n - 1, and one
+// barrier's parity could not tell the two apart.
+// Every wait is bounded (tc_ptx.cuh).
+#include "paged_attention.cuh"
+#include "tc_ptx.cuh"
+
+#include <atomic>
+
+namespace b200 {
+namespace paged {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 128, kKeys = kPrefillKeys;
+constexpr int kSoftmax = 128, kConvert = 128, kThreads = kSoftmax + kConvert + 32, kWarps = kThreads / 32;
+constexpr float kSlack = 8.f, kLift = 7.f;// w <= 2^15
+constexpr float kLeast = -90.f;
+constexpr int kMinUnits = 4;
+constexpr uint32_t kSuspendNs = 20000;
+// Two CTAs of 9 warps leave 96 registers a thread (5 warps on a quarter of the SM).  The softmax warps, which hold a
+// tile's 64 scores of a row, take what the converting warps can spare.
+constexpr int kLaunchRegs = 96, kSoftmaxRegs = 120, kConvertRegs = 72;
+static_assert(kSoftmax * kSoftmaxRegs + kConvert * kConvertRegs + 32 * kLaunchRegs <= kThreads * kLaunchRegs, "the split fits what the launch gave");
+constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
+
+// TMEM columns: S (and the weights over it) [0, 64) and [64, 128), O from 128
+__host__ __device__ constexpr uint32_t tmem_cols(int dhc) { return dhc <= 128 ? 256u : 512u; }
+
+enum Bar { kQFull, kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty1, kSFull, kSFull1, kWFull, kWFull1, kPvDone, kPvDone1,
+           kScFull, kBars = kScFull + kScaleSets };
+
+struct TileScales {
+    float ks[kKeys], vs[kKeys], lv[kKeys];// scales of the keys, of the values, log2 of the latter; one page: [0] only
+    uint32_t mask[2], pad[2];             // tokens that exist
+};
+
+__host__ __device__ constexpr uint32_t q_bytes(int dhc) { return (uint32_t) dhc * 2 * kRows; }
+__host__ __device__ constexpr uint32_t kv_bytes(int dhc) { return (uint32_t) dhc * 2 * kKeys; }
+__host__ __device__ constexpr uint32_t smem_bytes(int dhc) {
+    return q_bytes(dhc) + 4 * kv_bytes(dhc) + kScaleSets * (uint32_t) sizeof(TileScales) + kBars * 8 + 32;
+}
+static_assert(kPrefillMaxBatch * 8 <= q_bytes(64) + 4 * kv_bytes(64), "the sequences' unit counts fit the tiles' memory");
+
+// D[tmem] (+)= A[tmem] * B[smem desc]: the rows of A are TMEM lanes, two fp16 elements per column
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
+        "tcgen05.wait::st.sync.aligned;"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+          "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+          "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2f(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2f(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Tiles of a block of query rows: up to the last key that its last row sees, one at least (rows without keys get zeros).
+__device__ __forceinline__ int32_t tiles_of(const AttendParams &p, const Seq &s, int32_t rb) {
+    const uint32_t rows = (uint32_t) s.n * (uint32_t) p.group, end = ((uint32_t) rb + 1) * kRows;
+    const int32_t tok = (int32_t) p.group_div.div((end < rows ? end : rows) - 1);
+    const int32_t limit = min(s.len - s.n + tok + 1, held(s.len, p.t.cap));
+    return limit > 0 ? (limit - 1) / kKeys + 1 : 1;
+}
+__device__ __forceinline__ int32_t blocks_of(const AttendParams &p, const Seq &s) {
+    return (int32_t) (((uint32_t) s.n * (uint32_t) p.group + kRows - 1) / kRows);
+}
+
+// A stretch of units, item by item.  Every role keeps its own.
+struct Segment {
+    Seq s;
+    int32_t b, kvh, rb, t0, t1, tiles;
+    int64_t u;// unit of t0
+};
+struct Walker {
+    const AttendParams &p;
+    Seq s;
+    int32_t b, kvh, rb, t0, blocks;
+    int64_t u, end;
+    __device__ __forceinline__ bool next(Segment &g) {
+        if (u >= end) return false;
+        if (blocks < 0) s = seq_of(p.lens, p.offs, p.rows, b), blocks = blocks_of(p, s);
+        while (blocks == 0) s = seq_of(p.lens, p.offs, p.rows, ++b), blocks = blocks_of(p, s);// (units are left: there is one)
+        const int32_t tiles = tiles_of(p, s, rb);
+        const int32_t n = end - u < tiles - t0 ? (int32_t) (end - u) : tiles - t0;
+        g.s = s, g.b = b, g.kvh = kvh, g.rb = rb, g.t0 = t0, g.t1 = t0 + n, g.tiles = tiles, g.u = u;
+        u += n, t0 = 0;
+        if (g.t1 == tiles && ++rb == blocks) {
+            rb = 0;
+            if (++kvh == p.c.heads) kvh = 0, ++b, blocks = -1;
+        }
+        return true;
+    }
+};
+
+template<int DHC, bool ONE>
+__global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(const SplitParams sp) {
+    constexpr uint32_t kQ = q_bytes(DHC), kKV = kv_bytes(DHC);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ int64_t slot[kWarps], found_base;
+    __shared__ int32_t found_b, found_rb, found_t;
+    const AttendParams &p = sp.a;
+    // the swizzled tiles need 1024-byte alignment; two CTAs fill the SM, so there is no room to round up
+    if ((smem_u32(smem) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicAdd(&g_tc_gemm_timeouts, 1ull), sp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
+        return;
+    }
+    const uint32_t sq = smem_u32(smem), sk = sq + kQ, sv = sk + 2 * kKV;
+    TileScales *scales = reinterpret_cast<TileScales *>(smem + kQ + 4 * kKV);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kScaleSets);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- this CTA's stretch.  Units of a kv head of each sequence: a warp per sequence, a lane per block of rows.
+    int64_t *sums = reinterpret_cast<int64_t *>(smem);
+    for (int32_t b = (int32_t) warp; b < p.t.batch; b += kWarps) {
+        const Seq s = seq_of(p.lens, p.offs, p.rows, b);
+        const int32_t blocks = blocks_of(p, s);
+        int64_t n = 0;
+        for (int32_t rb = (int32_t) lane; rb < blocks; rb += 32) n += tiles_of(p, s, rb);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        if (lane == 0) sums[b] = n;
+    }
+    __syncthreads();
+    int64_t mine = 0, total;
+    for (int32_t b = (int32_t) threadIdx.x; b < p.t.batch; b += kThreads) mine += sums[b] * p.c.heads;
+    cta_exclusive_sum64<kWarps>(mine, slot, total);
+    const int64_t each = stretch_of(total, kMinUnits), u0 = each * blockIdx.x, u1 = u0 + each < total ? u0 + each : total;
+    if (u0 >= u1) {
+        if (threadIdx.x == 0) sp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
+        return;
+    }
+    {
+        int64_t base = 0;
+        for (int32_t b0 = 0; b0 < p.t.batch && base <= u0; b0 += kThreads) {
+            const int32_t b = b0 + (int32_t) threadIdx.x;
+            const int64_t n = b < p.t.batch ? sums[b] * p.c.heads : 0;
+            int64_t sum;
+            const int64_t before = base + cta_exclusive_sum64<kWarps>(n, slot, sum);
+            if (u0 >= before && u0 - before < n) found_b = b, found_base = before;
+            base += sum;
+        }
+        __syncthreads();
+    }
+    const int32_t b_first = found_b;
+    const int64_t per_head = sums[b_first];
+    const int32_t kvh_first = (int32_t) divide(u0 - found_base, per_head);
+    if (warp == 0) {
+        // the block of rows and its tile where the stretch begins
+        const Seq s = seq_of(p.lens, p.offs, p.rows, b_first);
+        const int32_t blocks = blocks_of(p, s);
+        const int64_t x = u0 - found_base - kvh_first * per_head;
+        int64_t base = 0;
+        for (int32_t rb0 = 0; rb0 < blocks && base <= x; rb0 += 32) {
+            const int32_t rb = rb0 + (int32_t) lane;
+            const int64_t n = rb < blocks ? tiles_of(p, s, rb) : 0;
+            int64_t incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                if ((int) lane >= o) incl += v;
+            }
+            const int64_t before = base + incl - n;
+            if (x >= before && x - before < n) found_rb = rb, found_t = (int32_t) (x - before);
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < kBars; ++i) {
+            const bool rows = i == kQFull || i == kWFull || i == kWFull1, keys = i >= kScFull;
+            const bool codes = i == kKFull || i == kKFull1 || i == kVFull || i == kVFull1;
+            mbar_init(&bars[i], rows ? kSoftmax : codes ? kConvert : keys ? kKeys : 1u);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, tmem_cols(DHC));
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();// (the sums are read, the tiles' memory is free)
+    tc_fence_after();
+    if (p.c.dh < DHC) {
+        // head elements beyond dh: zeros that nothing writes again
+        for (uint32_t i = threadIdx.x * 16; i < kQ + 4 * kKV; i += kThreads * 16) {
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sq + i), "r"(0) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+    }
+    const uint32_t tmem = *tmem_slot;
+    Walker walk{p, Seq{}, b_first, kvh_first, found_rb, found_t, -1, u0, u1};
+    Segment g;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ products
+        if (lane == 0) {
+            const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
+            const uint32_t idesc_s = make_idesc(kRows, kKeys, 0, 0), idesc_o = make_idesc(kRows, steps * 16, 0, 1);
+            bool ok = true;
+            uint32_t n = 0, seg = 0;
+            auto issue_s = [&](uint32_t i) -> bool {
+                const uint32_t b = i & 1u;
+                if (!mbar_wait<kSuspendNs>(&bars[kKFull + b], (i >> 1) & 1u, abort_flag)) return false;
+                tc_fence_after();
+                for (uint32_t k = 0; k < steps; ++k) {
+                    const uint64_t da = make_smem_desc(sq + (k >> 2) * (kRows * 128u) + (k & 3u) * 32u, 16, 1024);
+                    const uint64_t db = make_smem_desc(sk + b * kKV + (k >> 2) * (kKeys * 128u) + (k & 3u) * 32u, 16, 1024);
+                    umma_f16(tmem + b * kKeys, da, db, idesc_s, k > 0 ? 1u : 0u);
+                }
+                umma_commit(&bars[kKEmpty + b]);
+                umma_commit(&bars[kSFull + b]);
+                return true;
+            };
+            while (ok && walk.next(g)) {
+                const uint32_t tiles = (uint32_t) (g.t1 - g.t0);
+                if (!(ok = mbar_wait<kSuspendNs>(&bars[kQFull], seg & 1u, abort_flag)) || !(ok = issue_s(n))) break;
+                ++seg;
+                for (uint32_t j = 0; j < tiles; ++j, ++n) {
+                    const uint32_t b = n & 1u, ph = (n >> 1) & 1u;
+                    if (j + 1 < tiles && !(ok = issue_s(n + 1))) break;
+                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kVFull + b], ph, abort_flag))) break;
+                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kWFull + b], ph, abort_flag))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t k = 0; k < kKeys / 16; ++k) {
+                        const uint64_t db = make_smem_desc(sv + b * kKV + k * 2048u, kKeys * 128u, 1024);
+                        umma_f16_ts(tmem + 2 * kKeys, tmem + b * kKeys + k * 8u, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                    }
+                    umma_commit(&bars[kVEmpty + b]);
+                    umma_commit(&bars[kPvDone + b]);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ codes to fp16
+        if (DHC <= 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+        constexpr int kGroups = DHC / 64;// 4 lanes take 64 bytes of a row; 8 rows per warp and load
+        const uint32_t c = threadIdx.x - kSoftmax, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
+        // tile that is loaded next
+        bool more = walk.next(g);
+        int32_t tile = g.t0;
+        auto advance = [&]() {
+            if (++tile >= g.t1 && (more = walk.next(g))) tile = g.t0;
+        };
+        struct Ids {
+            int32_t row[2], key;// pages of this thread's two rows and of the key whose scales it loads; -1: none
+        };
+        auto page_of = [&](int32_t tok) -> int32_t {
+            if (tok >= held(g.s.len, p.t.cap)) return -1;
+            const int32_t id = p.table[(int64_t) g.b * p.t.stride + (int32_t) p.page_div.div((uint32_t) tok)];
+            return id >= 0 && id < p.c.pages ? id : -1;
+        };
+        auto ids_of = [&](Ids &x) {
+            x.row[0] = x.row[1] = x.key = -1;
+            if (!more) return;
+            const int32_t tok = tile * kKeys;
+            if (ONE) {
+                const int32_t id = page_of(tok), left = held(g.s.len, p.t.cap) - tok;
+                x.row[0] = (int32_t) r0 < left ? id : -1;
+                x.row[1] = (int32_t) r0 + 32 < left ? id : -1;
+                x.key = (int32_t) c < left ? id : -1;
+            } else {
+                x.row[0] = page_of(tok + (int32_t) r0);
+                x.row[1] = page_of(tok + (int32_t) r0 + 32);
+                if (c < kKeys) x.key = page_of(tok + (int32_t) c);
+            }
+        };
+        uint4 kd[2][kGroups], vd[2][kGroups];
+        float ks = 0.f, vs = 0.f;
+        bool key_ok = false;
+        // 16 codes of head elements d0 .. of one row
+        auto load16 = [&](const uint8_t *at, int32_t d0) -> uint4 {
+            if (p.vec) return *reinterpret_cast<const uint4 *>(at + d0);
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (d0 + i < p.c.dh) w[i >> 2] |= (uint32_t) at[d0 + i] << (8 * (i & 3));
+            }
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        auto load_tile = [&](const Ids &x, const PoolStrides &st, const uint8_t *pool, uint4 (&to)[2][kGroups]) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int32_t tok = tile * kKeys + (int32_t) r0 + 32 * i, in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
+                const uint8_t *at = pool + (int64_t) max(x.row[i], 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp;
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    const int32_t d0 = (q * 4 + (int32_t) c4) * 16;
+                    to[i][q] = x.row[i] >= 0 && d0 < p.c.dh ? load16(at, d0) : make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        };
+        auto load_scales = [&](const Ids &x) {
+            key_ok = x.key >= 0;
+            ks = vs = 0.f;
+            if (key_ok && c < (ONE ? 1u : (uint32_t) kKeys)) {
+                ks = p.ks[(int64_t) x.key * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch];
+                vs = p.vs[(int64_t) x.key * p.c.v.cn + (int64_t) g.kvh * p.c.v.ch];
+            }
+        };
+        // rows as TMA with 128-byte swizzle would lay them: 16-byte chunk j of row r at j ^ (r & 7)
+        auto store_tile = [&](uint32_t base, const uint4 (&from)[2][kGroups]) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t r = r0 + 32 * i;
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    if ((q * 4 + (int32_t) c4) * 16 >= p.c.dh) continue;
+                    const uint4 w = from[i][q];
+                    const uint32_t row = base + (uint32_t) q * (kKeys * 128u) + r * 128u;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4) ^ (r & 7u)) << 4)),
+                                 "r"(e4m3x2_to_f16x2((uint16_t) w.x)), "r"(e4m3x2_to_f16x2((uint16_t) (w.x >> 16))),
+                                 "r"(e4m3x2_to_f16x2((uint16_t) w.y)), "r"(e4m3x2_to_f16x2((uint16_t) (w.y >> 16)))
+                                 : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4 + 1) ^ (r & 7u)) << 4)),
+                                 "r"(e4m3x2_to_f16x2((uint16_t) w.z)), "r"(e4m3x2_to_f16x2((uint16_t) (w.z >> 16))),
+                                 "r"(e4m3x2_to_f16x2((uint16_t) w.w)), "r"(e4m3x2_to_f16x2((uint16_t) (w.w >> 16)))
+                                 : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");// the products read through the async proxy
+        };
+        Ids ids;
+        ids_of(ids);
+        load_tile(ids, p.c.k, p.kp, kd);
+        load_tile(ids, p.c.v, p.vp, vd);
+        load_scales(ids);
+        bool ok = true;
+        for (uint32_t n = 0; more; ++n) {
+            const uint32_t b = n & 1u, ph = ((n >> 1) & 1u) ^ 1u;
+            // scales of this tile, ids of the next
+            TileScales &sc = scales[n % kScaleSets];
+            const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
+            const float lv = log2_of(vs);
+            if (c < kKeys) {
+                if (!ONE || c == 0) sc.ks[c] = ks, sc.vs[c] = vs, sc.lv[c] = lv;
+                if (lane == 0) sc.mask[cw] = mask;
+                mbar_arrive(&bars[kScFull + n % kScaleSets]);
+            }
+            advance();
+            Ids next;
+            ids_of(next);
+            if (!(ok = mbar_wait<kSuspendNs>(&bars[kKEmpty + b], ph, abort_flag))) break;
+            store_tile(sk + b * kKV, kd);
+            mbar_arrive(&bars[kKFull + b]);
+            load_tile(next, p.c.k, p.kp, kd);
+            load_scales(next);
+            if (!(ok = mbar_wait<kSuspendNs>(&bars[kVEmpty + b], ph, abort_flag))) break;
+            store_tile(sv + b * kKV, vd);
+            mbar_arrive(&bars[kVFull + b]);
+            load_tile(next, p.c.v, p.vp, vd);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax and epilogue: a thread per row
+        if (DHC <= 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const uint32_t r = threadIdx.x, t_lane = tmem + ((warp * 32u) << 16);
+        CtaMeta meta{-1, 0, 0, 0};
+        bool ok = true;
+        uint32_t n = 0;
+        while (ok && walk.next(g)) {
+            const Seq s = g.s;
+            const uint32_t rr = (uint32_t) g.rb * kRows + r;
+            const bool have = rr < (uint32_t) s.n * (uint32_t) p.group;
+            const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0, hd = have ? (int32_t) rr - tok * p.group : 0;
+            const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
+            float rf;
+            {
+                // q: the row's largest magnitude, then its elements times a power of two (and the sign of the scale, so
+                // that the factor of the scores is not negative) into swizzled shared memory.  Every product of the item
+                // before has completed: its last S was waited for.
+                const uint16_t *q = p.q + (int64_t) (s.first + tok) * p.q_st + (int64_t) (g.kvh * p.group + hd) * p.q_sh;
+                auto load8 = [&](int32_t d) -> uint4 {
+                    if (!have || d >= p.c.dh) return make_uint4(0u, 0u, 0u, 0u);
+                    if (p.q_vec && d + 8 <= p.c.dh) return *reinterpret_cast<const uint4 *>(q + d);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = (uint32_t) (d + 2 * i < p.c.dh ? q[d + 2 * i] : 0) | ((uint32_t) (d + 2 * i + 1 < p.c.dh ? q[d + 2 * i + 1] : 0) << 16);
+                    }
+                    return make_uint4(w[0], w[1], w[2], w[3]);
+                };
+                uint32_t top = 0;
+#pragma unroll 4
+                for (int32_t d = 0; d < p.c.dh; d += 8) {
+                    const uint4 w = load8(d);
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+                }
+                top = max(top & 0xFFFFu, top >> 16);
+                const int32_t shift = query_shift(p.bf16, top);
+                const float up = copysignf(__uint_as_float(pow2_bits(shift)), p.scale_log2);
+                rf = __uint_as_float(pow2_bits(-shift)) * fabsf(p.scale_log2);
+#pragma unroll 4
+                for (int32_t d = 0; d < p.c.dh; d += 8) {
+                    const uint4 w = load8(d);
+                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = p.bf16 ? unpack2_t<kBF16>(x[i]) : unpack2(x[i]);
+                        x[i] = round16x2(false, f.x * up, f.y * up);
+                    }
+                    const uint32_t at = sq + ((uint32_t) d >> 6) * (kRows * 128u) + r * 128u + (((((uint32_t) d >> 3) & 7u) ^ (r & 7u)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&bars[kQFull]);
+            }
+            float m = -INFINITY, wm = -INFINITY, l = 0.f;
+#pragma unroll 1
+            for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n) {
+                const uint32_t b = n & 1u;
+                const TileScales &sc = scales[n % kScaleSets];
+                if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n % kScaleSets], (n / kScaleSets) & 1u, abort_flag))) break;
+                if (!(ok = mbar_wait<kSuspendNs>(&bars[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                tc_fence_after();
+                __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
+                float x[kKeys];
+                tmem_ld32(t_lane + b * kKeys, x);
+                tmem_ld32(t_lane + b * kKeys + 32, x + 32);
+                // scores are x * f; a tile that hides something from a row of this warp takes them one by one
+                float f = ONE ? sc.ks[0] * rf : 1.f;
+                if (!ONE) {
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) x[i] *= sc.ks[i] * rf;
+                }
+                const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
+                if (__any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && (int64_t) tile * kKeys + kKeys > limit))) {
+                    const int32_t left = limit - tile * kKeys;
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) {
+                        const bool seen = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u;
+                        x[i] = seen && i < left ? x[i] * f : -INFINITY;
+                    }
+                    f = 1.f;
+                }
+                float t4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < kKeys; i += 8) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t4[j] = i + 4 + j < kKeys ? fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]) : fmaxf(t4[j], x[i + j]);
+                }
+                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f;
+                float wtop;
+                if (ONE) {
+                    wtop = top + sc.lv[0];
+                } else {
+                    wtop = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
+                }
+                // references
+                if (top > m + kSlack || (m == -INFINITY && top > m)) {
+                    l *= fast_exp2(m - top);// (from -inf: 0)
+                    m = top;
+                }
+                const bool up = wtop > wm + kSlack || (wm == -INFINITY && wtop > wm);
+                const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
+                if (up) wm = wtop;
+                if (__any_sync(0xffffffffu, up) && tile > g.t0) {
+                    // O so far: every product into it must have completed
+                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+                    tc_fence_after();
+                    __syncwarp();
+                    for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
+                        float o[32];
+                        tmem_ld32(t_lane + 2 * kKeys + c0, o);
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
+                        tmem_st32(t_lane + 2 * kKeys + c0, w);
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.f : m, ww = wm == -INFINITY ? 0.f : wm;
+                uint32_t w[kKeys / 2];
+                if (ONE) {
+                    const float e = fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : sc.lv[0]), kLeast);
+                    const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
+                    uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int i = 0; i < kKeys / 2; ++i) {
+                        const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
+                        const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
+                        part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
+                        w[i] = round16x2(false, y0, y1);
+                    }
+                    const float2 sum = unpack2f(add2(part[0], part[1]));
+                    l = fmaf(sum.x + sum.y, fast_exp2(-e), l);
+                } else {
+                    // pages that end inside the tile: a factor per key
+                    const float gf = mm - ww + kLift;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kKeys / 2; ++i) {
+                        const float y0 = fast_exp2(x[2 * i] - mm), y1 = fast_exp2(x[2 * i + 1] - mm);
+                        sum += y0 + y1;
+                        w[i] = round16x2(false, x[2 * i] == -INFINITY ? 0.f : fast_exp2(x[2 * i] - mm + gf + sc.lv[2 * i]),
+                                         x[2 * i + 1] == -INFINITY ? 0.f : fast_exp2(x[2 * i + 1] - mm + gf + sc.lv[2 * i + 1]));
+                    }
+                    l += sum;
+                }
+                __syncwarp();
+                tmem_st32(t_lane + b * kKeys, w);
+                tc_fence_before();
+                mbar_arrive(&bars[kWFull + b]);
+            }
+            if (!ok) break;
+            // ---- the item's output, or its part
+            if (!(ok = mbar_wait<kSuspendNs>(&bars[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+            tc_fence_after();
+            const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+            const int part = g.t0 > 0 ? 0 : 1;
+            const int64_t at = ((int64_t) blockIdx.x * 2 + part) * kRows + r;
+            uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (g.kvh * p.group + hd) * p.o_sh;
+            const bool none = wm == -INFINITY;// (O holds products with weights of zero)
+            for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
+                float o[32];
+                __syncwarp();
+                tmem_ld32(t_lane + 2 * kKeys + c0, o);// every lane takes part
+#pragma unroll
+                for (int i = 0; have && i < 32; i += 4) {
+                    float4 y = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    if (none) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (whole) store_out(p, out, c0 + i, y, l, wm - kLift - m);
+                    else *reinterpret_cast<float4 *>(sp.parts + at * DHC + c0 + i) = y;
+                }
+            }
+            if (!whole && have) sp.heads[at] = PartHead{m, l, wm - kLift, 0.f};
+            if (!whole && part == 1) meta = CtaMeta{g.b, g.kvh, g.rb, (int32_t) divide(g.u + g.tiles - 1, each)};
+            tc_fence_before();
+        }
+        if (threadIdx.x == 0) sp.meta[blockIdx.x] = meta;
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, tmem_cols(DHC));
+    }
+}
+
+template<int DHC, bool ONE>
+cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};// devices on which the shared memory has been asked for
+    const uint64_t bit = device_id < 64 ? 1ull << device_id : 0;
+    cudaError_t e = cudaSuccess;
+    if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+        e = cudaFuncSetAttribute(prefill_kernel<DHC, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes(DHC));
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    prefill_kernel<DHC, ONE><<<ctas, kThreads, smem_bytes(DHC), st>>>(sp);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || ctas == 1) return e;
+    return launch_join<DHC, kRows>(sp, ctas, st);
+}
+template<int DHC>
+cudaError_t launch(const AttendParams &a, void *workspace, uint32_t ctas, int device_id, cudaStream_t st) {
+    const SplitParams sp = split_params(a, workspace, ctas, kRows, DHC);
+    return a.vec && a.c.page % kKeys == 0 ? launch_as<DHC, true>(sp, ctas, device_id, st) : launch_as<DHC, false>(sp, ctas, device_id, st);
+}
+
+}// namespace
+
+cudaError_t launch_prefill(const AttendParams &a, void *workspace, int dhc, uint32_t ctas, int device_id, cudaStream_t st) {
+    return dhc == 64 ? launch<64>(a, workspace, ctas, device_id, st) : dhc == 128 ? launch<128>(a, workspace, ctas, device_id, st)
+                                                                                  : launch<256>(a, workspace, ctas, device_id, st);
+}
+
+}// namespace paged
+
+unsigned long long paged_prefill_timeouts_read() {
+    unsigned long long v = 0;
+    if (cudaMemcpyFromSymbol(&v, tc::g_tc_gemm_timeouts, sizeof(v)) != cudaSuccess) {
+        cudaGetLastError();
+        return ~0ull;
+    }
+    return v;
+}
+
+}// namespace b200

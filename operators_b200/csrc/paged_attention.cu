@@ -84,8 +84,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-__device__ __forceinline__ uint32_t lo_f16x2(uint32_t w) { return e4m3x2_to_f16x2((uint16_t) w); }
-__device__ __forceinline__ uint32_t hi_f16x2(uint32_t w) { return e4m3x2_to_f16x2((uint16_t) (w >> 16)); }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
@@ -399,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, e[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t a0 = lo_f16x2(a[i]), a2 = hi_f16x2(a[i]), a1 = lo_f16x2(e[i]), a3 = hi_f16x2(e[i]);
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_to_f16x4(a[i], a0, a2), e4m3x4_to_f16x4(e[i], a1, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma_f16(x[sub][nt], a0, a1, a2, a3, qf[nt][h * 4 + i][0], qf[nt][h * 4 + i][1]);
                     }
@@ -522,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     // bytes of two tokens side by side: (a0 b0 a1 b1) and (a2 b2 a3 b3)
                     const uint32_t e0 = __byte_perm(v[0][i], v[1][i], 0x5140), e1 = __byte_perm(v[0][i], v[1][i], 0x7362);
                     const uint32_t f0 = __byte_perm(v[2][i], v[3][i], 0x5140), f1 = __byte_perm(v[2][i], v[3][i], 0x7362);
-                    const uint32_t a0 = lo_f16x2(e0), a1 = hi_f16x2(e0), a2 = lo_f16x2(f0), a3 = hi_f16x2(f0);
-                    const uint32_t c0 = lo_f16x2(e1), c1 = hi_f16x2(e1), c2 = lo_f16x2(f1), c3 = hi_f16x2(f1);
+                    uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
+                    e4m3x4_to_f16x4(e0, a0, a1), e4m3x4_to_f16x4(f0, a2, a3), e4m3x4_to_f16x4(e1, c0, c1), e4m3x4_to_f16x4(f1, c2, c3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma_f16(o[nt][2 * i], a0, a1, a2, a3, bw[sub][nt][0], bw[sub][nt][1]);

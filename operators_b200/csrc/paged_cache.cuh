@@ -113,6 +113,15 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
     return r;
 }
+// four codes of a word
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t c, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(c));
+}
 __device__ __forceinline__ uint16_t f32x2_to_e4m3x2(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));

@@ -90,6 +90,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
           "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// 16 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n\t"
+        "tcgen05.wait::st.sync.aligned;"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 // two fp32 operations per instruction
 __device__ __forceinline__ uint64_t pack2f(float lo, float hi) {
     uint64_t r;
@@ -305,7 +315,8 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
             if (++tile >= g.t1 && (more = walk.next(g))) tile = g.t0;
         };
         struct Ids {
-            int32_t row[2], key;// pages of this thread's two rows and of the key whose scales it loads; -1: none
+            int32_t row[2], key;// pages of this thread's two rows and of the key whose scales it loads (one page: the tile's); -1: none
+            bool has;           // this thread's key exists
         };
         auto page_of = [&](int32_t tok) -> int32_t {
             if (tok >= held(g.s.len, p.t.cap)) return -1;
@@ -313,47 +324,58 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
             return id >= 0 && id < p.c.pages ? id : -1;
         };
         auto ids_of = [&](Ids &x) {
-            x.row[0] = x.row[1] = x.key = -1;
+            x.row[0] = x.row[1] = x.key = -1, x.has = false;
             if (!more) return;
             const int32_t tok = tile * kKeys;
             if (ONE) {
                 const int32_t id = page_of(tok), left = held(g.s.len, p.t.cap) - tok;
                 x.row[0] = (int32_t) r0 < left ? id : -1;
                 x.row[1] = (int32_t) r0 + 32 < left ? id : -1;
-                x.key = (int32_t) c < left ? id : -1;
+                x.key = id, x.has = id >= 0 && (int32_t) c < left;
             } else {
                 x.row[0] = page_of(tok + (int32_t) r0);
                 x.row[1] = page_of(tok + (int32_t) r0 + 32);
-                if (c < kKeys) x.key = page_of(tok + (int32_t) c);
+                if (c < kKeys) x.key = page_of(tok + (int32_t) c), x.has = x.key >= 0;
             }
         };
         uint4 kd[2][kGroups], vd[2][kGroups];
         float ks = 0.f, vs = 0.f;
         bool key_ok = false;
-        // 16 codes of head elements d0 .. of one row
+        // 16 codes of a row from element d0 on, one by one
         auto load16 = [&](const uint8_t *at, int32_t d0) -> uint4 {
-            if (p.vec) return *reinterpret_cast<const uint4 *>(at + d0);
             uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < 16; ++i) {
-                if (d0 + i < p.c.dh) w[i >> 2] |= (uint32_t) at[d0 + i] << (8 * (i & 3));
+                if (d0 + i < p.c.dh) w[i >> 2] |= (uint32_t) at[i] << (8 * (i & 3));
             }
             return make_uint4(w[0], w[1], w[2], w[3]);
         };
         auto load_tile = [&](const Ids &x, const PoolStrides &st, const uint8_t *pool, uint4 (&to)[2][kGroups]) {
+            const uint8_t *at[2];
+            const int32_t tok = tile * kKeys + (int32_t) r0;
+            if (ONE) {
+                const int32_t in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
+                at[0] = pool + (int64_t) max(x.key, 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp + c4 * 16;
+                at[1] = at[0] + 32 * st.sp;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int32_t in_page = tok + 32 * i - (int32_t) p.page_div.div((uint32_t) (tok + 32 * i)) * p.c.page;
+                    at[i] = pool + (int64_t) max(x.row[i], 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp + c4 * 16;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int32_t tok = tile * kKeys + (int32_t) r0 + 32 * i, in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
-                const uint8_t *at = pool + (int64_t) max(x.row[i], 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp;
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
                     const int32_t d0 = (q * 4 + (int32_t) c4) * 16;
-                    to[i][q] = x.row[i] >= 0 && d0 < p.c.dh ? load16(at, d0) : make_uint4(0u, 0u, 0u, 0u);
+                    to[i][q] = make_uint4(0u, 0u, 0u, 0u);
+                    if (x.row[i] >= 0 && d0 < p.c.dh) to[i][q] = ONE || p.vec ? *reinterpret_cast<const uint4 *>(at[i] + q * 64) : load16(at[i] + q * 64, d0);
                 }
             }
         };
         auto load_scales = [&](const Ids &x) {
-            key_ok = x.key >= 0;
+            key_ok = x.has;
             ks = vs = 0.f;
             if (key_ok && c < (ONE ? 1u : (uint32_t) kKeys)) {
                 ks = p.ks[(int64_t) x.key * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch];
@@ -370,14 +392,11 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
                     if ((q * 4 + (int32_t) c4) * 16 >= p.c.dh) continue;
                     const uint4 w = from[i][q];
                     const uint32_t row = base + (uint32_t) q * (kKeys * 128u) + r * 128u;
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4) ^ (r & 7u)) << 4)),
-                                 "r"(e4m3x2_to_f16x2((uint16_t) w.x)), "r"(e4m3x2_to_f16x2((uint16_t) (w.x >> 16))),
-                                 "r"(e4m3x2_to_f16x2((uint16_t) w.y)), "r"(e4m3x2_to_f16x2((uint16_t) (w.y >> 16)))
-                                 : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4 + 1) ^ (r & 7u)) << 4)),
-                                 "r"(e4m3x2_to_f16x2((uint16_t) w.z)), "r"(e4m3x2_to_f16x2((uint16_t) (w.z >> 16))),
-                                 "r"(e4m3x2_to_f16x2((uint16_t) w.w)), "r"(e4m3x2_to_f16x2((uint16_t) (w.w >> 16)))
-                                 : "memory");
+                    uint32_t h[8];
+                    e4m3x4_to_f16x4(w.x, h[0], h[1]), e4m3x4_to_f16x4(w.y, h[2], h[3]);
+                    e4m3x4_to_f16x4(w.z, h[4], h[5]), e4m3x4_to_f16x4(w.w, h[6], h[7]);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");// the products read through the async proxy
@@ -475,40 +494,47 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
                 if (!(ok = mbar_wait<kSuspendNs>(&bars[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
                 tc_fence_after();
                 __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
-                float x[kKeys];
-                tmem_ld32(t_lane + b * kKeys, x);
-                tmem_ld32(t_lane + b * kKeys + 32, x + 32);
-                // scores are x * f; a tile that hides something from a row of this warp takes them one by one
+                // Scores are x * f; where the tile hides something from a row of this warp, x is the score itself and
+                // f is 1.  The 64 scores pass through 32 registers: half 0 for its maximum, half 1 for its maximum and
+                // its weights, half 0 again for its weights.
+                float x[32];
                 float f = ONE ? sc.ks[0] * rf : 1.f;
-                if (!ONE) {
+                const uint32_t mask[2] = {sc.mask[0], sc.mask[1]};
+                const bool hidden = __any_sync(0xffffffffu, (mask[0] & mask[1]) != 0xFFFFFFFFu || (have && (int64_t) tile * kKeys + kKeys > limit));
+                auto load_scores = [&](int half, float &lane_wtop) {
+                    tmem_ld32(t_lane + b * kKeys + half * 32, x);
+                    if (!ONE) {
 #pragma unroll
-                    for (int i = 0; i < kKeys; ++i) x[i] *= sc.ks[i] * rf;
-                }
-                const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
-                if (__any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && (int64_t) tile * kKeys + kKeys > limit))) {
-                    const int32_t left = limit - tile * kKeys;
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) {
-                        const bool seen = ((i < 32 ? m0 : m1) >> (i & 31)) & 1u;
-                        x[i] = seen && i < left ? x[i] * f : -INFINITY;
+                        for (int i = 0; i < 32; ++i) x[i] *= sc.ks[half * 32 + i] * rf;
                     }
-                    f = 1.f;
-                }
-                float t4[4] = {x[0], x[1], x[2], x[3]};
+                    if (hidden) {
+                        const int32_t left = limit - tile * kKeys - half * 32;
 #pragma unroll
-                for (int i = 4; i < kKeys; i += 8) {
+                        for (int i = 0; i < 32; ++i) x[i] = ((mask[half] >> i) & 1u) && i < left ? (ONE ? x[i] * f : x[i]) : -INFINITY;
+                    }
+                    if (!ONE) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t4[j] = i + 4 + j < kKeys ? fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]) : fmaxf(t4[j], x[i + j]);
-                }
-                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f;
-                float wtop;
-                if (ONE) {
-                    wtop = top + sc.lv[0];
-                } else {
-                    wtop = -INFINITY;
+                        for (int i = 0; i < 32; ++i) lane_wtop = fmaxf(lane_wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[half * 32 + i]);
+                    }
+                };
+                auto largest = [&]() -> float {
+                    float t4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
-                }
+                    for (int i = 4; i < 28; i += 8) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], x[28 + j]);
+                    return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                };
+                float wtop = -INFINITY;
+                load_scores(0, wtop);
+                float top = largest();
+                load_scores(1, wtop);
+                if (ONE && hidden) f = 1.f;
+                top = fmaxf(top, largest()) * f;
+                if (ONE) wtop = top + sc.lv[0];
                 // references
                 if (top > m + kSlack || (m == -INFINITY && top > m)) {
                     l *= fast_exp2(m - top);// (from -inf: 0)
@@ -532,35 +558,43 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
                     }
                 }
                 const float mm = m == -INFINITY ? 0.f : m, ww = wm == -INFINITY ? 0.f : wm;
-                uint32_t w[kKeys / 2];
-                if (ONE) {
-                    const float e = fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : sc.lv[0]), kLeast);
-                    const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
-                    uint64_t part[2] = {0ull, 0ull};
+                const float e = ONE ? fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : sc.lv[0]), kLeast) : mm - ww + kLift;
+                float sum = 0.f;
+                auto weigh = [&](int half, uint32_t (&w)[16]) {
+                    if (ONE) {
+                        const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
+                        uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int i = 0; i < kKeys / 2; ++i) {
-                        const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
-                        const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
-                        part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
-                        w[i] = round16x2(false, y0, y1);
-                    }
-                    const float2 sum = unpack2f(add2(part[0], part[1]));
-                    l = fmaf(sum.x + sum.y, fast_exp2(-e), l);
-                } else {
-                    // pages that end inside the tile: a factor per key
-                    const float gf = mm - ww + kLift;
-                    float sum = 0.f;
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
+                            const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
+                            part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
+                            w[i] = round16x2(false, y0, y1);
+                        }
+                        const float2 t = unpack2f(add2(part[0], part[1]));
+                        sum += t.x + t.y;
+                    } else {
+                        // pages that end inside the tile: a factor per key, so p and w take an exponential each
 #pragma unroll
-                    for (int i = 0; i < kKeys / 2; ++i) {
-                        const float y0 = fast_exp2(x[2 * i] - mm), y1 = fast_exp2(x[2 * i + 1] - mm);
-                        sum += y0 + y1;
-                        w[i] = round16x2(false, x[2 * i] == -INFINITY ? 0.f : fast_exp2(x[2 * i] - mm + gf + sc.lv[2 * i]),
-                                         x[2 * i + 1] == -INFINITY ? 0.f : fast_exp2(x[2 * i + 1] - mm + gf + sc.lv[2 * i + 1]));
+                        for (int i = 0; i < 16; ++i) {
+                            const float a0 = x[2 * i] - mm, a1 = x[2 * i + 1] - mm;
+                            sum += fast_exp2(a0) + fast_exp2(a1);
+                            w[i] = round16x2(false, a0 == -INFINITY ? 0.f : fast_exp2(a0 + (e + sc.lv[half * 32 + 2 * i])),
+                                             a1 == -INFINITY ? 0.f : fast_exp2(a1 + (e + sc.lv[half * 32 + 2 * i + 1])));
+                        }
                     }
-                    l += sum;
-                }
+                };
+                uint32_t w0[16], w1[16];
+                weigh(1, w1);
                 __syncwarp();
-                tmem_st32(t_lane + b * kKeys, w);
+                if (ONE) f = sc.ks[0] * rf;// (load_scores applies it again where something is hidden)
+                load_scores(0, wtop);
+                if (ONE && hidden) f = 1.f;
+                tmem_st16(t_lane + b * kKeys + 16, w1);// (over scores that are read)
+                weigh(0, w0);
+                __syncwarp();
+                tmem_st16(t_lane + b * kKeys, w0);
+                l = ONE ? fmaf(sum, fast_exp2(-e), l) : l + sum;
                 tc_fence_before();
                 mbar_arrive(&bars[kWFull + b]);
             }

@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     const float4 a = *reinterpret_cast<const float4 *>(so + (i * kRows + r) * DHC + ((grp ^ (uint32_t) (r & 7)) << 2));
                     if (f[i] != 0.f) y.x += f[i] * a.x, y.y += f[i] * a.y, y.z += f[i] * a.z, y.w += f[i] * a.w;
                 }
-                if (whole) store_out(p, out, (int32_t) grp * 4, y, lr, wr - kLift - mr);
+                if (whole) store_out(p, out, (int32_t) grp * 4, y, out_factors(lr, wr - kLift - mr));
                 else *reinterpret_cast<float4 *>(dp.parts + (slot0 + r) * DHC + grp * 4) = y;
             }
         }
@@ -614,7 +614,7 @@ struct AttendDesc {
     int64_t o_st, o_sh, q_st, q_sh;
     float scale;
     int dhc;      // head size rounded up to 64, 128 or 256
-    int block;    // query rows per block: 8 or 16 (mma.sync), 128 (tcgen05)
+    int block;    // query rows per item: 8 or 16 (mma.sync), 128 or 256 (tcgen05)
     uint32_t ctas;
 };
 
@@ -679,11 +679,12 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     if ((int64_t) d.rows * group > 0x7FFFFFFF) return STATUS_BAD_TENSOR_SHAPE;
     // query rows per sequence on average (only the device knows each one's)
     const int64_t rows_each = d.t.batch > 0 ? (int64_t) d.rows * group / d.t.batch : 0;
-    d.block = rows_each > kPrefillRows && d.t.batch <= kPrefillMaxBatch ? 128 : rows_each > 8 ? 16 : 8;
+    const bool prefill = rows_each > kPrefillRows && d.t.batch <= kPrefillMaxBatch;
+    d.block = prefill ? prefill_rows(d.dhc) : rows_each > 8 ? 16 : 8;
     // every CTA that fits the GPU at once, but no more than there can be units for
-    const int64_t blocks = ((int64_t) d.rows * group + d.block - 1) / d.block + d.t.batch, keys = d.block == 128 ? kPrefillKeys : kTile;
+    const int64_t blocks = ((int64_t) d.rows * group + d.block - 1) / d.block + d.t.batch, keys = prefill ? kPrefillKeys : kTile;
     const int64_t tiles = std::max<int64_t>(1, ((int64_t) d.t.cap + keys - 1) / keys);
-    const int64_t places = (int64_t) d.sm_count * (d.block == 128 ? (d.dhc == 256 ? 1 : 2) : ctas_per_sm(d.dhc, d.block / 8));
+    const int64_t places = (int64_t) d.sm_count * (prefill ? 1 : ctas_per_sm(d.dhc, d.block / 8));
     d.ctas = (uint32_t) places;
     if (blocks * d.c.heads < places * kMinUnits) {
         d.ctas = (uint32_t) std::max<int64_t>(1, std::min(places, (blocks * d.c.heads * tiles + kMinUnits - 1) / kMinUnits));
@@ -734,7 +735,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     p.o_vec = (uintptr_t) out % 8 == 0 && d->o_st % 4 == 0 && d->o_sh % 4 == 0 && d->c.dh % 4 == 0;
     auto st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (d->block == 128) {
+    if (d->block >= 128) {
         e = launch_prefill(p, workspace, d->dhc, d->ctas, d->device_id, st);
     } else {
         const bool few = d->block == 8;

@@ -37,15 +37,17 @@ __device__ __forceinline__ uint32_t round16x2(bool bf16, float lo, float hi) {
     return r;
 }
 
-// Elements d .. d + 3 of a row of out: y * 2^exponent / l, rounded once; rows that have seen no key get zeros.  The
-// power of two may leave fp32's range on the way, so it is applied in two halves.
-__device__ __forceinline__ void store_out(const AttendParams &p, uint16_t *out, int32_t d, float4 y, float l, float exponent) {
-    float a = 0.f, b = 0.f;
-    if (l != 0.f) {
-        const float h = truncf(exponent * 0.5f);
-        a = exp2f(h) / l, b = exp2f(exponent - h);
-    }
-    if (l == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+// A row's output is y * 2^exponent / l; the power of two may leave fp32's range on the way, so it is applied as two
+// factors.  Rows that have seen no key (l = 0) get zeros.
+__device__ __forceinline__ float2 out_factors(float l, float exponent) {
+    if (l == 0.f) return make_float2(0.f, 0.f);
+    const float h = truncf(exponent * 0.5f);
+    return make_float2(exp2f(h) / l, exp2f(exponent - h));
+}
+// Elements d .. d + 3 of a row of out, rounded once.
+__device__ __forceinline__ void store_out(const AttendParams &p, uint16_t *out, int32_t d, float4 y, float2 f) {
+    const float a = f.x, b = f.y;
+    if (a == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
     const uint32_t lo = round16x2(p.bf16, y.x * a * b, y.y * a * b), hi = round16x2(p.bf16, y.z * a * b, y.w * a * b);
     if (p.o_vec) {
         if (d < p.c.dh) *reinterpret_cast<uint2 *>(out + d) = make_uint2(lo, hi);
@@ -134,12 +136,17 @@ static inline SplitParams split_params(const AttendParams &a, void *workspace, u
     return s;
 }
 
-// Joins the parts of the item that begins in stretch blockIdx.x and goes on behind it.  A block takes two rows; for each,
-// four groups of threads add every fourth part (kBatch of them loaded at a time: the loads' latency is all there is to
-// this kernel), and the groups' sums are added in order.
-constexpr int kJoinRows = 2, kJoinGroups = 4, kBatch = 7;
+// Joins the parts of the item that begins in stretch blockIdx.x and goes on behind it.  A decoding item (ROWS 8 or 16) may
+// have dozens of parts: a block takes two rows, and for each, four groups of threads add every fourth part.  A block of
+// prompt rows has few: eight rows per block, one group.  kBatch parts are loaded at a time (the loads' latency is all there
+// is to this kernel), and everything is added in the order of the list.
+template<int ROWS>
+struct JoinShape {
+    static constexpr int kRows = ROWS >= 128 ? 8 : 2, kGroups = ROWS >= 128 ? 1 : 4, kBatch = ROWS >= 128 ? 3 : 7;
+};
 template<int DHC, int ROWS>
-__global__ void __launch_bounds__(kJoinRows * kJoinGroups * DHC / 4) join_kernel(const SplitParams dp) {
+__global__ void __launch_bounds__(JoinShape<ROWS>::kRows * JoinShape<ROWS>::kGroups * DHC / 4) join_kernel(const SplitParams dp) {
+    constexpr int kJoinRows = JoinShape<ROWS>::kRows, kJoinGroups = JoinShape<ROWS>::kGroups, kBatch = JoinShape<ROWS>::kBatch;
     constexpr int kLanes = DHC / 4;
     __shared__ float4 acc[kJoinRows][kJoinGroups][kLanes];
     __shared__ float stat[kJoinRows][kJoinGroups][3];
@@ -201,14 +208,14 @@ __global__ void __launch_bounds__(kJoinRows * kJoinGroups * DHC / 4) join_kernel
             y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
         }
     }
-    store_out(p, row_of_out(p, s, item.kvh, rr), ln * 4, y, l, w - m);
+    store_out(p, row_of_out(p, s, item.kvh, rr), ln * 4, y, out_factors(l, w - m));
 }
 
 template<int DHC, int ROWS>
 static inline cudaError_t launch_join(const SplitParams &sp, uint32_t ctas, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas - 1, ROWS / kJoinRows);
-    cfg.blockDim = dim3(kJoinRows * kJoinGroups * DHC / 4);
+    cfg.gridDim = dim3(ctas - 1, ROWS / JoinShape<ROWS>::kRows);
+    cfg.blockDim = dim3(JoinShape<ROWS>::kRows * JoinShape<ROWS>::kGroups * DHC / 4);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -217,8 +224,10 @@ static inline cudaError_t launch_join(const SplitParams &sp, uint32_t ctas, cuda
     return cudaLaunchKernelEx(&cfg, join_kernel<DHC, ROWS>, sp);
 }
 
-// Prompts and chunks (paged_prefill.cu): 128 query rows x 64 cached tokens per tile.
+// Prompts and chunks (paged_prefill.cu): tiles of 64 cached tokens, items of 256 query rows (128 for head sizes beyond 128),
+// one CTA per SM.
 constexpr int kPrefillKeys = 64;
+static inline int prefill_rows(int dhc) { return dhc <= 128 ? 256 : 128; }
 constexpr int64_t kPrefillMaxBatch = 4096;// sequences whose unit counts fit the kernel's shared memory
 cudaError_t launch_prefill(const AttendParams &a, void *workspace, int dhc, uint32_t ctas, int device_id, cudaStream_t st);
 

@@ -3,7 +3,7 @@
 // A block is 128 query rows (new tokens x the q heads that share a kv head, row = token * group + head), one TMEM lane
 // each; a tile is 64 cached tokens.  Per tile: S = q k^T into TMEM, weights in fp16 back into TMEM over S (operand A of
 // the second product), O += W v in TMEM.  The operands of kind::f16 are fp16: q is scaled per row by a power of two
-// (see paged_attention.cu), the codes become fp16 exactly on their way into shared memory, once per block of 128 rows.
+// (see paged_attention.cu), the codes become fp16 exactly on their way into shared memory, once per pair of blocks.
 //
 // Softmax in one pass: score 2^(s f - m) with f the row's and the page's factor and m the row's running reference,
 // which moves only when a score exceeds it by 2^8, so that O (which then has to be read, multiplied and written
@@ -14,14 +14,18 @@
 // and their sum must not underflow.
 //
 // What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x
-// dh multiply-adds (512 cycles at dh 128), so two CTAs share an SM and one's exponentials run beside the other's
-// products.
+// dh multiply-adds (512 cycles at dh 128).  One CTA per SM works on two blocks at a time (head sizes beyond 128: one), so
+// that one's exponentials run beside the other's products and both share the converted tiles.
 //
-// Roles (288 threads): warps 0-3 softmax and epilogue, a thread per row; warps 4-7 convert codes (their loads run a
-// tile ahead in registers); warp 8 allocates TMEM, one lane issues the products.  Shared memory: q, two tiles of K, two
-// of V (128-byte swizzled rows as TMA would lay them).  S is double-buffered: S of tile j + 1 is issued before W v of
-// tile j.  Work is divided into equal stretches of tiles as in paged_attention.cu (row blocks stop where their last row's
-// mask begins), and all roles walk the stretch's items by themselves.
+// Roles (416 threads; 288 with one block): a warpgroup per block for softmax and epilogue, a thread per row; a
+// warpgroup converts codes (its loads run a tile ahead in registers); the last warp allocates TMEM, one lane issues the
+// products.  Shared memory: q, two tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is
+// double-buffered: S of tile j + 1 is issued before W v of tile j.
+//
+// Work is divided into equal stretches as in paged_attention.cu; an item is a pair of blocks, stops where its last row's
+// mask begins, and counts kItemUnits tiles more for what its start and end cost.  All roles walk the stretch's items by
+// themselves.
+//
 // A product's completion is waited for only where O is touched, so it has a barrier for even and one for odd tiles: a row
 // that has seen S of tile n knows that W v of tile n - 2 (issued before it) is done, not that of tile n - 1, and one
 // barrier's parity could not tell the two apart.
@@ -39,34 +43,41 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = kPrefillKeys;
-constexpr int kSoftmax = 128, kConvert = 128, kThreads = kSoftmax + kConvert + 32, kWarps = kThreads / 32;
 constexpr float kSlack = 8.f, kLift = 7.f;// w <= 2^15
 constexpr float kLeast = -90.f;
-constexpr int kMinUnits = 4;
+constexpr int kItemUnits = 4;// what the start and the end of an item cost, in tiles
+constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;
-// Two CTAs of 9 warps leave 96 registers a thread (5 warps on a quarter of the SM).  The softmax warps, which hold a
-// tile's 64 scores of a row, take what the converting warps can spare.
-constexpr int kLaunchRegs = 96, kSoftmaxRegs = 120, kConvertRegs = 72;
-static_assert(kSoftmax * kSoftmaxRegs + kConvert * kConvertRegs + 32 * kLaunchRegs <= kThreads * kLaunchRegs, "the split fits what the launch gave");
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
 
-// TMEM columns: S (and the weights over it) [0, 64) and [64, 128), O from 128
-__host__ __device__ constexpr uint32_t tmem_cols(int dhc) { return dhc <= 128 ? 256u : 512u; }
+__host__ __device__ constexpr int blocks_at_once(int dhc) { return dhc <= 128 ? 2 : 1; }
+__host__ __device__ constexpr int threads_of(int nb) { return 128 * nb + 128 + 32; }
+// Registers per thread: at launch, and after the warpgroups have traded (the softmax holds the 64 scores of a row's tile)
+__host__ __device__ constexpr int launch_regs(int nb) { return nb == 2 ? 128 : 168; }
+__host__ __device__ constexpr int softmax_regs(int nb) { return nb == 2 ? 152 : 200; }
+__host__ __device__ constexpr int convert_regs(int nb) { return nb == 2 ? 80 : 136; }
+__host__ __device__ constexpr bool split_fits(int nb) {
+    return 128 * nb * softmax_regs(nb) + 128 * convert_regs(nb) + 32 * launch_regs(nb) <= threads_of(nb) * launch_regs(nb);
+}
+static_assert(split_fits(1) && split_fits(2), "the registers' split fits what the launch gave");
 
-enum Bar { kQFull, kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty1, kSFull, kSFull1, kWFull, kWFull1, kPvDone, kPvDone1,
-           kScFull, kBars = kScFull + kScaleSets };
+// TMEM columns of a block: S (and the weights over it) [0, 64) and [64, 128), O from 128; the second block from 256.
+constexpr uint32_t kTmemCols = 512;
+
+// barriers; the second block's own follow the first's
+enum Bar { kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty1, kScFull, kBlock = kScFull + kScaleSets,
+           kQFull = 0, kSFull, kSFull1, kWFull, kWFull1, kPvDone, kPvDone1, kBlockBars, kBars = kBlock + 2 * kBlockBars };
 
 struct TileScales {
     float ks[kKeys], vs[kKeys], lv[kKeys];// scales of the keys, of the values, log2 of the latter; one page: [0] only
     uint32_t mask[2], pad[2];             // tokens that exist
 };
 
-__host__ __device__ constexpr uint32_t q_bytes(int dhc) { return (uint32_t) dhc * 2 * kRows; }
+__host__ __device__ constexpr uint32_t q_bytes(int dhc) { return (uint32_t) dhc * 2 * kRows; }// of one block
 __host__ __device__ constexpr uint32_t kv_bytes(int dhc) { return (uint32_t) dhc * 2 * kKeys; }
-__host__ __device__ constexpr uint32_t smem_bytes(int dhc) {
-    return q_bytes(dhc) + 4 * kv_bytes(dhc) + kScaleSets * (uint32_t) sizeof(TileScales) + kBars * 8 + 32;
-}
-static_assert(kPrefillMaxBatch * 8 <= q_bytes(64) + 4 * kv_bytes(64), "the sequences' unit counts fit the tiles' memory");
+__host__ __device__ constexpr uint32_t tile_bytes(int dhc) { return (uint32_t) blocks_at_once(dhc) * q_bytes(dhc) + 4 * kv_bytes(dhc); }
+__host__ __device__ constexpr uint32_t smem_bytes(int dhc) { return tile_bytes(dhc) + kScaleSets * (uint32_t) sizeof(TileScales) + kBars * 8 + 32; }
+static_assert(kPrefillMaxBatch * 8 <= tile_bytes(64), "the sequences' unit counts fit the tiles' memory");
 
 // D[tmem] (+)= A[tmem] * B[smem desc]: the rows of A are TMEM lanes, two fp16 elements per column
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -122,70 +133,81 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// Tiles of a block of query rows: up to the last key that its last row sees, one at least (rows without keys get zeros).
+// Items of a sequence and kv head, and the tiles of one: up to the last key that its last row sees, one at least (rows
+// without keys get zeros).
+template<int ROWS>
+__device__ __forceinline__ int32_t items_of(const AttendParams &p, const Seq &s) {
+    return (int32_t) (((uint32_t) s.n * (uint32_t) p.group + ROWS - 1) / ROWS);
+}
+template<int ROWS>
 __device__ __forceinline__ int32_t tiles_of(const AttendParams &p, const Seq &s, int32_t rb) {
-    const uint32_t rows = (uint32_t) s.n * (uint32_t) p.group, end = ((uint32_t) rb + 1) * kRows;
+    const uint32_t rows = (uint32_t) s.n * (uint32_t) p.group, end = ((uint32_t) rb + 1) * ROWS;
     const int32_t tok = (int32_t) p.group_div.div((end < rows ? end : rows) - 1);
     const int32_t limit = min(s.len - s.n + tok + 1, held(s.len, p.t.cap));
     return limit > 0 ? (limit - 1) / kKeys + 1 : 1;
 }
-__device__ __forceinline__ int32_t blocks_of(const AttendParams &p, const Seq &s) {
-    return (int32_t) (((uint32_t) s.n * (uint32_t) p.group + kRows - 1) / kRows);
-}
 
-// A stretch of units, item by item.  Every role keeps its own.
+// A stretch of units, item by item.  Every role keeps its own.  The first kItemUnits units of an item hold no tile.
 struct Segment {
     Seq s;
     int32_t b, kvh, rb, t0, t1, tiles;
-    int64_t u;// unit of t0
+    int64_t last_unit;// of the item
 };
+template<int ROWS>
 struct Walker {
     const AttendParams &p;
     Seq s;
-    int32_t b, kvh, rb, t0, blocks;
+    int32_t b, kvh, rb, at, blocks;// `at`: unit of the item
     int64_t u, end;
     __device__ __forceinline__ bool next(Segment &g) {
-        if (u >= end) return false;
-        if (blocks < 0) s = seq_of(p.lens, p.offs, p.rows, b), blocks = blocks_of(p, s);
-        while (blocks == 0) s = seq_of(p.lens, p.offs, p.rows, ++b), blocks = blocks_of(p, s);// (units are left: there is one)
-        const int32_t tiles = tiles_of(p, s, rb);
-        const int32_t n = end - u < tiles - t0 ? (int32_t) (end - u) : tiles - t0;
-        g.s = s, g.b = b, g.kvh = kvh, g.rb = rb, g.t0 = t0, g.t1 = t0 + n, g.tiles = tiles, g.u = u;
-        u += n, t0 = 0;
-        if (g.t1 == tiles && ++rb == blocks) {
-            rb = 0;
-            if (++kvh == p.c.heads) kvh = 0, ++b, blocks = -1;
+        while (u < end) {
+            if (blocks < 0) s = seq_of(p.lens, p.offs, p.rows, b), blocks = items_of<ROWS>(p, s);
+            while (blocks == 0) s = seq_of(p.lens, p.offs, p.rows, ++b), blocks = items_of<ROWS>(p, s);// (units are left: there is one)
+            const int32_t tiles = tiles_of<ROWS>(p, s, rb), size = tiles + kItemUnits;
+            const int32_t n = end - u < size - at ? (int32_t) (end - u) : size - at;
+            g.s = s, g.b = b, g.kvh = kvh, g.rb = rb, g.tiles = tiles;
+            g.t0 = max(0, at - kItemUnits), g.t1 = max(0, at + n - kItemUnits);
+            g.last_unit = u - at + size - 1;
+            u += n;
+            const bool ends = at + n == size;
+            at = 0;
+            if (ends && ++rb == blocks) {
+                rb = 0;
+                if (++kvh == p.c.heads) kvh = 0, ++b, blocks = -1;
+            }
+            if (g.t1 > g.t0) return true;
         }
-        return true;
+        return false;
     }
 };
 
 template<int DHC, bool ONE>
-__global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(const SplitParams sp) {
+__global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_kernel(const SplitParams sp) {
+    constexpr int kNB = blocks_at_once(DHC), kItemRows = kNB * kRows, kThreads = threads_of(kNB), kWarps = kThreads / 32;
     constexpr uint32_t kQ = q_bytes(DHC), kKV = kv_bytes(DHC);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ int64_t slot[kWarps], found_base;
     __shared__ int32_t found_b, found_rb, found_t;
     const AttendParams &p = sp.a;
-    // the swizzled tiles need 1024-byte alignment; two CTAs fill the SM, so there is no room to round up
+    // the swizzled tiles need 1024-byte alignment
     if ((smem_u32(smem) & 1023u) != 0) {
         if (threadIdx.x == 0) atomicAdd(&g_tc_gemm_timeouts, 1ull), sp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
         return;
     }
-    const uint32_t sq = smem_u32(smem), sk = sq + kQ, sv = sk + 2 * kKV;
-    TileScales *scales = reinterpret_cast<TileScales *>(smem + kQ + 4 * kKV);
+    const uint32_t sq = smem_u32(smem), sk = sq + kNB * kQ, sv = sk + 2 * kKV;
+    TileScales *scales = reinterpret_cast<TileScales *>(smem + tile_bytes(DHC));
     uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kScaleSets);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // ---- this CTA's stretch.  Units of a kv head of each sequence: a warp per sequence, a lane per block of rows.
+    // ---- this CTA's stretch.  Units of a kv head of each sequence: a warp per sequence, a lane per item.
     int64_t *sums = reinterpret_cast<int64_t *>(smem);
     for (int32_t b = (int32_t) warp; b < p.t.batch; b += kWarps) {
         const Seq s = seq_of(p.lens, p.offs, p.rows, b);
-        const int32_t blocks = blocks_of(p, s);
+        const int32_t blocks = items_of<kItemRows>(p, s);
         int64_t n = 0;
-        for (int32_t rb = (int32_t) lane; rb < blocks; rb += 32) n += tiles_of(p, s, rb);
+        for (int32_t rb = (int32_t) lane; rb < blocks; rb += 32) n += tiles_of<kItemRows>(p, s, rb) + kItemUnits;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
         if (lane == 0) sums[b] = n;
@@ -215,14 +237,14 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
     const int64_t per_head = sums[b_first];
     const int32_t kvh_first = (int32_t) divide(u0 - found_base, per_head);
     if (warp == 0) {
-        // the block of rows and its tile where the stretch begins
+        // the item where the stretch begins, and the unit in it
         const Seq s = seq_of(p.lens, p.offs, p.rows, b_first);
-        const int32_t blocks = blocks_of(p, s);
+        const int32_t blocks = items_of<kItemRows>(p, s);
         const int64_t x = u0 - found_base - kvh_first * per_head;
         int64_t base = 0;
         for (int32_t rb0 = 0; rb0 < blocks && base <= x; rb0 += 32) {
             const int32_t rb = rb0 + (int32_t) lane;
-            const int64_t n = rb < blocks ? tiles_of(p, s, rb) : 0;
+            const int64_t n = rb < blocks ? tiles_of<kItemRows>(p, s, rb) + kItemUnits : 0;
             int64_t incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -236,78 +258,91 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
     }
     if (threadIdx.x == 32) {
         for (int i = 0; i < kBars; ++i) {
-            const bool rows = i == kQFull || i == kWFull || i == kWFull1, keys = i >= kScFull;
-            const bool codes = i == kKFull || i == kKFull1 || i == kVFull || i == kVFull1;
-            mbar_init(&bars[i], rows ? kSoftmax : codes ? kConvert : keys ? kKeys : 1u);
+            const int own = i >= kBlock ? (i - kBlock) % kBlockBars : -1;
+            const bool rows = own == kQFull || own == kWFull || own == kWFull1;
+            const bool codes = i == kKFull || i == kKFull1 || i == kVFull || i == kVFull1, keys = i >= kScFull && i < kBlock;
+            mbar_init(&bars[i], rows || codes ? 128u : keys ? (uint32_t) kKeys : 1u);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        tmem_alloc(tmem_slot, tmem_cols(DHC));
+    if (warp == kWarps - 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();// (the sums are read, the tiles' memory is free)
     tc_fence_after();
     if (p.c.dh < DHC) {
-        // head elements beyond dh: zeros that nothing writes again
-        for (uint32_t i = threadIdx.x * 16; i < kQ + 4 * kKV; i += kThreads * 16) {
+        // head elements beyond dh: zeros that no product's operand overwrites
+        for (uint32_t i = threadIdx.x * 16; i < tile_bytes(DHC); i += kThreads * 16) {
             asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sq + i), "r"(0) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
     }
     const uint32_t tmem = *tmem_slot;
-    Walker walk{p, Seq{}, b_first, kvh_first, found_rb, found_t, -1, u0, u1};
+    Walker<kItemRows> walk{p, Seq{}, b_first, kvh_first, found_rb, found_t, -1, u0, u1};
     Segment g;
+    // the second block of an item has rows
+    auto second = [&](const Segment &x) { return kNB == 2 && (uint32_t) x.s.n * (uint32_t) p.group > (uint32_t) x.rb * kItemRows + kRows; };
 
-    if (warp == 8) {
+    if (warp == kWarps - 1) {
         // ------------------------------------------------------------ products
         if (lane == 0) {
             const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
             const uint32_t idesc_s = make_idesc(kRows, kKeys, 0, 0), idesc_o = make_idesc(kRows, steps * 16, 0, 1);
             bool ok = true;
-            uint32_t n = 0, seg = 0;
-            auto issue_s = [&](uint32_t i) -> bool {
+            uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
+            // S of the n-th tile for the active blocks
+            auto issue_s = [&](uint32_t i, uint32_t ahead, int nb) -> bool {
                 const uint32_t b = i & 1u;
                 if (!mbar_wait<kSuspendNs>(&bars[kKFull + b], (i >> 1) & 1u, abort_flag)) return false;
                 tc_fence_after();
-                for (uint32_t k = 0; k < steps; ++k) {
-                    const uint64_t da = make_smem_desc(sq + (k >> 2) * (kRows * 128u) + (k & 3u) * 32u, 16, 1024);
-                    const uint64_t db = make_smem_desc(sk + b * kKV + (k >> 2) * (kKeys * 128u) + (k & 3u) * 32u, 16, 1024);
-                    umma_f16(tmem + b * kKeys, da, db, idesc_s, k > 0 ? 1u : 0u);
+                for (int x = 0; x < nb; ++x) {
+                    const uint32_t d = tmem + x * 256u + ((bn[x] + ahead) & 1u) * kKeys;
+                    for (uint32_t k = 0; k < steps; ++k) {
+                        const uint64_t da = make_smem_desc(sq + x * kQ + (k >> 2) * (kRows * 128u) + (k & 3u) * 32u, 16, 1024);
+                        const uint64_t db = make_smem_desc(sk + b * kKV + (k >> 2) * (kKeys * 128u) + (k & 3u) * 32u, 16, 1024);
+                        umma_f16(d, da, db, idesc_s, k > 0 ? 1u : 0u);
+                    }
+                    if (x + 1 == nb) umma_commit(&bars[kKEmpty + b]);
+                    umma_commit(&bars[kBlock + x * kBlockBars + kSFull + ((bn[x] + ahead) & 1u)]);
                 }
-                umma_commit(&bars[kKEmpty + b]);
-                umma_commit(&bars[kSFull + b]);
                 return true;
             };
             while (ok && walk.next(g)) {
                 const uint32_t tiles = (uint32_t) (g.t1 - g.t0);
-                if (!(ok = mbar_wait<kSuspendNs>(&bars[kQFull], seg & 1u, abort_flag)) || !(ok = issue_s(n))) break;
-                ++seg;
-                for (uint32_t j = 0; j < tiles; ++j, ++n) {
-                    const uint32_t b = n & 1u, ph = (n >> 1) & 1u;
-                    if (j + 1 < tiles && !(ok = issue_s(n + 1))) break;
-                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kVFull + b], ph, abort_flag))) break;
-                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kWFull + b], ph, abort_flag))) break;
-                    tc_fence_after();
+                const int nb = second(g) ? 2 : 1;
+                for (int x = 0; ok && x < nb; ++x) ok = mbar_wait<kSuspendNs>(&bars[kBlock + x * kBlockBars + kQFull], bseg[x]++ & 1u, abort_flag);
+                if (!ok || !(ok = issue_s(n, 0, nb))) break;
+                for (uint32_t j = 0; ok && j < tiles; ++j, ++n) {
+                    const uint32_t b = n & 1u;
+                    if (j + 1 < tiles && !(ok = issue_s(n + 1, 1, nb))) break;
+                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kVFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    for (int x = 0; x < nb; ++x) {
+                        uint64_t *own = bars + kBlock + x * kBlockBars;
+                        const uint32_t sb = bn[x] & 1u;
+                        if (!(ok = mbar_wait<kSuspendNs>(&own[kWFull + sb], (bn[x] >> 1) & 1u, abort_flag))) break;
+                        tc_fence_after();
 #pragma unroll
-                    for (uint32_t k = 0; k < kKeys / 16; ++k) {
-                        const uint64_t db = make_smem_desc(sv + b * kKV + k * 2048u, kKeys * 128u, 1024);
-                        umma_f16_ts(tmem + 2 * kKeys, tmem + b * kKeys + k * 8u, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                        for (uint32_t k = 0; k < kKeys / 16; ++k) {
+                            const uint64_t db = make_smem_desc(sv + b * kKV + k * 2048u, kKeys * 128u, 1024);
+                            umma_f16_ts(tmem + x * 256u + 2 * kKeys, tmem + x * 256u + sb * kKeys + k * 8u, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                        }
+                        if (x + 1 == nb) umma_commit(&bars[kVEmpty + b]);
+                        umma_commit(&own[kPvDone + sb]);
+                        ++bn[x];
                     }
-                    umma_commit(&bars[kVEmpty + b]);
-                    umma_commit(&bars[kPvDone + b]);
                 }
             }
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp >= 4 * kNB) {
         // ------------------------------------------------------------ codes to fp16
-        if (DHC <= 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(convert_regs(kNB)));
         constexpr int kGroups = DHC / 64;// 4 lanes take 64 bytes of a row; 8 rows per warp and load
-        const uint32_t c = threadIdx.x - kSoftmax, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
+        const uint32_t c = threadIdx.x - 128 * kNB, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
         // tile that is loaded next
         bool more = walk.next(g);
         int32_t tile = g.t0;
@@ -433,108 +468,122 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
         }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: a thread per row
-        if (DHC <= 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const uint32_t r = threadIdx.x, t_lane = tmem + ((warp * 32u) << 16);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(kNB)));
+        const uint32_t blk = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;// row of the block
+        const uint32_t t_lane = tmem + blk * 256u + ((quarter * 32u) << 16), myq = sq + blk * kQ;
+        uint64_t *own = bars + kBlock + blk * kBlockBars;
         CtaMeta meta{-1, 0, 0, 0};
         bool ok = true;
-        uint32_t n = 0;
+        uint32_t n_all = 0, n = 0;// tiles of the stretch, and of them this block's
         while (ok && walk.next(g)) {
+            if (blk == 1 && !second(g)) {
+                n_all += (uint32_t) (g.t1 - g.t0);
+                continue;
+            }
             const Seq s = g.s;
-            const uint32_t rr = (uint32_t) g.rb * kRows + r;
-            const bool have = rr < (uint32_t) s.n * (uint32_t) p.group;
-            const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0, hd = have ? (int32_t) rr - tok * p.group : 0;
+            const uint32_t rows = (uint32_t) s.n * (uint32_t) p.group, rr0 = (uint32_t) g.rb * kItemRows + blk * kRows;// first row of the block
+            const uint32_t rr = rr0 + r;
+            const bool have = rr < rows;
+            const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0;
             const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
-            float rf;
+            float rf = 0.f;
             {
-                // q: the row's largest magnitude, then its elements times a power of two (and the sign of the scale, so
-                // that the factor of the scores is not negative) into swizzled shared memory.  Every product of the item
-                // before has completed: its last S was waited for.
-                const uint16_t *q = p.q + (int64_t) (s.first + tok) * p.q_st + (int64_t) (g.kvh * p.group + hd) * p.q_sh;
-                auto load8 = [&](int32_t d) -> uint4 {
-                    if (!have || d >= p.c.dh) return make_uint4(0u, 0u, 0u, 0u);
-                    if (p.q_vec && d + 8 <= p.c.dh) return *reinterpret_cast<const uint4 *>(q + d);
-                    uint32_t w[4];
+                // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes: the row's largest
+                // magnitude, then its elements times a power of two (and the sign of the scale, so that the factor of
+                // the scores is not negative) into swizzled shared memory.  Every product of the item before is done.
+                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 4;// lanes per row, rows per load
+                const int32_t d = (int32_t) (lane % kPer) * 8;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
+                    uint4 w[kBatch];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        w[i] = (uint32_t) (d + 2 * i < p.c.dh ? q[d + 2 * i] : 0) | ((uint32_t) (d + 2 * i + 1 < p.c.dh ? q[d + 2 * i + 1] : 0) << 16);
-                    }
-                    return make_uint4(w[0], w[1], w[2], w[3]);
-                };
-                uint32_t top = 0;
-#pragma unroll 4
-                for (int32_t d = 0; d < p.c.dh; d += 8) {
-                    const uint4 w = load8(d);
-                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
-                }
-                top = max(top & 0xFFFFu, top >> 16);
-                const int32_t shift = query_shift(p.bf16, top);
-                const float up = copysignf(__uint_as_float(pow2_bits(shift)), p.scale_log2);
-                rf = __uint_as_float(pow2_bits(-shift)) * fabsf(p.scale_log2);
-#pragma unroll 4
-                for (int32_t d = 0; d < p.c.dh; d += 8) {
-                    const uint4 w = load8(d);
-                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                    for (int i = 0; i < kBatch; ++i) {
+                        const uint32_t row = rr0 + quarter * 32u + (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
+                        w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (row < rows && d < p.c.dh) {
+                            const int32_t tk = (int32_t) p.group_div.div(row), hd = (int32_t) row - tk * p.group;
+                            const uint16_t *q = p.q + (int64_t) (s.first + tk) * p.q_st + (int64_t) (g.kvh * p.group + hd) * p.q_sh + d;
+                            if (p.q_vec && d + 8 <= p.c.dh) {
+                                w[i] = *reinterpret_cast<const uint4 *>(q);
+                            } else {
+                                uint32_t e[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = p.bf16 ? unpack2_t<kBF16>(x[i]) : unpack2(x[i]);
-                        x[i] = round16x2(false, f.x * up, f.y * up);
+                                for (int j = 0; j < 8; ++j) e[j] = d + j < p.c.dh ? q[j] : 0u;
+                                w[i] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+                            }
+                        }
                     }
-                    const uint32_t at = sq + ((uint32_t) d >> 6) * (kRows * 128u) + r * 128u + (((((uint32_t) d >> 3) & 7u) ^ (r & 7u)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        uint32_t top = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
+                        top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+                        for (int o = 1; o < kPer; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int32_t shift = query_shift(p.bf16, top);
+                        const float up = copysignf(__uint_as_float(pow2_bits(shift)), p.scale_log2);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = p.bf16 ? unpack2_t<kBF16>(x[j]) : unpack2(x[j]);
+                            x[j] = round16x2(false, f.x * up, f.y * up);
+                        }
+                        const uint32_t br = quarter * 32u + (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
+                        if (d < p.c.dh) {
+                            const uint32_t at = myq + ((uint32_t) d >> 6) * (kRows * 128u) + br * 128u + (((((uint32_t) d >> 3) & 7u) ^ (br & 7u)) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                        }
+                        // the factor of row (i0 + i) * kAtOnce + .. to the lane that owns the row
+                        const int32_t its = __shfl_sync(0xffffffffu, shift, (int) (lane % kAtOnce) * kPer);
+                        if ((int) (lane / kAtOnce) == i0 + i) rf = __uint_as_float(pow2_bits(-its)) * fabsf(p.scale_log2);
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&bars[kQFull]);
+                mbar_arrive(&own[kQFull]);
             }
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
 #pragma unroll 1
-            for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n) {
+            for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
                 const uint32_t b = n & 1u;
-                const TileScales &sc = scales[n % kScaleSets];
-                if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n % kScaleSets], (n / kScaleSets) & 1u, abort_flag))) break;
-                if (!(ok = mbar_wait<kSuspendNs>(&bars[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                const TileScales &sc = scales[n_all % kScaleSets];
+                if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                // (after S: a block that sat out items may be ahead by more than a parity can tell)
+                if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
                 tc_fence_after();
                 __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
                 // Scores are x * f; where the tile hides something from a row of this warp, x is the score itself and
-                // f is 1.  The 64 scores pass through 32 registers: half 0 for its maximum, half 1 for its maximum and
-                // its weights, half 0 again for its weights.
-                float x[32];
+                // f is 1.
+                float x[kKeys];
+                tmem_ld32(t_lane + b * kKeys, x);
+                tmem_ld32(t_lane + b * kKeys + 32, x + 32);
                 float f = ONE ? sc.ks[0] * rf : 1.f;
-                const uint32_t mask[2] = {sc.mask[0], sc.mask[1]};
-                const bool hidden = __any_sync(0xffffffffu, (mask[0] & mask[1]) != 0xFFFFFFFFu || (have && (int64_t) tile * kKeys + kKeys > limit));
-                auto load_scores = [&](int half, float &lane_wtop) {
-                    tmem_ld32(t_lane + b * kKeys + half * 32, x);
-                    if (!ONE) {
+                if (!ONE) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] *= sc.ks[half * 32 + i] * rf;
-                    }
-                    if (hidden) {
-                        const int32_t left = limit - tile * kKeys - half * 32;
+                    for (int i = 0; i < kKeys; ++i) x[i] *= sc.ks[i] * rf;
+                }
+                const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
+                const int32_t left = limit - tile * kKeys;// (rows that do not exist see nothing)
+                if (__any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && left < kKeys))) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = ((mask[half] >> i) & 1u) && i < left ? (ONE ? x[i] * f : x[i]) : -INFINITY;
-                    }
-                    if (!ONE) {
+                    for (int i = 0; i < kKeys; ++i) x[i] = (((i < 32 ? m0 : m1) >> (i & 31)) & 1u) && i < left ? x[i] * f : -INFINITY;
+                    f = 1.f;
+                }
+                float t4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) lane_wtop = fmaxf(lane_wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[half * 32 + i]);
-                    }
-                };
-                auto largest = [&]() -> float {
-                    float t4[4] = {x[0], x[1], x[2], x[3]};
+                for (int i = 4; i < kKeys - 4; i += 8) {
 #pragma unroll
-                    for (int i = 4; i < 28; i += 8) {
+                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]);
+                }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]);
-                    }
+                for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], x[kKeys - 4 + j]);
+                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f;
+                float wtop;
+                if (ONE) {
+                    wtop = top + sc.lv[0];
+                } else {
+                    wtop = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], x[28 + j]);
-                    return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                };
-                float wtop = -INFINITY;
-                load_scores(0, wtop);
-                float top = largest();
-                load_scores(1, wtop);
-                if (ONE && hidden) f = 1.f;
-                top = fmaxf(top, largest()) * f;
-                if (ONE) wtop = top + sc.lv[0];
+                    for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
+                }
                 // references
                 if (top > m + kSlack || (m == -INFINITY && top > m)) {
                     l *= fast_exp2(m - top);// (from -inf: 0)
@@ -545,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
                 if (up) wm = wtop;
                 if (__any_sync(0xffffffffu, up) && tile > g.t0) {
                     // O so far: every product into it must have completed
-                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
                     tc_fence_after();
                     __syncwarp();
                     for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
@@ -559,68 +608,80 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
                 }
                 const float mm = m == -INFINITY ? 0.f : m, ww = wm == -INFINITY ? 0.f : wm;
                 const float e = ONE ? fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : sc.lv[0]), kLeast) : mm - ww + kLift;
-                float sum = 0.f;
-                auto weigh = [&](int half, uint32_t (&w)[16]) {
-                    if (ONE) {
-                        const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
-                        uint64_t part[2] = {0ull, 0ull};
+                uint32_t w[kKeys / 2];
+                if (ONE) {
+                    const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
+                    uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
-                            const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
-                            part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
-                            w[i] = round16x2(false, y0, y1);
-                        }
-                        const float2 t = unpack2f(add2(part[0], part[1]));
-                        sum += t.x + t.y;
-                    } else {
-                        // pages that end inside the tile: a factor per key, so p and w take an exponential each
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float a0 = x[2 * i] - mm, a1 = x[2 * i + 1] - mm;
-                            sum += fast_exp2(a0) + fast_exp2(a1);
-                            w[i] = round16x2(false, a0 == -INFINITY ? 0.f : fast_exp2(a0 + (e + sc.lv[half * 32 + 2 * i])),
-                                             a1 == -INFINITY ? 0.f : fast_exp2(a1 + (e + sc.lv[half * 32 + 2 * i + 1])));
-                        }
+                    for (int i = 0; i < kKeys / 2; ++i) {
+                        const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
+                        const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
+                        part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
+                        w[i] = round16x2(false, y0, y1);
                     }
-                };
-                uint32_t w0[16], w1[16];
-                weigh(1, w1);
+                    const float2 sum = unpack2f(add2(part[0], part[1]));
+                    l = fmaf(sum.x + sum.y, fast_exp2(-e), l);
+                } else {
+                    // pages that end inside the tile: a factor per key, so p and w take an exponential each
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kKeys / 2; ++i) {
+                        const float a0 = x[2 * i] - mm, a1 = x[2 * i + 1] - mm;
+                        sum += fast_exp2(a0) + fast_exp2(a1);
+                        w[i] = round16x2(false, a0 == -INFINITY ? 0.f : fast_exp2(a0 + (e + sc.lv[2 * i])),
+                                         a1 == -INFINITY ? 0.f : fast_exp2(a1 + (e + sc.lv[2 * i + 1])));
+                    }
+                    l += sum;
+                }
                 __syncwarp();
-                if (ONE) f = sc.ks[0] * rf;// (load_scores applies it again where something is hidden)
-                load_scores(0, wtop);
-                if (ONE && hidden) f = 1.f;
-                tmem_st16(t_lane + b * kKeys + 16, w1);// (over scores that are read)
-                weigh(0, w0);
-                __syncwarp();
-                tmem_st16(t_lane + b * kKeys, w0);
-                l = ONE ? fmaf(sum, fast_exp2(-e), l) : l + sum;
+                tmem_st32(t_lane + b * kKeys, w);
                 tc_fence_before();
-                mbar_arrive(&bars[kWFull + b]);
+                mbar_arrive(&own[kWFull + b]);
             }
             if (!ok) break;
             // ---- the item's output, or its part
-            if (!(ok = mbar_wait<kSuspendNs>(&bars[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+            if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
             const bool whole = g.t0 == 0 && g.t1 == g.tiles;
             const int part = g.t0 > 0 ? 0 : 1;
-            const int64_t at = ((int64_t) blockIdx.x * 2 + part) * kRows + r;
-            uint16_t *out = p.out + (int64_t) (s.first + tok) * p.o_st + (int64_t) (g.kvh * p.group + hd) * p.o_sh;
+            const int64_t at0 = ((int64_t) blockIdx.x * 2 + part) * kItemRows + blk * kRows + quarter * 32u;// this warp's first row
+            const float2 mine = out_factors(l, wm - kLift - m);
             const bool none = wm == -INFINITY;// (O holds products with weights of zero)
+            // 32 columns at a time through this warp's part of q's memory (16-byte pieces rotated by the row), so that a
+            // row's pieces leave side by side
+            const uint32_t stage = myq + quarter * 32u * 128u;
             for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
                 float o[32];
                 __syncwarp();
-                tmem_ld32(t_lane + 2 * kKeys + c0, o);// every lane takes part
+                tmem_ld32(t_lane + 2 * kKeys + c0, o);
 #pragma unroll
-                for (int i = 0; have && i < 32; i += 4) {
-                    float4 y = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    if (none) y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (whole) store_out(p, out, c0 + i, y, l, wm - kLift - m);
-                    else *reinterpret_cast<float4 *>(sp.parts + at * DHC + c0 + i) = y;
+                for (int i = 0; i < 8; ++i) {
+                    if (none) o[4 * i] = o[4 * i + 1] = o[4 * i + 2] = o[4 * i + 3] = 0.f;
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128u + (((uint32_t) i ^ (lane & 7u)) << 4)),
+                                 "f"(o[4 * i]), "f"(o[4 * i + 1]), "f"(o[4 * i + 2]), "f"(o[4 * i + 3]) : "memory");
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t wr = (uint32_t) i * 4u + (lane >> 3), piece = lane & 7u;// row of the warp
+                    float4 y;
+                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                                 : "r"(stage + wr * 128u + ((piece ^ (wr & 7u)) << 4)) : "memory");
+                    const float2 f = make_float2(__shfl_sync(0xffffffffu, mine.x, (int) wr), __shfl_sync(0xffffffffu, mine.y, (int) wr));
+                    const uint32_t row = rr0 + quarter * 32u + wr;
+                    if (row < rows) {
+                        if (whole) store_out(p, row_of_out(p, s, g.kvh, row), c0 + (int32_t) piece * 4, y, f);
+                        else *reinterpret_cast<float4 *>(sp.parts + (at0 + wr) * DHC + c0 + piece * 4) = y;
+                    }
                 }
             }
-            if (!whole && have) sp.heads[at] = PartHead{m, l, wm - kLift, 0.f};
-            if (!whole && part == 1) meta = CtaMeta{g.b, g.kvh, g.rb, (int32_t) divide(g.u + g.tiles - 1, each)};
+            __syncwarp();
+            if (p.c.dh < DHC) {// the zeros beyond dh in q's rows were written over
+                for (uint32_t i = lane * 16; i < 32 * 128; i += 512) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(stage + i), "r"(0) : "memory");
+                __syncwarp();
+            }
+            if (!whole && have) sp.heads[at0 + lane] = PartHead{m, l, wm - kLift, 0.f};
+            if (!whole && part == 1) meta = CtaMeta{g.b, g.kvh, g.rb, (int32_t) divide(g.last_unit, each)};
             tc_fence_before();
         }
         if (threadIdx.x == 0) sp.meta[blockIdx.x] = meta;
@@ -629,9 +690,9 @@ __global__ void __launch_bounds__(kThreads, DHC <= 128 ? 2 : 1) prefill_kernel(c
     tc_fence_before();
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;");
-    if (warp == 8) {
+    if (warp == kWarps - 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, tmem_cols(DHC));
+        tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -645,14 +706,14 @@ cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaS
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    prefill_kernel<DHC, ONE><<<ctas, kThreads, smem_bytes(DHC), st>>>(sp);
+    prefill_kernel<DHC, ONE><<<ctas, threads_of(blocks_at_once(DHC)), smem_bytes(DHC), st>>>(sp);
     e = cudaGetLastError();
     if (e != cudaSuccess || ctas == 1) return e;
-    return launch_join<DHC, kRows>(sp, ctas, st);
+    return launch_join<DHC, blocks_at_once(DHC) * kRows>(sp, ctas, st);
 }
 template<int DHC>
 cudaError_t launch(const AttendParams &a, void *workspace, uint32_t ctas, int device_id, cudaStream_t st) {
-    const SplitParams sp = split_params(a, workspace, ctas, kRows, DHC);
+    const SplitParams sp = split_params(a, workspace, ctas, (uint64_t) prefill_rows(DHC), DHC);
     return a.vec && a.c.page % kKeys == 0 ? launch_as<DHC, true>(sp, ctas, device_id, st) : launch_as<DHC, false>(sp, ctas, device_id, st);
 }
 

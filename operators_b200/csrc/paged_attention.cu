@@ -733,6 +733,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     for (int64_t s : {d->c.k.sn, d->c.k.sh, d->c.k.sp, d->c.v.sn, d->c.v.sh, d->c.v.sp}) p.vec = p.vec && s % 16 == 0;
     p.q_vec = aligned16(q) && d->q_st % 8 == 0 && d->q_sh % 8 == 0;
     p.o_vec = (uintptr_t) out % 8 == 0 && d->o_st % 4 == 0 && d->o_sh % 4 == 0 && d->c.dh % 4 == 0;
+    p.o_vec8 = aligned16(out) && d->o_st % 8 == 0 && d->o_sh % 8 == 0 && d->c.dh % 8 == 0;
     auto st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (d->block >= 128) {

@@ -15,7 +15,7 @@ struct AttendParams {
     const int32_t *table, *lens, *offs;
     int32_t rows, group;
     float scale_log2;// scale * log2(e)
-    bool bf16, vec, q_vec, o_vec;
+    bool bf16, vec, q_vec, o_vec, o_vec8;// whole vectors: 16 bytes of codes, q and out, 8 bytes of out
     FastDiv page_div, group_div;// by the page size and by the q heads per kv head
     CacheShape c;
     TableShape t;

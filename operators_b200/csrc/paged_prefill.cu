@@ -101,14 +101,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
           "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// 16 columns of this warp's 32 lanes
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+// 64 columns of this warp's 32 lanes; the load and its wait are one statement
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float *v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
-        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n\t"
-        "tcgen05.wait::st.sync.aligned;"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+        : "r"(taddr)
         : "memory");
 }
 // two fp32 operations per instruction
@@ -290,8 +289,11 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     if (warp == kWarps - 1) {
         // ------------------------------------------------------------ products
         if (lane == 0) {
+            // One thread issues two dozen products per tile, so each may cost it a few instructions only: the descriptors
+            // of a tile's start are kept, a product adds its constant offset (>> 4, as the descriptors count).
             const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
             const uint32_t idesc_s = make_idesc(kRows, kKeys, 0, 0), idesc_o = make_idesc(kRows, steps * 16, 0, 1);
+            const uint64_t dq = make_smem_desc(sq, 16, 1024), dk = make_smem_desc(sk, 16, 1024), dv = make_smem_desc(sv, kKeys * 128u, 1024);
             bool ok = true;
             uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
             // S of the n-th tile for the active blocks
@@ -299,15 +301,23 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 const uint32_t b = i & 1u;
                 if (!mbar_wait<kSuspendNs>(&bars[kKFull + b], (i >> 1) & 1u, abort_flag)) return false;
                 tc_fence_after();
-                for (int x = 0; x < nb; ++x) {
-                    const uint32_t d = tmem + x * 256u + ((bn[x] + ahead) & 1u) * kKeys;
-                    for (uint32_t k = 0; k < steps; ++k) {
-                        const uint64_t da = make_smem_desc(sq + x * kQ + (k >> 2) * (kRows * 128u) + (k & 3u) * 32u, 16, 1024);
-                        const uint64_t db = make_smem_desc(sk + b * kKV + (k >> 2) * (kKeys * 128u) + (k & 3u) * 32u, 16, 1024);
-                        umma_f16(d, da, db, idesc_s, k > 0 ? 1u : 0u);
+                const uint64_t db = dk + b * (kKV >> 4);
+#pragma unroll
+                for (int x = 0; x < kNB; ++x) {
+                    if (x >= nb) break;
+                    const uint32_t sb = (bn[x] + ahead) & 1u;
+                    // 64 elements (four products) at a time; unrolled no further: with all 16 products of head size 256 in
+                    // a row the compiled code issued wrong descriptors (scores of mismatched elements)
+#pragma unroll 1
+                    for (uint32_t box = 0; box * 4 < steps; ++box) {
+                        const uint64_t dqb = dq + ((x * kQ + box * (kRows * 128u)) >> 4), dkb = db + ((box * (kKeys * 128u)) >> 4);
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            if (box * 4 + k < steps) umma_f16(tmem + x * 256u + sb * kKeys, dqb + 2 * k, dkb + 2 * k, idesc_s, (box | k) > 0 ? 1u : 0u);
+                        }
                     }
                     if (x + 1 == nb) umma_commit(&bars[kKEmpty + b]);
-                    umma_commit(&bars[kBlock + x * kBlockBars + kSFull + ((bn[x] + ahead) & 1u)]);
+                    umma_commit(&bars[kBlock + x * kBlockBars + kSFull + sb]);
                 }
                 return true;
             };
@@ -320,15 +330,18 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const uint32_t b = n & 1u;
                     if (j + 1 < tiles && !(ok = issue_s(n + 1, 1, nb))) break;
                     if (!(ok = mbar_wait<kSuspendNs>(&bars[kVFull + b], (n >> 1) & 1u, abort_flag))) break;
-                    for (int x = 0; x < nb; ++x) {
+                    const uint64_t db = dv + b * (kKV >> 4);
+#pragma unroll
+                    for (int x = 0; x < kNB; ++x) {
+                        if (x >= nb) break;
                         uint64_t *own = bars + kBlock + x * kBlockBars;
                         const uint32_t sb = bn[x] & 1u;
                         if (!(ok = mbar_wait<kSuspendNs>(&own[kWFull + sb], (bn[x] >> 1) & 1u, abort_flag))) break;
                         tc_fence_after();
 #pragma unroll
                         for (uint32_t k = 0; k < kKeys / 16; ++k) {
-                            const uint64_t db = make_smem_desc(sv + b * kKV + k * 2048u, kKeys * 128u, 1024);
-                            umma_f16_ts(tmem + x * 256u + 2 * kKeys, tmem + x * 256u + sb * kKeys + k * 8u, db, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                            umma_f16_ts(tmem + x * 256u + 2 * kKeys, tmem + x * 256u + sb * kKeys + k * 8u, db + k * (2048u >> 4), idesc_o,
+                                        (j > 0 || k > 0) ? 1u : 0u);
                         }
                         if (x + 1 == nb) umma_commit(&bars[kVEmpty + b]);
                         umma_commit(&own[kPvDone + sb]);
@@ -343,36 +356,26 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(convert_regs(kNB)));
         constexpr int kGroups = DHC / 64;// 4 lanes take 64 bytes of a row; 8 rows per warp and load
         const uint32_t c = threadIdx.x - 128 * kNB, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
-        // tile that is loaded next
+        // Three tiles are in flight here: one whose codes are in registers, the next one, whose page ids are (`cur`), and
+        // the one after, whose ids are being read (`fut`): the ids' latency, the codes' and the conversion overlap.
+        struct Ids {
+            const int32_t *row;// of the block table
+            int32_t id[3];     // pages of this thread's two rows and of its key (one page per tile: [0] only)
+            int32_t tile, keys, kvh;
+            bool some;
+        };
         bool more = walk.next(g);
-        int32_t tile = g.t0;
-        auto advance = [&]() {
+        int32_t tile = more ? g.t0 : 0;
+        auto read_ids = [&](Ids &x) {
+            x.some = more;
+            if (!more) return;
+            x.tile = tile, x.keys = held(g.s.len, p.t.cap), x.kvh = g.kvh, x.row = p.table + (int64_t) g.b * p.t.stride;
+            const int32_t tok[3] = {tile * kKeys + (ONE ? 0 : (int32_t) r0), tile * kKeys + (int32_t) r0 + 32, tile * kKeys + (int32_t) (c % kKeys)};
+#pragma unroll
+            for (int i = 0; i < (ONE ? 1 : 3); ++i) x.id[i] = tok[i] < x.keys ? x.row[p.page_div.div((uint32_t) tok[i])] : -1;
             if (++tile >= g.t1 && (more = walk.next(g))) tile = g.t0;
         };
-        struct Ids {
-            int32_t row[2], key;// pages of this thread's two rows and of the key whose scales it loads (one page: the tile's); -1: none
-            bool has;           // this thread's key exists
-        };
-        auto page_of = [&](int32_t tok) -> int32_t {
-            if (tok >= held(g.s.len, p.t.cap)) return -1;
-            const int32_t id = p.table[(int64_t) g.b * p.t.stride + (int32_t) p.page_div.div((uint32_t) tok)];
-            return id >= 0 && id < p.c.pages ? id : -1;
-        };
-        auto ids_of = [&](Ids &x) {
-            x.row[0] = x.row[1] = x.key = -1, x.has = false;
-            if (!more) return;
-            const int32_t tok = tile * kKeys;
-            if (ONE) {
-                const int32_t id = page_of(tok), left = held(g.s.len, p.t.cap) - tok;
-                x.row[0] = (int32_t) r0 < left ? id : -1;
-                x.row[1] = (int32_t) r0 + 32 < left ? id : -1;
-                x.key = id, x.has = id >= 0 && (int32_t) c < left;
-            } else {
-                x.row[0] = page_of(tok + (int32_t) r0);
-                x.row[1] = page_of(tok + (int32_t) r0 + 32);
-                if (c < kKeys) x.key = page_of(tok + (int32_t) c), x.has = x.key >= 0;
-            }
-        };
+        auto in_pool = [&](int32_t id) { return id >= 0 && id < p.c.pages; };
         uint4 kd[2][kGroups], vd[2][kGroups];
         float ks = 0.f, vs = 0.f;
         bool key_ok = false;
@@ -386,17 +389,20 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             return make_uint4(w[0], w[1], w[2], w[3]);
         };
         auto load_tile = [&](const Ids &x, const PoolStrides &st, const uint8_t *pool, uint4 (&to)[2][kGroups]) {
+            const int32_t tok = x.tile * kKeys + (int32_t) r0;
             const uint8_t *at[2];
-            const int32_t tok = tile * kKeys + (int32_t) r0;
+            bool ok[2];
             if (ONE) {
                 const int32_t in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
-                at[0] = pool + (int64_t) max(x.key, 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp + c4 * 16;
+                ok[0] = x.some && in_pool(x.id[0]) && tok < x.keys, ok[1] = ok[0] && tok + 32 < x.keys;
+                at[0] = pool + (ok[0] ? (int64_t) x.id[0] * st.sn + (int64_t) x.kvh * st.sh + (int64_t) in_page * st.sp : 0) + c4 * 16;
                 at[1] = at[0] + 32 * st.sp;
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int32_t in_page = tok + 32 * i - (int32_t) p.page_div.div((uint32_t) (tok + 32 * i)) * p.c.page;
-                    at[i] = pool + (int64_t) max(x.row[i], 0) * st.sn + (int64_t) g.kvh * st.sh + (int64_t) in_page * st.sp + c4 * 16;
+                    ok[i] = x.some && in_pool(x.id[i]);
+                    at[i] = pool + (ok[i] ? (int64_t) x.id[i] * st.sn + (int64_t) x.kvh * st.sh + (int64_t) in_page * st.sp : 0) + c4 * 16;
                 }
             }
 #pragma unroll
@@ -405,16 +411,17 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 for (int q = 0; q < kGroups; ++q) {
                     const int32_t d0 = (q * 4 + (int32_t) c4) * 16;
                     to[i][q] = make_uint4(0u, 0u, 0u, 0u);
-                    if (x.row[i] >= 0 && d0 < p.c.dh) to[i][q] = ONE || p.vec ? *reinterpret_cast<const uint4 *>(at[i] + q * 64) : load16(at[i] + q * 64, d0);
+                    if (ok[i] && d0 < p.c.dh) to[i][q] = ONE || p.vec ? *reinterpret_cast<const uint4 *>(at[i] + q * 64) : load16(at[i] + q * 64, d0);
                 }
             }
         };
         auto load_scales = [&](const Ids &x) {
-            key_ok = x.has;
+            const int32_t id = x.id[ONE ? 0 : 2], key = (int32_t) (c % kKeys);
+            key_ok = x.some && in_pool(id) && x.tile * kKeys + key < x.keys;
             ks = vs = 0.f;
-            if (key_ok && c < (ONE ? 1u : (uint32_t) kKeys)) {
-                ks = p.ks[(int64_t) x.key * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch];
-                vs = p.vs[(int64_t) x.key * p.c.v.cn + (int64_t) g.kvh * p.c.v.ch];
+            if (ONE ? x.some && in_pool(id) && c == 0 : key_ok && c < kKeys) {
+                ks = p.ks[(int64_t) id * p.c.k.cn + (int64_t) x.kvh * p.c.k.ch];
+                vs = p.vs[(int64_t) id * p.c.v.cn + (int64_t) x.kvh * p.c.v.ch];
             }
         };
         // rows as TMA with 128-byte swizzle would lay them: 16-byte chunk j of row r at j ^ (r & 7)
@@ -436,35 +443,36 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");// the products read through the async proxy
         };
-        Ids ids;
-        ids_of(ids);
-        load_tile(ids, p.c.k, p.kp, kd);
-        load_tile(ids, p.c.v, p.vp, vd);
-        load_scales(ids);
-        bool ok = true;
-        for (uint32_t n = 0; more; ++n) {
+        Ids cur, fut;
+        read_ids(cur);
+        load_tile(cur, p.c.k, p.kp, kd);
+        load_tile(cur, p.c.v, p.vp, vd);
+        load_scales(cur);
+        bool have = cur.some, ok = true;
+        read_ids(cur);
+        for (uint32_t n = 0; have; ++n) {
             const uint32_t b = n & 1u, ph = ((n >> 1) & 1u) ^ 1u;
-            // scales of this tile, ids of the next
+            read_ids(fut);
+            if (!(ok = mbar_wait<kSuspendNs>(&bars[kKEmpty + b], ph, abort_flag))) break;
+            // the scales go first: the rows that see K see them
             TileScales &sc = scales[n % kScaleSets];
             const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
-            const float lv = log2_of(vs);
             if (c < kKeys) {
+                const float lv = log2_of(vs);
                 if (!ONE || c == 0) sc.ks[c] = ks, sc.vs[c] = vs, sc.lv[c] = lv;
                 if (lane == 0) sc.mask[cw] = mask;
                 mbar_arrive(&bars[kScFull + n % kScaleSets]);
             }
-            advance();
-            Ids next;
-            ids_of(next);
-            if (!(ok = mbar_wait<kSuspendNs>(&bars[kKEmpty + b], ph, abort_flag))) break;
             store_tile(sk + b * kKV, kd);
             mbar_arrive(&bars[kKFull + b]);
-            load_tile(next, p.c.k, p.kp, kd);
-            load_scales(next);
+            load_tile(cur, p.c.k, p.kp, kd);
+            load_scales(cur);
             if (!(ok = mbar_wait<kSuspendNs>(&bars[kVEmpty + b], ph, abort_flag))) break;
             store_tile(sv + b * kKV, vd);
             mbar_arrive(&bars[kVFull + b]);
-            load_tile(next, p.c.v, p.vp, vd);
+            load_tile(cur, p.c.v, p.vp, vd);
+            have = cur.some;
+            cur = fut;
         }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: a thread per row
@@ -491,7 +499,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes: the row's largest
                 // magnitude, then its elements times a power of two (and the sign of the scale, so that the factor of
                 // the scores is not negative) into swizzled shared memory.  Every product of the item before is done.
-                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 4;// lanes per row, rows per load
+                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 32 / kAtOnce < 16 ? 32 / kAtOnce : 16;// lanes per row, rows per load, loads in flight
                 const int32_t d = (int32_t) (lane % kPer) * 8;
 #pragma unroll 1
                 for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
@@ -541,6 +549,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 mbar_arrive(&own[kQFull]);
             }
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
+            float e = 0.f, e_back = 1.f, lv_of_e = NAN;// exponent from p to w, 2^-e, and the scale (log2) that e is for
 #pragma unroll 1
             for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
                 const uint32_t b = n & 1u;
@@ -553,8 +562,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 // Scores are x * f; where the tile hides something from a row of this warp, x is the score itself and
                 // f is 1.
                 float x[kKeys];
-                tmem_ld32(t_lane + b * kKeys, x);
-                tmem_ld32(t_lane + b * kKeys + 32, x + 32);
+                tmem_ld64(t_lane + b * kKeys, x);
                 float f = ONE ? sc.ks[0] * rf : 1.f;
                 if (!ONE) {
 #pragma unroll
@@ -584,30 +592,39 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
                 }
-                // references
-                if (top > m + kSlack || (m == -INFINITY && top > m)) {
-                    l *= fast_exp2(m - top);// (from -inf: 0)
-                    m = top;
-                }
-                const bool up = wtop > wm + kSlack || (wm == -INFINITY && wtop > wm);
-                const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
-                if (up) wm = wtop;
-                if (__any_sync(0xffffffffu, up) && tile > g.t0) {
-                    // O so far: every product into it must have completed
-                    if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
-                    tc_fence_after();
-                    __syncwarp();
-                    for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
-                        float o[32];
-                        tmem_ld32(t_lane + 2 * kKeys + c0, o);
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
-                        tmem_st32(t_lane + 2 * kKeys + c0, w);
+                // references: moved when a score or a weight of a row of this warp exceeds its own by more than the slack
+                const bool up_m = top > m + kSlack || (m == -INFINITY && top > m), up = wtop > wm + kSlack || (wm == -INFINITY && wtop > wm);
+                if (__any_sync(0xffffffffu, up_m || up)) {
+                    if (up_m) {
+                        l *= fast_exp2(m - top);// (from -inf: 0)
+                        m = top;
                     }
+                    const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
+                    if (up) wm = wtop;
+                    if (tile > g.t0 && __any_sync(0xffffffffu, up)) {
+                        // O so far: every product into it must have completed
+                        if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+                        tc_fence_after();
+                        __syncwarp();
+                        for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
+                            float o[32];
+                            tmem_ld32(t_lane + 2 * kKeys + c0, o);
+                            uint32_t w[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
+                            tmem_st32(t_lane + 2 * kKeys + c0, w);
+                        }
+                    }
+                    lv_of_e = NAN;
                 }
-                const float mm = m == -INFINITY ? 0.f : m, ww = wm == -INFINITY ? 0.f : wm;
-                const float e = ONE ? fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : sc.lv[0]), kLeast) : mm - ww + kLift;
+                const float mm = m == -INFINITY ? 0.f : m;
+                const float lv = ONE ? sc.lv[0] : 0.f;
+                if (!(lv == lv_of_e)) {// (the references or the scale have changed)
+                    const float ww = wm == -INFINITY ? 0.f : wm;
+                    e = ONE ? fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : lv), kLeast) : mm - ww + kLift;
+                    e_back = fast_exp2(-e);
+                    lv_of_e = lv;
+                }
                 uint32_t w[kKeys / 2];
                 if (ONE) {
                     const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
@@ -620,7 +637,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         w[i] = round16x2(false, y0, y1);
                     }
                     const float2 sum = unpack2f(add2(part[0], part[1]));
-                    l = fmaf(sum.x + sum.y, fast_exp2(-e), l);
+                    l = fmaf(sum.x + sum.y, e_back, l);
                 } else {
                     // pages that end inside the tile: a factor per key, so p and w take an exponential each
                     float sum = 0.f;
@@ -645,33 +662,71 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const bool whole = g.t0 == 0 && g.t1 == g.tiles;
             const int part = g.t0 > 0 ? 0 : 1;
             const int64_t at0 = ((int64_t) blockIdx.x * 2 + part) * kItemRows + blk * kRows + quarter * 32u;// this warp's first row
-            const float2 mine = out_factors(l, wm - kLift - m);
             const bool none = wm == -INFINITY;// (O holds products with weights of zero)
-            // 32 columns at a time through this warp's part of q's memory (16-byte pieces rotated by the row), so that a
-            // row's pieces leave side by side
-            const uint32_t stage = myq + quarter * 32u * 128u;
-            for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
-                float o[32];
-                __syncwarp();
-                tmem_ld32(t_lane + 2 * kKeys + c0, o);
+            // Through this warp's part of q's memory (rows of 128 bytes, their 16-byte pieces rotated by the row), so that a
+            // row's pieces leave side by side: finished outputs 64 columns at a time, parts 32 columns in fp32.
+            const uint32_t stage = myq + quarter * 32u * 128u, piece = lane & 7u, sub = lane >> 3;
+            auto put = [&](uint32_t i, uint32_t a, uint32_t c, uint32_t d, uint32_t f) {
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128u + ((i ^ (lane & 7u)) << 4)), "r"(a), "r"(c), "r"(d), "r"(f) : "memory");
+            };
+            auto take = [&](uint32_t wr) -> uint4 {
+                uint4 y;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w) : "r"(stage + wr * 128u + ((piece ^ (wr & 7u)) << 4)) : "memory");
+                return y;
+            };
+            if (whole) {
+                const float2 fac = none ? make_float2(0.f, 0.f) : out_factors(l, wm - kLift - m);
+                for (int32_t c0 = 0; c0 < p.c.dh; c0 += 64) {
+                    float o[64];
+                    __syncwarp();
+                    tmem_ld64(t_lane + 2 * kKeys + c0, o);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (none) o[4 * i] = o[4 * i + 1] = o[4 * i + 2] = o[4 * i + 3] = 0.f;
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128u + (((uint32_t) i ^ (lane & 7u)) << 4)),
-                                 "f"(o[4 * i]), "f"(o[4 * i + 1]), "f"(o[4 * i + 2]), "f"(o[4 * i + 3]) : "memory");
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            const float y0 = o[8 * i + 2 * j], y1 = o[8 * i + 2 * j + 1];
+                            h[j] = fac.x == 0.f ? 0u : round16x2(p.bf16, y0 * fac.x * fac.y, y1 * fac.x * fac.y);
+                        }
+                        put(i, h[0], h[1], h[2], h[3]);
+                    }
+                    __syncwarp();
+                    const int32_t d = c0 + (int32_t) piece * 8;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint32_t wr = i * 4u + sub, row = rr0 + quarter * 32u + wr;
+                        const uint4 y = take(wr);
+                        if (row < rows && d < p.c.dh) {
+                            uint16_t *out = row_of_out(p, s, g.kvh, row) + d;
+                            if (p.o_vec8) {
+                                *reinterpret_cast<uint4 *>(out) = y;
+                            } else {
+                                const uint32_t h[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    if (d + j < p.c.dh) out[j] = (uint16_t) (h[j >> 1] >> (16 * (j & 1)));
+                                }
+                            }
+                        }
+                    }
                 }
-                __syncwarp();
+            } else {
+                float *parts = sp.parts + at0 * DHC;
+                for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
+                    float o[32];
+                    __syncwarp();
+                    tmem_ld32(t_lane + 2 * kKeys + c0, o);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t wr = (uint32_t) i * 4u + (lane >> 3), piece = lane & 7u;// row of the warp
-                    float4 y;
-                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
-                                 : "r"(stage + wr * 128u + ((piece ^ (wr & 7u)) << 4)) : "memory");
-                    const float2 f = make_float2(__shfl_sync(0xffffffffu, mine.x, (int) wr), __shfl_sync(0xffffffffu, mine.y, (int) wr));
-                    const uint32_t row = rr0 + quarter * 32u + wr;
-                    if (row < rows) {
-                        if (whole) store_out(p, row_of_out(p, s, g.kvh, row), c0 + (int32_t) piece * 4, y, f);
-                        else *reinterpret_cast<float4 *>(sp.parts + (at0 + wr) * DHC + c0 + piece * 4) = y;
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        if (none) o[4 * i] = o[4 * i + 1] = o[4 * i + 2] = o[4 * i + 3] = 0.f;
+                        put(i, __float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint32_t wr = i * 4u + sub;
+                        const uint4 y = take(wr);
+                        if (rr0 + quarter * 32u + wr < rows) *reinterpret_cast<uint4 *>(parts + wr * DHC + c0 + piece * 4u) = y;
                     }
                 }
             }

@@ -18,8 +18,8 @@
 // that one's exponentials run beside the other's products and both share the converted tiles.
 //
 // Roles (416 threads; 288 with one block): a warpgroup per block for softmax and epilogue, a thread per row; a
-// warpgroup converts codes (its loads run a tile ahead in registers); the last warp allocates TMEM, one lane issues the
-// products.  Shared memory: q, two tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is
+// warpgroup converts codes (its loads run a tile ahead in registers); the last warp allocates TMEM and issues the
+// products (the warp as one, see umma_f16_ss).  Shared memory: q, two tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is
 // double-buffered: S of tile j + 1 is issued before W v of tile j.
 //
 // Work is divided into equal stretches as in paged_attention.cu; an item is a pair of blocks, stops where its last row's
@@ -79,13 +79,39 @@ __host__ __device__ constexpr uint32_t tile_bytes(int dhc) { return (uint32_t) b
 __host__ __device__ constexpr uint32_t smem_bytes(int dhc) { return tile_bytes(dhc) + kScaleSets * (uint32_t) sizeof(TileScales) + kBars * 8 + 32; }
 static_assert(kPrefillMaxBatch * 8 <= tile_bytes(64), "the sequences' unit counts fit the tiles' memory");
 
-// D[tmem] (+)= A[tmem] * B[smem desc]: the rows of A are TMEM lanes, two fp16 elements per column
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// Products issued by a warp as a whole, the instruction itself by its elected lane: D[tmem] (+)= A * B[smem desc], A from
+// shared memory or from TMEM (rows are lanes, two fp16 elements per column).  Code that the compiler knows to be the same
+// in all lanes keeps descriptors in uniform registers; in a branch of one lane each product took 96 cycles to issue
+// whatever its size, here 48 (64 columns of B) and 64 (128 columns), the tensor core's own pace.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(lead));
+    return lead;
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint64_t *bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_u32(bar)), "r"(lead)
         : "memory");
 }
 // 32 columns of this warp's 32 lanes
@@ -198,7 +224,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kScaleSets);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     // ---- this CTA's stretch.  Units of a kv head of each sequence: a warp per sequence, a lane per item.
     int64_t *sums = reinterpret_cast<int64_t *>(smem);
@@ -288,65 +314,62 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
 
     if (warp == kWarps - 1) {
         // ------------------------------------------------------------ products
-        if (lane == 0) {
-            // One thread issues two dozen products per tile, so each may cost it a few instructions only: the descriptors
-            // of a tile's start are kept, a product adds its constant offset (>> 4, as the descriptors count).
-            const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
-            const uint32_t idesc_s = make_idesc(kRows, kKeys, 0, 0), idesc_o = make_idesc(kRows, steps * 16, 0, 1);
-            const uint64_t dq = make_smem_desc(sq, 16, 1024), dk = make_smem_desc(sk, 16, 1024), dv = make_smem_desc(sv, kKeys * 128u, 1024);
-            bool ok = true;
-            uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
-            // S of the n-th tile for the active blocks
-            auto issue_s = [&](uint32_t i, uint32_t ahead, int nb) -> bool {
-                const uint32_t b = i & 1u;
-                if (!mbar_wait<kSuspendNs>(&bars[kKFull + b], (i >> 1) & 1u, abort_flag)) return false;
-                tc_fence_after();
-                const uint64_t db = dk + b * (kKV >> 4);
+        // (the shuffles and votes tell the compiler what is the same in all lanes)
+        const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
+        const uint32_t idesc_s = make_idesc(kRows, kKeys, 0, 0), idesc_o = make_idesc(kRows, steps * 16, 0, 1);
+        const uint64_t dq = make_smem_desc(sq, 16, 1024), dk = make_smem_desc(sk, 16, 1024), dv = make_smem_desc(sv, kKeys * 128u, 1024);
+        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
+        auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+            const bool done = __all_sync(0xffffffffu, mbar_wait<kSuspendNs>(bar, parity, abort_flag));
+            tc_fence_after();
+            return done;
+        };
+        // S of the n-th tile for the active blocks
+        auto issue_s = [&](uint32_t i, uint32_t ahead, int nb) -> bool {
+            const uint32_t b = i & 1u;
+            if (!wait(&bars[kKFull + b], (i >> 1) & 1u)) return false;
+#pragma unroll
+            for (int x = 0; x < kNB; ++x) {
+                if (x >= nb) break;
+                const uint32_t sb = (bn[x] + ahead) & 1u;
+#pragma unroll 1
+                for (uint32_t box = 0; box * 4 < steps; ++box) {// 64 elements (four products) at a time
+                    const uint64_t dqb = dq + ((x * kQ + box * (kRows * 128u)) >> 4), dkb = dk + ((b * kKV + box * (kKeys * 128u)) >> 4);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        if (box * 4 + k < steps) umma_f16_ss(tm + x * 256u + sb * kKeys, dqb + 2 * k, dkb + 2 * k, idesc_s, (box | k) > 0 ? 1u : 0u, lead);
+                    }
+                }
+                if (x + 1 == nb) umma_commit_by(&bars[kKEmpty + b], lead);
+                umma_commit_by(&bars[kBlock + x * kBlockBars + kSFull + sb], lead);
+            }
+            return true;
+        };
+        bool ok = true;
+        while (ok && __any_sync(0xffffffffu, walk.next(g))) {
+            const uint32_t tiles = __shfl_sync(0xffffffffu, (uint32_t) (g.t1 - g.t0), 0);
+            const int nb = __any_sync(0xffffffffu, second(g)) ? 2 : 1;
+            for (int x = 0; ok && x < nb; ++x) ok = wait(&bars[kBlock + x * kBlockBars + kQFull], bseg[x]++ & 1u);
+            if (!ok || !(ok = issue_s(n, 0, nb))) break;
+            for (uint32_t j = 0; ok && j < tiles; ++j, ++n) {
+                const uint32_t b = n & 1u;
+                if (j + 1 < tiles && !(ok = issue_s(n + 1, 1, nb))) break;
+                if (!(ok = wait(&bars[kVFull + b], (n >> 1) & 1u))) break;
 #pragma unroll
                 for (int x = 0; x < kNB; ++x) {
                     if (x >= nb) break;
-                    const uint32_t sb = (bn[x] + ahead) & 1u;
-                    // 64 elements (four products) at a time; unrolled no further: with all 16 products of head size 256 in
-                    // a row the compiled code issued wrong descriptors (scores of mismatched elements)
-#pragma unroll 1
-                    for (uint32_t box = 0; box * 4 < steps; ++box) {
-                        const uint64_t dqb = dq + ((x * kQ + box * (kRows * 128u)) >> 4), dkb = db + ((box * (kKeys * 128u)) >> 4);
+                    uint64_t *own = bars + kBlock + x * kBlockBars;
+                    const uint32_t sb = bn[x] & 1u;
+                    if (!(ok = wait(&own[kWFull + sb], (bn[x] >> 1) & 1u))) break;
 #pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            if (box * 4 + k < steps) umma_f16(tmem + x * 256u + sb * kKeys, dqb + 2 * k, dkb + 2 * k, idesc_s, (box | k) > 0 ? 1u : 0u);
-                        }
+                    for (uint32_t k = 0; k < kKeys / 16; ++k) {
+                        umma_f16_ts(tm + x * 256u + 2 * kKeys, tm + x * 256u + sb * kKeys + k * 8u, dv + ((b * kKV + k * 2048u) >> 4), idesc_o,
+                                    (j > 0 || k > 0) ? 1u : 0u, lead);
                     }
-                    if (x + 1 == nb) umma_commit(&bars[kKEmpty + b]);
-                    umma_commit(&bars[kBlock + x * kBlockBars + kSFull + sb]);
-                }
-                return true;
-            };
-            while (ok && walk.next(g)) {
-                const uint32_t tiles = (uint32_t) (g.t1 - g.t0);
-                const int nb = second(g) ? 2 : 1;
-                for (int x = 0; ok && x < nb; ++x) ok = mbar_wait<kSuspendNs>(&bars[kBlock + x * kBlockBars + kQFull], bseg[x]++ & 1u, abort_flag);
-                if (!ok || !(ok = issue_s(n, 0, nb))) break;
-                for (uint32_t j = 0; ok && j < tiles; ++j, ++n) {
-                    const uint32_t b = n & 1u;
-                    if (j + 1 < tiles && !(ok = issue_s(n + 1, 1, nb))) break;
-                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kVFull + b], (n >> 1) & 1u, abort_flag))) break;
-                    const uint64_t db = dv + b * (kKV >> 4);
-#pragma unroll
-                    for (int x = 0; x < kNB; ++x) {
-                        if (x >= nb) break;
-                        uint64_t *own = bars + kBlock + x * kBlockBars;
-                        const uint32_t sb = bn[x] & 1u;
-                        if (!(ok = mbar_wait<kSuspendNs>(&own[kWFull + sb], (bn[x] >> 1) & 1u, abort_flag))) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16; ++k) {
-                            umma_f16_ts(tmem + x * 256u + 2 * kKeys, tmem + x * 256u + sb * kKeys + k * 8u, db + k * (2048u >> 4), idesc_o,
-                                        (j > 0 || k > 0) ? 1u : 0u);
-                        }
-                        if (x + 1 == nb) umma_commit(&bars[kVEmpty + b]);
-                        umma_commit(&own[kPvDone + sb]);
-                        ++bn[x];
-                    }
+                    if (x + 1 == nb) umma_commit_by(&bars[kVEmpty + b], lead);
+                    umma_commit_by(&own[kPvDone + sb], lead);
+                    ++bn[x];
                 }
             }
         }

@@ -17,8 +17,8 @@
 // dh multiply-adds (512 cycles at dh 128).  One CTA per SM works on two blocks at a time (head sizes beyond 128: one), so
 // that one's exponentials run beside the other's products and both share the converted tiles.
 //
-// Roles (416 threads; 288 with one block): a warpgroup per block for softmax and epilogue, a thread per row; a
-// warpgroup converts codes (its loads run a tile ahead in registers); the last warp allocates TMEM and issues the
+// Roles (544 threads; 416 with one block): a warpgroup per block for softmax and epilogue, a thread per row; one
+// warpgroup converts the codes of K, one those of V (their loads run a tile ahead in registers); the last warp allocates TMEM and issues the
 // products (the warp as one, see umma_f16_ss).  Shared memory: q, two tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is
 // double-buffered: S of tile j + 1 is issued before W v of tile j.
 //
@@ -51,13 +51,13 @@ constexpr uint32_t kSuspendNs = 20000;
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
 
 __host__ __device__ constexpr int blocks_at_once(int dhc) { return dhc <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int threads_of(int nb) { return 128 * nb + 128 + 32; }
+__host__ __device__ constexpr int threads_of(int nb) { return 128 * nb + 256 + 32; }
 // Registers per thread: at launch, and after the warpgroups have traded (the softmax holds the 64 scores of a row's tile)
-__host__ __device__ constexpr int launch_regs(int nb) { return nb == 2 ? 128 : 168; }
-__host__ __device__ constexpr int softmax_regs(int nb) { return nb == 2 ? 152 : 200; }
-__host__ __device__ constexpr int convert_regs(int nb) { return nb == 2 ? 80 : 136; }
+__host__ __device__ constexpr int launch_regs(int nb) { return nb == 2 ? 96 : 128; }
+__host__ __device__ constexpr int softmax_regs(int nb) { return nb == 2 ? 144 : 200; }
+__host__ __device__ constexpr int convert_regs(int nb) { return nb == 2 ? 48 : 88; }
 __host__ __device__ constexpr bool split_fits(int nb) {
-    return 128 * nb * softmax_regs(nb) + 128 * convert_regs(nb) + 32 * launch_regs(nb) <= threads_of(nb) * launch_regs(nb);
+    return 128 * nb * softmax_regs(nb) + 256 * convert_regs(nb) + 32 * launch_regs(nb) <= threads_of(nb) * launch_regs(nb);
 }
 static_assert(split_fits(1) && split_fits(2), "the registers' split fits what the launch gave");
 
@@ -135,6 +135,16 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float *v) {
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]), "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]), "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
         : "r"(taddr)
         : "memory");
+}
+// 32 columns without the wait, and the wait that hands them over
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_finish(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]) :: "memory");
 }
 // two fp32 operations per instruction
 __device__ __forceinline__ uint64_t pack2f(float lo, float hi) {
@@ -375,127 +385,159 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         }
         __syncwarp();
     } else if (warp >= 4 * kNB) {
-        // ------------------------------------------------------------ codes to fp16
+        // ------------------------------------------------------------ codes to fp16: a warpgroup for K and the scales, one for V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(convert_regs(kNB)));
         constexpr int kGroups = DHC / 64;// 4 lanes take 64 bytes of a row; 8 rows per warp and load
-        const uint32_t c = threadIdx.x - 128 * kNB, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
-        // Three tiles are in flight here: one whose codes are in registers, the next one, whose page ids are (`cur`), and
-        // the one after, whose ids are being read (`fut`): the ids' latency, the codes' and the conversion overlap.
-        struct Ids {
-            const int32_t *row;// of the block table
-            int32_t id[3];     // pages of this thread's two rows and of its key (one page per tile: [0] only)
-            int32_t tile, keys, kvh;
-            bool some;
-        };
-        bool more = walk.next(g);
-        int32_t tile = more ? g.t0 : 0;
-        auto read_ids = [&](Ids &x) {
-            x.some = more;
-            if (!more) return;
-            x.tile = tile, x.keys = held(g.s.len, p.t.cap), x.kvh = g.kvh, x.row = p.table + (int64_t) g.b * p.t.stride;
-            const int32_t tok[3] = {tile * kKeys + (ONE ? 0 : (int32_t) r0), tile * kKeys + (int32_t) r0 + 32, tile * kKeys + (int32_t) (c % kKeys)};
-#pragma unroll
-            for (int i = 0; i < (ONE ? 1 : 3); ++i) x.id[i] = tok[i] < x.keys ? x.row[p.page_div.div((uint32_t) tok[i])] : -1;
-            if (++tile >= g.t1 && (more = walk.next(g))) tile = g.t0;
-        };
-        auto in_pool = [&](int32_t id) { return id >= 0 && id < p.c.pages; };
-        uint4 kd[2][kGroups], vd[2][kGroups];
-        float ks = 0.f, vs = 0.f;
-        bool key_ok = false;
-        // 16 codes of a row from element d0 on, one by one
-        auto load16 = [&](const uint8_t *at, int32_t d0) -> uint4 {
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                if (d0 + i < p.c.dh) w[i >> 2] |= (uint32_t) at[i] << (8 * (i & 3));
-            }
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        };
-        auto load_tile = [&](const Ids &x, const PoolStrides &st, const uint8_t *pool, uint4 (&to)[2][kGroups]) {
-            const int32_t tok = x.tile * kKeys + (int32_t) r0;
-            const uint8_t *at[2];
-            bool ok[2];
-            if (ONE) {
-                const int32_t in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
-                ok[0] = x.some && in_pool(x.id[0]) && tok < x.keys, ok[1] = ok[0] && tok + 32 < x.keys;
-                at[0] = pool + (ok[0] ? (int64_t) x.id[0] * st.sn + (int64_t) x.kvh * st.sh + (int64_t) in_page * st.sp : 0) + c4 * 16;
-                at[1] = at[0] + 32 * st.sp;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int32_t in_page = tok + 32 * i - (int32_t) p.page_div.div((uint32_t) (tok + 32 * i)) * p.c.page;
-                    ok[i] = x.some && in_pool(x.id[i]);
-                    at[i] = pool + (ok[i] ? (int64_t) x.id[i] * st.sn + (int64_t) x.kvh * st.sh + (int64_t) in_page * st.sp : 0) + c4 * 16;
-                }
-            }
+        const bool is_v = warp >= 4 * kNB + 4;
+        const uint32_t c = (threadIdx.x - 128 * kNB) & 127u, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
+        uint64_t *full = bars + (is_v ? kVFull : kKFull), *empty = bars + (is_v ? kVEmpty : kKEmpty);
+        const PoolStrides st = is_v ? p.c.v : p.c.k;
+        const uint8_t *pool = (is_v ? p.vp : p.kp) + c4 * 16;
+        // rows as TMA with 128-byte swizzle would lay them: 16-byte chunk j of row r at j ^ (r & 7); this thread's rows are
+        // r0 and r0 + 32, its chunks 2 c4 and 2 c4 + 1 of every box of 64 elements
+        const uint32_t row_at = (is_v ? sv : sk) + r0 * 128u, chunk0 = ((2 * c4) ^ (r0 & 7u)) << 4, chunk1 = ((2 * c4 + 1) ^ (r0 & 7u)) << 4;
+        uint4 data[2][kGroups];
+        auto store_tile = [&](uint32_t b) {
+            const uint32_t at = row_at + b * kKV;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int q = 0; q < kGroups; ++q) {
-                    const int32_t d0 = (q * 4 + (int32_t) c4) * 16;
-                    to[i][q] = make_uint4(0u, 0u, 0u, 0u);
-                    if (ok[i] && d0 < p.c.dh) to[i][q] = ONE || p.vec ? *reinterpret_cast<const uint4 *>(at[i] + q * 64) : load16(at[i] + q * 64, d0);
-                }
-            }
-        };
-        auto load_scales = [&](const Ids &x) {
-            const int32_t id = x.id[ONE ? 0 : 2], key = (int32_t) (c % kKeys);
-            key_ok = x.some && in_pool(id) && x.tile * kKeys + key < x.keys;
-            ks = vs = 0.f;
-            if (ONE ? x.some && in_pool(id) && c == 0 : key_ok && c < kKeys) {
-                ks = p.ks[(int64_t) id * p.c.k.cn + (int64_t) x.kvh * p.c.k.ch];
-                vs = p.vs[(int64_t) id * p.c.v.cn + (int64_t) x.kvh * p.c.v.ch];
-            }
-        };
-        // rows as TMA with 128-byte swizzle would lay them: 16-byte chunk j of row r at j ^ (r & 7)
-        auto store_tile = [&](uint32_t base, const uint4 (&from)[2][kGroups]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t r = r0 + 32 * i;
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
                     if ((q * 4 + (int32_t) c4) * 16 >= p.c.dh) continue;
-                    const uint4 w = from[i][q];
-                    const uint32_t row = base + (uint32_t) q * (kKeys * 128u) + r * 128u;
+                    const uint4 w = data[i][q];
                     uint32_t h[8];
                     e4m3x4_to_f16x4(w.x, h[0], h[1]), e4m3x4_to_f16x4(w.y, h[2], h[3]);
                     e4m3x4_to_f16x4(w.z, h[4], h[5]), e4m3x4_to_f16x4(w.w, h[6], h[7]);
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                    const uint32_t row = at + (uint32_t) (q * (kKeys * 128) + i * (32 * 128));
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + chunk0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + chunk1), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");// the products read through the async proxy
         };
-        Ids cur, fut;
-        read_ids(cur);
-        load_tile(cur, p.c.k, p.kp, kd);
-        load_tile(cur, p.c.v, p.vp, vd);
-        load_scales(cur);
-        bool have = cur.some, ok = true;
-        read_ids(cur);
-        for (uint32_t n = 0; have; ++n) {
-            const uint32_t b = n & 1u, ph = ((n >> 1) & 1u) ^ 1u;
-            read_ids(fut);
-            if (!(ok = mbar_wait<kSuspendNs>(&bars[kKEmpty + b], ph, abort_flag))) break;
-            // the scales go first: the rows that see K see them
-            TileScales &sc = scales[n % kScaleSets];
-            const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
-            if (c < kKeys) {
-                const float lv = log2_of(vs);
-                if (!ONE || c == 0) sc.ks[c] = ks, sc.vs[c] = vs, sc.lv[c] = lv;
-                if (lane == 0) sc.mask[cw] = mask;
-                mbar_arrive(&bars[kScFull + n % kScaleSets]);
+        bool ok = true;
+        uint32_t n = 0;
+        while (ok && walk.next(g)) {
+            // The codes of a tile are loaded while the tile before is converted.
+            const int32_t keys = held(g.s.len, p.t.cap), t1 = g.t1;
+            const int32_t *ids = p.table + (int64_t) g.b * p.t.stride;
+            const uint8_t *head = pool + (int64_t) g.kvh * st.sh;
+            if (ONE) {
+                // One page per tile: lane j holds the page of the j-th of 32 tiles, and its scales, so that these are read
+                // once in 32 tiles; the next 32 are requested while the last of these are converted.
+                int32_t id = -1, id_next = -1, first = g.t0;// `first`: the tile of lane 0
+                float ks = 0.f, vs = 0.f, lv = 0.f;
+                auto page_of = [&](int32_t tile) -> int32_t {
+                    if (tile >= t1 || tile * kKeys >= keys) return -1;
+                    const int32_t x = ids[p.page_div.div((uint32_t) (tile * kKeys))];
+                    return x >= 0 && x < p.c.pages ? x : -1;
+                };
+                auto scales_of = [&]() {
+                    ks = id >= 0 ? p.ks[(int64_t) id * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch] : 0.f;
+                    vs = id >= 0 ? p.vs[(int64_t) id * p.c.v.cn + (int64_t) g.kvh * p.c.v.ch] : 0.f;
+                    lv = log2_of(vs);
+                };
+                const int32_t start = g.t0 * kKeys;
+                int32_t in_page = start - (int32_t) p.page_div.div((uint32_t) start) * p.c.page;
+                auto load = [&](int32_t tile, int32_t page) {
+                    const int32_t left = page < 0 ? 0 : keys - tile * kKeys;
+                    const uint8_t *at = head + (int64_t) max(page, 0) * st.sn + (int64_t) (in_page + (int32_t) r0) * st.sp;
+                    in_page = in_page + kKeys == p.c.page ? 0 : in_page + kKeys;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q) {
+                            data[i][q] = make_uint4(0u, 0u, 0u, 0u);
+                            if ((int32_t) r0 + 32 * i < left && (q * 4 + (int32_t) c4) * 16 < p.c.dh) data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
+                        }
+                        at += 32 * st.sp;
+                    }
+                };
+                id = page_of(first + (int32_t) lane);
+                if (cw == 0 && !is_v) scales_of();
+                load(g.t0, __shfl_sync(0xffffffffu, id, 0));
+                for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
+                    const uint32_t b = n & 1u;
+                    const int32_t j = tile - first;
+                    if (j == 24) id_next = page_of(first + 32 + (int32_t) lane);
+                    if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
+                    __syncwarp();
+                    if (cw < 2 && !is_v) {
+                        // the scales go first: the rows that see K see them
+                        const float k1 = __shfl_sync(0xffffffffu, ks, j), v1 = __shfl_sync(0xffffffffu, vs, j), l1 = __shfl_sync(0xffffffffu, lv, j);
+                        const int32_t left = __shfl_sync(0xffffffffu, id, j) < 0 ? 0 : keys - tile * kKeys - (int32_t) cw * 32;
+                        TileScales &sc = scales[n % kScaleSets];
+                        if (c == 0) sc.ks[0] = k1, sc.vs[0] = v1, sc.lv[0] = l1;
+                        if (lane == 0) sc.mask[cw] = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+                        mbar_arrive(&bars[kScFull + n % kScaleSets]);
+                    }
+                    store_tile(b);
+                    mbar_arrive(&full[b]);
+                    if (j == 31) {
+                        first += 32, id = id_next;
+                        if (cw == 0 && !is_v) scales_of();
+                    }
+                    if (tile + 1 < t1) load(tile + 1, __shfl_sync(0xffffffffu, id, tile + 1 - first));
+                }
+            } else {
+                // pages that end inside a tile: a page per row and per key
+                auto page_of = [&](int32_t tok) -> int32_t {
+                    if (tok >= keys) return -1;
+                    const int32_t x = ids[p.page_div.div((uint32_t) tok)];
+                    return x >= 0 && x < p.c.pages ? x : -1;
+                };
+                float ks = 0.f, vs = 0.f;
+                bool key_ok = false;
+                auto load = [&](int32_t tile) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int32_t tok = tile * kKeys + (int32_t) r0 + 32 * i, page = page_of(tok);
+                        const int32_t in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
+                        const uint8_t *at = head + (int64_t) max(page, 0) * st.sn + (int64_t) in_page * st.sp;
+#pragma unroll
+                        for (int q = 0; q < kGroups; ++q) {
+                            const int32_t d0 = (q * 4 + (int32_t) c4) * 16;
+                            data[i][q] = make_uint4(0u, 0u, 0u, 0u);
+                            if (page < 0 || d0 >= p.c.dh) continue;
+                            if (p.vec) {
+                                data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
+                            } else {// rows that are no whole aligned vectors: code by code
+                                uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+#pragma unroll 1
+                                    for (int y = 0; y < 4; ++y) {
+                                        if (d0 + 4 * x + y < p.c.dh) w[x] |= (uint32_t) at[q * 64 + 4 * x + y] << (8 * y);
+                                    }
+                                }
+                                data[i][q] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                    if (!is_v && c < kKeys) {
+                        const int32_t page = page_of(tile * kKeys + (int32_t) c);
+                        key_ok = page >= 0;
+                        ks = key_ok ? p.ks[(int64_t) page * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch] : 0.f;
+                        vs = key_ok ? p.vs[(int64_t) page * p.c.v.cn + (int64_t) g.kvh * p.c.v.ch] : 0.f;
+                    }
+                };
+                load(g.t0);
+                for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
+                    const uint32_t b = n & 1u;
+                    if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
+                    __syncwarp();
+                    if (cw < 2 && !is_v) {
+                        TileScales &sc = scales[n % kScaleSets];
+                        const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
+                        sc.ks[c] = ks, sc.vs[c] = vs, sc.lv[c] = log2_of(vs);
+                        if (lane == 0) sc.mask[cw] = mask;
+                        mbar_arrive(&bars[kScFull + n % kScaleSets]);
+                    }
+                    store_tile(b);
+                    mbar_arrive(&full[b]);
+                    if (tile + 1 < t1) load(tile + 1);
+                }
             }
-            store_tile(sk + b * kKV, kd);
-            mbar_arrive(&bars[kKFull + b]);
-            load_tile(cur, p.c.k, p.kp, kd);
-            load_scales(cur);
-            if (!(ok = mbar_wait<kSuspendNs>(&bars[kVEmpty + b], ph, abort_flag))) break;
-            store_tile(sv + b * kKV, vd);
-            mbar_arrive(&bars[kVFull + b]);
-            load_tile(cur, p.c.v, p.vp, vd);
-            have = cur.some;
-            cur = fut;
         }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: a thread per row
@@ -519,53 +561,62 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
             float rf = 0.f;
             {
-                // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes: the row's largest
-                // magnitude, then its elements times a power of two (and the sign of the scale, so that the factor of
-                // the scores is not negative) into swizzled shared memory.  Every product of the item before is done.
-                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 32 / kAtOnce < 16 ? 32 / kAtOnce : 16;// lanes per row, rows per load, loads in flight
+                // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes, into swizzled shared memory.
+                // fp16 rows go as they are; bf16 rows are multiplied by a power of two after their largest magnitude.  The
+                // sign of the scale goes with q, so that the factor of the scores is not negative.  (Every product of the
+                // item before is done.)
+                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 32 / kAtOnce < 8 ? 32 / kAtOnce : 8;// lanes per row, rows per load, loads in flight
                 const int32_t d = (int32_t) (lane % kPer) * 8;
+                const bool vec = p.q_vec && p.c.dh % 8 == 0;
+                const int64_t mine = (int64_t) (s.first + tok) * p.q_st + (int64_t) (g.kvh * p.group + (have ? (int32_t) rr - tok * p.group : 0)) * p.q_sh;
+                const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+                rf = fabsf(p.scale_log2);
 #pragma unroll 1
                 for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
                     uint4 w[kBatch];
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
-                        const uint32_t row = rr0 + quarter * 32u + (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
+                        const uint32_t row = (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
+                        const int64_t at = __shfl_sync(0xffffffffu, mine, (int) row);
                         w[i] = make_uint4(0u, 0u, 0u, 0u);
-                        if (row < rows && d < p.c.dh) {
-                            const int32_t tk = (int32_t) p.group_div.div(row), hd = (int32_t) row - tk * p.group;
-                            const uint16_t *q = p.q + (int64_t) (s.first + tk) * p.q_st + (int64_t) (g.kvh * p.group + hd) * p.q_sh + d;
-                            if (p.q_vec && d + 8 <= p.c.dh) {
-                                w[i] = *reinterpret_cast<const uint4 *>(q);
+                        if (rr0 + quarter * 32u + row < rows && d < p.c.dh) {
+                            if (vec) {
+                                w[i] = *reinterpret_cast<const uint4 *>(p.q + at + d);
                             } else {
-                                uint32_t e[8];
+                                uint32_t e[4];
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) e[j] = d + j < p.c.dh ? q[j] : 0u;
-                                w[i] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+                                for (int j = 0; j < 4; ++j) {
+                                    e[j] = (uint32_t) p.q[at + min(d + 2 * j, p.c.dh - 1)] | ((uint32_t) p.q[at + min(d + 2 * j + 1, p.c.dh - 1)] << 16);
+                                    if (d + 2 * j >= p.c.dh) e[j] = 0u;
+                                    else if (d + 2 * j + 1 >= p.c.dh) e[j] &= 0xFFFFu;
+                                }
+                                w[i] = make_uint4(e[0], e[1], e[2], e[3]);
                             }
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                        uint32_t top = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
-                        top = max(top & 0xFFFFu, top >> 16);
-#pragma unroll
-                        for (int o = 1; o < kPer; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        const int32_t shift = query_shift(p.bf16, top);
-                        const float up = copysignf(__uint_as_float(pow2_bits(shift)), p.scale_log2);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 f = p.bf16 ? unpack2_t<kBF16>(x[j]) : unpack2(x[j]);
-                            x[j] = round16x2(false, f.x * up, f.y * up);
-                        }
                         const uint32_t br = quarter * 32u + (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
+                        if (p.bf16) {
+                            uint32_t top = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
+#pragma unroll
+                            for (int o = 1; o < kPer; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            const int32_t shift = query_shift(true, max(top & 0xFFFFu, top >> 16));
+                            const float up = __uint_as_float(pow2_bits(shift));
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float2 f = unpack2_t<kBF16>(x[j]);
+                                x[j] = round16x2(false, f.x * up, f.y * up);
+                            }
+                            // the factor of row (i0 + i) * kAtOnce + .. to the lane that owns the row
+                            const int32_t its = __shfl_sync(0xffffffffu, shift, (int) (lane % kAtOnce) * kPer);
+                            if ((int) (lane / kAtOnce) == i0 + i) rf *= __uint_as_float(pow2_bits(-its));
+                        }
                         if (d < p.c.dh) {
                             const uint32_t at = myq + ((uint32_t) d >> 6) * (kRows * 128u) + br * 128u + (((((uint32_t) d >> 3) & 7u) ^ (br & 7u)) << 4);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0] ^ flip), "r"(x[1] ^ flip), "r"(x[2] ^ flip), "r"(x[3] ^ flip) : "memory");
                         }
-                        // the factor of row (i0 + i) * kAtOnce + .. to the lane that owns the row
-                        const int32_t its = __shfl_sync(0xffffffffu, shift, (int) (lane % kAtOnce) * kPer);
-                        if ((int) (lane / kAtOnce) == i0 + i) rf = __uint_as_float(pow2_bits(-its)) * fabsf(p.scale_log2);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -585,28 +636,39 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 // Scores are x * f; where the tile hides something from a row of this warp, x is the score itself and
                 // f is 1.
                 float x[kKeys];
-                tmem_ld64(t_lane + b * kKeys, x);
+                tmem_ld32(t_lane + b * kKeys, x);
+                tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);// (while the first half is looked through)
                 float f = ONE ? sc.ks[0] * rf : 1.f;
-                if (!ONE) {
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) x[i] *= sc.ks[i] * rf;
-                }
                 const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
                 const int32_t left = limit - tile * kKeys;// (rows that do not exist see nothing)
-                if (__any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && left < kKeys))) {
+                const bool hidden = __any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && left < kKeys));
+                auto finish_scores = [&](int half) {
+                    if (!ONE) {
 #pragma unroll
-                    for (int i = 0; i < kKeys; ++i) x[i] = (((i < 32 ? m0 : m1) >> (i & 31)) & 1u) && i < left ? x[i] * f : -INFINITY;
-                    f = 1.f;
-                }
-                float t4[4] = {x[0], x[1], x[2], x[3]};
+                        for (int i = half * 32; i < half * 32 + 32; ++i) x[i] *= sc.ks[i] * rf;
+                    }
+                    if (hidden) {
 #pragma unroll
-                for (int i = 4; i < kKeys - 4; i += 8) {
+                        for (int i = half * 32; i < half * 32 + 32; ++i) x[i] = (((half ? m1 : m0) >> (i & 31)) & 1u) && i < left ? x[i] * f : -INFINITY;
+                    }
+                };
+                auto largest = [&](const float *v) -> float {
+                    float t4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], x[i + j]), x[i + 4 + j]);
-                }
+                    for (int i = 4; i < 28; i += 8) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], x[kKeys - 4 + j]);
-                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f;
+                        for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], v[i + j]), v[i + 4 + j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[28 + j]);
+                    return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                };
+                finish_scores(0);
+                float top = largest(x);
+                tmem_ld32_finish(x + 32);
+                finish_scores(1);
+                if (hidden) f = 1.f;
+                top = fmaxf(top, largest(x + 32)) * f;
                 float wtop;
                 if (ONE) {
                     wtop = top + sc.lv[0];
@@ -686,6 +748,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const int part = g.t0 > 0 ? 0 : 1;
             const int64_t at0 = ((int64_t) blockIdx.x * 2 + part) * kItemRows + blk * kRows + quarter * 32u;// this warp's first row
             const bool none = wm == -INFINITY;// (O holds products with weights of zero)
+            const int64_t out_at = (int64_t) (s.first + tok) * p.o_st + (int64_t) (g.kvh * p.group + (have ? (int32_t) rr - tok * p.group : 0)) * p.o_sh;
             // Through this warp's part of q's memory (rows of 128 bytes, their 16-byte pieces rotated by the row), so that a
             // row's pieces leave side by side: finished outputs 64 columns at a time, parts 32 columns in fp32.
             const uint32_t stage = myq + quarter * 32u * 128u, piece = lane & 7u, sub = lane >> 3;
@@ -719,8 +782,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     for (uint32_t i = 0; i < 8; ++i) {
                         const uint32_t wr = i * 4u + sub, row = rr0 + quarter * 32u + wr;
                         const uint4 y = take(wr);
+                        uint16_t *out = p.out + __shfl_sync(0xffffffffu, out_at, (int) wr) + d;
                         if (row < rows && d < p.c.dh) {
-                            uint16_t *out = row_of_out(p, s, g.kvh, row) + d;
                             if (p.o_vec8) {
                                 *reinterpret_cast<uint4 *>(out) = y;
                             } else {

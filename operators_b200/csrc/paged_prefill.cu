@@ -5,12 +5,13 @@
 // the second product), O += W v in TMEM.  The operands of kind::f16 are fp16: q is scaled per row by a power of two
 // (see paged_attention.cu), the codes become fp16 exactly on their way into shared memory, once per pair of blocks.
 //
-// Softmax in one pass: score 2^(s f - m) with f the row's and the page's factor and m the row's running reference,
-// which moves only when a score exceeds it by 2^8, so that O (which then has to be read, multiplied and written
-// back) almost never moves after the first tiles.  The weight of a value is w = p * 2^c with
-// 2^c = 2^(m - M + 7) * (scale of the values' page) and M the weights' own reference, so fp16 holds weights between
-// 2^15 and 2^-21 of the reference (2^-32 with subnormals) however the pages' scales differ, and one exponential gives
-// w; the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way,
+// Softmax in one pass: p = 2^(s f - m) with f the row's and the page's factor and m the row's reference, the largest
+// score of its first tile.  The weight of a value is w = p * 2^c with 2^c = 2^(m - M + 2) * (scale of the values' page) and
+// M the weights' own reference; it moves (and O, which has to be read, multiplied and written back) only when a weight
+// exceeds it by 2^13.  Scores of later tiles rarely exceed the first tile's largest by that much, so hardly any tile is
+// looked through for its largest score: sums of 16 weights, formed anyway, tell when one may have grown too large.  fp16
+// holds weights between 2^13 and 2^-16 times the reference with all their bits, smaller ones to 2^-27 of it.  One
+// exponential gives w; the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way,
 // and their sum must not underflow.
 //
 // What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x
@@ -43,8 +44,9 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = kPrefillKeys;
-constexpr float kSlack = 8.f, kLift = 7.f;// w <= 2^15
+constexpr float kSlack = 13.f, kLift = 2.f;// w <= 2^15
 constexpr float kLeast = -90.f;
+constexpr float kMostWeight = 32768.f;// 2^(lift + slack)
 constexpr int kItemUnits = 4;// what the start and the end of an item cost, in tiles
 constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;
@@ -69,7 +71,7 @@ enum Bar { kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty
            kQFull = 0, kSFull, kSFull1, kWFull, kWFull1, kPvDone, kPvDone1, kBlockBars, kBars = kBlock + 2 * kBlockBars };
 
 struct TileScales {
-    float ks[kKeys], vs[kKeys], lv[kKeys];// scales of the keys, of the values, log2 of the latter; one page: [0] only
+    float ks[kKeys], lv[kKeys];// scales of the keys, log2 of the values'
     uint32_t mask[2], pad[2];             // tokens that exist
 };
 
@@ -423,19 +425,13 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const int32_t *ids = p.table + (int64_t) g.b * p.t.stride;
             const uint8_t *head = pool + (int64_t) g.kvh * st.sh;
             if (ONE) {
-                // One page per tile: lane j holds the page of the j-th of 32 tiles, and its scales, so that these are read
-                // once in 32 tiles; the next 32 are requested while the last of these are converted.
-                int32_t id = -1, id_next = -1, first = g.t0;// `first`: the tile of lane 0
-                float ks = 0.f, vs = 0.f, lv = 0.f;
+                // One page per tile: lane j holds the page of the j-th of 32 tiles, so that these are read once in 32 tiles;
+                // the next 32 are requested while the last of these are converted.
+                int32_t first = g.t0, id_next = -1;// `first`: the tile of lane 0
                 auto page_of = [&](int32_t tile) -> int32_t {
                     if (tile >= t1 || tile * kKeys >= keys) return -1;
                     const int32_t x = ids[p.page_div.div((uint32_t) (tile * kKeys))];
                     return x >= 0 && x < p.c.pages ? x : -1;
-                };
-                auto scales_of = [&]() {
-                    ks = id >= 0 ? p.ks[(int64_t) id * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch] : 0.f;
-                    vs = id >= 0 ? p.vs[(int64_t) id * p.c.v.cn + (int64_t) g.kvh * p.c.v.ch] : 0.f;
-                    lv = log2_of(vs);
                 };
                 const int32_t start = g.t0 * kKeys;
                 int32_t in_page = start - (int32_t) p.page_div.div((uint32_t) start) * p.c.page;
@@ -453,8 +449,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         at += 32 * st.sp;
                     }
                 };
-                id = page_of(first + (int32_t) lane);
-                if (cw == 0 && !is_v) scales_of();
+                int32_t id = page_of(first + (int32_t) lane);
                 load(g.t0, __shfl_sync(0xffffffffu, id, 0));
                 for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
@@ -462,21 +457,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     if (j == 24) id_next = page_of(first + 32 + (int32_t) lane);
                     if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     __syncwarp();
-                    if (cw < 2 && !is_v) {
-                        // the scales go first: the rows that see K see them
-                        const float k1 = __shfl_sync(0xffffffffu, ks, j), v1 = __shfl_sync(0xffffffffu, vs, j), l1 = __shfl_sync(0xffffffffu, lv, j);
-                        const int32_t left = __shfl_sync(0xffffffffu, id, j) < 0 ? 0 : keys - tile * kKeys - (int32_t) cw * 32;
-                        TileScales &sc = scales[n % kScaleSets];
-                        if (c == 0) sc.ks[0] = k1, sc.vs[0] = v1, sc.lv[0] = l1;
-                        if (lane == 0) sc.mask[cw] = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
-                        mbar_arrive(&bars[kScFull + n % kScaleSets]);
-                    }
                     store_tile(b);
                     mbar_arrive(&full[b]);
-                    if (j == 31) {
-                        first += 32, id = id_next;
-                        if (cw == 0 && !is_v) scales_of();
-                    }
+                    if (j == 31) first += 32, id = id_next;
                     if (tile + 1 < t1) load(tile + 1, __shfl_sync(0xffffffffu, id, tile + 1 - first));
                 }
             } else {
@@ -529,7 +512,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     if (cw < 2 && !is_v) {
                         TileScales &sc = scales[n % kScaleSets];
                         const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
-                        sc.ks[c] = ks, sc.vs[c] = vs, sc.lv[c] = log2_of(vs);
+                        sc.ks[c] = ks, sc.lv[c] = log2_of(vs);
                         if (lane == 0) sc.mask[cw] = mask;
                         mbar_arrive(&bars[kScFull + n % kScaleSets]);
                     }
@@ -559,6 +542,17 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const bool have = rr < rows;
             const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0;
             const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
+            // ONE: the pages and scales of 32 tiles in the lanes, as in the converting warps (requested ahead of q)
+            const int32_t *ids = p.table + (int64_t) g.b * p.t.stride;
+            const int32_t keys = held(s.len, p.t.cap);
+            auto page_of = [&](int32_t tile) -> int32_t {
+                if (tile >= g.t1 || tile * kKeys >= keys) return -1;
+                const int32_t x = ids[p.page_div.div((uint32_t) (tile * kKeys))];
+                return x >= 0 && x < p.c.pages ? x : -1;
+            };
+            const float *kscale = p.ks + (int64_t) g.kvh * p.c.k.ch, *vscale = p.vs + (int64_t) g.kvh * p.c.v.ch;
+            int32_t first = g.t0, id = ONE ? page_of(first + (int32_t) lane) : -1, id_next = -1;
+            float ks = id >= 0 ? kscale[(int64_t) id * p.c.k.cn] : 0.f, vs = id >= 0 ? vscale[(int64_t) id * p.c.v.cn] : 0.f, ks_next = 0.f, vs_next = 0.f;
             float rf = 0.f;
             {
                 // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes, into swizzled shared memory.
@@ -623,108 +617,167 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 mbar_arrive(&own[kQFull]);
             }
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
-            float e = 0.f, e_back = 1.f, lv_of_e = NAN;// exponent from p to w, 2^-e, and the scale (log2) that e is for
-#pragma unroll 1
-            for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
-                const uint32_t b = n & 1u;
-                const TileScales &sc = scales[n_all % kScaleSets];
-                if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
-                // (after S: a block that sat out items may be ahead by more than a parity can tell)
-                if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
-                tc_fence_after();
-                __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
-                // Scores are x * f; where the tile hides something from a row of this warp, x is the score itself and
-                // f is 1.
-                float x[kKeys];
-                tmem_ld32(t_lane + b * kKeys, x);
-                tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);// (while the first half is looked through)
-                float f = ONE ? sc.ks[0] * rf : 1.f;
-                const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
-                const int32_t left = limit - tile * kKeys;// (rows that do not exist see nothing)
-                const bool hidden = __any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && left < kKeys));
-                auto finish_scores = [&](int half) {
-                    if (!ONE) {
+            auto largest = [&](const float *v) -> float {
+                float t4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                        for (int i = half * 32; i < half * 32 + 32; ++i) x[i] *= sc.ks[i] * rf;
-                    }
-                    if (hidden) {
+                for (int i = 4; i < 28; i += 8) {
 #pragma unroll
-                        for (int i = half * 32; i < half * 32 + 32; ++i) x[i] = (((half ? m1 : m0) >> (i & 31)) & 1u) && i < left ? x[i] * f : -INFINITY;
-                    }
-                };
-                auto largest = [&](const float *v) -> float {
-                    float t4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                    for (int i = 4; i < 28; i += 8) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], v[i + j]), v[i + 4 + j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[28 + j]);
-                    return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                };
-                finish_scores(0);
-                float top = largest(x);
-                tmem_ld32_finish(x + 32);
-                finish_scores(1);
-                if (hidden) f = 1.f;
-                top = fmaxf(top, largest(x + 32)) * f;
-                float wtop;
-                if (ONE) {
-                    wtop = top + sc.lv[0];
-                } else {
-                    wtop = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
+                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], v[i + j]), v[i + 4 + j]);
                 }
-                // references: moved when a score or a weight of a row of this warp exceeds its own by more than the slack
-                const bool up_m = top > m + kSlack || (m == -INFINITY && top > m), up = wtop > wm + kSlack || (wm == -INFINITY && wtop > wm);
-                if (__any_sync(0xffffffffu, up_m || up)) {
-                    if (up_m) {
-                        l *= fast_exp2(m - top);// (from -inf: 0)
-                        m = top;
-                    }
-                    const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
-                    if (up) wm = wtop;
-                    if (tile > g.t0 && __any_sync(0xffffffffu, up)) {
-                        // O so far: every product into it must have completed
-                        if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + (b ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
-                        tc_fence_after();
-                        __syncwarp();
-                        for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
-                            float o[32];
-                            tmem_ld32(t_lane + 2 * kKeys + c0, o);
-                            uint32_t w[32];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
-                            tmem_st32(t_lane + 2 * kKeys + c0, w);
+                for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[28 + j]);
+                return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+            };
+            // The references of the rows that ask for it move to this tile's largest: O so far and the sum follow.
+            auto move_references = [&](bool up, float top, float wtop, int32_t tile) -> bool {
+                const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
+                if (up) {
+                    const float m_new = fmaxf(m, top);
+                    l *= fast_exp2(m - m_new);// (from -inf: 0)
+                    m = m_new, wm = wtop;
+                }
+                if (tile > g.t0 && __any_sync(0xffffffffu, up)) {
+                    // every product into O must have completed
+                    const bool done = mbar_wait<kSuspendNs>(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag);
+                    if (!__all_sync(0xffffffffu, done)) return false;
+                    tc_fence_after();
+                    for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
+                        float o[32];
+                        tmem_ld32(t_lane + 2 * kKeys + c0, o);
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
+                        tmem_st32(t_lane + 2 * kKeys + c0, w);
+                    }
+                }
+                return true;
+            };
+            if (ONE) {
+                float lv_lane = log2_of(vs);
+                float e = 0.f, e_back = 1.f, shift = 0.f, lv_of_e = NAN;// exponent from p to w, 2^-e, e - m, and the scale (log2) they are for
+#pragma unroll 1
+                for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n) {
+                    const uint32_t b = n & 1u;
+                    const int32_t j = tile - first;
+                    if (j == 18) id_next = page_of(first + 32 + (int32_t) lane);
+                    if (j == 25) {
+                        ks_next = id_next >= 0 ? kscale[(int64_t) id_next * p.c.k.cn] : 0.f;
+                        vs_next = id_next >= 0 ? vscale[(int64_t) id_next * p.c.v.cn] : 0.f;
+                    }
+                    const float factor = __shfl_sync(0xffffffffu, ks, j) * rf, lv = __shfl_sync(0xffffffffu, lv_lane, j);
+                    // keys of the tile that this row sees
+                    const int32_t left = __shfl_sync(0xffffffffu, id, j) >= 0 ? limit - tile * kKeys : 0;
+                    const bool hidden = __any_sync(0xffffffffu, have && left < kKeys);
+                    // a row without a reference (its first keys are in this tile) looks through the tile for its largest score
+                    bool move = m == -INFINITY && left > 0;
+                    const bool some = __any_sync(0xffffffffu, move);
+                    if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    tc_fence_after();
+                    __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
+                    uint32_t w[kKeys / 2];
+                    float sum = 0.f;
+                    auto exponents = [&]() {
+                        if (!(lv == lv_of_e)) {// (the references or the scale have changed)
+                            e = wm == -INFINITY ? 0.f : fmaxf(m - wm + kLift + lv, kLeast);
+                            e_back = fast_exp2(-e);
+                            shift = e - (m == -INFINITY ? 0.f : m);
+                            lv_of_e = lv;
+                        }
+                    };
+                    // weights of 16 pairs, and what they add up to in four sums
+                    auto weigh = [&](const float *x, uint32_t *to, uint64_t f2, uint64_t e2, uint64_t (&part)[2]) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
+                            const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
+                            part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
+                            to[i] = round16x2(false, y0, y1);
+                        }
+                    };
+                    // Most tiles hide nothing and move no reference: their weights are formed at once, and the sums tell
+                    // whether one may have grown beyond what fp16 holds (2^(lift + slack)).  A row that finds so moves its
+                    // reference to the tile's largest score and forms its weights anew.  What a row does depends on its own
+                    // scores alone.
+                    if (!hidden && !some) {
+                        float x[kKeys];
+                        tmem_ld32(t_lane + b * kKeys, x);
+                        tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);
+                        exponents();
+                        const uint64_t f2 = pack2f(factor, factor), e2 = pack2f(shift, shift);
+                        uint64_t part[2] = {0ull, 0ull};
+                        weigh(x, w, f2, e2, part);
+                        tmem_ld32_finish(x + 32);
+                        weigh(x + 32, w + 16, f2, e2, part);
+                        const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
+                        sum = (s0.x + s0.y) + (s1.x + s1.y);
+                        move = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y)) > kMostWeight;
+                    }
+                    if (hidden || __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                        for (int pass = 0; pass < 3; ++pass) {// (a row that has moved has weights of 2^lift at most: it ends here)
+                            float x[kKeys];
+                            tmem_ld64(t_lane + b * kKeys, x);
+#pragma unroll
+                            for (int i = 0; i < kKeys; ++i) x[i] = i < left ? x[i] * factor : -INFINITY;
+                            if (__any_sync(0xffffffffu, move)) {
+                                const float top = fmaxf(largest(x), largest(x + 32));
+                                if (!(ok = move_references(move && top > -INFINITY, top, top + lv, tile))) break;
+                                lv_of_e = NAN;
+                            }
+                            exponents();
+                            uint64_t part[2] = {0ull, 0ull};
+                            const uint64_t one = pack2f(1.f, 1.f), e2 = pack2f(shift, shift);
+                            weigh(x, w, one, e2, part);
+                            weigh(x + 32, w + 16, one, e2, part);
+                            const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
+                            sum = (s0.x + s0.y) + (s1.x + s1.y);
+                            move = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y)) > kMostWeight;
+                            if (!__any_sync(0xffffffffu, move)) break;
                         }
                     }
-                    lv_of_e = NAN;
+                    if (!ok) break;
+                    l = fmaf(sum, e_back, l);
+                    __syncwarp();
+                    tmem_st32(t_lane + b * kKeys, w);
+                    tc_fence_before();
+                    mbar_arrive(&own[kWFull + b]);
+                    if (j == 31) first += 32, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                 }
-                const float mm = m == -INFINITY ? 0.f : m;
-                const float lv = ONE ? sc.lv[0] : 0.f;
-                if (!(lv == lv_of_e)) {// (the references or the scale have changed)
-                    const float ww = wm == -INFINITY ? 0.f : wm;
-                    e = ONE ? fmaxf(mm - ww + kLift + (wm == -INFINITY ? 0.f : lv), kLeast) : mm - ww + kLift;
-                    e_back = fast_exp2(-e);
-                    lv_of_e = lv;
-                }
-                uint32_t w[kKeys / 2];
-                if (ONE) {
-                    const uint64_t f2 = pack2f(f, f), e2 = pack2f(e - mm, e - mm);
-                    uint64_t part[2] = {0ull, 0ull};
+            } else {
+                // pages that end inside a tile: a factor, a scale and a mask bit per key, from shared memory
+#pragma unroll 1
+                for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
+                    const uint32_t b = n & 1u;
+                    const TileScales &sc = scales[n_all % kScaleSets];
+                    if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    // (after S: a block that sat out items may be ahead by more than a parity can tell)
+                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
+                    tc_fence_after();
+                    __syncwarp();
+                    float x[kKeys];
+                    tmem_ld64(t_lane + b * kKeys, x);
+                    const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
+                    const int32_t left = limit - tile * kKeys;
+                    const bool hidden = __any_sync(0xffffffffu, (m0 & m1) != 0xFFFFFFFFu || (have && left < kKeys));
 #pragma unroll
-                    for (int i = 0; i < kKeys / 2; ++i) {
-                        const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
-                        const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
-                        part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
-                        w[i] = round16x2(false, y0, y1);
+                    for (int i = 0; i < kKeys; ++i) x[i] *= sc.ks[i] * rf;
+                    if (hidden) {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) {
+                            if (!(((i < 32 ? m0 : m1) >> (i & 31)) & 1u) || i >= left) x[i] = -INFINITY;
+                        }
                     }
-                    const float2 sum = unpack2f(add2(part[0], part[1]));
-                    l = fmaf(sum.x + sum.y, e_back, l);
-                } else {
-                    // pages that end inside the tile: a factor per key, so p and w take an exponential each
+                    const float top = fmaxf(largest(x), largest(x + 32));
+                    float wtop = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
+                    // (the sum's own reference: it may exceed the weights' by what the scales differ)
+                    const bool far = top > m + 64.f && m != -INFINITY;
+                    if (far) l *= fast_exp2(m - top), m = top;
+                    const bool up = wtop > wm + kSlack || (wm == -INFINITY && wtop > wm);
+                    if (__any_sync(0xffffffffu, up) && !(ok = move_references(up, top, wtop, tile))) break;
+                    const float mm = m == -INFINITY ? 0.f : m, e = wm == -INFINITY ? 0.f : mm - wm + kLift;
+                    uint32_t w[kKeys / 2];
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < kKeys / 2; ++i) {
@@ -734,11 +787,11 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                                          a1 == -INFINITY ? 0.f : fast_exp2(a1 + (e + sc.lv[2 * i + 1])));
                     }
                     l += sum;
+                    __syncwarp();
+                    tmem_st32(t_lane + b * kKeys, w);
+                    tc_fence_before();
+                    mbar_arrive(&own[kWFull + b]);
                 }
-                __syncwarp();
-                tmem_st32(t_lane + b * kKeys, w);
-                tc_fence_before();
-                mbar_arrive(&own[kWFull + b]);
             }
             if (!ok) break;
             // ---- the item's output, or its part

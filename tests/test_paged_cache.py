@@ -158,14 +158,14 @@ def attend_bound(y, mean_abs, v_max, mag, dh, keys, dtype):
     each relative; numerator and denominator count once each: mean |v| times twice their sum.  Sums over the keys are in
     fp32, in parts of at most 2^15 terms that grow by 2^-23 of the running sum: 2 * (2^-8) would be the worst case, but the
     products of a step of 16 keys are summed before they join, so keys / 16 * 2^-23 counts.  Weights are stored times
-    2^7 at least relative to a reference that is one row's weight (so at most the largest); below fp16's normal range,
-    2^-14, a rounding is off by half a step of 2^-24, that is by 2^-25 / 2^7 = 2^-32 of the reference, and a key's codes
-    reach 448 where its page's largest value is at least half of that: keys * 2^-31 * max |v| in all.  One rounding of
+    2^2 at least relative to a reference that is one row's weight (so at most the largest); below fp16's normal range,
+    2^-14, a rounding is off by half a step of 2^-24, that is by 2^-25 / 2^2 = 2^-27 of the reference, and a key's codes
+    reach 448 where its page's largest value is at least half of that: keys * 2^-26 * max |v| in all.  One rounding of
     the result at the end."""
     half = torch.finfo(dtype).eps / 2
     e = (dh + 8) * 2.0 ** -23 * mag
     weight = 2.0 ** -11 + 2.0 ** -20 + 2.0 * e + (keys / 16 + 16) * 2.0 ** -23
-    return half * np.abs(y) + 2 * weight * mean_abs + keys * 2.0 ** -31 * v_max + float(torch.finfo(dtype).tiny) * half
+    return half * np.abs(y) + 2 * weight * mean_abs + keys * 2.0 ** -26 * v_max + float(torch.finfo(dtype).tiny) * half
 
 
 def close(got, want, tol):

@@ -71,10 +71,6 @@ __device__ __forceinline__ uint16_t *row_of_out(const AttendParams &p, const Seq
 // stretch is finished there; of any other, each CTA stores its part (unnormalised output and the rows' references) and
 // join_kernel adds the parts in the order of the list.
 
-// a / b of values that mostly fit 32 bits (a 64-bit division takes a few hundred cycles)
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    return ((a | b) >> 32) == 0 ? (int64_t) ((uint32_t) a / (uint32_t) b) : a / b;
-}
 __device__ __forceinline__ int64_t stretch_of(int64_t total, int64_t least) {
     const int64_t each = divide(total + gridDim.x - 1, gridDim.x);
     return each < least ? least : each;

@@ -29,6 +29,7 @@ struct AppendParams {
     float *ks, *vs;
     const int32_t *table, *lens, *offs;
     int32_t rows;
+    FastDiv per_row;// by the vectors of a row
     CacheShape c;
     TableShape t;
 };
@@ -60,37 +61,53 @@ __device__ __forceinline__ int32_t cta_exclusive_sum(int32_t v, int32_t *slot, i
 // VEC new elements of one row at a time: 8 (16-byte loads, 8-byte stores of codes) or 1.
 template<bool BF, int VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
-    __shared__ int32_t slot[33], found[2];
     __shared__ uint32_t wmax[kAppendThreads / 32];
     const int32_t item = (int32_t) blockIdx.x, head = (int32_t) blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const int32_t P = p.c.page, D = p.c.dh;
+    const int32_t P = p.c.page, D = p.c.dh, lane = (int32_t) (threadIdx.x & 31);
 
-    // the item-th touched page of the call: sequence b, its k-th page
-    int32_t b, nth;
+    // the item-th touched page of the call: sequence b, its nth page.  Every warp looks for it by itself, 128 sequences at
+    // a time (no barrier ahead of the loads).
+    int32_t b = item, nth = 0;// one token, one page per sequence
     if (p.offs == nullptr) {
-        b = item, nth = 0;// one token, one page per sequence
         if (b >= p.t.batch) return;
     } else {
         int32_t base = 0;
         bool hit = false;
-        for (int32_t b0 = 0; b0 < p.t.batch && !hit; b0 += (int32_t) blockDim.x) {
-            const int32_t mine = b0 + (int32_t) threadIdx.x;
-            int32_t count = 0;
-            if (mine < p.t.batch) {
-                int32_t lo, hi;
-                written(seq_of(p.lens, p.offs, p.rows, mine), p.t.cap, lo, hi);
-                count = pages_touched(lo, hi, P);
+        for (int32_t b0 = 0; b0 < p.t.batch && !hit; b0 += 128) {
+            int32_t count[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int32_t x = b0 + lane * 4 + i;
+                count[i] = 0;
+                if (x < p.t.batch) {
+                    int32_t lo, hi;
+                    written(seq_of(p.lens, p.offs, p.rows, x), p.t.cap, lo, hi);
+                    count[i] = pages_touched(lo, hi, P);
+                }
+                mine += count[i];
             }
-            int32_t total;
-            const int32_t before = base + cta_exclusive_sum(count, slot, total);
-            if (item >= before && item - before < count) found[0] = mine, found[1] = item - before;
-            base += total;
-            hit = item < base;// the same in every thread
+            int32_t incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += u;
+            }
+            int32_t before = base + incl - mine;
+            const uint32_t who = __ballot_sync(0xffffffffu, item >= before && item - before < mine);
+            if (who != 0) {
+                int32_t f = 0, k = item - before;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    if (f == i && k >= count[i]) k -= count[i], f = i + 1;
+                }
+                const int src = __ffs((int) who) - 1;
+                b = b0 + src * 4 + __shfl_sync(0xffffffffu, f, src), nth = __shfl_sync(0xffffffffu, k, src);
+                hit = true;
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
         }
         if (!hit) return;
-        __syncthreads();
-        b = found[0], nth = found[1];
     }
     const Seq s = seq_of(p.lens, p.offs, p.rows, b);
     int32_t lo, hi;
@@ -98,24 +115,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     if (hi <= lo) return;
     const int32_t col = lo / P + nth, page0 = col * P;
     const int32_t p0 = lo > page0 ? lo : page0, p1 = hi - page0 < P ? hi : page0 + P;
-    const int32_t page = p.table[(int64_t) b * p.t.stride + col];
-    if (page < 0 || page >= p.c.pages) return;
+    const int32_t page = p.table[(int64_t) b * p.t.stride + col];// (looked at once the new rows are on their way)
     const int32_t kept = p0 - page0, m = p1 - p0;
 
     const PoolStrides st = is_v ? p.c.v : p.c.k;
     const int64_t x_st = is_v ? p.v_st : p.k_st;
     const uint16_t *x = (is_v ? p.v + (int64_t) head * p.v_sh : p.k + (int64_t) head * p.k_sh) + (int64_t) (s.first + (p0 - (s.len - s.n))) * x_st;
-    uint8_t *codes = (is_v ? p.vp : p.kp) + (int64_t) page * st.sn + (int64_t) head * st.sh;
-    float *scale = (is_v ? p.vs : p.ks) + (int64_t) page * st.cn + (int64_t) head * st.ch;
-    const float old = kept > 0 ? *scale : 0.f;
-
     // the new rows: into registers, and their largest finite magnitude
-    const int32_t per_row = D / VEC;
+    const uint32_t per_row = (uint32_t) (D / VEC);
     const int64_t nv = (int64_t) m * per_row;
     uint4 held_v[kHeld];
     uint32_t top = 0;
+    // row and element of the i-th vector of a block (below 2^32: one multiplication instead of a division)
+    auto row_of = [&](int64_t i) -> int64_t { return i <= 0xFFFFFFFFll ? (int64_t) p.per_row.div((uint32_t) i) : i / per_row; };
     auto load = [&](int64_t i) -> uint4 {
-        const int64_t r = i / per_row;
+        const int64_t r = row_of(i);
         const uint16_t *src = x + r * x_st + (i - r * per_row) * VEC;
         if (VEC == 8) return *reinterpret_cast<const uint4 *>(src);
         return make_uint4(*src, 0u, 0u, 0u);
@@ -129,6 +143,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
         const int64_t i = threadIdx.x + (int64_t) j * blockDim.x;
         held_v[j] = i < nv ? load(i) : make_uint4(0u, 0u, 0u, 0u);
     }
+    if (page < 0 || page >= p.c.pages) return;
+    uint8_t *codes = (is_v ? p.vp : p.kp) + (int64_t) page * st.sn + (int64_t) head * st.sh;
+    float *scale = (is_v ? p.vs : p.ks) + (int64_t) page * st.cn + (int64_t) head * st.ch;
+    const float old = kept > 0 ? *scale : 0.f;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) grow(held_v[j]);
     for (int64_t i = threadIdx.x + (int64_t) kHeld * blockDim.x; i < nv; i += blockDim.x) grow(load(i));
@@ -148,10 +166,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     // rows that stay, where the scale has grown
     if (kept > 0 && now != old) {
         const float ratio = old / now;
-        const int32_t n = kept * per_row;
-        for (int32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const int32_t r = i / per_row;
-            uint8_t *at = codes + (int64_t) r * st.sp + (i - r * per_row) * VEC;
+        const int64_t n = (int64_t) kept * per_row;
+        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+            const int64_t r = row_of(i);
+            uint8_t *at = codes + r * st.sp + (i - r * per_row) * VEC;
             if (VEC == 8) {
                 uint2 w = *reinterpret_cast<uint2 *>(at);
                 uint32_t out[2] = {w.x, w.y};
@@ -169,7 +187,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     }
     // the new rows
     auto store = [&](int64_t i, uint4 w) {
-        const int64_t r = i / per_row;
+        const int64_t r = row_of(i);
         uint8_t *at = codes + (kept + r) * st.sp + (i - r * per_row) * VEC;
         if (VEC == 8) {
             *reinterpret_cast<uint2 *>(at) = make_uint2(code2(f16or_bf16x2<BF>(w.x)) | (code2(f16or_bf16x2<BF>(w.y)) << 16),
@@ -209,6 +227,7 @@ struct MoveParams {
     float *ks, *vs;
     PageRuns k, v;
     int32_t pages, heads;
+    int64_t k_pieces, v_pieces;// of a page
 };
 
 constexpr int kMoveThreads = 256;
@@ -232,10 +251,11 @@ int run_unit(const PageRuns &r, const void *base) {
     return (all & 15u) == 0 ? 16 : (all & 3u) == 0 ? 4 : 1;
 }
 
-// Units [begin, begin + 4 * threads) of one page of one pool, and with the first of them the page's scales.
-template<typename U>
+// Units [begin, begin + 4 * threads) of one page of one pool, and with the first of them the page's scales.  ONE: a page
+// is one run of bytes.
+template<typename U, bool ONE>
 __device__ __forceinline__ void move_piece(uint8_t *pool, float *scales, const PageRuns &r, int32_t heads, int64_t src, int64_t dst, int64_t begin) {
-    const int64_t per_run = r.len / (int32_t) sizeof(U), units = per_run * r.n1 * r.n0;
+    const int64_t per_run = r.len / (int32_t) sizeof(U), units = ONE ? per_run : per_run * r.n1 * r.n0;
     const uint8_t *from = pool + src * r.page;
     uint8_t *to = pool + dst * r.page;
     U v[4];
@@ -245,8 +265,12 @@ __device__ __forceinline__ void move_piece(uint8_t *pool, float *scales, const P
         const int64_t u = begin + threadIdx.x + (int64_t) j * kMoveThreads;
         at[j] = -1;
         if (u < units) {
-            const int64_t run = u / per_run;
-            at[j] = (run / r.n1) * r.s0 + (run % r.n1) * r.s1 + (u - run * per_run) * (int64_t) sizeof(U);
+            if (ONE) {
+                at[j] = u * (int64_t) sizeof(U);
+            } else {
+                const int64_t run = divide(u, per_run), outer = divide(run, r.n1);
+                at[j] = outer * r.s0 + (run - outer * r.n1) * r.s1 + (u - run * per_run) * (int64_t) sizeof(U);
+            }
             v[j] = *reinterpret_cast<const U *>(from + at[j]);
         }
     }
@@ -263,18 +287,18 @@ int64_t pieces_of(const PageRuns &r) {
     const int64_t units = (int64_t) (r.len / (int32_t) sizeof(U)) * r.n1 * r.n0;
     return (units + 4 * kMoveThreads - 1) / (4 * kMoveThreads);
 }
+bool one_run(const MoveParams &m) { return m.k.n0 * m.k.n1 == 1 && m.v.n0 * m.v.n1 == 1; }
 
-template<typename U>
-__global__ void __launch_bounds__(kMoveThreads) copy_pairs_kernel(const MoveParams p, const int32_t *pairs, int64_t stride, int64_t count, int64_t pieces) {
-    // work: (pair, pool, piece), piece fastest
-    for (int64_t w = blockIdx.x; w < count * 2 * pieces; w += gridDim.x) {
-        const int64_t i = w / (2 * pieces), rest = w - i * 2 * pieces;
-        const bool is_v = rest >= pieces;
+// A block moves 16 KB (U 16 bytes): piece blockIdx.x of pool blockIdx.y of the pairs blockIdx.z ..
+template<typename U, bool ONE>
+__global__ void __launch_bounds__(kMoveThreads) copy_pairs_kernel(const MoveParams p, const int32_t *pairs, int64_t stride, int64_t count) {
+    const bool is_v = blockIdx.y != 0;
+    for (int64_t i = blockIdx.z; i < count; i += gridDim.z) {
         const int32_t src = pairs[i * stride], dst = pairs[i * stride + 1];
         if (src < 0 || src >= p.pages || dst < 0 || dst >= p.pages || src == dst) continue;
-        const int64_t begin = (is_v ? rest - pieces : rest) * 4 * kMoveThreads;
-        if (is_v) move_piece<U>(p.vp, p.vs, p.v, p.heads, src, dst, begin);
-        else move_piece<U>(p.kp, p.ks, p.k, p.heads, src, dst, begin);
+        for (int64_t piece = blockIdx.x; piece < (is_v ? p.v_pieces : p.k_pieces); piece += gridDim.x) {
+            move_piece<U, ONE>(is_v ? p.vp : p.kp, is_v ? p.vs : p.ks, is_v ? p.v : p.k, p.heads, src, dst, piece * 4 * kMoveThreads);
+        }
     }
 }
 
@@ -287,7 +311,7 @@ struct CopyDesc {
 
 MoveParams move_params(const CacheShape &c, void *kp, void *vp, void *ks, void *vs) {
     return MoveParams{reinterpret_cast<uint8_t *>(kp), reinterpret_cast<uint8_t *>(vp), reinterpret_cast<float *>(ks),
-                      reinterpret_cast<float *>(vs), page_runs(c, c.k), page_runs(c, c.v), c.pages, c.heads};
+                      reinterpret_cast<float *>(vs), page_runs(c, c.k), page_runs(c, c.v), c.pages, c.heads, 0, 0};
 }
 
 // ---------------------------------------------------------------------------------------------------- compacting --
@@ -395,8 +419,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
 
 // Renames the table's entries, fills the map and moves the pages.  Sources lie at or above the live count,
 // destinations below it, so no page is both.
-template<typename U>
-__global__ void __launch_bounds__(kMoveThreads) compact_apply_kernel(const CompactParams p, const MoveParams m, int64_t pieces) {
+template<typename U, bool ONE>
+__global__ void __launch_bounds__(kMoveThreads, 5) compact_apply_kernel(const CompactParams p, const MoveParams m) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int32_t live = p.plan.head->live;
     const int64_t moves = p.plan.head->moves;
@@ -413,12 +437,12 @@ __global__ void __launch_bounds__(kMoveThreads) compact_apply_kernel(const Compa
         if ((int64_t) col * p.page < len && id >= live && id < p.pages) id = p.page_map[id];// a mover: written by the plan
         p.new_table[(int64_t) b * p.new_stride + col] = id;
     }
-    for (int64_t w = blockIdx.x; w < moves * 2 * pieces; w += gridDim.x) {
-        const int64_t i = w / (2 * pieces), rest = w - i * 2 * pieces;
-        const bool is_v = rest >= pieces;
-        const int64_t begin = (is_v ? rest - pieces : rest) * 4 * kMoveThreads;
-        if (is_v) move_piece<U>(m.vp, m.vs, m.v, m.heads, p.plan.src[i], p.plan.dst[i], begin);
-        else move_piece<U>(m.kp, m.ks, m.k, m.heads, p.plan.src[i], p.plan.dst[i], begin);
+    const int64_t each = m.k_pieces + m.v_pieces;
+    for (int64_t w = blockIdx.x; w < moves * each; w += gridDim.x) {
+        const int64_t i = divide(w, each), rest = w - i * each;
+        const bool is_v = rest >= m.k_pieces;
+        move_piece<U, ONE>(is_v ? m.vp : m.kp, is_v ? m.vs : m.ks, is_v ? m.v : m.k, m.heads, p.plan.src[i], p.plan.dst[i],
+                           (is_v ? rest - m.k_pieces : rest) * 4 * kMoveThreads);
     }
 }
 
@@ -489,10 +513,11 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheAppend(infiniopPagedCacheAppendD
     AppendParams p{reinterpret_cast<const uint16_t *>(k), reinterpret_cast<const uint16_t *>(v), d->k_st, d->k_sh, d->v_st, d->v_sh,
                    reinterpret_cast<uint8_t *>(k_pages), reinterpret_cast<uint8_t *>(v_pages), reinterpret_cast<float *>(k_scales),
                    reinterpret_cast<float *>(v_scales), reinterpret_cast<const int32_t *>(block_table),
-                   reinterpret_cast<const int32_t *>(seq_lens), reinterpret_cast<const int32_t *>(q_offsets), d->rows, d->c, d->t};
+                   reinterpret_cast<const int32_t *>(seq_lens), reinterpret_cast<const int32_t *>(q_offsets), d->rows, FastDiv(1), d->c, d->t};
     // 8 elements at a time where every row of the new tokens starts on 16 bytes and every row of codes on 8
     bool vec = d->c.dh % 8 == 0 && aligned16(k) && aligned16(v) && ((uintptr_t) k_pages | (uintptr_t) v_pages) % 8 == 0;
     for (int64_t s : {d->k_st, d->k_sh, d->v_st, d->v_sh, d->c.k.sn, d->c.k.sh, d->c.k.sp, d->c.v.sn, d->c.v.sh, d->c.v.sp}) vec = vec && s % 8 == 0;
+    p.per_row = FastDiv((uint32_t) (vec ? d->c.dh / 8 : d->c.dh));
     const int64_t items = d->t.offsets ? pages_bound(d->rows, d->t.batch, d->c.page) : d->rows;
     const dim3 grid((unsigned) items, (unsigned) d->c.heads, 2);
     // one token per sequence is 16 vectors of 8: a small block leaves the SM to more of them
@@ -553,18 +578,20 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheCopy(infiniopPagedCacheCopyDescr
     if (d->count == 0 || d->c.pages == 0) return STATUS_SUCCESS;
     if (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || pairs == nullptr) return STATUS_BAD_PARAM;
     DeviceGuard guard(d->device_id);
-    const MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
+    MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
     const int unit = std::min(run_unit(m.k, k_pages), run_unit(m.v, v_pages));
     auto st = reinterpret_cast<cudaStream_t>(stream);
     const auto *list = reinterpret_cast<const int32_t *>(pairs);
-    auto run = [&](auto u, auto *kernel) {
+    auto run = [&](auto u, auto *whole, auto *runs) {
         using U = decltype(u);
-        const int64_t pieces = std::max(pieces_of<U>(m.k), pieces_of<U>(m.v)), work = d->count * 2 * pieces;
-        kernel<<<(unsigned) std::min<int64_t>(work, 0x7FFFFFFF), kMoveThreads, 0, st>>>(m, list, d->stride, d->count, pieces);
+        m.k_pieces = pieces_of<U>(m.k), m.v_pieces = pieces_of<U>(m.v);
+        const dim3 grid((unsigned) std::min<int64_t>(std::max(m.k_pieces, m.v_pieces), 1 << 20), 2, (unsigned) std::min<int64_t>(d->count, 65535));
+        if (one_run(m)) whole<<<grid, kMoveThreads, 0, st>>>(m, list, d->stride, d->count);
+        else runs<<<grid, kMoveThreads, 0, st>>>(m, list, d->stride, d->count);
     };
-    if (unit == 16) run(uint4{}, copy_pairs_kernel<uint4>);
-    else if (unit == 4) run(uint32_t{}, copy_pairs_kernel<uint32_t>);
-    else run(uint8_t{}, copy_pairs_kernel<uint8_t>);
+    if (unit == 16) run(uint4{}, copy_pairs_kernel<uint4, true>, copy_pairs_kernel<uint4, false>);
+    else if (unit == 4) run(uint32_t{}, copy_pairs_kernel<uint32_t, true>, copy_pairs_kernel<uint32_t, false>);
+    else run(uint8_t{}, copy_pairs_kernel<uint8_t, true>, copy_pairs_kernel<uint8_t, false>);
     return check_launch("paged cache copy");
 }
 
@@ -634,22 +661,24 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheCompact(infiniopPagedCacheCompac
     if (no_rows) p.t.batch = 0;
     p.plan = plan_view(workspace, (uint64_t) d->c.pages);
     if (launch_cluster(compact_plan_kernel, kPlanCtas, kPlanThreads, kPlanCtas, st, p) != cudaSuccess) return check_launch("paged cache compact (plan)");
-    const MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
+    MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
     const int unit = std::min(run_unit(m.k, k_pages), run_unit(m.v, v_pages));
-    auto run = [&](auto u, auto *kernel) {
+    auto run = [&](auto u, auto *whole, auto *runs) {
         using U = decltype(u);
+        m.k_pieces = pieces_of<U>(m.k), m.v_pieces = pieces_of<U>(m.v);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned) d->sm_count * 8);
+        cfg.gridDim = dim3((unsigned) d->sm_count * 5);
         cfg.blockDim = dim3(kMoveThreads);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr, cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, kernel, p, m, std::max(pieces_of<U>(m.k), pieces_of<U>(m.v)));
+        return one_run(m) ? cudaLaunchKernelEx(&cfg, whole, p, m) : cudaLaunchKernelEx(&cfg, runs, p, m);
     };
-    const cudaError_t e = unit == 16 ? run(uint4{}, compact_apply_kernel<uint4>) : unit == 4 ? run(uint32_t{}, compact_apply_kernel<uint32_t>)
-                                                                                             : run(uint8_t{}, compact_apply_kernel<uint8_t>);
+    const cudaError_t e = unit == 16 ? run(uint4{}, compact_apply_kernel<uint4, true>, compact_apply_kernel<uint4, false>)
+        : unit == 4                 ? run(uint32_t{}, compact_apply_kernel<uint32_t, true>, compact_apply_kernel<uint32_t, false>)
+                                    : run(uint8_t{}, compact_apply_kernel<uint8_t, true>, compact_apply_kernel<uint8_t, false>);
     (void) e;// reported by the check below
     return check_launch("paged cache compact");
 }

@@ -128,6 +128,11 @@ __device__ __forceinline__ uint16_t f32x2_to_e4m3x2(float lo, float hi) {
     return r;
 }
 
+// a / b of values that mostly fit 32 bits (a 64-bit division takes a few hundred cycles)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t) ((uint32_t) a / (uint32_t) b) : a / b;
+}
+
 // Largest finite magnitudes of two 16-bit floats, as bit patterns per half (the patterns of one sign are ordered like
 // the values); infinities and NaN count as zero.
 template<bool BF>

@@ -296,7 +296,7 @@ INFINIOP_API infiniopStatus_t infiniopDestroyAttentionDescriptor(infiniopAttenti
  *                      positions seq_lens[b] - n .. seq_lens[b] - 1 of b.  May
  *                      be NULL where every sequence has one new token (rows ==
  *                      batch).  Rows behind the last sequence's are left alone.
- * dh <= 256; columns * page_size < 2^31.  Table entries behind a sequence's
+ * dh <= 256, page_size < 2^22, columns * page_size < 2^31.  Table entries behind a sequence's
  * last page are never read.  Values that lead nowhere do no harm: a page id
  * outside the pool is a page whose tokens are masked (attention) or dropped
  * (append, copy, compact), offsets outside the rows are clamped, tokens beyond

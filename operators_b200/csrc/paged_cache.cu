@@ -121,26 +121,23 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     const PoolStrides st = is_v ? p.c.v : p.c.k;
     const int64_t x_st = is_v ? p.v_st : p.k_st;
     const uint16_t *x = (is_v ? p.v + (int64_t) head * p.v_sh : p.k + (int64_t) head * p.k_sh) + (int64_t) (s.first + (p0 - (s.len - s.n))) * x_st;
-    // the new rows: into registers, and their largest finite magnitude
-    const uint32_t per_row = (uint32_t) (D / VEC);
-    const int64_t nv = (int64_t) m * per_row;
+    // the new rows: into registers, and their largest magnitude.  (A block has fewer than 2^31 elements.)
+    const uint32_t per_row = (uint32_t) (D / VEC), nv = (uint32_t) m * per_row, step = blockDim.x;
     uint4 held_v[kHeld];
-    uint32_t top = 0;
-    // row and element of the i-th vector of a block (below 2^32: one multiplication instead of a division)
-    auto row_of = [&](int64_t i) -> int64_t { return i <= 0xFFFFFFFFll ? (int64_t) p.per_row.div((uint32_t) i) : i / per_row; };
-    auto load = [&](int64_t i) -> uint4 {
-        const int64_t r = row_of(i);
-        const uint16_t *src = x + r * x_st + (i - r * per_row) * VEC;
+    auto load = [&](uint32_t i) -> uint4 {
+        const uint32_t r = p.per_row.div(i);
+        const uint16_t *src = x + (int64_t) r * x_st + (i - r * per_row) * VEC;
         if (VEC == 8) return *reinterpret_cast<const uint4 *>(src);
         return make_uint4(*src, 0u, 0u, 0u);
     };
+    uint32_t top = 0;
     auto grow = [&](uint4 w) {
-        top = __vmaxu2(top, finite_abs2<BF>(w.x));
-        if (VEC == 8) top = __vmaxu2(__vmaxu2(top, finite_abs2<BF>(w.y)), __vmaxu2(finite_abs2<BF>(w.z), finite_abs2<BF>(w.w)));
+        top = abs_max2<BF>(top, w.x);
+        if (VEC == 8) top = abs_max2<BF>(abs_max2<BF>(abs_max2<BF>(top, w.y), w.z), w.w);
     };
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-        const int64_t i = threadIdx.x + (int64_t) j * blockDim.x;
+        const uint32_t i = threadIdx.x + (uint32_t) j * step;
         held_v[j] = i < nv ? load(i) : make_uint4(0u, 0u, 0u, 0u);
     }
     if (page < 0 || page >= p.c.pages) return;
@@ -149,27 +146,38 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     const float old = kept > 0 ? *scale : 0.f;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) grow(held_v[j]);
-    for (int64_t i = threadIdx.x + (int64_t) kHeld * blockDim.x; i < nv; i += blockDim.x) grow(load(i));
-    top = __vmaxu2(top, top >> 16) & 0xFFFFu;
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (uint32_t w = 0; w < blockDim.x / 32; ++w) top = max(top, wmax[w]);
+    for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) grow(load(i));
+    const uint32_t kInf = BF ? 0x7F80u : 0x7C00u;
+    auto block_max = [&]() {// patterns of one sign are ordered like their values
+        top = max(top & 0xFFFFu, top >> 16);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) wmax[threadIdx.x >> 5] = top;
+        __syncthreads();
+        for (uint32_t w = 0; w < step / 32; ++w) top = max(top, wmax[w]);
+    };
+    block_max();
+    if (top >= kInf) {
+        // an infinity (NaN is passed over by the maximum): once more, finite elements only
+        __syncthreads();
+        top = 0;
+        for (uint32_t i = threadIdx.x; i < nv; i += step) {
+            const uint4 w = load(i);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < (VEC == 8 ? 4 : 1); ++j) top = __vmaxu2(top, finite_abs2<BF>(words[j]));
+        }
+        block_max();
+    }
     const float amax = BF ? __uint_as_float(top << 16) : f16_to_f32((uint16_t) top);
-    const int32_t e = scale_exponent(__float_as_uint(amax));
-    const float fresh = __uint_as_float(pow2_bits(e)), now = fmaxf(old, fresh);
-    // 1 / now: exact for powers of two (an old scale that is none is divided by as it stands)
-    const bool pow2 = (__float_as_uint(now) & 0x7FFFFFu) == 0;
-    const float inv = 1.f / now;
-    auto code2 = [&](float2 f) -> uint32_t { return pow2 ? f32x2_to_e4m3x2(f.x * inv, f.y * inv) : f32x2_to_e4m3x2(f.x / now, f.y / now); };
+    const float fresh = __uint_as_float(pow2_bits(scale_exponent(__float_as_uint(amax)))), now = fmaxf(old, fresh);
 
     // rows that stay, where the scale has grown
     if (kept > 0 && now != old) {
         const float ratio = old / now;
-        const int64_t n = (int64_t) kept * per_row;
-        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const int64_t r = row_of(i);
-            uint8_t *at = codes + r * st.sp + (i - r * per_row) * VEC;
+        const uint32_t n = (uint32_t) kept * per_row;
+        for (uint32_t i = threadIdx.x; i < n; i += step) {
+            const uint32_t r = p.per_row.div(i);
+            uint8_t *at = codes + (int64_t) r * st.sp + (i - r * per_row) * VEC;
             if (VEC == 8) {
                 uint2 w = *reinterpret_cast<uint2 *>(at);
                 uint32_t out[2] = {w.x, w.y};
@@ -185,23 +193,33 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
             }
         }
     }
-    // the new rows
-    auto store = [&](int64_t i, uint4 w) {
-        const int64_t r = row_of(i);
-        uint8_t *at = codes + (kept + r) * st.sp + (i - r * per_row) * VEC;
-        if (VEC == 8) {
-            *reinterpret_cast<uint2 *>(at) = make_uint2(code2(f16or_bf16x2<BF>(w.x)) | (code2(f16or_bf16x2<BF>(w.y)) << 16),
-                                                        code2(f16or_bf16x2<BF>(w.z)) | (code2(f16or_bf16x2<BF>(w.w)) << 16));
-        } else {
-            *at = (uint8_t) code2(f16or_bf16x2<BF>(w.x));
-        }
-    };
+    // the new rows.  `code2`: two elements to two codes
+    auto write = [&](auto code2) {
+        auto store = [&](uint32_t i, uint4 w) {
+            const uint32_t r = p.per_row.div(i);
+            uint8_t *at = codes + (int64_t) (kept + (int32_t) r) * st.sp + (i - r * per_row) * VEC;
+            if (VEC == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(code2(w.x) | (code2(w.y) << 16), code2(w.z) | (code2(w.w) << 16));
+            else *at = (uint8_t) code2(w.x);
+        };
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-        const int64_t i = threadIdx.x + (int64_t) j * blockDim.x;
-        if (i < nv) store(i, held_v[j]);
+        for (int j = 0; j < kHeld; ++j) {
+            const uint32_t i = threadIdx.x + (uint32_t) j * step;
+            if (i < nv) store(i, held_v[j]);
+        }
+        for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) store(i, load(i));
+    };
+    if ((__float_as_uint(now) & 0x7FFFFFu) == 0) {
+        const float inv = 1.f / now;// exact, and so are the products
+        write([&](uint32_t w) -> uint32_t {
+            const float2 f = f16or_bf16x2<BF>(w);
+            return f32x2_to_e4m3x2(f.x * inv, f.y * inv);
+        });
+    } else {// an old scale that is no power of two
+        write([&](uint32_t w) -> uint32_t {
+            const float2 f = f16or_bf16x2<BF>(w);
+            return f32x2_to_e4m3x2(f.x / now, f.y / now);
+        });
     }
-    for (int64_t i = threadIdx.x + (int64_t) kHeld * blockDim.x; i < nv; i += blockDim.x) store(i, load(i));
     if (threadIdx.x == 0) *scale = now;// (every read of the old scale lies before the barrier)
 }
 

@@ -64,7 +64,7 @@ static inline infiniopStatus_t check_cache(const TensorDescriptor *kp, const Ten
         if (ks->shape[i] != kp->shape[i] || vs->shape[i] != kp->shape[i]) return STATUS_BAD_TENSOR_SHAPE;
     }
     if (kp->shape[0] > 0x7FFFFFFFull || kp->shape[1] == 0 || kp->shape[1] > 0xFFFFull || kp->shape[2] == 0 ||
-        kp->shape[2] > 0x3FFFFFFFull || kp->shape[3] == 0 || kp->shape[3] > 256) {
+        kp->shape[2] > 0x3FFFFFull || kp->shape[3] == 0 || kp->shape[3] > 256) {
         return STATUS_BAD_TENSOR_SHAPE;
     }
     if (!dt_eq(kp->dt, F8E4M3) || !dt_eq(vp->dt, F8E4M3) || !dt_eq(ks->dt, F32) || !dt_eq(vs->dt, F32)) {
@@ -139,6 +139,14 @@ template<bool BF>
 __device__ __forceinline__ uint32_t finite_abs2(uint32_t w) {
     const uint32_t inf = BF ? 0x7F807F80u : 0x7C007C00u, a = w & 0x7FFF7FFFu;
     return a & ~__vcmpgeu2(a, inf);
+}
+// max(top, |w|) per half; NaN in w is passed over
+template<bool BF>
+__device__ __forceinline__ uint32_t abs_max2(uint32_t top, uint32_t w) {
+    uint32_t r;
+    if (BF) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(top), "r"(w & 0x7FFF7FFFu));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(top), "r"(w & 0x7FFF7FFFu));
+    return r;
 }
 template<bool BF>
 __device__ __forceinline__ float2 f16or_bf16x2(uint32_t w) {

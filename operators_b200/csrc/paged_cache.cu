@@ -8,7 +8,8 @@
 // e4m3 carries its own exponent, so a power of two costs no precision against an exact 448 / max (the step relative to
 // the value is the same in every binade), division by it is exact, and when the scale of a half-filled page grows the
 // kept codes only move in their exponent: nothing is lost but bits of codes that become subnormal, however often it
-// happens.  One CTA owns a block: it reads the new rows once into registers, takes the maximum, and writes codes.
+// happens.  One CTA owns the K and the V block of a page and head (the page is looked up once, and both blocks' loads are
+// under way together): it reads the new rows once into registers, takes the maxima, and writes codes.
 //
 // Copy and compact move whole pages; compact first finds the live pages (one cluster, a bitmap in the workspace).
 #include "paged_cache.cuh"
@@ -29,7 +30,7 @@ struct AppendParams {
     float *ks, *vs;
     const int32_t *table, *lens, *offs;
     int32_t rows;
-    FastDiv per_row;// by the vectors of a row
+    FastDiv per_row, page_div;// by the vectors of a row and by the page size
     CacheShape c;
     TableShape t;
 };
@@ -61,29 +62,29 @@ __device__ __forceinline__ int32_t cta_exclusive_sum(int32_t v, int32_t *slot, i
 // VEC new elements of one row at a time: 8 (16-byte loads, 8-byte stores of codes) or 1.
 template<bool BF, int VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
-    __shared__ uint32_t wmax[kAppendThreads / 32];
+    __shared__ uint32_t wmax[2][kAppendThreads / 32];
     const int32_t item = (int32_t) blockIdx.x, head = (int32_t) blockIdx.y;
-    const bool is_v = blockIdx.z != 0;
     const int32_t P = p.c.page, D = p.c.dh, lane = (int32_t) (threadIdx.x & 31);
 
-    // the item-th touched page of the call: sequence b, its nth page.  Every warp looks for it by itself, 128 sequences at
-    // a time (no barrier ahead of the loads).
+    // the item-th touched page of the call: sequence b, its nth page.  Every warp looks for it by itself (no barrier ahead
+    // of the loads), a sequence per lane, four where there are many.
     int32_t b = item, nth = 0;// one token, one page per sequence
     if (p.offs == nullptr) {
         if (b >= p.t.batch) return;
     } else {
+        const int32_t each = p.t.batch <= 32 ? 1 : 4;
         int32_t base = 0;
         bool hit = false;
-        for (int32_t b0 = 0; b0 < p.t.batch && !hit; b0 += 128) {
+        for (int32_t b0 = 0; b0 < p.t.batch && !hit; b0 += 32 * each) {
             int32_t count[4], mine = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int32_t x = b0 + lane * 4 + i;
+                const int32_t x = b0 + lane * each + i;
                 count[i] = 0;
-                if (x < p.t.batch) {
+                if (i < each && x < p.t.batch) {
                     int32_t lo, hi;
                     written(seq_of(p.lens, p.offs, p.rows, x), p.t.cap, lo, hi);
-                    count[i] = pages_touched(lo, hi, P);
+                    if (hi > lo) count[i] = (int32_t) (p.page_div.div((uint32_t) hi - 1) - p.page_div.div((uint32_t) lo)) + 1;
                 }
                 mine += count[i];
             }
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                 const int32_t u = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += u;
             }
-            int32_t before = base + incl - mine;
+            const int32_t before = base + incl - mine;
             const uint32_t who = __ballot_sync(0xffffffffu, item >= before && item - before < mine);
             if (who != 0) {
                 int32_t f = 0, k = item - before;
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
                     if (f == i && k >= count[i]) k -= count[i], f = i + 1;
                 }
                 const int src = __ffs((int) who) - 1;
-                b = b0 + src * 4 + __shfl_sync(0xffffffffu, f, src), nth = __shfl_sync(0xffffffffu, k, src);
+                b = b0 + src * each + __shfl_sync(0xffffffffu, f, src), nth = __shfl_sync(0xffffffffu, k, src);
                 hit = true;
             }
             base += __shfl_sync(0xffffffffu, incl, 31);
@@ -113,114 +114,131 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     int32_t lo, hi;
     written(s, p.t.cap, lo, hi);
     if (hi <= lo) return;
-    const int32_t col = lo / P + nth, page0 = col * P;
+    const int32_t col = (int32_t) p.page_div.div((uint32_t) lo) + nth, page0 = col * P;
     const int32_t p0 = lo > page0 ? lo : page0, p1 = hi - page0 < P ? hi : page0 + P;
     const int32_t page = p.table[(int64_t) b * p.t.stride + col];// (looked at once the new rows are on their way)
     const int32_t kept = p0 - page0, m = p1 - p0;
 
-    const PoolStrides st = is_v ? p.c.v : p.c.k;
-    const int64_t x_st = is_v ? p.v_st : p.k_st;
-    const uint16_t *x = (is_v ? p.v + (int64_t) head * p.v_sh : p.k + (int64_t) head * p.k_sh) + (int64_t) (s.first + (p0 - (s.len - s.n))) * x_st;
-    // the new rows: into registers, and their largest magnitude.  (A block has fewer than 2^31 elements.)
+    const int64_t row0 = s.first + (p0 - (s.len - s.n));
+    const uint16_t *x[2] = {p.k + row0 * p.k_st + (int64_t) head * p.k_sh, p.v + row0 * p.v_st + (int64_t) head * p.v_sh};
+    const int64_t x_st[2] = {p.k_st, p.v_st};
+
+    // the new rows: into registers, and their largest magnitudes.  (A block has fewer than 2^31 elements.)
     const uint32_t per_row = (uint32_t) (D / VEC), nv = (uint32_t) m * per_row, step = blockDim.x;
-    uint4 held_v[kHeld];
-    auto load = [&](uint32_t i) -> uint4 {
+    uint4 held_v[2][kHeld];
+    auto load = [&](int side, uint32_t i) -> uint4 {
         const uint32_t r = p.per_row.div(i);
-        const uint16_t *src = x + (int64_t) r * x_st + (i - r * per_row) * VEC;
+        const uint16_t *src = x[side] + (int64_t) r * x_st[side] + (i - r * per_row) * VEC;
         if (VEC == 8) return *reinterpret_cast<const uint4 *>(src);
         return make_uint4(*src, 0u, 0u, 0u);
     };
-    uint32_t top = 0;
-    auto grow = [&](uint4 w) {
-        top = abs_max2<BF>(top, w.x);
-        if (VEC == 8) top = abs_max2<BF>(abs_max2<BF>(abs_max2<BF>(top, w.y), w.z), w.w);
+    uint32_t top[2] = {0u, 0u};
+    auto grow = [&](int side, uint4 w) {
+        top[side] = abs_max2<BF>(top[side], w.x);
+        if (VEC == 8) top[side] = abs_max2<BF>(abs_max2<BF>(abs_max2<BF>(top[side], w.y), w.z), w.w);
     };
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
         const uint32_t i = threadIdx.x + (uint32_t) j * step;
-        held_v[j] = i < nv ? load(i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int side = 0; side < 2; ++side) held_v[side][j] = i < nv ? load(side, i) : make_uint4(0u, 0u, 0u, 0u);
     }
     if (page < 0 || page >= p.c.pages) return;
-    uint8_t *codes = (is_v ? p.vp : p.kp) + (int64_t) page * st.sn + (int64_t) head * st.sh;
-    float *scale = (is_v ? p.vs : p.ks) + (int64_t) page * st.cn + (int64_t) head * st.ch;
-    const float old = kept > 0 ? *scale : 0.f;
+    uint8_t *codes[2] = {p.kp + (int64_t) page * p.c.k.sn + (int64_t) head * p.c.k.sh, p.vp + (int64_t) page * p.c.v.sn + (int64_t) head * p.c.v.sh};
+    const int64_t sp[2] = {p.c.k.sp, p.c.v.sp};
+    float *scale[2] = {p.ks + (int64_t) page * p.c.k.cn + (int64_t) head * p.c.k.ch, p.vs + (int64_t) page * p.c.v.cn + (int64_t) head * p.c.v.ch};
+    const float old[2] = {kept > 0 ? *scale[0] : 0.f, kept > 0 ? *scale[1] : 0.f};
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) grow(held_v[j]);
-    for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) grow(load(i));
+    for (int side = 0; side < 2; ++side) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) grow(side, held_v[side][j]);
+        for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) grow(side, load(side, i));
+    }
     const uint32_t kInf = BF ? 0x7F80u : 0x7C00u;
     auto block_max = [&]() {// patterns of one sign are ordered like their values
-        top = max(top & 0xFFFFu, top >> 16);
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) wmax[threadIdx.x >> 5] = top;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const uint32_t t = __reduce_max_sync(0xffffffffu, max(top[side] & 0xFFFFu, top[side] >> 16));
+            if (lane == 0) wmax[side][threadIdx.x >> 5] = t;
+        }
         __syncthreads();
-        for (uint32_t w = 0; w < step / 32; ++w) top = max(top, wmax[w]);
+        const uint32_t w = (uint32_t) lane < step / 32 ? (uint32_t) lane : 0u;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) top[side] = __reduce_max_sync(0xffffffffu, wmax[side][w]);
     };
     block_max();
-    if (top >= kInf) {
+    if (max(top[0], top[1]) >= kInf) {
         // an infinity (NaN is passed over by the maximum): once more, finite elements only
         __syncthreads();
-        top = 0;
-        for (uint32_t i = threadIdx.x; i < nv; i += step) {
-            const uint4 w = load(i);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < (VEC == 8 ? 4 : 1); ++j) top = __vmaxu2(top, finite_abs2<BF>(words[j]));
+        for (int side = 0; side < 2; ++side) {
+            uint32_t t = 0;
+            for (uint32_t i = threadIdx.x; i < nv; i += step) {
+                const uint4 w = load(side, i);
+                t = __vmaxu2(t, finite_abs2<BF>(w.x));
+                if (VEC == 8) t = __vmaxu2(__vmaxu2(t, finite_abs2<BF>(w.y)), __vmaxu2(finite_abs2<BF>(w.z), finite_abs2<BF>(w.w)));
+            }
+            top[side] = t;
         }
         block_max();
     }
-    const float amax = BF ? __uint_as_float(top << 16) : f16_to_f32((uint16_t) top);
-    const float fresh = __uint_as_float(pow2_bits(scale_exponent(__float_as_uint(amax)))), now = fmaxf(old, fresh);
-
-    // rows that stay, where the scale has grown
-    if (kept > 0 && now != old) {
-        const float ratio = old / now;
-        const uint32_t n = (uint32_t) kept * per_row;
-        for (uint32_t i = threadIdx.x; i < n; i += step) {
-            const uint32_t r = p.per_row.div(i);
-            uint8_t *at = codes + (int64_t) r * st.sp + (i - r * per_row) * VEC;
-            if (VEC == 8) {
-                uint2 w = *reinterpret_cast<uint2 *>(at);
-                uint32_t out[2] = {w.x, w.y};
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) out[j])), c = unpack2(e4m3x2_to_f16x2((uint16_t) (out[j] >> 16)));
-                    out[j] = (uint32_t) f32x2_to_e4m3x2(a.x * ratio, a.y * ratio) | ((uint32_t) f32x2_to_e4m3x2(c.x * ratio, c.y * ratio) << 16);
+    for (int side = 0; side < 2; ++side) {
+        const float amax = BF ? __uint_as_float(top[side] << 16) : f16_to_f32((uint16_t) top[side]);
+        const float fresh = __uint_as_float(pow2_bits(scale_exponent(__float_as_uint(amax)))), now = fmaxf(old[side], fresh);
+
+        // rows that stay, where the scale has grown
+        if (kept > 0 && now != old[side]) {
+            const float ratio = old[side] / now;
+            const uint32_t n = (uint32_t) kept * per_row;
+            for (uint32_t i = threadIdx.x; i < n; i += step) {
+                const uint32_t r = p.per_row.div(i);
+                uint8_t *at = codes[side] + (int64_t) r * sp[side] + (i - r * per_row) * VEC;
+                if (VEC == 8) {
+                    uint2 w = *reinterpret_cast<uint2 *>(at);
+                    uint32_t out[2] = {w.x, w.y};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) out[j])), c = unpack2(e4m3x2_to_f16x2((uint16_t) (out[j] >> 16)));
+                        out[j] = (uint32_t) f32x2_to_e4m3x2(a.x * ratio, a.y * ratio) | ((uint32_t) f32x2_to_e4m3x2(c.x * ratio, c.y * ratio) << 16);
+                    }
+                    *reinterpret_cast<uint2 *>(at) = make_uint2(out[0], out[1]);
+                } else {
+                    const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) *at));
+                    *at = (uint8_t) f32x2_to_e4m3x2(a.x * ratio, 0.f);
                 }
-                *reinterpret_cast<uint2 *>(at) = make_uint2(out[0], out[1]);
-            } else {
-                const float2 a = unpack2(e4m3x2_to_f16x2((uint16_t) *at));
-                *at = (uint8_t) f32x2_to_e4m3x2(a.x * ratio, 0.f);
             }
         }
-    }
-    // the new rows.  `code2`: two elements to two codes
-    auto write = [&](auto code2) {
-        auto store = [&](uint32_t i, uint4 w) {
+        // the new rows
+        uint8_t *first = codes[side] + (int64_t) kept * sp[side];
+        auto store = [&](uint32_t i, uint4 w, auto code2) {// `code2`: two elements to two codes
             const uint32_t r = p.per_row.div(i);
-            uint8_t *at = codes + (int64_t) (kept + (int32_t) r) * st.sp + (i - r * per_row) * VEC;
+            uint8_t *at = first + (int64_t) r * sp[side] + (i - r * per_row) * VEC;
             if (VEC == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(code2(w.x) | (code2(w.y) << 16), code2(w.z) | (code2(w.w) << 16));
             else *at = (uint8_t) code2(w.x);
         };
+        if ((__float_as_uint(now) & 0x7FFFFFu) == 0) {
+            const float inv = 1.f / now;// exact, and so are the products
+            auto code2 = [&](uint32_t w) -> uint32_t {
+                const float2 f = f16or_bf16x2<BF>(w);
+                return f32x2_to_e4m3x2(f.x * inv, f.y * inv);
+            };
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const uint32_t i = threadIdx.x + (uint32_t) j * step;
-            if (i < nv) store(i, held_v[j]);
+            for (int j = 0; j < kHeld; ++j) {
+                const uint32_t i = threadIdx.x + (uint32_t) j * step;
+                if (i < nv) store(i, held_v[side][j], code2);
+            }
+            for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) store(i, load(side, i), code2);
+        } else {// an old scale that is no power of two
+            for (uint32_t i = threadIdx.x; i < nv; i += step) {
+                store(i, load(side, i), [&](uint32_t w) -> uint32_t {
+                    const float2 f = f16or_bf16x2<BF>(w);
+                    return f32x2_to_e4m3x2(f.x / now, f.y / now);
+                });
+            }
         }
-        for (uint32_t i = threadIdx.x + kHeld * step; i < nv; i += step) store(i, load(i));
-    };
-    if ((__float_as_uint(now) & 0x7FFFFFu) == 0) {
-        const float inv = 1.f / now;// exact, and so are the products
-        write([&](uint32_t w) -> uint32_t {
-            const float2 f = f16or_bf16x2<BF>(w);
-            return f32x2_to_e4m3x2(f.x * inv, f.y * inv);
-        });
-    } else {// an old scale that is no power of two
-        write([&](uint32_t w) -> uint32_t {
-            const float2 f = f16or_bf16x2<BF>(w);
-            return f32x2_to_e4m3x2(f.x / now, f.y / now);
-        });
+        if (threadIdx.x == 0) *scale[side] = now;// (every read of the old scale lies before the barrier)
     }
-    if (threadIdx.x == 0) *scale = now;// (every read of the old scale lies before the barrier)
 }
 
 struct AppendDesc {
@@ -531,13 +549,13 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheAppend(infiniopPagedCacheAppendD
     AppendParams p{reinterpret_cast<const uint16_t *>(k), reinterpret_cast<const uint16_t *>(v), d->k_st, d->k_sh, d->v_st, d->v_sh,
                    reinterpret_cast<uint8_t *>(k_pages), reinterpret_cast<uint8_t *>(v_pages), reinterpret_cast<float *>(k_scales),
                    reinterpret_cast<float *>(v_scales), reinterpret_cast<const int32_t *>(block_table),
-                   reinterpret_cast<const int32_t *>(seq_lens), reinterpret_cast<const int32_t *>(q_offsets), d->rows, FastDiv(1), d->c, d->t};
+                   reinterpret_cast<const int32_t *>(seq_lens), reinterpret_cast<const int32_t *>(q_offsets), d->rows, FastDiv(1), FastDiv((uint32_t) d->c.page), d->c, d->t};
     // 8 elements at a time where every row of the new tokens starts on 16 bytes and every row of codes on 8
     bool vec = d->c.dh % 8 == 0 && aligned16(k) && aligned16(v) && ((uintptr_t) k_pages | (uintptr_t) v_pages) % 8 == 0;
     for (int64_t s : {d->k_st, d->k_sh, d->v_st, d->v_sh, d->c.k.sn, d->c.k.sh, d->c.k.sp, d->c.v.sn, d->c.v.sh, d->c.v.sp}) vec = vec && s % 8 == 0;
     p.per_row = FastDiv((uint32_t) (vec ? d->c.dh / 8 : d->c.dh));
     const int64_t items = d->t.offsets ? pages_bound(d->rows, d->t.batch, d->c.page) : d->rows;
-    const dim3 grid((unsigned) items, (unsigned) d->c.heads, 2);
+    const dim3 grid((unsigned) items, (unsigned) d->c.heads);
     // one token per sequence is 16 vectors of 8: a small block leaves the SM to more of them
     const unsigned threads = d->t.offsets ? kAppendThreads : 128;
     auto st = reinterpret_cast<cudaStream_t>(stream);

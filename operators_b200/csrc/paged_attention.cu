@@ -37,6 +37,8 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;      // cached tokens per warp and step
 constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
 constexpr int kPrefillRows = 32;// query rows per sequence from which on the tcgen05 kernel takes the call
+constexpr uint32_t kMaxCluster = 8;
+constexpr int64_t kClusterRounds = 4;
 constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
 constexpr float kLift = 14.f;  // weights are stored times 2^14: at most 2^(14 + slack) < 65504
 
@@ -124,6 +126,15 @@ __device__ __forceinline__ float log2_of(float v) {
     return (float) ((int32_t) (u >> 23) - 127);
 }
 
+// 16 bytes at the same place of another CTA's shared memory
+__device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t rank) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
 // The state of a warp's ring while it walks tiles first, first + kWarps, .. of one item.
 struct Walk {
     int32_t b, keys;
@@ -146,18 +157,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
     const uint32_t ring = (uint32_t) __cvta_generic_to_shared(smem) + warp * kStages * kStage;
 
     // ---- this CTA's stretch of the units
+    // (with clusters: item blockIdx.x / CTAs of a cluster, and of its tiles this CTA's share)
+    const uint32_t cl = dp.cluster, rank = cl > 0 ? blockIdx.x % cl : 0u;
     auto units_of = [&](int32_t b) -> int64_t {
         int32_t blocks, tiles;
         extent_of<kRows>(p, seq_of(p.lens, p.offs, p.rows, b), blocks, tiles);
-        return (int64_t) blocks * tiles * p.c.heads;
+        return (int64_t) blocks * (cl > 0 ? 1 : tiles) * p.c.heads;
     };
     int64_t mine = 0, total;
     for (int32_t b = (int32_t) threadIdx.x; b < p.t.batch; b += kThreads) mine += units_of(b);
     cta_exclusive_sum64<kWarps>(mine, slot, total);
-    const int64_t each = stretch_of(total, kMinUnits);
-    int64_t u = each * blockIdx.x;
+    const int64_t each = cl > 0 ? 1 : stretch_of(total, kMinUnits);
+    int64_t u = cl > 0 ? (int64_t) (blockIdx.x / cl) : each * blockIdx.x;
     const int64_t u_end = u + each < total ? u + each : total;
-    if (u >= u_end) {
+    if (u >= u_end) {// (a cluster's CTAs leave together)
+        if (cl > 0) return;
         if (threadIdx.x == 0) dp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
         asm volatile("griddepcontrol.launch_dependents;");
         return;
@@ -188,16 +202,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
         Seq s = seq_of(p.lens, p.offs, p.rows, b);
         int32_t blocks, tiles;
         extent_of<kRows>(p, s, blocks, tiles);
-        const int64_t units = (int64_t) blocks * tiles * p.c.heads;
+        const int64_t units = (int64_t) blocks * (cl > 0 ? 1 : tiles) * p.c.heads;
         if (units == 0 || u - base >= units) {// on to the next sequence (u < total: there is one)
             base += units, ++b;
             continue;
         }
-        const int64_t item = divide(u - base, tiles);
-        const int32_t t0 = (int32_t) (u - base - item * tiles);
-        const int32_t t1 = u_end - u < tiles - t0 ? t0 + (int32_t) (u_end - u) : tiles;
+        const int64_t item = cl > 0 ? u - base : divide(u - base, tiles);
+        int32_t t0, t1;
+        if (cl > 0) {
+            t0 = (int32_t) (rank * (uint32_t) tiles / cl), t1 = (int32_t) ((rank + 1) * (uint32_t) tiles / cl);
+        } else {
+            t0 = (int32_t) (u - base - item * tiles);
+            t1 = u_end - u < tiles - t0 ? t0 + (int32_t) (u_end - u) : tiles;
+        }
         const int32_t kvh = (int32_t) divide(item, blocks), rb = (int32_t) (item - (int64_t) kvh * blocks);
-        u += t1 - t0;
+        u += cl > 0 ? 1 : t1 - t0;
 
         Walk w;
         w.b = b, w.keys = held(s.len, p.t.cap);
@@ -557,8 +576,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == tiles;
+        const bool whole = cl > 0 ? cl == 1 : t0 == 0 && t1 == tiles;
         const int part = t0 > 0 ? 0 : 1;
+        float *po = reinterpret_cast<float *>(sh + kWarps * kRows);// this CTA's part, for its cluster
+        PartHead *ph = reinterpret_cast<PartHead *>(po + kRows * DHC);
         const int64_t slot0 = ((int64_t) blockIdx.x * 2 + part) * kRows;
         for (int r = (int) warp; r < n_rows; r += kWarps) {
             float mr = -INFINITY, wr = -INFINITY, lr = 0.f, f[kWarps];
@@ -571,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 f[i] = h.w == -INFINITY ? 0.f : fast_exp2(h.w - wr);
             }
             uint16_t *out = row_of_out(p, s, kvh, (uint32_t) rb * kRows + (uint32_t) r);
-            if (!whole && lane == 0) dp.heads[slot0 + r] = PartHead{mr, lr, wr - kLift, 0.f};
+            if (!whole && lane == 0) (cl > 0 ? ph[r] : dp.heads[slot0 + r]) = PartHead{mr, lr, wr - kLift, 0.f};
 #pragma unroll
             for (int j = 0; j < (DHC + 127) / 128; ++j) {
                 const uint32_t grp = lane + 32 * j;
@@ -583,8 +604,46 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     if (f[i] != 0.f) y.x += f[i] * a.x, y.y += f[i] * a.y, y.z += f[i] * a.z, y.w += f[i] * a.w;
                 }
                 if (whole) store_out(p, out, (int32_t) grp * 4, y, out_factors(lr, wr - kLift - mr));
-                else *reinterpret_cast<float4 *>(dp.parts + (slot0 + r) * DHC + grp * 4) = y;
+                else *reinterpret_cast<float4 *>(cl > 0 ? po + r * DHC + grp * 4 : dp.parts + (slot0 + r) * DHC + grp * 4) = y;
             }
+        }
+        if (cl > 1) {
+            // the CTAs of the cluster meet: each adds the parts of its share of the rows, in the order of the tiles
+            cluster_sync_all();
+            const uint32_t po_at = (uint32_t) __cvta_generic_to_shared(po), ph_at = (uint32_t) __cvta_generic_to_shared(ph);
+            for (int r = (int) (rank + cl * warp); r < n_rows; r += (int) (cl * kWarps)) {
+                float mr = -INFINITY, wr = -INFINITY, lr = 0.f;
+                PartHead h[kMaxCluster];
+#pragma unroll
+                for (uint32_t i = 0; i < kMaxCluster; ++i) {
+                    h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0.f};
+                    if (i < cl) {
+                        const float4 v = ld_cluster4(ph_at + (uint32_t) r * 16u, i);
+                        h[i] = PartHead{v.x, v.y, v.z, v.w};
+                    }
+                    mr = fmaxf(mr, h[i].m), wr = fmaxf(wr, h[i].w);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kMaxCluster; ++i) lr += h[i].m == -INFINITY ? 0.f : h[i].l * fast_exp2(h[i].m - mr);
+                uint16_t *out = row_of_out(p, s, kvh, (uint32_t) rb * kRows + (uint32_t) r);
+#pragma unroll
+                for (int j = 0; j < (DHC + 127) / 128; ++j) {
+                    const uint32_t grp = lane + 32 * j;
+                    if (DHC == 64 && grp >= 16) break;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (uint32_t i = 0; i < kMaxCluster; ++i) {
+                        if (i < cl && h[i].w != -INFINITY) {
+                            const float f = fast_exp2(h[i].w - wr);
+                            const float4 a = ld_cluster4(po_at + ((uint32_t) r * DHC + grp * 4) * 4u, i);
+                            y.x += f * a.x, y.y += f * a.y, y.z += f * a.z, y.w += f * a.w;
+                        }
+                    }
+                    store_out(p, out, (int32_t) grp * 4, y, out_factors(lr, wr - mr));
+                }
+            }
+            cluster_sync_all();// nobody leaves while its part may still be read
+            return;
         }
         if (!whole && part == 1) {
             meta.b = b, meta.kvh = kvh, meta.rb = rb;
@@ -600,6 +659,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             }
         }
     }
+    if (cl > 0) return;
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) dp.meta[blockIdx.x] = meta;
 }
@@ -616,16 +676,18 @@ struct AttendDesc {
     int dhc;      // head size rounded up to 64, 128 or 256
     int block;    // query rows per item: 8 or 16 (mma.sync), 128 or 256 (tcgen05)
     uint32_t ctas;
+    uint32_t cluster;// CTAs that share an item over distributed shared memory; 0: equal stretches, joined by a second kernel
 };
 
-uint64_t workspace_of_desc(const AttendDesc &d) { return split_bytes(d.ctas, (uint64_t) d.block, (uint64_t) d.dhc); }
+uint64_t workspace_of_desc(const AttendDesc &d) { return d.cluster > 0 ? 0 : split_bytes(d.ctas, (uint64_t) d.block, (uint64_t) d.dhc); }
 
 template<int DHC, int NT, bool ONE>
 cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
     constexpr int kSmem = smem_bytes(DHC, NT);
-    static_assert(kWarps * 8 * NT * DHC * 4 + kWarps * 8 * NT * (int) sizeof(PartHead) <= kSmem, "the warps' results fit their rings");
+    static_assert((kWarps + 1) * 8 * NT * (DHC * 4 + (int) sizeof(PartHead)) <= kSmem, "the warps' results and their sum fit the rings");
     static_assert(stage_bytes(DHC) % 16 == 0, "stages start on 16 bytes");
-    const SplitParams dp = split_params(a, workspace, d.ctas, 8 * NT, DHC);
+    SplitParams dp = split_params(a, workspace, d.ctas, 8 * NT, DHC);
+    dp.cluster = d.cluster;
     // more shared memory than the default: asked for once per device (again, where two threads come first)
     static std::atomic<uint64_t> ready{0};
     const uint64_t bit = d.device_id < 64 ? 1ull << d.device_id : 0;
@@ -635,6 +697,7 @@ cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *w
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
+    if (d.cluster > 0) return launch_cluster_smem(decode_kernel<DHC, NT, ONE>, d.ctas, kThreads, d.cluster, kSmem, st, dp);
     decode_kernel<DHC, NT, ONE><<<d.ctas, kThreads, kSmem, st>>>(dp);
     e = cudaGetLastError();
     if (e != cudaSuccess || d.ctas == 1) return e;
@@ -689,6 +752,16 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     if (blocks * d.c.heads < places * kMinUnits) {
         d.ctas = (uint32_t) std::max<int64_t>(1, std::min(places, (blocks * d.c.heads * tiles + kMinUnits - 1) / kMinUnits));
     }
+    // Few items over a table of few columns: a cluster of CTAs per item, one launch.  A CTA of four warps takes up to
+    // kClusterRounds tiles per warp; beyond that equal stretches over all SMs are faster although they take a second launch.
+    d.cluster = 0;
+    if (!prefill) {
+        const int64_t exact = d.t.offsets ? blocks : (int64_t) d.t.batch * ((group + d.block - 1) / d.block);
+        const int64_t items = exact * d.c.heads;
+        uint32_t c = 1;
+        while (c < kMaxCluster && items * c * 2 <= places && tiles > (int64_t) c * kWarps) c *= 2;
+        if (items <= places && tiles <= (int64_t) c * kWarps * kClusterRounds) d.cluster = c, d.ctas = (uint32_t) (items * c);
+    }
     auto *r = new (std::nothrow) AttendDesc(d);
     if (r == nullptr) return STATUS_MEMORY_NOT_ALLOCATED;
     *desc_ptr = reinterpret_cast<infiniopPagedAttentionDescriptor_t>(r);
@@ -714,7 +787,8 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     // a table without columns or a pool without pages has no keys: every token gets zeros
     const bool empty = d->t.cols == 0 || d->c.pages == 0;
     if (!empty && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || block_table == nullptr)) return STATUS_BAD_PARAM;
-    if (workspace == nullptr || workspace_size < workspace_of_desc(*d)) return STATUS_MEMORY_NOT_ALLOCATED;
+    const uint64_t need = workspace_of_desc(*d);
+    if (need > 0 && (workspace == nullptr || workspace_size < need)) return STATUS_MEMORY_NOT_ALLOCATED;
     DeviceGuard guard(d->device_id);
     AttendParams p{};
     p.out = reinterpret_cast<uint16_t *>(out), p.q = reinterpret_cast<const uint16_t *>(q);

@@ -119,6 +119,7 @@ struct SplitParams {
     float *parts;   // [cta][2][rows][DHC]: the part of an item that began before the stretch, and of one that goes on
     PartHead *heads;// [cta][2][rows]
     CtaMeta *meta;  // [cta]
+    uint32_t cluster;// decoding: CTAs of a cluster that share an item (0: equal stretches)
 };
 static inline uint64_t split_bytes(uint64_t ctas, uint64_t rows, uint64_t dhc) {
     return ctas * (2 * rows * (sizeof(PartHead) + dhc * 4) + sizeof(CtaMeta));

@@ -15,8 +15,8 @@
 //    (p . v) as its rows and the query rows as its 8 columns: the contraction is far below a tcgen05 tile.  Codes
 //    become fp16 exactly in registers.  The contraction index is only a label, so every lane reads 16 consecutive
 //    bytes of a row; for p . v the bytes of two tokens are paired with one byte permutation per 4 elements.
-//  * q in fp16 too: each row is multiplied by a power of two that brings its largest element to [2^14, 2^15), which
-//    holds every bf16 element that is not 2^-29 of the largest exactly, and is undone in the score's factor.
+//  * q in fp16 too: each bf16 row is multiplied by a power of two that brings its largest element to [2^14, 2^15), which
+//    holds every element that is not 2^-29 of the largest exactly, and is undone in the score's factor.
 //  * The running maximum m of a row moves only when a score exceeds it by more than a factor 2, so most tiles rescale
 //    nothing.  The weight of a value is w_j = p_j * (scale of v_j): its own reference M keeps fp16 weights
 //    between 2^15 and what is 2^-28 of the largest (2^-39 with subnormals), however the pages' scales differ.  Sums
@@ -37,6 +37,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;      // cached tokens per warp and step
 constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
 constexpr int kPrefillRows = 32;// query rows per sequence from which on the tcgen05 kernel takes the call
+constexpr int kItemUnits = 8;  // what the start and the end of an item cost, in tiles
 constexpr uint32_t kMaxCluster = 8;
 constexpr int64_t kClusterRounds = 4;
 constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
     auto units_of = [&](int32_t b) -> int64_t {
         int32_t blocks, tiles;
         extent_of<kRows>(p, seq_of(p.lens, p.offs, p.rows, b), blocks, tiles);
-        return (int64_t) blocks * (cl > 0 ? 1 : tiles) * p.c.heads;
+        return (int64_t) blocks * (cl > 0 ? 1 : tiles + kItemUnits) * p.c.heads;
     };
     int64_t mine = 0, total;
     for (int32_t b = (int32_t) threadIdx.x; b < p.t.batch; b += kThreads) mine += units_of(b);
@@ -202,21 +203,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
         Seq s = seq_of(p.lens, p.offs, p.rows, b);
         int32_t blocks, tiles;
         extent_of<kRows>(p, s, blocks, tiles);
-        const int64_t units = (int64_t) blocks * (cl > 0 ? 1 : tiles) * p.c.heads;
+        const int32_t size = tiles + kItemUnits;// the first kItemUnits units of an item hold no tile
+        const int64_t units = (int64_t) blocks * (cl > 0 ? 1 : size) * p.c.heads;
         if (units == 0 || u - base >= units) {// on to the next sequence (u < total: there is one)
             base += units, ++b;
             continue;
         }
-        const int64_t item = cl > 0 ? u - base : divide(u - base, tiles);
+        const int64_t item = cl > 0 ? u - base : divide(u - base, size);
         int32_t t0, t1;
         if (cl > 0) {
             t0 = (int32_t) (rank * (uint32_t) tiles / cl), t1 = (int32_t) ((rank + 1) * (uint32_t) tiles / cl);
         } else {
-            t0 = (int32_t) (u - base - item * tiles);
-            t1 = u_end - u < tiles - t0 ? t0 + (int32_t) (u_end - u) : tiles;
+            const int32_t at = (int32_t) (u - base - item * size), n = u_end - u < size - at ? (int32_t) (u_end - u) : size - at;
+            t0 = max(0, at - kItemUnits), t1 = max(0, at + n - kItemUnits);
+            u += n;
+            if (t1 == t0) continue;
         }
         const int32_t kvh = (int32_t) divide(item, blocks), rb = (int32_t) (item - (int64_t) kvh * blocks);
-        u += cl > 0 ? 1 : t1 - t0;
+        if (cl > 0) ++u;
 
         Walk w;
         w.b = b, w.keys = held(s.len, p.t.cap);
@@ -302,22 +306,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             }
         };
 
-        // ---- start the ring, then read q
-        int32_t ahead = t0 + (int32_t) warp, page = page_of(ahead);
-        __syncwarp();
-#pragma unroll 1
-        for (int i = 0; i < kStages - 1; ++i) {
-            const int32_t next = page_of(ahead + kWarps);
-            if (ahead < t1) fetch((uint32_t) i, ahead, page);
-            cp_async_commit();
-            page = next, ahead += kWarps;
-        }
-
-        // q: lane (g, t) holds the elements of row g that its chunks of a key row meet.  Row r of the block is new token
-        // (rb * kRows + r) / group, q head kvh * group + (..) % group.
-        uint32_t qf[NT][kSteps][2];
-        float factor[NT];
+        // ---- request q, start the ring, then look at q.  Lane (g, t) holds the elements of row g that its chunks of a key
+        // row meet.  Row r of the block is new token (rb * kRows + r) / group, q head kvh * group + (..) % group.
         const int32_t n_rows = min(kRows, s.n * p.group - rb * kRows);
+        uint32_t qf[NT][kSteps][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int32_t r = nt * 8 + (int32_t) g;
@@ -325,7 +317,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             const uint32_t rr = (uint32_t) rb * kRows + (uint32_t) r;
             const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0, hd = have ? (int32_t) rr - tok * p.group : 0;
             const uint16_t *q = p.q + (int64_t) (s.first + tok) * p.q_st + (int64_t) (kvh * p.group + hd) * p.q_sh;
-            uint32_t top = 0;
 #pragma unroll
             for (int h = 0; h < kHalf; ++h) {
                 const int32_t d0 = (int32_t) key_chunk<DHC>(t, (uint32_t) h) * 16;
@@ -342,26 +333,41 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    qf[nt][h * 4 + i / 2][i % 2] = x[i];
-                    top = __vmaxu2(top, x[i] & 0x7FFF7FFFu);
-                }
+                for (int i = 0; i < 8; ++i) qf[nt][h * 4 + i / 2][i % 2] = x[i];
             }
-            top = __vmaxu2(top, top >> 16) & 0xFFFFu;
+        }
+        int32_t ahead = t0 + (int32_t) warp, page = page_of(ahead);
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < kStages - 1; ++i) {
+            const int32_t next = page_of(ahead + kWarps);
+            if (ahead < t1) fetch((uint32_t) i, ahead, page);
+            cp_async_commit();
+            page = next, ahead += kWarps;
+        }
+        float factor[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) top = __vmaxu2(top, __vmaxu2(qf[nt][i][0] & 0x7FFF7FFFu, qf[nt][i][1] & 0x7FFF7FFFu));
+            top = max(top & 0xFFFFu, top >> 16);
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int32_t shift = query_shift(p.bf16, top);
             const float up = __uint_as_float(pow2_bits(shift));
+            if (p.bf16) {// (fp16 elements go as they are)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
+                for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 f = p.bf16 ? unpack2_t<kBF16>(qf[nt][i][j]) : unpack2(qf[nt][i][j]);
-                    const __half2 v = __floats2half2_rn(f.x * up, f.y * up);
-                    qf[nt][i][j] = *reinterpret_cast<const uint32_t *>(&v);
+                    for (int j = 0; j < 2; ++j) {
+                        const float2 f = unpack2_t<kBF16>(qf[nt][i][j]);
+                        const __half2 v = __floats2half2_rn(f.x * up, f.y * up);
+                        qf[nt][i][j] = *reinterpret_cast<const uint32_t *>(&v);
+                    }
                 }
             }
-            factor[nt] = __uint_as_float(pow2_bits(-shift)) * p.scale_log2;
+            factor[nt] = (p.bf16 ? __uint_as_float(pow2_bits(-shift)) : 1.f) * p.scale_log2;
         }
         // scores come as (token g, rows 2t and 2t + 1): the factors and limits of those rows
         float rf[NT][2];
@@ -647,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
         }
         if (!whole && part == 1) {
             meta.b = b, meta.kvh = kvh, meta.rb = rb;
-            meta.last = (int32_t) divide(base + (item + 1) * tiles - 1, each);
+            meta.last = (int32_t) divide(base + (item + 1) * size - 1, each);
         }
         if (u < u_end) {
             __syncthreads();// the ring is loaded again

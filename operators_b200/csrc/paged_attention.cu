@@ -36,7 +36,6 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;      // cached tokens per warp and step
 constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
-constexpr int kPrefillRows = 32;// query rows per sequence from which on the tcgen05 kernel takes the call
 constexpr int kItemUnits = 8;  // what the start and the end of an item cost, in tiles
 constexpr uint32_t kMaxCluster = 8;
 constexpr int64_t kClusterRounds = 4;
@@ -687,6 +686,20 @@ struct AttendDesc {
 
 uint64_t workspace_of_desc(const AttendDesc &d) { return d.cluster > 0 ? 0 : split_bytes(d.ctas, (uint64_t) d.block, (uint64_t) d.dhc); }
 
+// Whether the tcgen05 kernel takes a call with rows_each query rows per sequence and kv head, from what both cost in ns
+// x SMs if every sequence fills its table.  Measured over 1 and 16 sequences of 2000 to 30000 tokens and 2 to 64 new ones:
+// this kernel takes 130, 270 or 600 ns for 16 rows and 32 cached tokens at a head size of 64, 128 or 256, the other one
+// about 1050 ns for a block of rows and 64 cached tokens and 10 us more to start and end.  32 heads on 8 of 128 elements,
+// 16 sequences of 8000 tokens: 8 new tokens 122 us here and 150 us there, 16 new tokens 220 us and 153 us; one sequence of
+// 2000 tokens: 24 new ones 19 us and 28 us.
+bool prefill_is_faster(const AttendDesc &d, int64_t rows_each) {
+    if (rows_each <= 16 || d.t.batch > kPrefillMaxBatch) return false;
+    const auto cost = [&](int64_t block, int64_t keys, int64_t each) {
+        return (double) d.t.batch * (double) d.c.heads * (double) ((rows_each + block - 1) / block) * (double) (((int64_t) d.t.cap + keys - 1) / keys) * (double) each;
+    };
+    return cost(16, kTile, d.dhc == 64 ? 130 : d.dhc == 128 ? 270 : 600) > cost(prefill_rows(d.dhc), kPrefillKeys, 1050) + 10000. * d.sm_count;
+}
+
 template<int DHC, int NT, bool ONE>
 cudaError_t launch_decode_as(const AttendDesc &d, const AttendParams &a, void *workspace, cudaStream_t st) {
     constexpr int kSmem = smem_bytes(DHC, NT);
@@ -748,7 +761,7 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     if ((int64_t) d.rows * group > 0x7FFFFFFF) return STATUS_BAD_TENSOR_SHAPE;
     // query rows per sequence on average (only the device knows each one's)
     const int64_t rows_each = d.t.batch > 0 ? (int64_t) d.rows * group / d.t.batch : 0;
-    const bool prefill = rows_each > kPrefillRows && d.t.batch <= kPrefillMaxBatch;
+    const bool prefill = prefill_is_faster(d, rows_each);
     d.block = prefill ? prefill_rows(d.dhc) : rows_each > 8 ? 16 : 8;
     // every CTA that fits the GPU at once, but no more than there can be units for
     const int64_t blocks = ((int64_t) d.rows * group + d.block - 1) / d.block + d.t.batch, keys = prefill ? kPrefillKeys : kTile;

@@ -379,9 +379,18 @@ def test_refused_sizes_and_calls(host):
         size = ctypes.c_uint64()
         assert getattr(lib, "infiniopGet%sWorkspaceSize" % name)(None, ctypes.byref(size)) == DEVICE
         assert getattr(lib, "infiniopDestroy%sDescriptor" % name)(None) == DEVICE
+    # more pairs of a new token and a q head than 31 bits hold, in descriptors alone
+    t = _small(dh=1, heads=1, pages=1, page=1)
+    t["q"] = t["out"] = torch.empty(1 << 16, 1 << 15, 1, dtype=torch.float16, device="meta")
+    with pytest.raises(InfiniopError) as e:
+        ops.PagedAttentionOp(lib, handle, *[t[f] for f in OPS["attend"][1]])
+    assert e.value.status == SHAPE
     # null pointers, offsets that the descriptor does not know, a short workspace
-    for name, (op, fields) in OPS.items():
+    t = _small()
+    t["long_table"] = torch.zeros(3, 100000, dtype=torch.int32)
+    for name, (op, fields) in [*OPS.items(), ("attend", (ops.PagedAttentionOp, [f.replace("block", "long") for f in OPS["attend"][1]]))]:
         with op(lib, handle, *[t[f] for f in fields]) as o:
+            assert o.workspace is not None or name != "attend" or "long_table" not in fields
             if o.workspace is not None:
                 o.workspace_size -= 1
                 with pytest.raises(InfiniopError) as e:
@@ -555,15 +564,24 @@ def run_attend(cuda_lib, q, cache, table, lens, offs, scale, out, stream=None):
     return d[0]
 
 
+def wide(table, page):
+    """The same sequences in a table with room for 2^20 tokens each: the operator's kernels are chosen by how long a
+    sequence may become, so this is how short ones reach those for long ones."""
+    room = torch.full((table.shape[0], max(2 ** 20 // page, table.shape[1])), -7, dtype=torch.int32)
+    room[:, :table.shape[1]] = table
+    return room
+
+
 def check_attend(cuda_lib, q, cache, table, lens, offs, scale=None, out=None):
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     out = torch.full_like(q, 3.0) if out is None else out
     lens_t = torch.tensor(lens, dtype=torch.int32)
     offs_t = None if offs is None else torch.tensor(offs, dtype=torch.int32)
-    want, tol = attend_ref(q, *cache, table, lens, offs, scale, out)
-    got = run_attend(cuda_lib, q, cache, table, lens_t, offs_t, scale, out)
-    close(got, want, tol)
-    return got
+    page = cache[0].shape[2]
+    for room in (table, wide(table, page)):
+        if room is table or max(lens) > table.shape[1] * page:
+            want, tol = attend_ref(q, *cache, room, lens, offs, scale, out)
+        close(run_attend(cuda_lib, q, cache, room, lens_t, offs_t, scale, out), want, tol)
 
 
 def poison(cache, table, lens, page):
@@ -686,7 +704,7 @@ def test_attend_row_with_infinity_stays_alone(cuda_lib):
     H, P, D = 1, 32, 64
     cache = make_cache(12, H, P, D, 71)
     table = make_tables([350], P, 12, 72)
-    for new in (1, 150):
+    for new, table in ((1, table), (1, wide(table, P)), (150, table), (150, wide(table, P))):
         q = new_rows(new, 4, D, torch.float16, 73)
         clean = run_attend(cuda_lib, q, cache, table, torch.tensor([350], dtype=torch.int32), torch.tensor([0, new], dtype=torch.int32), 0.125, torch.zeros_like(q))
         bad = q.clone()
@@ -714,11 +732,54 @@ def test_attend_strided_rows(cuda_lib, new):
 
 
 @gpu
+@pytest.mark.parametrize("new", [1, 5, 40, 150])
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("course", ["up", "down", "steps", "last"])
+def test_attend_scores_that_wander(cuda_lib, course, dh, new):
+    """The running maximum rises all the way, never, by leaps, or at the very last key only."""
+    H, P, n = 1, 32, 700
+    cache = make_cache(24, H, P, dh, 161)
+    table = make_tables([n], P, 24, 162)
+    pos = np.arange(n)
+    level = {"up": pos / 10.0, "down": -pos / 10.0, "steps": 7.0 * (pos // 150), "last": np.where(pos >= n - 2, 60.0, 0.0)}[course]
+    k = cache[0].float()
+    for j in range(n):                                        # element 0 of a key holds its level, to e4m3's 4 bits
+        k[int(table[0, j // P]), 0, j % P, 0] = float(level[j])
+    cache[0].copy_(k.to(CODE))
+    cache[2].fill_(1.0 / 16)
+    q = new_rows(new, 2, dh, torch.float16, 163) * 0.1
+    q[:, :, 0] = 16.0
+    check_attend(cuda_lib, q, cache, table, [n], [0, new], scale=1.0)
+
+
+@gpu
+@pytest.mark.parametrize("kv_heads,n", [(1, 128), (1, 129), (1, 4096), (2, 300), (40, 1000), (130, 500), (500, 70), (3, 4097)])
+def test_attend_one_token_of_every_size_of_call(cuda_lib, kv_heads, n):
+    """From one head over a few tokens to more heads than the GPU has places for, with sequences of all lengths up to n."""
+    lens = [n, n // 2, 1]
+    need = sum(-(-x // 64) for x in lens)
+    cache = make_cache(need, kv_heads, 64, 64, 171)
+    check_attend(cuda_lib, new_rows(3, kv_heads, 64, torch.bfloat16, 173), cache, make_tables(lens, 64, need, 172), lens, None)
+
+
+@gpu
+@pytest.mark.parametrize("batch", [700, 4100])
+def test_attend_many_sequences(cuda_lib, batch):
+    rng = np.random.default_rng(181)
+    news = [int(x) for x in rng.integers(0, 5, batch)]
+    lens = [n + int(x) for n, x in zip(news, rng.integers(0, 40, batch))]
+    need = sum(-(-x // 16) for x in lens)
+    cache = make_cache(need, 1, 16, 8, 182)
+    offs = [0] + [int(x) for x in np.cumsum(news)]
+    check_attend(cuda_lib, new_rows(offs[-1], 24, 8, torch.float16, 183), cache, make_tables(lens, 16, need, 184), lens, offs)
+
+
+@gpu
 def test_attend_is_repeatable(cuda_lib):
     """The same call gives the same bits: partial results are joined in a fixed order."""
     cache = make_cache(300, 2, 64, 128, 91)
     table = make_tables([9000, 700], 64, 300, 92)
-    for new in (1, 100):
+    for new, table in ((1, table), (100, table), (100, wide(table, 64))):
         q = new_rows(2 * new, 8, 128, torch.bfloat16, 93)
         offs = torch.tensor([0, new, 2 * new], dtype=torch.int32)
         a, b = (run_attend(cuda_lib, q, cache, table, torch.tensor([9000, 700], dtype=torch.int32), offs, 0.09, torch.zeros_like(q)) for _ in range(2))
@@ -738,7 +799,7 @@ def test_attend_offsets_beyond_32_bits(cuda_lib):
     for pool, src in ((kp, cache[0]), (vp, cache[1])):
         pool.view(torch.uint8)[at] = src.view(torch.uint8).to(DEV)
     ks[at], vs[at] = cache[2].to(DEV), cache[3].to(DEV)
-    for new in (1, 100):
+    for new, ids in ((1, ids), (1, wide(ids, P)), (100, wide(ids, P)), (100, ids)):
         q = new_rows(new, 16, D, torch.float16, 103)
         want, tol = attend_ref(q, *cache, torch.arange(4, dtype=torch.int32)[None], [250], [0, new], 0.1, torch.zeros_like(q))
         out = torch.zeros_like(q, device=DEV)
@@ -977,7 +1038,7 @@ def test_two_streams_at_once(cuda_lib):
     H, P, D = 4, 64, 128
     cache = [to_dev(x) for x in make_cache(400, H, P, D, 151)]
     jobs = []
-    for i, (lens, new) in enumerate((([9000, 3000], 1), ([12000], 130))):
+    for i, (lens, new) in enumerate((([9000, 3000], 1), ([12000], 300))):
         table = make_tables(lens, P, 400, 152 + i).to(DEV)
         T = new * len(lens)
         q = new_rows(T, 16, D, torch.float16, 154 + i).to(DEV)

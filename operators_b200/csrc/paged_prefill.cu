@@ -46,20 +46,22 @@ using namespace tc;
 constexpr int kRows = 128, kKeys = kPrefillKeys;
 constexpr float kSlack = 13.f, kLift = 2.f;// w <= 2^15
 constexpr float kLeast = -90.f;
-constexpr float kMostWeight = 32768.f;// 2^(lift + slack)
+constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
 constexpr int kItemUnits = 4;// what the start and the end of an item cost, in tiles
 constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
 
 __host__ __device__ constexpr int blocks_at_once(int dhc) { return dhc <= 128 ? 2 : 1; }
-__host__ __device__ constexpr int threads_of(int nb) { return 128 * nb + 256 + 32; }
-// Registers per thread: at launch, and after the warpgroups have traded (the softmax holds the 64 scores of a row's tile)
-__host__ __device__ constexpr int launch_regs(int nb) { return nb == 2 ? 96 : 128; }
-__host__ __device__ constexpr int softmax_regs(int nb) { return nb == 2 ? 144 : 200; }
-__host__ __device__ constexpr int convert_regs(int nb) { return nb == 2 ? 48 : 88; }
+__host__ __device__ constexpr int threads_of(int nb) { return 128 * nb + 256; }
+// Registers per thread: at launch (all of the SM's), and after the warpgroups have traded: the softmax holds the 64 scores of
+// a row's tile and their weights.  Whole warpgroups only: a 17th warp would cost the launch 32 registers per thread.
+__host__ __device__ constexpr int launch_regs(int nb) { return nb == 2 ? 128 : 168; }
+__host__ __device__ constexpr int softmax_regs(int nb) { return nb == 2 ? 184 : 240; }
+__host__ __device__ constexpr int convert_regs(int nb) { return nb == 2 ? 88 : 152; }
+__host__ __device__ constexpr int issue_regs(int nb) { return nb == 2 ? 56 : 112; }
 __host__ __device__ constexpr bool split_fits(int nb) {
-    return 128 * nb * softmax_regs(nb) + 256 * convert_regs(nb) + 32 * launch_regs(nb) <= threads_of(nb) * launch_regs(nb);
+    return nb * softmax_regs(nb) + convert_regs(nb) + issue_regs(nb) <= (nb + 2) * launch_regs(nb) && threads_of(nb) * launch_regs(nb) <= 65536;
 }
 static_assert(split_fits(1) && split_fits(2), "the registers' split fits what the launch gave");
 
@@ -129,6 +131,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
           "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// 32 columns without the wait, and the wait
+__device__ __forceinline__ void tmem_st32_start(uint32_t taddr, const float *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+          "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]),
+          "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]),
+          "f"(r[30]), "f"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_finish() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 64 columns of this warp's 32 lanes; the load and its wait are one statement
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float *v) {
     asm volatile(
@@ -298,7 +313,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const int own = i >= kBlock ? (i - kBlock) % kBlockBars : -1;
             const bool rows = own == kQFull || own == kWFull || own == kWFull1;
             const bool codes = i == kKFull || i == kKFull1 || i == kVFull || i == kVFull1, keys = i >= kScFull && i < kBlock;
-            mbar_init(&bars[i], rows || codes ? 128u : keys ? (uint32_t) kKeys : 1u);
+            mbar_init(&bars[i], rows ? 128u : codes || keys ? 64u : 1u);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -324,7 +339,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     // the second block of an item has rows
     auto second = [&](const Segment &x) { return kNB == 2 && (uint32_t) x.s.n * (uint32_t) p.group > (uint32_t) x.rb * kItemRows + kRows; };
 
-    if (warp == kWarps - 1) {
+    if (warp >= kWarps - 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(issue_regs(kNB)));
+        if (warp == kWarps - 1) {
         // ------------------------------------------------------------ products
         // (the shuffles and votes tell the compiler what is the same in all lanes)
         const uint32_t steps = (uint32_t) (p.c.dh + 15) / 16;// of 16 head elements
@@ -386,23 +403,25 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             }
         }
         __syncwarp();
+        }
     } else if (warp >= 4 * kNB) {
-        // ------------------------------------------------------------ codes to fp16: a warpgroup for K and the scales, one for V
+        // ------------------------------------------------------------ codes to fp16: two warps for K and the scales, two for V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(convert_regs(kNB)));
         constexpr int kGroups = DHC / 64;// 4 lanes take 64 bytes of a row; 8 rows per warp and load
-        const bool is_v = warp >= 4 * kNB + 4;
-        const uint32_t c = (threadIdx.x - 128 * kNB) & 127u, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
+        constexpr int kLoads = 4;// rows per thread, 16 apart
+        const bool is_v = warp >= 4 * kNB + 2;
+        const uint32_t c = (threadIdx.x - 128 * kNB) & 63u, cw = c >> 5, c4 = lane & 3u, r0 = cw * 8 + (lane >> 2);
         uint64_t *full = bars + (is_v ? kVFull : kKFull), *empty = bars + (is_v ? kVEmpty : kKEmpty);
         const PoolStrides st = is_v ? p.c.v : p.c.k;
         const uint8_t *pool = (is_v ? p.vp : p.kp) + c4 * 16;
         // rows as TMA with 128-byte swizzle would lay them: 16-byte chunk j of row r at j ^ (r & 7); this thread's rows are
-        // r0 and r0 + 32, its chunks 2 c4 and 2 c4 + 1 of every box of 64 elements
+        // r0, r0 + 16, .., its chunks 2 c4 and 2 c4 + 1 of every box of 64 elements
         const uint32_t row_at = (is_v ? sv : sk) + r0 * 128u, chunk0 = ((2 * c4) ^ (r0 & 7u)) << 4, chunk1 = ((2 * c4 + 1) ^ (r0 & 7u)) << 4;
-        uint4 data[2][kGroups];
+        uint4 data[kLoads][kGroups];
         auto store_tile = [&](uint32_t b) {
             const uint32_t at = row_at + b * kKV;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kLoads; ++i) {
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
                     if ((q * 4 + (int32_t) c4) * 16 >= p.c.dh) continue;
@@ -410,7 +429,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     uint32_t h[8];
                     e4m3x4_to_f16x4(w.x, h[0], h[1]), e4m3x4_to_f16x4(w.y, h[2], h[3]);
                     e4m3x4_to_f16x4(w.z, h[4], h[5]), e4m3x4_to_f16x4(w.w, h[6], h[7]);
-                    const uint32_t row = at + (uint32_t) (q * (kKeys * 128) + i * (32 * 128));
+                    const uint32_t row = at + (uint32_t) (q * (kKeys * 128) + i * (16 * 128));
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + chunk0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + chunk1), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                 }
@@ -440,13 +459,13 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const uint8_t *at = head + (int64_t) max(page, 0) * st.sn + (int64_t) (in_page + (int32_t) r0) * st.sp;
                     in_page = in_page + kKeys == p.c.page ? 0 : in_page + kKeys;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < kLoads; ++i) {
 #pragma unroll
                         for (int q = 0; q < kGroups; ++q) {
                             data[i][q] = make_uint4(0u, 0u, 0u, 0u);
-                            if ((int32_t) r0 + 32 * i < left && (q * 4 + (int32_t) c4) * 16 < p.c.dh) data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
+                            if ((int32_t) r0 + 16 * i < left && (q * 4 + (int32_t) c4) * 16 < p.c.dh) data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
                         }
-                        at += 32 * st.sp;
+                        at += 16 * st.sp;
                     }
                 };
                 int32_t id = page_of(first + (int32_t) lane);
@@ -454,12 +473,15 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
                     const int32_t j = tile - first;
-                    if (j == 24) id_next = page_of(first + 32 + (int32_t) lane);
+                    if (j == 20) {
+                        const int32_t ahead = first + 32 + (int32_t) lane;
+                        id_next = ahead >= t1 || ahead * kKeys >= keys ? -1 : ids[p.page_div.div((uint32_t) (ahead * kKeys))];
+                    }
                     if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     __syncwarp();
                     store_tile(b);
                     mbar_arrive(&full[b]);
-                    if (j == 31) first += 32, id = id_next;
+                    if (j == 31) first += 32, id = id_next < p.c.pages ? id_next : -1;// (looked at long after the request)
                     if (tile + 1 < t1) load(tile + 1, __shfl_sync(0xffffffffu, id, tile + 1 - first));
                 }
             } else {
@@ -473,8 +495,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 bool key_ok = false;
                 auto load = [&](int32_t tile) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int32_t tok = tile * kKeys + (int32_t) r0 + 32 * i, page = page_of(tok);
+                    for (int i = 0; i < kLoads; ++i) {
+                        const int32_t tok = tile * kKeys + (int32_t) r0 + 16 * i, page = page_of(tok);
                         const int32_t in_page = tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page;
                         const uint8_t *at = head + (int64_t) max(page, 0) * st.sn + (int64_t) in_page * st.sp;
 #pragma unroll
@@ -497,7 +519,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             }
                         }
                     }
-                    if (!is_v && c < kKeys) {
+                    if (!is_v) {
                         const int32_t page = page_of(tile * kKeys + (int32_t) c);
                         key_ok = page >= 0;
                         ks = key_ok ? p.ks[(int64_t) page * p.c.k.cn + (int64_t) g.kvh * p.c.k.ch] : 0.f;
@@ -509,7 +531,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const uint32_t b = n & 1u;
                     if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     __syncwarp();
-                    if (cw < 2 && !is_v) {
+                    if (!is_v) {
                         TileScales &sc = scales[n % kScaleSets];
                         const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
                         sc.ks[c] = ks, sc.lv[c] = log2_of(vs);
@@ -552,6 +574,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             };
             const float *kscale = p.ks + (int64_t) g.kvh * p.c.k.ch, *vscale = p.vs + (int64_t) g.kvh * p.c.v.ch;
             int32_t first = g.t0, id = ONE ? page_of(first + (int32_t) lane) : -1, id_next = -1;
+            // (without the upper bound, so that nothing waits for the load)
+            auto page_at = [&](int32_t tile) -> int32_t { return tile >= g.t1 || tile * kKeys >= keys ? -1 : ids[p.page_div.div((uint32_t) (tile * kKeys))]; };
             float ks = id >= 0 ? kscale[(int64_t) id * p.c.k.cn] : 0.f, vs = id >= 0 ? vscale[(int64_t) id * p.c.v.cn] : 0.f, ks_next = 0.f, vs_next = 0.f;
             float rf = 0.f;
             {
@@ -628,6 +652,22 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[28 + j]);
                 return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
             };
+            // O so far is multiplied by a factor per row.  Every product into it must have completed.
+            auto scale_o = [&](float by) -> bool {
+                const bool done = mbar_wait<kSuspendNs>(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, done)) return false;
+                tc_fence_after();
+                for (int32_t c0 = 0; c0 < p.c.dh; c0 += 64) {
+                    float o[64];
+                    tmem_ld64(t_lane + 2 * kKeys + c0, o);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) o[i] *= by;
+                    tmem_st32_start(t_lane + 2 * kKeys + c0, o);
+                    tmem_st32_start(t_lane + 2 * kKeys + c0 + 32, o + 32);
+                }
+                tmem_st_finish();
+                return true;
+            };
             // The references of the rows that ask for it move to this tile's largest: O so far and the sum follow.
             auto move_references = [&](bool up, float top, float wtop, int32_t tile) -> bool {
                 const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
@@ -636,92 +676,109 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     l *= fast_exp2(m - m_new);// (from -inf: 0)
                     m = m_new, wm = wtop;
                 }
-                if (tile > g.t0 && __any_sync(0xffffffffu, up)) {
-                    // every product into O must have completed
-                    const bool done = mbar_wait<kSuspendNs>(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag);
-                    if (!__all_sync(0xffffffffu, done)) return false;
-                    tc_fence_after();
-                    for (int32_t c0 = 0; c0 < p.c.dh; c0 += 32) {
-                        float o[32];
-                        tmem_ld32(t_lane + 2 * kKeys + c0, o);
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * shrink);
-                        tmem_st32(t_lane + 2 * kKeys + c0, w);
-                    }
-                }
-                return true;
+                return tile == g.t0 || !__any_sync(0xffffffffu, up) || scale_o(shrink);
             };
             if (ONE) {
                 float lv_lane = log2_of(vs);
                 float e = 0.f, e_back = 1.f, shift = 0.f, lv_of_e = NAN;// exponent from p to w, 2^-e, e - m, and the scale (log2) they are for
+                // the tile's factor, scale and how many of its keys this row sees; formed while the tile before is worked on
+                float factor, lv;
+                int32_t left;
+                bool hidden;
+                auto look_at = [&](int32_t tile) {
+                    const int32_t j = tile - first;
+                    factor = __shfl_sync(0xffffffffu, ks, j) * rf, lv = __shfl_sync(0xffffffffu, lv_lane, j);
+                    left = __shfl_sync(0xffffffffu, id, j) >= 0 ? limit - tile * kKeys : 0;
+                    hidden = __any_sync(0xffffffffu, have && left < kKeys);
+                };
+                look_at(g.t0);
 #pragma unroll 1
                 for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
-                    const int32_t j = tile - first;
-                    if (j == 18) id_next = page_of(first + 32 + (int32_t) lane);
-                    if (j == 25) {
-                        ks_next = id_next >= 0 ? kscale[(int64_t) id_next * p.c.k.cn] : 0.f;
-                        vs_next = id_next >= 0 ? vscale[(int64_t) id_next * p.c.v.cn] : 0.f;
-                    }
-                    const float factor = __shfl_sync(0xffffffffu, ks, j) * rf, lv = __shfl_sync(0xffffffffu, lv_lane, j);
-                    // keys of the tile that this row sees
-                    const int32_t left = __shfl_sync(0xffffffffu, id, j) >= 0 ? limit - tile * kKeys : 0;
-                    const bool hidden = __any_sync(0xffffffffu, have && left < kKeys);
+                    const int32_t j = tile - first, left_now = left;
+                    const float factor_now = factor, lv_now = lv;
+                    const bool hidden_now = hidden;
                     // a row without a reference (its first keys are in this tile) looks through the tile for its largest score
                     bool move = m == -INFINITY && left > 0;
                     const bool some = __any_sync(0xffffffffu, move);
+                    auto next = [&]() {
+                        // pages and scales of the next 32 tiles: requested and looked at some tiles apart
+                        if (j == 16) id_next = page_at(first + 32 + (int32_t) lane);
+                        if (j == 22) {
+                            if (id_next >= p.c.pages) id_next = -1;
+                            ks_next = id_next >= 0 ? kscale[(int64_t) id_next * p.c.k.cn] : 0.f;
+                            vs_next = id_next >= 0 ? vscale[(int64_t) id_next * p.c.v.cn] : 0.f;
+                        }
+                        if (j == 31) first += 32, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
+                        if (tile + 1 < g.t1) look_at(tile + 1);
+                    };
                     if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
                     tc_fence_after();
                     __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
                     uint32_t w[kKeys / 2];
-                    float sum = 0.f;
+                    float sum = 0.f, most = 0.f;
                     auto exponents = [&]() {
-                        if (!(lv == lv_of_e)) {// (the references or the scale have changed)
-                            e = wm == -INFINITY ? 0.f : fmaxf(m - wm + kLift + lv, kLeast);
+                        if (!(lv_now == lv_of_e)) {// (the references or the scale have changed)
+                            e = wm == -INFINITY ? 0.f : fmaxf(m - wm + kLift + lv_now, kLeast);
                             e_back = fast_exp2(-e);
                             shift = e - (m == -INFINITY ? 0.f : m);
-                            lv_of_e = lv;
+                            lv_of_e = lv_now;
                         }
                     };
                     // weights of 16 pairs, and what they add up to in four sums
-                    auto weigh = [&](const float *x, uint32_t *to, uint64_t f2, uint64_t e2, uint64_t (&part)[2]) {
+                    auto weigh = [&](float *x, uint32_t *to, uint64_t f2, uint64_t e2, uint64_t (&part)[2]) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
-                            const float y0 = fast_exp2(a.x), y1 = fast_exp2(a.y);
-                            part[i & 1] = add2(part[i & 1], pack2f(y0, y1));
-                            to[i] = round16x2(false, y0, y1);
+                            x[2 * i] = fast_exp2(a.x), x[2 * i + 1] = fast_exp2(a.y);
+                            part[i & 1] = add2(part[i & 1], pack2f(x[2 * i], x[2 * i + 1]));
+                            to[i] = round16x2(false, x[2 * i], x[2 * i + 1]);
                         }
                     };
+                    auto add_up = [&](const uint64_t (&part)[2]) {
+                        const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
+                        sum = (s0.x + s0.y) + (s1.x + s1.y);
+                        most = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y));
+                    };
                     // Most tiles hide nothing and move no reference: their weights are formed at once, and the sums tell
-                    // whether one may have grown beyond what fp16 holds (2^(lift + slack)).  A row that finds so moves its
-                    // reference to the tile's largest score and forms its weights anew.  What a row does depends on its own
-                    // scores alone.
-                    if (!hidden && !some) {
+                    // whether one may have grown beyond what fp16 holds.  A row that finds so lets its references follow by a
+                    // power of two, which its weights (still in fp32), sum and O are divided by, exactly.  What a row does
+                    // depends on its own scores alone.
+                    if (!hidden_now && !some) {
                         float x[kKeys];
                         tmem_ld32(t_lane + b * kKeys, x);
                         tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);
                         exponents();
-                        const uint64_t f2 = pack2f(factor, factor), e2 = pack2f(shift, shift);
+                        const uint64_t f2 = pack2f(factor_now, factor_now), e2 = pack2f(shift, shift);
                         uint64_t part[2] = {0ull, 0ull};
                         weigh(x, w, f2, e2, part);
+                        next();
                         tmem_ld32_finish(x + 32);
                         weigh(x + 32, w + 16, f2, e2, part);
-                        const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
-                        sum = (s0.x + s0.y) + (s1.x + s1.y);
-                        move = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y)) > kMostWeight;
+                        add_up(part);
+                        if (__any_sync(0xffffffffu, most > kMostWeight)) {
+                            move = most > kFarWeight;
+                            const float top = fmaxf(largest(x), largest(x + 32));
+                            const int32_t up = most > kMostWeight && !move ? (int32_t) (__float_as_uint(top) >> 23) - (127 + (int32_t) kLift) : 0;
+                            const float by = __uint_as_float(pow2_bits(-up));
+#pragma unroll
+                            for (int i = 0; i < kKeys / 2; ++i) w[i] = round16x2(false, x[2 * i] * by, x[2 * i + 1] * by);
+                            sum *= by, l *= by, m += (float) up, wm += (float) up, lv_of_e = NAN;
+                            if (tile > g.t0 && !(ok = scale_o(by))) break;
+                        }
+                    } else {
+                        next();
                     }
-                    if (hidden || __any_sync(0xffffffffu, move)) {
+                    if (hidden_now || __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
                         for (int pass = 0; pass < 3; ++pass) {// (a row that has moved has weights of 2^lift at most: it ends here)
                             float x[kKeys];
                             tmem_ld64(t_lane + b * kKeys, x);
 #pragma unroll
-                            for (int i = 0; i < kKeys; ++i) x[i] = i < left ? x[i] * factor : -INFINITY;
+                            for (int i = 0; i < kKeys; ++i) x[i] = i < left_now ? x[i] * factor_now : -INFINITY;
                             if (__any_sync(0xffffffffu, move)) {
                                 const float top = fmaxf(largest(x), largest(x + 32));
-                                if (!(ok = move_references(move && top > -INFINITY, top, top + lv, tile))) break;
+                                if (!(ok = move_references(move && top > -INFINITY, top, top + lv_now, tile))) break;
                                 lv_of_e = NAN;
                             }
                             exponents();
@@ -729,9 +786,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             const uint64_t one = pack2f(1.f, 1.f), e2 = pack2f(shift, shift);
                             weigh(x, w, one, e2, part);
                             weigh(x + 32, w + 16, one, e2, part);
-                            const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
-                            sum = (s0.x + s0.y) + (s1.x + s1.y);
-                            move = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y)) > kMostWeight;
+                            add_up(part);
+                            move = most > kMostWeight;
                             if (!__any_sync(0xffffffffu, move)) break;
                         }
                     }
@@ -741,7 +797,6 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     tmem_st32(t_lane + b * kKeys, w);
                     tc_fence_before();
                     mbar_arrive(&own[kWFull + b]);
-                    if (j == 31) first += 32, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                 }
             } else {
                 // pages that end inside a tile: a factor, a scale and a mask bit per key, from shared memory

@@ -79,8 +79,11 @@ struct TileScales {
 
 __host__ __device__ constexpr uint32_t q_bytes(int dhc) { return (uint32_t) dhc * 2 * kRows; }// of one block
 __host__ __device__ constexpr uint32_t kv_bytes(int dhc) { return (uint32_t) dhc * 2 * kKeys; }
-__host__ __device__ constexpr uint32_t tile_bytes(int dhc) { return (uint32_t) blocks_at_once(dhc) * q_bytes(dhc) + 4 * kv_bytes(dhc); }
+// q of an item and, where it fits, of the next one
+__host__ __device__ constexpr uint32_t q_buffers(int dhc) { return dhc <= 128 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t tile_bytes(int dhc) { return q_buffers(dhc) * (uint32_t) blocks_at_once(dhc) * q_bytes(dhc) + 4 * kv_bytes(dhc); }
 __host__ __device__ constexpr uint32_t smem_bytes(int dhc) { return tile_bytes(dhc) + kScaleSets * (uint32_t) sizeof(TileScales) + kBars * 8 + 32; }
+static_assert(smem_bytes(64) <= 232448 && smem_bytes(128) <= 232448 && smem_bytes(256) <= 232448, "a CTA's shared memory");
 static_assert(kPrefillMaxBatch * 8 <= tile_bytes(64), "the sequences' unit counts fit the tiles' memory");
 
 // Products issued by a warp as a whole, the instruction itself by its elected lane: D[tmem] (+)= A * B[smem desc], A from
@@ -246,7 +249,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         if (threadIdx.x == 0) atomicAdd(&g_tc_gemm_timeouts, 1ull), sp.meta[blockIdx.x] = CtaMeta{-1, 0, 0, 0};
         return;
     }
-    const uint32_t sq = smem_u32(smem), sk = sq + kNB * kQ, sv = sk + 2 * kKV;
+    constexpr uint32_t kQBufs = q_buffers(DHC);
+    const uint32_t sq = smem_u32(smem), sk = sq + kQBufs * kNB * kQ, sv = sk + 2 * kKV;
     TileScales *scales = reinterpret_cast<TileScales *>(smem + tile_bytes(DHC));
     uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kScaleSets);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
@@ -326,9 +330,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     __syncthreads();// (the sums are read, the tiles' memory is free)
     tc_fence_after();
     if (p.c.dh < DHC) {
-        // head elements beyond dh: zeros that no product's operand overwrites
-        for (uint32_t i = threadIdx.x * 16; i < tile_bytes(DHC); i += kThreads * 16) {
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sq + i), "r"(0) : "memory");
+        // codes of head elements beyond dh: zeros that nothing overwrites
+        for (uint32_t i = threadIdx.x * 16; i < 4 * kKV; i += kThreads * 16) {
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sk + i), "r"(0) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 const uint32_t sb = (bn[x] + ahead) & 1u;
 #pragma unroll 1
                 for (uint32_t box = 0; box * 4 < steps; ++box) {// 64 elements (four products) at a time
-                    const uint64_t dqb = dq + ((x * kQ + box * (kRows * 128u)) >> 4), dkb = dk + ((b * kKV + box * (kKeys * 128u)) >> 4);
+                    const uint64_t dqb = dq + ((((kQBufs == 2 ? (bseg[x] - 1) & 1u : 0u) * kNB + x) * kQ + box * (kRows * 128u)) >> 4), dkb = dk + ((b * kKV + box * (kKeys * 128u)) >> 4);
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
                         if (box * 4 + k < steps) umma_f16_ss(tm + x * 256u + sb * kKeys, dqb + 2 * k, dkb + 2 * k, idesc_s, (box | k) > 0 ? 1u : 0u, lead);
@@ -548,98 +552,142 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         // ------------------------------------------------------------ softmax and epilogue: a thread per row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(kNB)));
         const uint32_t blk = warp >> 2, quarter = warp & 3u, r = quarter * 32u + lane;// row of the block
-        const uint32_t t_lane = tmem + blk * 256u + ((quarter * 32u) << 16), myq = sq + blk * kQ;
+        const uint32_t t_lane = tmem + blk * 256u + ((quarter * 32u) << 16);
         uint64_t *own = bars + kBlock + blk * kBlockBars;
         CtaMeta meta{-1, 0, 0, 0};
         bool ok = true;
         uint32_t n_all = 0, n = 0;// tiles of the stretch, and of them this block's
-        while (ok && walk.next(g)) {
-            if (blk == 1 && !second(g)) {
-                n_all += (uint32_t) (g.t1 - g.t0);
-                continue;
+        // the next item with rows in this block; tiles of those without
+        auto next_item = [&](Segment &x, uint32_t &skipped) -> bool {
+            skipped = 0;
+            while (walk.next(x)) {
+                if (blk == 0 || second(x)) return true;
+                skipped += (uint32_t) (x.t1 - x.t0);
             }
-            const Seq s = g.s;
-            const uint32_t rows = (uint32_t) s.n * (uint32_t) p.group, rr0 = (uint32_t) g.rb * kItemRows + blk * kRows;// first row of the block
-            const uint32_t rr = rr0 + r;
-            const bool have = rr < rows;
-            const int32_t tok = have ? (int32_t) p.group_div.div(rr) : 0;
-            const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
-            // ONE: the pages and scales of 32 tiles in the lanes, as in the converting warps (requested ahead of q)
-            const int32_t *ids = p.table + (int64_t) g.b * p.t.stride;
-            const int32_t keys = held(s.len, p.t.cap);
-            auto page_of = [&](int32_t tile) -> int32_t {
-                if (tile >= g.t1 || tile * kKeys >= keys) return -1;
-                const int32_t x = ids[p.page_div.div((uint32_t) (tile * kKeys))];
-                return x >= 0 && x < p.c.pages ? x : -1;
-            };
-            const float *kscale = p.ks + (int64_t) g.kvh * p.c.k.ch, *vscale = p.vs + (int64_t) g.kvh * p.c.v.ch;
-            int32_t first = g.t0, id = ONE ? page_of(first + (int32_t) lane) : -1, id_next = -1;
-            // (without the upper bound, so that nothing waits for the load)
-            auto page_at = [&](int32_t tile) -> int32_t { return tile >= g.t1 || tile * kKeys >= keys ? -1 : ids[p.page_div.div((uint32_t) (tile * kKeys))]; };
-            float ks = id >= 0 ? kscale[(int64_t) id * p.c.k.cn] : 0.f, vs = id >= 0 ? vscale[(int64_t) id * p.c.v.cn] : 0.f, ks_next = 0.f, vs_next = 0.f;
-            float rf = 0.f;
-            {
-                // q: a warp takes its 32 rows, a row's 16-byte pieces side by side in the lanes, into swizzled shared memory.
-                // fp16 rows go as they are; bf16 rows are multiplied by a power of two after their largest magnitude.  The
-                // sign of the scale goes with q, so that the factor of the scores is not negative.  (Every product of the
-                // item before is done.)
-                constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer, kBatch = 32 / kAtOnce < 8 ? 32 / kAtOnce : 8;// lanes per row, rows per load, loads in flight
-                const int32_t d = (int32_t) (lane % kPer) * 8;
-                const bool vec = p.q_vec && p.c.dh % 8 == 0;
-                const int64_t mine = (int64_t) (s.first + tok) * p.q_st + (int64_t) (g.kvh * p.group + (have ? (int32_t) rr - tok * p.group : 0)) * p.q_sh;
-                const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-                rf = fabsf(p.scale_log2);
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
-                    uint4 w[kBatch];
+            return false;
+        };
+        // q of a row: its first row in the block, the row's token, whether it exists, where it is
+        struct Place {
+            uint32_t rr0, rows;
+            int32_t tok, head;
+            bool have;
+        };
+        auto place_of = [&](const Segment &x) -> Place {
+            Place y;
+            y.rows = (uint32_t) x.s.n * (uint32_t) p.group, y.rr0 = (uint32_t) x.rb * kItemRows + blk * kRows;
+            y.have = y.rr0 + r < y.rows;
+            y.tok = y.have ? (int32_t) p.group_div.div(y.rr0 + r) : 0;
+            y.head = x.kvh * p.group + (y.have ? (int32_t) (y.rr0 + r) - y.tok * p.group : 0);
+            return y;
+        };
+        // q: a warp requests its 32 rows, a row's 16-byte pieces side by side in the lanes, into swizzled shared memory, zeros
+        // for rows that there are not and head elements beyond dh.
+        auto request_q = [&](const Segment &x, uint32_t to) {
+            constexpr int kPer = DHC / 8, kAtOnce = 32 / kPer;// lanes per row, rows at once
+            const Place y = place_of(x);
+            const int32_t d = (int32_t) (lane % kPer) * 8;
+            const bool vec = p.q_vec && p.c.dh % 8 == 0;
+            const int64_t mine = (int64_t) (x.s.first + y.tok) * p.q_st + (int64_t) y.head * p.q_sh;
+#pragma unroll 4
+            for (int i = 0; i < 32 / kAtOnce; ++i) {
+                const uint32_t row = (uint32_t) i * kAtOnce + lane / kPer, br = quarter * 32u + row;
+                const uint16_t *from = p.q + __shfl_sync(0xffffffffu, mine, (int) row);
+                const bool valid = y.rr0 + br < y.rows && d < p.c.dh;
+                const uint32_t at = to + ((uint32_t) d >> 6) * (kRows * 128u) + br * 128u + (((((uint32_t) d >> 3) & 7u) ^ (br & 7u)) << 4);
+                if (vec) {
+                    cp_async16(at, valid ? from + d : p.q, valid);
+                } else {
+                    uint32_t e[4] = {0u, 0u, 0u, 0u};
+                    if (valid) {
 #pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        const uint32_t row = (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
-                        const int64_t at = __shfl_sync(0xffffffffu, mine, (int) row);
-                        w[i] = make_uint4(0u, 0u, 0u, 0u);
-                        if (rr0 + quarter * 32u + row < rows && d < p.c.dh) {
-                            if (vec) {
-                                w[i] = *reinterpret_cast<const uint4 *>(p.q + at + d);
-                            } else {
-                                uint32_t e[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    e[j] = (uint32_t) p.q[at + min(d + 2 * j, p.c.dh - 1)] | ((uint32_t) p.q[at + min(d + 2 * j + 1, p.c.dh - 1)] << 16);
-                                    if (d + 2 * j >= p.c.dh) e[j] = 0u;
-                                    else if (d + 2 * j + 1 >= p.c.dh) e[j] &= 0xFFFFu;
-                                }
-                                w[i] = make_uint4(e[0], e[1], e[2], e[3]);
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            if (d + 2 * k < p.c.dh) e[k] = (uint32_t) from[d + 2 * k];
+                            if (d + 2 * k + 1 < p.c.dh) e[k] |= (uint32_t) from[d + 2 * k + 1] << 16;
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                        const uint32_t br = quarter * 32u + (uint32_t) (i0 + i) * kAtOnce + lane / kPer;
-                        if (p.bf16) {
-                            uint32_t top = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
-#pragma unroll
-                            for (int o = 1; o < kPer; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            const int32_t shift = query_shift(true, max(top & 0xFFFFu, top >> 16));
-                            const float up = __uint_as_float(pow2_bits(shift));
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float2 f = unpack2_t<kBF16>(x[j]);
-                                x[j] = round16x2(false, f.x * up, f.y * up);
-                            }
-                            // the factor of row (i0 + i) * kAtOnce + .. to the lane that owns the row
-                            const int32_t its = __shfl_sync(0xffffffffu, shift, (int) (lane % kAtOnce) * kPer);
-                            if ((int) (lane / kAtOnce) == i0 + i) rf *= __uint_as_float(pow2_bits(-its));
-                        }
-                        if (d < p.c.dh) {
-                            const uint32_t at = myq + ((uint32_t) d >> 6) * (kRows * 128u) + br * 128u + (((((uint32_t) d >> 3) & 7u) ^ (br & 7u)) << 4);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0] ^ flip), "r"(x[1] ^ flip), "r"(x[2] ^ flip), "r"(x[3] ^ flip) : "memory");
-                        }
-                    }
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&own[kQFull]);
             }
+            cp_async_commit();
+        };
+        // q has come: fp16 rows stay as they are; bf16 rows are multiplied by a power of two after their largest magnitude, a
+        // thread per row.  The sign of the scale goes with q, so that the factor of the scores (returned) is not negative.
+        auto finish_q = [&](uint32_t at0) -> float {
+            float f = fabsf(p.scale_log2);
+            cp_async_wait<0>();
+            __syncwarp();
+            const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+            if (p.bf16 || flip != 0u) {
+                const uint32_t row = at0 + r * 128u;
+                float up = 1.f;
+                if (p.bf16) {
+                    uint32_t top = 0u;
+#pragma unroll
+                    for (uint32_t i = 0; i < DHC / 8; ++i) {
+                        const uint4 x = lds128(row + (i >> 3) * (kRows * 128u) + (((i & 7u) ^ (r & 7u)) << 4));
+                        top = __vmaxu2(__vmaxu2(__vmaxu2(top, x.x & 0x7FFF7FFFu), __vmaxu2(x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu)), x.w & 0x7FFF7FFFu);
+                    }
+                    const int32_t shift = query_shift(true, max(top & 0xFFFFu, top >> 16));
+                    up = __uint_as_float(pow2_bits(shift)), f *= __uint_as_float(pow2_bits(-shift));
+                }
+#pragma unroll 4
+                for (uint32_t i = 0; i < DHC / 8; ++i) {
+                    const uint32_t at = row + (i >> 3) * (kRows * 128u) + (((i & 7u) ^ (r & 7u)) << 4);
+                    const uint4 v = lds128(at);
+                    uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (p.bf16) {
+                            const float2 y = unpack2_t<kBF16>(x[k]);
+                            x[k] = round16x2(false, y.x * up, y.y * up);
+                        }
+                        x[k] ^= flip;
+                    }
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&own[kQFull]);
+            return f;
+        };
+        // ONE: the pages and scales of 32 tiles in the lanes, as in the converting warps.  (The upper bound is looked at later,
+        // so that nothing waits for the load.)
+        auto page_at = [&](const Segment &x, int32_t tile) -> int32_t {
+            if (tile >= x.t1 || tile * kKeys >= held(x.s.len, p.t.cap)) return -1;
+            return p.table[(int64_t) x.b * p.t.stride + (int64_t) p.page_div.div((uint32_t) (tile * kKeys))];
+        };
+        auto scales_of = [&](const Segment &x, int32_t page, float &k, float &v) {
+            k = page >= 0 ? p.ks[(int64_t) page * p.c.k.cn + (int64_t) x.kvh * p.c.k.ch] : 0.f;
+            v = page >= 0 ? p.vs[(int64_t) page * p.c.v.cn + (int64_t) x.kvh * p.c.v.ch] : 0.f;
+        };
+        // What the next item needs is requested while this one is worked on, and its q is made ready before this one's output
+        // leaves, so that its first scores are computed meanwhile.
+        Segment gn;
+        uint32_t skipped, buf = 0;
+        int32_t id = -1;
+        float rf_next = 0.f, ks = 0.f, vs = 0.f;
+        bool more = next_item(gn, skipped);
+        if (more) {
+            request_q(gn, sq + blk * kQ);
+            if (ONE) id = page_at(gn, gn.t0 + (int32_t) lane);
+            rf_next = finish_q(sq + blk * kQ);
+            if (id >= p.c.pages) id = -1;
+            if (ONE) scales_of(gn, id, ks, vs);
+        }
+        while (ok && more) {
+            g = gn, n_all += skipped;
+            const float rf = rf_next;
+            const uint32_t myq = sq + (buf * kNB + blk) * kQ, other = kQBufs == 2 ? sq + ((buf ^ 1u) * kNB + blk) * kQ : myq;
+            const Seq s = g.s;
+            const Place at_q = place_of(g);
+            const uint32_t rows = at_q.rows, rr0 = at_q.rr0;
+            const bool have = at_q.have;
+            const int32_t tok = at_q.tok;
+            const int32_t limit = have ? max(0, min(s.len - s.n + tok + 1, held(s.len, p.t.cap))) : 0;// keys this row sees
+            more = next_item(gn, skipped);
+            if (kQBufs == 2 && more) request_q(gn, other);
+            int32_t first = g.t0, id_next = -1;
+            float ks_next = 0.f, vs_next = 0.f;
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
             auto largest = [&](const float *v) -> float {
                 float t4[4] = {v[0], v[1], v[2], v[3]};
@@ -703,11 +751,10 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const bool some = __any_sync(0xffffffffu, move);
                     auto next = [&]() {
                         // pages and scales of the next 32 tiles: requested and looked at some tiles apart
-                        if (j == 16) id_next = page_at(first + 32 + (int32_t) lane);
+                        if (j == 16) id_next = page_at(g, first + 32 + (int32_t) lane);
                         if (j == 22) {
                             if (id_next >= p.c.pages) id_next = -1;
-                            ks_next = id_next >= 0 ? kscale[(int64_t) id_next * p.c.k.cn] : 0.f;
-                            vs_next = id_next >= 0 ? vscale[(int64_t) id_next * p.c.v.cn] : 0.f;
+                            scales_of(g, id_next, ks_next, vs_next);
                         }
                         if (j == 31) first += 32, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                         if (tile + 1 < g.t1) look_at(tile + 1);
@@ -849,14 +896,22 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 }
             }
             if (!ok) break;
+            if (more) {
+                if (ONE) id = page_at(gn, gn.t0 + (int32_t) lane);
+                if (kQBufs == 2) rf_next = finish_q(other);
+            }
             // ---- the item's output, or its part
             if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
+            if (more && ONE) {
+                if (id >= p.c.pages) id = -1;
+                scales_of(gn, id, ks, vs);
+            }
             const bool whole = g.t0 == 0 && g.t1 == g.tiles;
             const int part = g.t0 > 0 ? 0 : 1;
             const int64_t at0 = ((int64_t) blockIdx.x * 2 + part) * kItemRows + blk * kRows + quarter * 32u;// this warp's first row
             const bool none = wm == -INFINITY;// (O holds products with weights of zero)
-            const int64_t out_at = (int64_t) (s.first + tok) * p.o_st + (int64_t) (g.kvh * p.group + (have ? (int32_t) rr - tok * p.group : 0)) * p.o_sh;
+            const int64_t out_at = (int64_t) (s.first + tok) * p.o_st + (int64_t) at_q.head * p.o_sh;
             // Through this warp's part of q's memory (rows of 128 bytes, their 16-byte pieces rotated by the row), so that a
             // row's pieces leave side by side: finished outputs 64 columns at a time, parts 32 columns in fp32.
             const uint32_t stage = myq + quarter * 32u * 128u, piece = lane & 7u, sub = lane >> 3;
@@ -925,13 +980,15 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 }
             }
             __syncwarp();
-            if (p.c.dh < DHC) {// the zeros beyond dh in q's rows were written over
-                for (uint32_t i = lane * 16; i < 32 * 128; i += 512) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(stage + i), "r"(0) : "memory");
-                __syncwarp();
-            }
             if (!whole && have) sp.heads[at0 + lane] = PartHead{m, l, wm - kLift, 0.f};
             if (!whole && part == 1) meta = CtaMeta{g.b, g.kvh, g.rb, (int32_t) divide(g.last_unit, each)};
             tc_fence_before();
+            if (kQBufs == 2) {
+                buf ^= 1u;
+            } else if (more) {
+                request_q(gn, myq);
+                rf_next = finish_q(myq);
+            }
         }
         if (threadIdx.x == 0) sp.meta[blockIdx.x] = meta;
     }

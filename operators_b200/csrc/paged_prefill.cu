@@ -47,7 +47,7 @@ constexpr int kRows = 128, kKeys = kPrefillKeys;
 constexpr float kSlack = 13.f, kLift = 2.f;// w <= 2^15
 constexpr float kLeast = -90.f;
 constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
-constexpr int kItemUnits = 8;// what the start and the end of an item cost, in tiles
+constexpr int kItemUnits = 6;// what the start and the end of an item cost, in tiles
 constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done

@@ -673,15 +673,15 @@ uint64_t workspace_of_desc(const AttendDesc &d) { return d.cluster > 0 ? 0 : spl
 // Whether the tcgen05 kernel takes a call with rows_each query rows per sequence and kv head, from what both cost in ns
 // x SMs if every sequence fills its table.  Measured over 1 and 16 sequences of 2000 to 30000 tokens and 2 to 64 new ones:
 // this kernel takes 130, 270 or 600 ns for 16 rows and 32 cached tokens at a head size of 64, 128 or 256, the other one
-// about 1050 ns for a block of rows and 64 cached tokens and 10 us more to start and end.  32 heads on 8 of 128 elements,
-// 16 sequences of 8000 tokens: 8 new tokens 122 us here and 150 us there, 16 new tokens 220 us and 153 us; one sequence of
-// 2000 tokens: 24 new ones 19 us and 28 us.
+// 950, 950 or 1250 ns for a block of rows and 64 cached tokens and 6 us more to start and end.  32 heads on 8 of 128
+// elements, 16 sequences of 8000 tokens: 8 new tokens 122 us here and 130 us there, 16 new tokens 220 us and 132 us; one
+// sequence of 2000 tokens: 12 new ones 15 us and 21 us, 64 new ones 33 us and 28 us.
 bool prefill_is_faster(const AttendDesc &d, int64_t rows_each) {
     if (rows_each <= 16 || d.t.batch > kPrefillMaxBatch) return false;
     const auto cost = [&](int64_t block, int64_t keys, int64_t each) {
         return (double) d.t.batch * (double) d.c.heads * (double) ((rows_each + block - 1) / block) * (double) (((int64_t) d.t.cap + keys - 1) / keys) * (double) each;
     };
-    return cost(16, kTile, d.dhc == 64 ? 130 : d.dhc == 128 ? 270 : 600) > cost(prefill_rows(d.dhc), kPrefillKeys, 1050) + 10000. * d.sm_count;
+    return cost(16, kTile, d.dhc == 64 ? 130 : d.dhc == 128 ? 270 : 600) > cost(prefill_rows(d.dhc), kPrefillKeys, d.dhc == 256 ? 1250 : 950) + 6000. * d.sm_count;
 }
 
 template<int DHC, int NT, bool ONE>

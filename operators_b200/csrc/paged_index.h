@@ -44,9 +44,10 @@ B200_HD void written(const Seq &s, int32_t cap, int32_t &lo, int32_t &hi) {
     lo = s.len > s.n ? s.len - s.n : 0;
     hi = held(s.len, cap);
 }
-// Pages that [lo, hi) touches.
-B200_HD int32_t pages_touched(int32_t lo, int32_t hi, int32_t page) {
-    return hi > lo ? (hi - 1) / page - lo / page + 1 : 0;
+// Pages that [lo, hi) touches; page_of(token) is a token's column of the table.
+template<class PageOf>
+B200_HD int32_t pages_touched(int32_t lo, int32_t hi, const PageOf &page_of) {
+    return hi > lo ? page_of(hi - 1) - page_of(lo) + 1 : 0;
 }
 // More pages than all appends of a call can touch: m tokens touch at most m pages, and at most m / page + 2.
 B200_HD int64_t pages_bound(int64_t rows, int64_t batch, int64_t page) {

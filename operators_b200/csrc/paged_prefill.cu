@@ -5,23 +5,28 @@
 // the second product), O += W v in TMEM.  The operands of kind::f16 are fp16: q is scaled per row by a power of two
 // (see paged_attention.cu), the codes become fp16 exactly on their way into shared memory, once per pair of blocks.
 //
-// Softmax in one pass: p = 2^(s f - m) with f the row's and the page's factor and m the row's reference, the largest
-// score of its first tile.  The weight of a value is w = p * 2^c with 2^c = 2^(m - M + 2) * (scale of the values' page) and
-// M the weights' own reference; it moves (and O, which has to be read, multiplied and written back) only when a weight
-// exceeds it by 2^13.  Scores of later tiles rarely exceed the first tile's largest by that much, so hardly any tile is
-// looked through for its largest score: sums of 16 weights, formed anyway, tell when one may have grown too large.  fp16
-// holds weights between 2^13 and 2^-16 times the reference with all their bits, smaller ones to 2^-27 of it.  One
-// exponential gives w; the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way,
-// and their sum must not underflow.
+// Softmax in one pass: p = 2^(s f - m) with f the row's and the page's factor and m the row's reference, at first the largest
+// score of its first tile.  The weight of a value is w = p * 2^c with 2^c = 2^(m - M + 2) * (scale of the values' page) and M
+// the weights' own reference.  No tile is looked through for its largest score: sums of 16 weights, formed anyway, tell when a
+// weight may have grown beyond fp16.  Then both references of the row follow by the power of two that brings the tile's largest
+// weight back to [2^2, 2^3), and the tile's weights (still in fp32 in registers), l and O are divided by it, exactly.  (Looking
+// for the maximum and forming the weights anew took 187 us where this takes 162, in heads whose scores spread widely.)  fp16
+// holds weights down to 2^-16 of the reference with all their bits, smaller ones to 2^-27 of it.  One exponential gives w;
+// the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way, and
+// their sum must not underflow.
 //
-// What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x
-// dh multiply-adds (512 cycles at dh 128).  One CTA per SM works on two blocks at a time (head sizes beyond 128: one), so
-// that one's exponentials run beside the other's products and both share the converted tiles.
+// What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x dh
+// multiply-adds (at dh 128: 256 cycles at full rate; S with its 64 columns runs at two thirds of it, 640 in all).  One CTA per SM
+// works on two blocks at a time (head sizes beyond 128: one), so that one's exponentials run beside the other's products and
+// both share the converted tiles.  Measured: 2000 cycles per pair of blocks and tile, of which the tensor pipe is busy 1280
+// and the exponentials 1024; the softmax warps' chain (S from TMEM, exponentials, weights to TMEM, barriers) is what is left.
 //
-// Roles (544 threads; 416 with one block): a warpgroup per block for softmax and epilogue, a thread per row; one
-// warpgroup converts the codes of K, one those of V (their loads run a tile ahead in registers); the last warp allocates TMEM and issues the
-// products (the warp as one, see umma_f16_ss).  Shared memory: q, two tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is
-// double-buffered: S of tile j + 1 is issued before W v of tile j.
+// Roles (512 threads; 384 with one block): a warpgroup per block for softmax and epilogue, a thread per row; two warps
+// convert the codes of K, two those of V (their loads run a tile ahead in registers); of the last warpgroup one warp allocates
+// TMEM and issues the products (the warp as one, see umma_f16_ss).  Shared memory: q of this item and (head sizes up to 128)
+// of the next, copied and made ready while this one is worked on (160 -> 150 us for a chunk, 170 -> 152 us for prompts); two
+// tiles of K, two of V (128-byte swizzled rows as TMA would lay them).  S is double-buffered: S of tile j + 1 is issued before
+// W v of tile j.
 //
 // Work is divided into equal stretches as in paged_attention.cu; an item is a pair of blocks, stops where its last row's
 // mask begins, and counts kItemUnits tiles more for what its start and end cost.  All roles walk the stretch's items by
@@ -31,6 +36,9 @@
 // that has seen S of tile n knows that W v of tile n - 2 (issued before it) is done, not that of tile n - 1, and one
 // barrier's parity could not tell the two apart.
 // Every wait is bounded (tc_ptx.cuh).
+//
+// 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 150 us, 935 TFLOP/s.  Two prompts of up to 4096
+// tokens, nothing cached before them, fp16: 151 us, 695 TFLOP/s of the visible products.
 #include "paged_attention.cuh"
 #include "tc_ptx.cuh"
 
@@ -236,10 +244,25 @@ struct Walker {
     }
 };
 
-template<int DHC, bool ONE>
+template<int N>
+__device__ __forceinline__ float largest(const float *v) {
+    float t4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < N; i += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[i + j]);
+    }
+    return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+}
+
+// GROUPS of a tile's keys that each lie in one page: 1 (page sizes that are multiples of 64), 4 (of 16), 0 (any other, and
+// codes whose rows are no aligned vectors: a page, a scale and a mask bit per key).  512 new tokens over 16384 cached ones, 32
+// heads on 8 of 128 elements: 150 us with pages of 64 tokens (1), 163 us with 16 (4), where the general form takes 412 us.
+template<int DHC, int GROUPS>
 __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_kernel(const SplitParams sp) {
     constexpr int kNB = blocks_at_once(DHC), kItemRows = kNB * kRows, kThreads = threads_of(kNB), kWarps = kThreads / 32;
     constexpr uint32_t kQ = q_bytes(DHC), kKV = kv_bytes(DHC);
+    constexpr int kGroupsOr1 = GROUPS > 0 ? GROUPS : 1;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ int64_t slot[kWarps], found_base;
     __shared__ int32_t found_b, found_rb, found_t;
@@ -447,46 +470,48 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             const int32_t keys = held(g.s.len, p.t.cap), t1 = g.t1;
             const int32_t *ids = p.table + (int64_t) g.b * p.t.stride;
             const uint8_t *head = pool + (int64_t) g.kvh * st.sh;
-            if (ONE) {
-                // One page per tile: lane j holds the page of the j-th of 32 tiles, so that these are read once in 32 tiles;
-                // the next 32 are requested while the last of these are converted.
-                int32_t first = g.t0, id_next = -1;// `first`: the tile of lane 0
-                auto page_of = [&](int32_t tile) -> int32_t {
-                    if (tile >= t1 || tile * kKeys >= keys) return -1;
-                    const int32_t x = ids[p.page_div.div((uint32_t) (tile * kKeys))];
-                    return x >= 0 && x < p.c.pages ? x : -1;
+            if constexpr (GROUPS > 0) {
+                // Lane j holds where the codes of the j-th of 32 groups begin (-1: no page), so that pages are read once in
+                // kChunk tiles; the next 32 are requested long before they are looked at.
+                constexpr int kChunk = 32 / kGroupsOr1, kTokens = kKeys / kGroupsOr1;
+                auto page_at = [&](int32_t group) -> int32_t {
+                    return group >= t1 * kGroupsOr1 || group * kTokens >= keys ? -1 : ids[p.page_div.div((uint32_t) (group * kTokens))];
                 };
-                const int32_t start = g.t0 * kKeys;
-                int32_t in_page = start - (int32_t) p.page_div.div((uint32_t) start) * p.c.page;
-                auto load = [&](int32_t tile, int32_t page) {
-                    const int32_t left = page < 0 ? 0 : keys - tile * kKeys;
-                    const uint8_t *at = head + (int64_t) max(page, 0) * st.sn + (int64_t) (in_page + (int32_t) r0) * st.sp;
-                    in_page = in_page + kKeys == p.c.page ? 0 : in_page + kKeys;
+                auto base_of = [&](int32_t group, int32_t page) -> int64_t {
+                    if (page < 0 || page >= p.c.pages) return -1;
+                    const int32_t tok = group * kTokens;
+                    return (int64_t) page * st.sn + (int64_t) (tok - (int32_t) p.page_div.div((uint32_t) tok) * p.c.page) * st.sp;
+                };
+                int32_t first = g.t0, id_next = -1;// `first`: the tile of lane 0
+                int64_t base = base_of(first * kGroupsOr1 + (int32_t) lane, page_at(first * kGroupsOr1 + (int32_t) lane));
+                const uint8_t *mine = head + (int64_t) r0 * st.sp;
+                const int64_t step = 16 * st.sp;
+                auto load = [&](int32_t tile) {
+                    const int32_t left = keys - tile * kKeys;
+                    int64_t from = __shfl_sync(0xffffffffu, base, (tile - first) * kGroupsOr1);
 #pragma unroll
-                    for (int i = 0; i < kLoads; ++i) {
+                    for (int i = 0; i < kLoads; ++i) {// (16 rows apart: the i-th group's where there are four)
+                        if (GROUPS == 4 && i > 0) from = __shfl_sync(0xffffffffu, base, (tile - first) * kGroupsOr1 + i);
+                        const uint8_t *at = mine + from + (GROUPS == 4 ? 0 : i * step);
 #pragma unroll
                         for (int q = 0; q < kGroups; ++q) {
                             data[i][q] = make_uint4(0u, 0u, 0u, 0u);
-                            if ((int32_t) r0 + 16 * i < left && (q * 4 + (int32_t) c4) * 16 < p.c.dh) data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
+                            if (from >= 0 && (int32_t) r0 + 16 * i < left && (q * 4 + (int32_t) c4) * 16 < p.c.dh) data[i][q] = *reinterpret_cast<const uint4 *>(at + q * 64);
                         }
-                        at += 16 * st.sp;
                     }
                 };
-                int32_t id = page_of(first + (int32_t) lane);
-                load(g.t0, __shfl_sync(0xffffffffu, id, 0));
+                load(g.t0);
+#pragma unroll 1
                 for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
                     const int32_t j = tile - first;
-                    if (j == 20) {
-                        const int32_t ahead = first + 32 + (int32_t) lane;
-                        id_next = ahead >= t1 || ahead * kKeys >= keys ? -1 : ids[p.page_div.div((uint32_t) (ahead * kKeys))];
-                    }
+                    if (j == kChunk / 2) id_next = page_at((first + kChunk) * kGroupsOr1 + (int32_t) lane);
                     if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     __syncwarp();
                     store_tile(b);
                     mbar_arrive(&full[b]);
-                    if (j == 31) first += 32, id = id_next < p.c.pages ? id_next : -1;// (looked at long after the request)
-                    if (tile + 1 < t1) load(tile + 1, __shfl_sync(0xffffffffu, id, tile + 1 - first));
+                    if (j == kChunk - 1) first += kChunk, base = base_of(first * kGroupsOr1 + (int32_t) lane, id_next);
+                    if (tile + 1 < t1) load(tile + 1);
                 }
             } else {
                 // pages that end inside a tile: a page per row and per key
@@ -650,11 +675,13 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             mbar_arrive(&own[kQFull]);
             return f;
         };
-        // ONE: the pages and scales of 32 tiles in the lanes, as in the converting warps.  (The upper bound is looked at later,
-        // so that nothing waits for the load.)
+        // The pages and scales of 32 groups in the lanes, as in the converting warps.  (The upper bound is looked at later, so
+        // that nothing waits for the load.)
+        constexpr int kChunk = 32 / kGroupsOr1, kTokens = kKeys / kGroupsOr1;
         auto page_at = [&](const Segment &x, int32_t tile) -> int32_t {
-            if (tile >= x.t1 || tile * kKeys >= held(x.s.len, p.t.cap)) return -1;
-            return p.table[(int64_t) x.b * p.t.stride + (int64_t) p.page_div.div((uint32_t) (tile * kKeys))];
+            const int32_t group = tile * kGroupsOr1 + (int32_t) lane;
+            if (group >= x.t1 * kGroupsOr1 || group * kTokens >= held(x.s.len, p.t.cap)) return -1;
+            return p.table[(int64_t) x.b * p.t.stride + (int64_t) p.page_div.div((uint32_t) (group * kTokens))];
         };
         auto scales_of = [&](const Segment &x, int32_t page, float &k, float &v) {
             k = page >= 0 ? p.ks[(int64_t) page * p.c.k.cn + (int64_t) x.kvh * p.c.k.ch] : 0.f;
@@ -669,10 +696,10 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         bool more = next_item(gn, skipped);
         if (more) {
             request_q(gn, sq + blk * kQ);
-            if (ONE) id = page_at(gn, gn.t0 + (int32_t) lane);
+            if (GROUPS > 0) id = page_at(gn, gn.t0);
             rf_next = finish_q(sq + blk * kQ);
             if (id >= p.c.pages) id = -1;
-            if (ONE) scales_of(gn, id, ks, vs);
+            if (GROUPS > 0) scales_of(gn, id, ks, vs);
         }
         while (ok && more) {
             g = gn, n_all += skipped;
@@ -689,17 +716,6 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             int32_t first = g.t0, id_next = -1;
             float ks_next = 0.f, vs_next = 0.f;
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
-            auto largest = [&](const float *v) -> float {
-                float t4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int i = 4; i < 28; i += 8) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) t4[j] = fmaxf(fmaxf(t4[j], v[i + j]), v[i + 4 + j]);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) t4[j] = fmaxf(t4[j], v[28 + j]);
-                return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-            };
             // O so far is multiplied by a factor per row.  Every product into it must have completed.
             auto scale_o = [&](float by) -> bool {
                 const bool done = mbar_wait<kSuspendNs>(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag);
@@ -726,66 +742,99 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 }
                 return tile == g.t0 || !__any_sync(0xffffffffu, up) || scale_o(shrink);
             };
-            if (ONE) {
+            if constexpr (GROUPS > 0) {
                 float lv_lane = log2_of(vs);
-                float e = 0.f, e_back = 1.f, shift = 0.f, lv_of_e = NAN;// exponent from p to w, 2^-e, e - m, and the scale (log2) they are for
-                // the tile's factor, scale and how many of its keys this row sees; formed while the tile before is worked on
-                float factor, lv;
+                // per group: exponent from p to w, 2^-e, e - m, and the scale (log2) they are for
+                float e[GROUPS], e_back[GROUPS], shift[GROUPS], lv_of_e[GROUPS];
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) lv_of_e[i] = NAN;
+                auto forget = [&]() {
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) lv_of_e[i] = NAN;
+                };
+                // the groups' factors and scales, those without a page, and how many of the tile's keys this row sees; formed
+                // while the tile before is worked on
+                float factor[GROUPS], lv[GROUPS];
                 int32_t left;
+                uint32_t gone;
                 bool hidden;
                 auto look_at = [&](int32_t tile) {
-                    const int32_t j = tile - first;
-                    factor = __shfl_sync(0xffffffffu, ks, j) * rf, lv = __shfl_sync(0xffffffffu, lv_lane, j);
-                    left = __shfl_sync(0xffffffffu, id, j) >= 0 ? limit - tile * kKeys : 0;
-                    hidden = __any_sync(0xffffffffu, have && left < kKeys);
+                    const int32_t j = (tile - first) * GROUPS;
+                    gone = __ballot_sync(0xffffffffu, id < 0) >> j & ((1u << GROUPS) - 1u);
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) factor[i] = __shfl_sync(0xffffffffu, ks, j + i) * rf, lv[i] = __shfl_sync(0xffffffffu, lv_lane, j + i);
+                    left = limit - tile * kKeys;
+                    if (GROUPS == 1 && gone != 0u) left = 0, gone = 0u;
+                    hidden = __any_sync(0xffffffffu, have && (left < kKeys || gone != 0u));
                 };
                 look_at(g.t0);
 #pragma unroll 1
                 for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n) {
-                    const uint32_t b = n & 1u;
+                    const uint32_t b = n & 1u, gone_now = gone;
                     const int32_t j = tile - first, left_now = left;
-                    const float factor_now = factor, lv_now = lv;
+                    float factor_now[GROUPS], lv_now[GROUPS];
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) factor_now[i] = factor[i], lv_now[i] = lv[i];
                     const bool hidden_now = hidden;
                     // a row without a reference (its first keys are in this tile) looks through the tile for its largest score
                     bool move = m == -INFINITY && left > 0;
                     const bool some = __any_sync(0xffffffffu, move);
                     auto next = [&]() {
-                        // pages and scales of the next 32 tiles: requested and looked at some tiles apart
-                        if (j == 16) id_next = page_at(g, first + 32 + (int32_t) lane);
-                        if (j == 22) {
+                        // pages and scales of the next 32 groups: requested and looked at some tiles apart
+                        if (j == kChunk / 2) id_next = page_at(g, first + kChunk);
+                        if (j == kChunk * 3 / 4 - 2 + GROUPS / 2) {
                             if (id_next >= p.c.pages) id_next = -1;
                             scales_of(g, id_next, ks_next, vs_next);
                         }
-                        if (j == 31) first += 32, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
+                        if (j == kChunk - 1) first += kChunk, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                         if (tile + 1 < g.t1) look_at(tile + 1);
                     };
                     if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
                     tc_fence_after();
                     __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
                     uint32_t w[kKeys / 2];
-                    float sum = 0.f, most = 0.f;
+                    float gain = 0.f, most = 0.f;// what the tile adds to l; the largest sum of 16 (or 8) weights
                     auto exponents = [&]() {
-                        if (!(lv_now == lv_of_e)) {// (the references or the scale have changed)
-                            e = wm == -INFINITY ? 0.f : fmaxf(m - wm + kLift + lv_now, kLeast);
-                            e_back = fast_exp2(-e);
-                            shift = e - (m == -INFINITY ? 0.f : m);
-                            lv_of_e = lv_now;
+#pragma unroll
+                        for (int i = 0; i < GROUPS; ++i) {
+                            if (!(lv_now[i] == lv_of_e[i])) {// (the references or the scale have changed)
+                                e[i] = wm == -INFINITY ? 0.f : fmaxf(m - wm + kLift + lv_now[i], kLeast);
+                                e_back[i] = fast_exp2(-e[i]);
+                                shift[i] = e[i] - (m == -INFINITY ? 0.f : m);
+                                lv_of_e[i] = lv_now[i];
+                            }
                         }
                     };
-                    // weights of 16 pairs, and what they add up to in four sums
-                    auto weigh = [&](float *x, uint32_t *to, uint64_t f2, uint64_t e2, uint64_t (&part)[2]) {
+                    // Weights of half a tile (the `half`-th), and what they add up to: four sums of 16 keys of the tile, or two
+                    // of 8 keys of each group.
+                    uint64_t part[GROUPS == 4 ? 4 : 2];
+                    auto weigh = [&](float *x, uint32_t *to, const float *f, int half) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), f2, e2));
+                            const int gr = GROUPS == 4 ? 2 * half + (i >> 3) : 0, at = GROUPS == 4 ? gr : i & 1;
+                            const float2 a = unpack2f(fma2(pack2f(x[2 * i], x[2 * i + 1]), pack2f(f[gr], f[gr]), pack2f(shift[gr], shift[gr])));
                             x[2 * i] = fast_exp2(a.x), x[2 * i + 1] = fast_exp2(a.y);
-                            part[i & 1] = add2(part[i & 1], pack2f(x[2 * i], x[2 * i + 1]));
+                            part[at] = add2(part[at], pack2f(x[2 * i], x[2 * i + 1]));
                             to[i] = round16x2(false, x[2 * i], x[2 * i + 1]);
                         }
                     };
-                    auto add_up = [&](const uint64_t (&part)[2]) {
-                        const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
-                        sum = (s0.x + s0.y) + (s1.x + s1.y);
-                        most = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y));
+                    auto add_up = [&]() {
+                        gain = most = 0.f;
+                        if (GROUPS == 4) {
+#pragma unroll
+                            for (int i = 0; i < GROUPS; ++i) {
+                                const float2 y = unpack2f(part[i]);
+                                gain = fmaf(y.x + y.y, e_back[i], gain), most = fmaxf(most, fmaxf(y.x, y.y));
+                            }
+                        } else {
+                            const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
+                            gain = ((s0.x + s0.y) + (s1.x + s1.y)) * e_back[0];
+                            most = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y));
+                        }
+                    };
+                    auto clear = [&]() {
+#pragma unroll
+                        for (int i = 0; i < (GROUPS == 4 ? 4 : 2); ++i) part[i] = 0ull;
                     };
                     // Most tiles hide nothing and move no reference: their weights are formed at once, and the sums tell
                     // whether one may have grown beyond what fp16 holds.  A row that finds so lets its references follow by a
@@ -796,21 +845,20 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         tmem_ld32(t_lane + b * kKeys, x);
                         tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);
                         exponents();
-                        const uint64_t f2 = pack2f(factor_now, factor_now), e2 = pack2f(shift, shift);
-                        uint64_t part[2] = {0ull, 0ull};
-                        weigh(x, w, f2, e2, part);
+                        clear();
+                        weigh(x, w, factor_now, 0);
                         next();
                         tmem_ld32_finish(x + 32);
-                        weigh(x + 32, w + 16, f2, e2, part);
-                        add_up(part);
+                        weigh(x + 32, w + 16, factor_now, 1);
+                        add_up();
                         if (__any_sync(0xffffffffu, most > kMostWeight)) {
                             move = most > kFarWeight;
-                            const float top = fmaxf(largest(x), largest(x + 32));
+                            const float top = fmaxf(largest<32>(x), largest<32>(x + 32));
                             const int32_t up = most > kMostWeight && !move ? (int32_t) (__float_as_uint(top) >> 23) - (127 + (int32_t) kLift) : 0;
                             const float by = __uint_as_float(pow2_bits(-up));
 #pragma unroll
                             for (int i = 0; i < kKeys / 2; ++i) w[i] = round16x2(false, x[2 * i] * by, x[2 * i + 1] * by);
-                            sum *= by, l *= by, m += (float) up, wm += (float) up, lv_of_e = NAN;
+                            gain *= by, l *= by, m += (float) up, wm += (float) up, forget();
                             if (tile > g.t0 && !(ok = scale_o(by))) break;
                         }
                     } else {
@@ -822,24 +870,34 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             float x[kKeys];
                             tmem_ld64(t_lane + b * kKeys, x);
 #pragma unroll
-                            for (int i = 0; i < kKeys; ++i) x[i] = i < left_now ? x[i] * factor_now : -INFINITY;
+                            for (int i = 0; i < kKeys; ++i) {
+                                const int gr = i / kTokens;
+                                x[i] = i < left_now && (GROUPS == 1 || !(gone_now >> gr & 1u)) ? x[i] * factor_now[gr] : -INFINITY;
+                            }
                             if (__any_sync(0xffffffffu, move)) {
-                                const float top = fmaxf(largest(x), largest(x + 32));
-                                if (!(ok = move_references(move && top > -INFINITY, top, top + lv_now, tile))) break;
-                                lv_of_e = NAN;
+                                float top = -INFINITY, wtop = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < GROUPS; ++i) {
+                                    const float y = GROUPS == 4 ? largest<16>(x + i * kTokens) : fmaxf(largest<32>(x), largest<32>(x + 32));
+                                    if (y > -INFINITY) top = fmaxf(top, y), wtop = fmaxf(wtop, y + lv_now[i]);
+                                }
+                                if (!(ok = move_references(move && top > -INFINITY, top, wtop, tile))) break;
+                                forget();
                             }
                             exponents();
-                            uint64_t part[2] = {0ull, 0ull};
-                            const uint64_t one = pack2f(1.f, 1.f), e2 = pack2f(shift, shift);
-                            weigh(x, w, one, e2, part);
-                            weigh(x + 32, w + 16, one, e2, part);
-                            add_up(part);
+                            float one[GROUPS];
+#pragma unroll
+                            for (int i = 0; i < GROUPS; ++i) one[i] = 1.f;
+                            clear();
+                            weigh(x, w, one, 0);
+                            weigh(x + 32, w + 16, one, 1);
+                            add_up();
                             move = most > kMostWeight;
                             if (!__any_sync(0xffffffffu, move)) break;
                         }
                     }
                     if (!ok) break;
-                    l = fmaf(sum, e_back, l);
+                    l += gain;
                     __syncwarp();
                     tmem_st32(t_lane + b * kKeys, w);
                     tc_fence_before();
@@ -869,7 +927,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             if (!(((i < 32 ? m0 : m1) >> (i & 31)) & 1u) || i >= left) x[i] = -INFINITY;
                         }
                     }
-                    const float top = fmaxf(largest(x), largest(x + 32));
+                    const float top = fmaxf(largest<32>(x), largest<32>(x + 32));
                     float wtop = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i) wtop = fmaxf(wtop, x[i] == -INFINITY ? -INFINITY : x[i] + sc.lv[i]);
@@ -897,13 +955,13 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             }
             if (!ok) break;
             if (more) {
-                if (ONE) id = page_at(gn, gn.t0 + (int32_t) lane);
+                if (GROUPS > 0) id = page_at(gn, gn.t0);
                 if (kQBufs == 2) rf_next = finish_q(other);
             }
             // ---- the item's output, or its part
             if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
-            if (more && ONE) {
+            if (more && GROUPS > 0) {
                 if (id >= p.c.pages) id = -1;
                 scales_of(gn, id, ks, vs);
             }
@@ -1002,17 +1060,17 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     }
 }
 
-template<int DHC, bool ONE>
+template<int DHC, int GROUPS>
 cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};// devices on which the shared memory has been asked for
     const uint64_t bit = device_id < 64 ? 1ull << device_id : 0;
     cudaError_t e = cudaSuccess;
     if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-        e = cudaFuncSetAttribute(prefill_kernel<DHC, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes(DHC));
+        e = cudaFuncSetAttribute(prefill_kernel<DHC, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes(DHC));
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    prefill_kernel<DHC, ONE><<<ctas, threads_of(blocks_at_once(DHC)), smem_bytes(DHC), st>>>(sp);
+    prefill_kernel<DHC, GROUPS><<<ctas, threads_of(blocks_at_once(DHC)), smem_bytes(DHC), st>>>(sp);
     e = cudaGetLastError();
     if (e != cudaSuccess || ctas == 1) return e;
     return launch_join<DHC, blocks_at_once(DHC) * kRows>(sp, ctas, st);
@@ -1020,7 +1078,8 @@ cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaS
 template<int DHC>
 cudaError_t launch(const AttendParams &a, void *workspace, uint32_t ctas, int device_id, cudaStream_t st) {
     const SplitParams sp = split_params(a, workspace, ctas, (uint64_t) prefill_rows(DHC), DHC);
-    return a.vec && a.c.page % kKeys == 0 ? launch_as<DHC, true>(sp, ctas, device_id, st) : launch_as<DHC, false>(sp, ctas, device_id, st);
+    if (a.vec && a.c.page % kKeys == 0) return launch_as<DHC, 1>(sp, ctas, device_id, st);
+    return a.vec && a.c.page % 16 == 0 ? launch_as<DHC, 4>(sp, ctas, device_id, st) : launch_as<DHC, 0>(sp, ctas, device_id, st);
 }
 
 }// namespace

@@ -226,7 +226,7 @@ int main() {
             if (pos / page != last) ++touched, last = pos / page;
         }
         CHECK(count == (hi > lo ? hi - lo : 0));
-        CHECK(pages_touched(lo, hi, page) == touched);
+        CHECK(pages_touched(lo, hi, [&](int x) { return x / page; }) == touched);
         CHECK(touched <= pages_bound(n, 1, page));
     }
     // 2^x is the smallest power with amax <= 448 * 2^x

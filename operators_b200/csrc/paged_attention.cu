@@ -25,8 +25,8 @@
 //    of 128 elements, 8 rows 27 us with one and 12 rows 33 us with two; more rows take further items, or the tcgen05 kernel
 //    (prefill_is_faster).  Tiles that lie in one page (page sizes that are multiples of 32) read one page id and scale per
 //    tile: 32 sequences of 2048 tokens 36 us with pages of 64, 41 us in the general form with pages of 16.
-// Measured: 32 sequences of 1024 to 8192 tokens, 32 heads on 8 of 128 elements: 65.6 us, 4.8 TB/s; one sequence of 131072:
-// 57.7 us, 4.65 TB/s.  The loop itself runs at 6.7 TB/s; the rest is the start (5 us), SMs that get less bandwidth than
+// Measured: 32 sequences of 1024 to 8192 tokens, 32 heads on 8 of 128 elements: 65 us, 4.8 TB/s; one sequence of 131072:
+// 57.6 us, 4.65 TB/s.  The loop itself runs at 6.7 TB/s; the rest is the start (5 us), SMs that get less bandwidth than
 // others (7 us), and the join (5 us).
 #include "paged_cache.cuh"
 #include "paged_attention.cuh"

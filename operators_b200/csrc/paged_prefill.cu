@@ -129,6 +129,12 @@ __device__ __forceinline__ void umma_commit_by(uint64_t *bar, uint32_t lead) {
         ::"r"(smem_u32(bar)), "r"(lead)
         : "memory");
 }
+// A warp waits as one: lanes leave a wait at different times, what follows (TMEM accesses, votes) is the whole warp's, and a
+// wait that runs out ends the loop for all of its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait<kSuspendNs>(bar, parity, abort_flag));
+}
+
 // 32 columns of this warp's 32 lanes
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile(
@@ -377,7 +383,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
         auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-            const bool done = __all_sync(0xffffffffu, mbar_wait<kSuspendNs>(bar, parity, abort_flag));
+            const bool done = warp_wait(bar, parity, abort_flag);
             tc_fence_after();
             return done;
         };
@@ -506,8 +512,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const uint32_t b = n & 1u;
                     const int32_t j = tile - first;
                     if (j == kChunk / 2) id_next = page_at((first + kChunk) * kGroupsOr1 + (int32_t) lane);
-                    if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
-                    __syncwarp();
+                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     store_tile(b);
                     mbar_arrive(&full[b]);
                     if (j == kChunk - 1) first += kChunk, base = base_of(first * kGroupsOr1 + (int32_t) lane, id_next);
@@ -558,8 +563,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 load(g.t0);
                 for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
-                    if (!(ok = mbar_wait<kSuspendNs>(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
-                    __syncwarp();
+                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
                     if (!is_v) {
                         TileScales &sc = scales[n % kScaleSets];
                         const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
@@ -718,8 +722,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
             // O so far is multiplied by a factor per row.  Every product into it must have completed.
             auto scale_o = [&](float by) -> bool {
-                const bool done = mbar_wait<kSuspendNs>(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag);
-                if (!__all_sync(0xffffffffu, done)) return false;
+                if (!warp_wait(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag)) return false;
                 tc_fence_after();
                 for (int32_t c0 = 0; c0 < p.c.dh; c0 += 64) {
                     float o[64];
@@ -789,9 +792,8 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         if (j == kChunk - 1) first += kChunk, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                         if (tile + 1 < g.t1) look_at(tile + 1);
                     };
-                    if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
                     tc_fence_after();
-                    __syncwarp();// lanes leave a wait at different times; the TMEM accesses are the whole warp's
                     uint32_t w[kKeys / 2];
                     float gain = 0.f, most = 0.f;// what the tile adds to l; the largest sum of 16 (or 8) weights
                     auto exponents = [&]() {
@@ -909,11 +911,10 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
                     const uint32_t b = n & 1u;
                     const TileScales &sc = scales[n_all % kScaleSets];
-                    if (!(ok = mbar_wait<kSuspendNs>(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
                     // (after S: a block that sat out items may be ahead by more than a parity can tell)
-                    if (!(ok = mbar_wait<kSuspendNs>(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
                     tc_fence_after();
-                    __syncwarp();
                     float x[kKeys];
                     tmem_ld64(t_lane + b * kKeys, x);
                     const uint32_t m0 = sc.mask[0], m1 = sc.mask[1];
@@ -959,7 +960,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 if (kQBufs == 2) rf_next = finish_q(other);
             }
             // ---- the item's output, or its part
-            if (!(ok = mbar_wait<kSuspendNs>(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+            if (!(ok = warp_wait(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
             if (more && GROUPS > 0) {
                 if (id >= p.c.pages) id = -1;

@@ -641,12 +641,15 @@ def test_attend(cuda_lib, q_heads, kv_heads, page, dh, lens, news, layout, spare
 @gpu
 @pytest.mark.parametrize("new", [1, 4, 150])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attend_values_that_lead_nowhere(cuda_lib, dtype, new):
+@pytest.mark.parametrize("P", [16, 64, 20])
+def test_attend_values_that_lead_nowhere(cuda_lib, P, dtype, new):
     """Missing pages are masked (a row that sees none of its keys gets zeros), offsets outside the rows are clamped,
     lengths may be below the new tokens (their first rows see nothing), beyond the table, zero or negative."""
-    H, P, D, G = 2, 16, 64, 3
+    H, D, G = 2, 64, 3
     lens = [40, 3, 200, -5, 0, 33, 5]
-    table = make_tables([40, 16, 64, 16, 16, 33, 5], P, 20, 32, cols=4)
+    table = make_tables([40, 16, min(4 * P, 200), 16, 16, 33, 5], P, 20, 32, cols=4)
+    if P > 16:
+        table[2, 0], table[5, 1] = 20, -3                     # the first keys are missing
     table[0, 1], table[5, 2], table[6, 0] = 20, -2147483648, -1
     cache = make_cache(20, H, P, D, 31)
     if new == 1:

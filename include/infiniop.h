@@ -340,7 +340,7 @@ INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheAppendDescriptor(infiniop
  * q, out F16 or BF16 [rows, n_q_head, dh], unit innermost stride, free positive
  * outer strides; `scale` finite; n_q_head <= 65535, and rows * n_q_head /
  * n_kv_head < 2^31.  The new tokens' own k and v are read from the pages: append
- * them first.  A token without visible keys gets zeros.  What the pages hold
+ * them first.  out may be q itself.  A token without visible keys gets zeros.  What the pages hold
  * behind a sequence's last token is not used, NaN included; a NaN among the
  * cached values of a later new token of the call may reach the outputs of the
  * sequence's earlier ones (it is multiplied by a weight of zero). */

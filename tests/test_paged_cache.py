@@ -1065,3 +1065,39 @@ def test_two_streams_at_once(cuda_lib):
             assert torch.equal(j[0], a)
     for o in plans:
         o.destroy()
+
+
+@gpu
+@pytest.mark.parametrize("new,D", [(1, 128), (3, 64), (150, 128), (150, 256)])
+def test_captured_attention_over_long_tables(cuda_lib, new, D):
+    """The forms that split work over CTAs and join it in a second kernel, captured with a table in a wider tensor and
+    replayed twice as often as the lengths change; the outputs written over the queries, on another stream, agree."""
+    lib, handle = cuda_lib
+    H, G, P = 2, 4, 32
+    cache = [to_dev(x) for x in make_cache(120, H, P, D, 191)]
+    table = wide(make_tables([1500, 700], P, 120, 192, cols=60), P).to(DEV)
+    table = table[:, :table.shape[1] - 5]
+    offs = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([new, new], dtype=torch.int32, device=DEV)
+    q = new_rows(2 * new, H * G, D, torch.bfloat16, 193).to(DEV)
+    out, s, other = torch.zeros_like(q), torch.cuda.Stream(), torch.cuda.Stream()
+    with ops.PagedAttentionOp(lib, handle, out, q, *cache, table, lens, offs) as att:
+        assert att.workspace is not None
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            att(out, q, *cache, table, lens, offs, stream=s)
+        for l0, l1 in ((new, new), (1500, 700), (151, 0), (1, 650)):
+            lens.copy_(torch.tensor([l0, l1], dtype=torch.int32))
+            out.fill_(7.0)
+            g.replay()
+            g.replay()
+            torch.cuda.synchronize()
+            over = q.clone()
+            torch.cuda.synchronize()
+            ops.paged_attention(lib, handle, over, over, *cache, table, lens, offs, stream=other)
+            torch.cuda.synchronize()
+            assert torch.equal(out, over)
+            want, tol = attend_ref(q.cpu(), *(x.cpu() for x in cache), table.cpu(), [l0, l1], offs.tolist(), D ** -0.5, torch.zeros_like(q).cpu())
+            close(out, want, tol)
+        del g

@@ -37,8 +37,8 @@
 // barrier's parity could not tell the two apart.
 // Every wait is bounded (tc_ptx.cuh).
 //
-// 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 150 us, 935 TFLOP/s.  Two prompts of up to 4096
-// tokens, nothing cached before them, fp16: 151 us, 695 TFLOP/s of the visible products.
+// 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 152 us, 920 TFLOP/s.  Two prompts of up to 4096
+// tokens, nothing cached before them, fp16: 150 us, 700 TFLOP/s of the visible products.
 #include "paged_attention.cuh"
 #include "tc_ptx.cuh"
 
@@ -52,7 +52,7 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = kPrefillKeys;
-constexpr float kSlack = 13.f, kLift = 2.f;// w <= 2^15
+constexpr float kSlack = 13.f, kLift = 2.f;// kSlack: of the general form, w <= 2^15 there
 constexpr float kLeast = -90.f;
 constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
 constexpr int kItemUnits = 6;// what the start and the end of an item cost, in tiles
@@ -869,30 +869,32 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     if (hidden_now || __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
                         for (int pass = 0; pass < 3; ++pass) {// (a row that has moved has weights of 2^lift at most: it ends here)
-                            float x[kKeys];
+                            // (the same arithmetic as above: a row's weights are the same whichever way its warp goes; a
+                            // factor of zero, which would make NaN of -inf, becomes scores of zero)
+                            float x[kKeys], f[GROUPS];
                             tmem_ld64(t_lane + b * kKeys, x);
+#pragma unroll
+                            for (int i = 0; i < GROUPS; ++i) f[i] = factor_now[i] > 0.f ? factor_now[i] : 1.f;
 #pragma unroll
                             for (int i = 0; i < kKeys; ++i) {
                                 const int gr = i / kTokens;
-                                x[i] = i < left_now && (GROUPS == 1 || !(gone_now >> gr & 1u)) ? x[i] * factor_now[gr] : -INFINITY;
+                                if (!(factor_now[gr] > 0.f)) x[i] = 0.f;
+                                if (i >= left_now || (GROUPS > 1 && (gone_now >> gr & 1u))) x[i] = -INFINITY;
                             }
                             if (__any_sync(0xffffffffu, move)) {
                                 float top = -INFINITY, wtop = -INFINITY;
 #pragma unroll
                                 for (int i = 0; i < GROUPS; ++i) {
                                     const float y = GROUPS == 4 ? largest<16>(x + i * kTokens) : fmaxf(largest<32>(x), largest<32>(x + 32));
-                                    if (y > -INFINITY) top = fmaxf(top, y), wtop = fmaxf(wtop, y + lv_now[i]);
+                                    if (y > -INFINITY) top = fmaxf(top, y * f[i]), wtop = fmaxf(wtop, y * f[i] + lv_now[i]);
                                 }
                                 if (!(ok = move_references(move && top > -INFINITY, top, wtop, tile))) break;
                                 forget();
                             }
                             exponents();
-                            float one[GROUPS];
-#pragma unroll
-                            for (int i = 0; i < GROUPS; ++i) one[i] = 1.f;
                             clear();
-                            weigh(x, w, one, 0);
-                            weigh(x + 32, w + 16, one, 1);
+                            weigh(x, w, f, 0);
+                            weigh(x + 32, w + 16, f, 1);
                             add_up();
                             move = most > kMostWeight;
                             if (!__any_sync(0xffffffffu, move)) break;

@@ -719,6 +719,28 @@ def test_attend_row_with_infinity_stays_alone(cuda_lib):
 
 
 @gpu
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("new", [2, 150])
+def test_attend_rows_do_not_touch_each_other(cuda_lib, P, new):
+    """A row's bits do not depend on what the rows beside it attend to: half of the rows become ones whose running maximum
+    keeps rising."""
+    H, D, n = 1, 64, 700
+    cache = make_cache(-(-n // P), H, P, D, 75)
+    table = wide(make_tables([n], P, -(-n // P), 76), P)
+    k = cache[0].float()
+    for j in range(n):
+        k[int(table[0, j // P]), 0, j % P, 0] = j / 8.0
+    cache[0].copy_(k.to(CODE))
+    cache[2].fill_(1.0 / 16)
+    q = new_rows(new, 4, D, torch.bfloat16, 77)
+    q[:, :, 0] = 0
+    risen = q.clone()
+    risen[:, ::2, 0] = 16.0
+    args = (table, torch.tensor([n], dtype=torch.int32), torch.tensor([0, new], dtype=torch.int32), 1.0 / 3, torch.zeros_like(q))
+    assert torch.equal(run_attend(cuda_lib, q, cache, *args)[:, 1::2], run_attend(cuda_lib, risen, cache, *args)[:, 1::2])
+
+
+@gpu
 @pytest.mark.parametrize("new", [1, 6, 70])
 def test_attend_strided_rows(cuda_lib, new):
     """q as a slice of a fused projection, out with heads outermost, storage bases off 16 bytes."""

@@ -55,6 +55,7 @@ constexpr int kRows = 128, kKeys = kPrefillKeys;
 constexpr float kSlack = 13.f, kLift = 2.f;// kSlack: of the general form, w <= 2^15 there
 constexpr float kLeast = -90.f;
 constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
+constexpr float kFarGain = 0x1p64f;// what a tile may add to a row's sum: 2^25 such tiles stay below 2^90
 constexpr int kItemUnits = 6;// what the start and the end of an item cost, in tiles
 constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;
@@ -735,13 +736,15 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 tmem_st_finish();
                 return true;
             };
-            // The references of the rows that ask for it move to this tile's largest: O so far and the sum follow.
+            // The references of the rows that ask for it rise to this tile's largest: O so far and the sum follow.  (A score
+            // may be the largest so far and its weight a small one, by its values' scale, and the other way round.)
             auto move_references = [&](bool up, float top, float wtop, int32_t tile) -> bool {
-                const float shrink = up ? fast_exp2(wm - wtop) : 1.f;
+                float shrink = 1.f;
                 if (up) {
-                    const float m_new = fmaxf(m, top);
-                    l *= fast_exp2(m - m_new);// (from -inf: 0)
-                    m = m_new, wm = wtop;
+                    const float m_new = fmaxf(m, top), wm_new = fmaxf(wm, wtop);
+                    if (wm_new > wm) shrink = fast_exp2(wm - wm_new);// (from -inf: 0)
+                    l *= fast_exp2(m - m_new);
+                    m = m_new, wm = wm_new;
                 }
                 return tile == g.t0 || !__any_sync(0xffffffffu, up) || scale_o(shrink);
             };
@@ -853,8 +856,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         tmem_ld32_finish(x + 32);
                         weigh(x + 32, w + 16, factor_now, 1);
                         add_up();
-                        if (__any_sync(0xffffffffu, most > kMostWeight)) {
-                            move = most > kFarWeight;
+                        if (__any_sync(0xffffffffu, most > kMostWeight || gain > kFarGain)) {
+                            // (the sum of p may be far beyond what the weights tell, where the values' scale is small)
+                            move = most > kFarWeight || gain > kFarGain;
                             const float top = fmaxf(largest<32>(x), largest<32>(x + 32));
                             const int32_t up = most > kMostWeight && !move ? (int32_t) (__float_as_uint(top) >> 23) - (127 + (int32_t) kLift) : 0;
                             const float by = __uint_as_float(pow2_bits(-up));
@@ -896,7 +900,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             weigh(x, w, f, 0);
                             weigh(x + 32, w + 16, f, 1);
                             add_up();
-                            move = most > kMostWeight;
+                            move = most > kMostWeight || gain > kFarGain;
                             if (!__any_sync(0xffffffffu, move)) break;
                         }
                     }

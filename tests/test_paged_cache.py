@@ -741,6 +741,33 @@ def test_attend_rows_do_not_touch_each_other(cuda_lib, P, new):
 
 
 @gpu
+@pytest.mark.parametrize("P", [16, 64, 20])
+@pytest.mark.parametrize("new", [1, 140])
+def test_attend_leap_over_a_page_of_zeros(cuda_lib, P, new):
+    """A score leaps by 2^130 at a key whose page holds nothing but zeros (scale 2^-40, as the append writes): its weight is
+    small, its share of the sum is not.  A later key of an ordinary page counts for more still."""
+    H, D, n = 1, 64, 400
+    cache = make_cache(-(-n // P), H, P, D, 221)
+    table = make_tables([n], P, -(-n // P), 222)
+    k, v = cache[0].float(), cache[1].float()
+    k[..., 0] = 0.0
+    cache[2].fill_(1.0 / 16)
+    cache[3].fill_(2.0 ** -7)
+    for j in range(n):
+        if 128 // P <= j // P <= 191 // P:
+            v[int(table[0, j // P])] = 0.0
+            cache[3][int(table[0, j // P])] = 2.0 ** -40
+    k[int(table[0, 150 // P]), 0, 150 % P, 0] = 88.0
+    k[int(table[0, 245 // P]), 0, 245 % P, 0] = 96.0
+    cache[0].copy_(k.to(CODE)), cache[1].copy_(v.to(CODE))
+    q = new_rows(new, 4, D, torch.float16, 223) * 0.1
+    q[:, :, 0] = 16.0
+    # (the leap in powers of two at scale s: 88 s log2(e), 128 to 131 from s = 1.01 on)
+    for scale in (1.0, 90 / 88, 1.03):
+        check_attend(cuda_lib, q, cache, table, [n], [0, new], scale=scale)
+
+
+@gpu
 @pytest.mark.parametrize("new", [1, 6, 70])
 def test_attend_strided_rows(cuda_lib, new):
     """q as a slice of a fused projection, out with heads outermost, storage bases off 16 bytes."""

@@ -8,12 +8,14 @@
 // Softmax in one pass: p = 2^(s f - m) with f the row's and the page's factor and m the row's reference, at first the largest
 // score of its first tile.  The weight of a value is w = p * 2^c with 2^c = 2^(m - M + 2) * (scale of the values' page) and M
 // the weights' own reference.  No tile is looked through for its largest score: sums of 16 weights, formed anyway, tell when a
-// weight may have grown beyond fp16.  Then both references of the row follow by the power of two that brings the tile's largest
-// weight back to [2^2, 2^3), and the tile's weights (still in fp32 in registers), l and O are divided by it, exactly.  (Looking
-// for the maximum and forming the weights anew took 187 us where this takes 162, in heads whose scores spread widely.)  fp16
+// weight may have grown beyond fp16.  Then M follows by the power of two that brings the tile's largest weight back to
+// [2^2, 2^3), and the tile's weights (still in fp32 in registers) and O are divided by it, exactly.  (Looking for the maximum
+// and forming the weights anew took 187 us where this takes 162, in heads whose scores spread widely.)  m is no part of that:
+// weights also grow with the scales of the values' pages, which the sum of p must not follow.  m moves to the tile's largest
+// score, and M to its largest weight, where the tile would add more than 2^64 to the sum or weights pass 2^100.  fp16
 // holds weights down to 2^-16 of the reference with all their bits, smaller ones to 2^-27 of it.  One exponential gives w;
-// the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way, and
-// their sum must not underflow.
+// the sum of p takes the tile's sum of w times 2^-c.  c is kept above -90: such weights are zero in fp16 either way (p < 2^64),
+// and their sum must not underflow.
 //
 // What bounds it: per tile and block 64 x 128 exponentials (16 a cycle and SM: 512 cycles) stand against 2 x 64 x 128 x dh
 // multiply-adds (at dh 128: 256 cycles at full rate; S with its 64 columns runs at two thirds of it, 640 in all).  One CTA per SM
@@ -842,9 +844,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         for (int i = 0; i < (GROUPS == 4 ? 4 : 2); ++i) part[i] = 0ull;
                     };
                     // Most tiles hide nothing and move no reference: their weights are formed at once, and the sums tell
-                    // whether one may have grown beyond what fp16 holds.  A row that finds so lets its references follow by a
-                    // power of two, which its weights (still in fp32), sum and O are divided by, exactly.  What a row does
-                    // depends on its own scores alone.
+                    // whether one may have grown beyond what fp16 holds.  A row that finds so lets the weights' reference
+                    // follow by a power of two, which its weights (still in fp32) and O are divided by, exactly.  What a row
+                    // does depends on its own scores alone.
                     if (!hidden_now && !some) {
                         float x[kKeys];
                         tmem_ld32(t_lane + b * kKeys, x);
@@ -864,7 +866,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             const float by = __uint_as_float(pow2_bits(-up));
 #pragma unroll
                             for (int i = 0; i < kKeys / 2; ++i) w[i] = round16x2(false, x[2 * i] * by, x[2 * i + 1] * by);
-                            gain *= by, l *= by, m += (float) up, wm += (float) up, forget();
+                            wm += (float) up, forget();
                             if (tile > g.t0 && !(ok = scale_o(by))) break;
                         }
                     } else {

@@ -768,6 +768,35 @@ def test_attend_leap_over_a_page_of_zeros(cuda_lib, P, new):
 
 
 @gpu
+@pytest.mark.parametrize("P", [16, 64, 20])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("step,level", [(30, 0.0), (15, 0.0), (30, 4.0), (-30, 0.0), (75, -8.0)])
+def test_attend_scales_in_stairs(cuda_lib, P, new, step, level):
+    """The values' scales climb from 2^-40 to 2^110 (or fall) in steps of pages while the scores stay or move a little:
+    however far the weights' reference goes, every key keeps its place in the denominator.  300 sequences that are all the
+    same, enough for a CTA to walk one from its first key to its last."""
+    H, D, B, stair, steps = 1, 64, 300, 192, 150 // abs(step) + 1
+    n = stair * steps
+    cache = make_cache(-(-n // P), H, P, D, 231)
+    table = make_tables([n], P, -(-n // P), 232)
+    k = cache[0].float()
+    cache[2].fill_(1.0 / 16)
+    for j in range(0, n, P):
+        p, i = int(table[0, j // P]), j // stair
+        k[p, 0, :, 0] = level * i
+        cache[3][p] = 2.0 ** ((-40 if step > 0 else 110) + step * i)
+    cache[0].copy_(k.to(CODE))
+    q = new_rows(new, 4, D, torch.bfloat16, 233) * 0.1
+    q[:, :, 0] = 16.0
+    want, tol = attend_ref(q, *cache, table, [n], [0, new], 1.0, torch.zeros_like(q))
+    lens, offs = torch.full((B,), n, dtype=torch.int32), torch.arange(0, B * new + 1, new, dtype=torch.int32)
+    for room in (table, wide(table, P)):
+        got = run_attend(cuda_lib, q.repeat(B, 1, 1), cache, room.expand(B, -1).contiguous(), lens, offs, 1.0, torch.zeros(B * new, 4, D, dtype=q.dtype))
+        for b in (0, 1, 150, B - 1):
+            close(got[b * new:b * new + new], want, tol)
+
+
+@gpu
 @pytest.mark.parametrize("new", [1, 6, 70])
 def test_attend_strided_rows(cuda_lib, new):
     """q as a slice of a fused projection, out with heads outermost, storage bases off 16 bytes."""

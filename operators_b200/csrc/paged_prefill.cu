@@ -835,20 +835,28 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             }
                         } else {
                             const float2 s0 = unpack2f(part[0]), s1 = unpack2f(part[1]);
-                            gain = ((s0.x + s0.y) + (s1.x + s1.y)) * e_back[0];
+                            gain = __fmul_rn((s0.x + s0.y) + (s1.x + s1.y), e_back[0]);
                             most = fmaxf(fmaxf(s0.x, s0.y), fmaxf(s1.x, s1.y));
                         }
                     };
+                    // (the sum of p may go far where the weights tell nothing, where the values' scale is small)
+                    auto far = [&]() -> bool { return most > kFarWeight || gain > kFarGain; };
                     auto clear = [&]() {
 #pragma unroll
                         for (int i = 0; i < (GROUPS == 4 ? 4 : 2); ++i) part[i] = 0ull;
                     };
                     // Most tiles hide nothing and move no reference: their weights are formed at once, and the sums tell
                     // whether one may have grown beyond what fp16 holds.  A row that finds so lets the weights' reference
-                    // follow by a power of two, which its weights (still in fp32) and O are divided by, exactly.  What a row
-                    // does depends on its own scores alone.
-                    if (!hidden_now && !some) {
-                        float x[kKeys];
+                    // follow by a power of two, which its weights (still in fp32) and O are divided by, exactly.
+                    //
+                    // What a row does, and so its bits, depends on its own scores alone, whichever way its warp goes: a row
+                    // without references takes its tile's largest; one whose weights or sum went far moves them there; one
+                    // whose weights outgrew fp16 follows.  A tile taken a second time for the sake of one row gives the
+                    // others the weights that they had: the same references, the same arithmetic (products and sums that
+                    // the compiler may not contract).
+                    float x[kKeys];
+                    bool again = hidden_now || some;
+                    if (!again) {
                         tmem_ld32(t_lane + b * kKeys, x);
                         tmem_ld32_start(t_lane + b * kKeys + 32, x + 32);
                         exponents();
@@ -858,26 +866,16 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         tmem_ld32_finish(x + 32);
                         weigh(x + 32, w + 16, factor_now, 1);
                         add_up();
-                        if (__any_sync(0xffffffffu, most > kMostWeight || gain > kFarGain)) {
-                            // (the sum of p may be far beyond what the weights tell, where the values' scale is small)
-                            move = most > kFarWeight || gain > kFarGain;
-                            const float top = fmaxf(largest<32>(x), largest<32>(x + 32));
-                            const int32_t up = most > kMostWeight && !move ? (int32_t) (__float_as_uint(top) >> 23) - (127 + (int32_t) kLift) : 0;
-                            const float by = __uint_as_float(pow2_bits(-up));
-#pragma unroll
-                            for (int i = 0; i < kKeys / 2; ++i) w[i] = round16x2(false, x[2 * i] * by, x[2 * i + 1] * by);
-                            wm += (float) up, forget();
-                            if (tile > g.t0 && !(ok = scale_o(by))) break;
-                        }
+                        move = far();
+                        again = __any_sync(0xffffffffu, move);
                     } else {
                         next();
                     }
-                    if (hidden_now || __any_sync(0xffffffffu, move)) {
+                    if (again) {
 #pragma unroll 1
                         for (int pass = 0; pass < 3; ++pass) {// (a row that has moved has weights of 2^lift at most: it ends here)
-                            // (the same arithmetic as above: a row's weights are the same whichever way its warp goes; a
-                            // factor of zero, which would make NaN of -inf, becomes scores of zero)
-                            float x[kKeys], f[GROUPS];
+                            // (a factor of zero, which would make NaN of -inf, becomes scores of zero)
+                            float f[GROUPS];
                             tmem_ld64(t_lane + b * kKeys, x);
 #pragma unroll
                             for (int i = 0; i < GROUPS; ++i) f[i] = factor_now[i] > 0.f ? factor_now[i] : 1.f;
@@ -892,7 +890,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
 #pragma unroll
                                 for (int i = 0; i < GROUPS; ++i) {
                                     const float y = GROUPS == 4 ? largest<16>(x + i * kTokens) : fmaxf(largest<32>(x), largest<32>(x + 32));
-                                    if (y > -INFINITY) top = fmaxf(top, y * f[i]), wtop = fmaxf(wtop, y * f[i] + lv_now[i]);
+                                    if (y > -INFINITY) top = fmaxf(top, __fmul_rn(y, f[i])), wtop = fmaxf(wtop, __fadd_rn(__fmul_rn(y, f[i]), lv_now[i]));
                                 }
                                 if (!(ok = move_references(move && top > -INFINITY, top, wtop, tile))) break;
                                 forget();
@@ -902,11 +900,20 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                             weigh(x, w, f, 0);
                             weigh(x + 32, w + 16, f, 1);
                             add_up();
-                            move = most > kMostWeight || gain > kFarGain;
+                            move = far();
                             if (!__any_sync(0xffffffffu, move)) break;
                         }
+                        if (!ok) break;
                     }
-                    if (!ok) break;
+                    if (__any_sync(0xffffffffu, most > kMostWeight)) {
+                        const float top = fmaxf(largest<32>(x), largest<32>(x + 32));
+                        const int32_t up = most > kMostWeight ? (int32_t) (__float_as_uint(top) >> 23) - (127 + (int32_t) kLift) : 0;
+                        const float by = __uint_as_float(pow2_bits(-up));
+#pragma unroll
+                        for (int i = 0; i < kKeys / 2; ++i) w[i] = round16x2(false, x[2 * i] * by, x[2 * i + 1] * by);
+                        wm += (float) up, forget();
+                        if (tile > g.t0 && !(ok = scale_o(by))) break;
+                    }
                     l += gain;
                     __syncwarp();
                     tmem_st32(t_lane + b * kKeys, w);

@@ -797,6 +797,33 @@ def test_attend_scales_in_stairs(cuda_lib, P, new, step, level):
 
 
 @gpu
+@pytest.mark.parametrize("P", [16, 64, 20])
+@pytest.mark.parametrize("new", [2, 150])
+@pytest.mark.parametrize("start,width", [(200, 300), (200, 1), (690, 5), (511, 2), (64, 64)])
+@pytest.mark.parametrize("dh", [64, 256])
+def test_attend_rows_beside_leaping_ones(cuda_lib, dh, start, width, new, P):
+    """A row's bits do not depend on the rows beside it, where its own weights outgrow fp16 in the very tile in which theirs
+    leap beyond 2^100, or where those rows are NaN."""
+    H, n = 1, 700
+    cache = make_cache(-(-n // P), H, P, dh, 241)
+    table = wide(make_tables([n], P, -(-n // P), 242), P)
+    k = cache[0].float()
+    k[..., 0] = 0.0
+    for j in range(start, start + width):
+        k[int(table[0, j // P]), 0, j % P, 0] = 14.0 + 0.25 * (j % 8)
+    cache[0].copy_(k.to(CODE))
+    cache[2].fill_(1.0 / 16)
+    q = new_rows(new, 4, dh, torch.bfloat16, 243)
+    q[:, :, 0] = 32.0                                         # 28 and more: 40 powers of two
+    args = (table, torch.tensor([n], dtype=torch.int32), torch.tensor([0, new], dtype=torch.int32), 1.0 / 0.97, torch.zeros_like(q))
+    quiet = run_attend(cuda_lib, q, cache, *args)
+    for level in (0.0, 400.0, -400.0, math.nan, math.inf):
+        other = q.clone()
+        other[:, ::2, 0] = level
+        assert torch.equal(run_attend(cuda_lib, other, cache, *args)[:, 1::2], quiet[:, 1::2]), level
+
+
+@gpu
 @pytest.mark.parametrize("new", [1, 6, 70])
 def test_attend_strided_rows(cuda_lib, new):
     """q as a slice of a fused projection, out with heads outermost, storage bases off 16 bytes."""

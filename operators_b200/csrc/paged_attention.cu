@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 float sum = l[nt][i];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                if (g == 0) sh[warp * kRows + r] = PartHead{m[nt][i], sum, wm[nt][i], 0.f};
+                if (g == 0) sh[warp * kRows + r] = PartHead{m[nt][i], sum, wm[nt][i], limit[nt][i]};
                 // elements g * DHC / 8 .. of this row; 16-byte groups rotated by the row, so that the four rows of a
                 // store spread over the banks
                 float *dst = so + (warp * kRows + r) * DHC;
@@ -581,14 +581,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
             float mr = -INFINITY, wr = -INFINITY, lr = 0.f, f[kWarps];
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) mr = fmaxf(mr, sh[i * kRows + r].m), wr = fmaxf(wr, sh[i * kRows + r].w);
+            const float m0 = mr == -INFINITY ? 0.f : mr;// (warps without a reference: their l is 0 or NaN)
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
                 const PartHead h = sh[i * kRows + r];
-                lr += h.m == -INFINITY ? 0.f : h.l * fast_exp2(h.m - mr);
+                lr += h.l * fast_exp2(h.m - m0);
                 f[i] = h.w == -INFINITY ? 0.f : fast_exp2(h.w - wr);
             }
             uint16_t *out = row_of_out(p, s, kvh, (uint32_t) rb * kRows + (uint32_t) r);
-            if (!whole && lane == 0) (cl > 0 ? ph[r] : dp.heads[slot0 + r]) = PartHead{mr, lr, wr - kLift, 0.f};
+            if (!whole && lane == 0) (cl > 0 ? ph[r] : dp.heads[slot0 + r]) = PartHead{mr, lr, wr - kLift, sh[r].keys};
 #pragma unroll
             for (int j = 0; j < (DHC + 127) / 128; ++j) {
                 const uint32_t grp = lane + 32 * j;
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     const float4 a = *reinterpret_cast<const float4 *>(so + (i * kRows + r) * DHC + ((grp ^ (uint32_t) (r & 7)) << 2));
                     if (f[i] != 0.f) y.x += f[i] * a.x, y.y += f[i] * a.y, y.z += f[i] * a.z, y.w += f[i] * a.w;
                 }
-                if (whole) store_out(p, out, (int32_t) grp * 4, y, out_factors(lr, wr - kLift - mr));
+                if (whole) store_out(p, out, (int32_t) grp * 4, y, out_factors(p, b, sh[r].keys, lr, wr - kLift - mr));
                 else *reinterpret_cast<float4 *>(cl > 0 ? po + r * DHC + grp * 4 : dp.parts + (slot0 + r) * DHC + grp * 4) = y;
             }
         }
@@ -612,15 +613,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 PartHead h[kMaxCluster];
 #pragma unroll
                 for (uint32_t i = 0; i < kMaxCluster; ++i) {
-                    h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0.f};
+                    h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0};
                     if (i < cl) {
                         const float4 v = ld_cluster4(ph_at + (uint32_t) r * 16u, i);
-                        h[i] = PartHead{v.x, v.y, v.z, v.w};
+                        h[i] = PartHead{v.x, v.y, v.z, __float_as_int(v.w)};
                     }
                     mr = fmaxf(mr, h[i].m), wr = fmaxf(wr, h[i].w);
                 }
 #pragma unroll
-                for (uint32_t i = 0; i < kMaxCluster; ++i) lr += h[i].m == -INFINITY ? 0.f : h[i].l * fast_exp2(h[i].m - mr);
+                for (uint32_t i = 0; i < kMaxCluster; ++i) lr += h[i].l * fast_exp2(h[i].m - (mr == -INFINITY ? 0.f : mr));
                 uint16_t *out = row_of_out(p, s, kvh, (uint32_t) rb * kRows + (uint32_t) r);
 #pragma unroll
                 for (int j = 0; j < (DHC + 127) / 128; ++j) {
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                             y.x += f * a.x, y.y += f * a.y, y.z += f * a.z, y.w += f * a.w;
                         }
                     }
-                    store_out(p, out, (int32_t) grp * 4, y, out_factors(lr, wr - mr));
+                    store_out(p, out, (int32_t) grp * 4, y, out_factors(p, b, sh[r].keys, lr, wr - mr));
                 }
             }
             cluster_sync_all();// nobody leaves while its part may still be read

@@ -55,10 +55,28 @@ __device__ __forceinline__ uint32_t round16x2(bool bf16, float lo, float hi) {
     return r;
 }
 
+// Keys that the rr-th query row (new token x q head of the group) of a sequence may see (pages may be missing among them).
+__device__ __forceinline__ int32_t keys_of_row(const AttendParams &p, const Seq &s, uint32_t rr) {
+    return max(0, min(s.len - s.n + (int32_t) p.group_div.div(rr) + 1, held(s.len, p.t.cap)));
+}
+// One of the first `keys` tokens of sequence b lies in a page.
+__device__ __forceinline__ bool any_page(const AttendParams &p, int32_t b, int32_t keys) {
+    const int32_t cols = keys > 0 ? (int32_t) p.page_div.div((uint32_t) keys - 1) + 1 : 0;
+#pragma unroll 1
+    for (int32_t i = 0; i < cols; ++i) {
+        const int32_t id = p.table[(int64_t) b * p.t.stride + i];
+        if (id >= 0 && id < p.c.pages) return true;
+    }
+    return false;
+}
 // A row's output is y * 2^exponent / l; the power of two may leave fp32's range on the way, so it is applied as two
-// factors.  Rows that have seen no key (l = 0) get zeros.
-__device__ __forceinline__ float2 out_factors(float l, float exponent) {
-    if (l == 0.f) return make_float2(0.f, 0.f);
+// factors.  l = 0: a row that sees no key gets zeros; one whose scores are all -inf is 0 / 0.  (A score of NaN makes l
+// NaN, also where the row has no reference for it: l is added up and scaled, never left out.)
+__device__ __forceinline__ float2 out_factors(const AttendParams &p, int32_t b, int32_t keys, float l, float exponent) {
+    if (l == 0.f) {
+        const float none = any_page(p, b, keys) ? NAN : 0.f;
+        return make_float2(none, none);
+    }
     const float h = truncf(exponent * 0.5f);
     return make_float2(exp2f(h) / l, exp2f(exponent - h));
 }
@@ -126,7 +144,8 @@ __device__ __forceinline__ float log2_of(float v) {
 
 // A row's part: sum over its keys of 2^(score - m) = l, and of 2^(score - w) * scale of the value * code = the output
 struct PartHead {
-    float m, l, w, pad;
+    float m, l, w;
+    int32_t keys;// decoding: keys_of_row
 };
 struct CtaMeta {
     int32_t b, kvh, rb;// the item that begins in this CTA's stretch and goes on behind it; b < 0: none
@@ -183,19 +202,18 @@ __global__ void __launch_bounds__(JoinShape<ROWS>::kRows * JoinShape<ROWS>::kGro
         for (int i = 0; i < kBatch; ++i) {
             const int32_t c = c0 + i * kJoinGroups;
             const int64_t at = ((int64_t) c * 2 + (c == first ? 1 : 0)) * ROWS + r;
-            h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0.f};
+            h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0};
             v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (c <= item.last) h[i] = dp.heads[at], v[i] = *reinterpret_cast<const float4 *>(dp.parts + at * DHC + ln * 4);
         }
         float m1 = m, w1 = w;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) m1 = fmaxf(m1, h[i].m), w1 = fmaxf(w1, h[i].w);
-        if (m1 != -INFINITY) {
-            l *= fast_exp2(m - m1);// (from -inf: 0)
+        const float m0 = m1 == -INFINITY ? 0.f : m1;// (parts without a reference: their l is 0 or NaN)
+        l *= fast_exp2(m - m0);// (from -inf: 0)
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) l += h[i].l * fast_exp2(h[i].m - m1);
-            m = m1;
-        }
+        for (int i = 0; i < kBatch; ++i) l += h[i].l * fast_exp2(h[i].m - m0);
+        m = m1;
         if (w1 != -INFINITY) {
             const float f0 = fast_exp2(w - w1);
             y.x *= f0, y.y *= f0, y.z *= f0, y.w *= f0;
@@ -216,14 +234,14 @@ __global__ void __launch_bounds__(JoinShape<ROWS>::kRows * JoinShape<ROWS>::kGro
     for (int i = 0; i < kJoinGroups; ++i) m = fmaxf(m, stat[sub][i][0]), w = fmaxf(w, stat[sub][i][2]);
 #pragma unroll
     for (int i = 0; i < kJoinGroups; ++i) {
-        if (stat[sub][i][0] != -INFINITY) l += stat[sub][i][1] * fast_exp2(stat[sub][i][0] - m);
+        l += stat[sub][i][1] * fast_exp2(stat[sub][i][0] - (m == -INFINITY ? 0.f : m));
         if (stat[sub][i][2] != -INFINITY) {
             const float f = fast_exp2(stat[sub][i][2] - w);
             const float4 v = acc[sub][i][ln];
             y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
         }
     }
-    store_out(p, row_of_out(p, s, item.kvh, rr), ln * 4, y, out_factors(l, w - m));
+    store_out(p, row_of_out(p, s, item.kvh, rr), ln * 4, y, out_factors(p, item.b, keys_of_row(p, s, rr), l, w - m));
 }
 
 template<int DHC, int ROWS>

@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
 #pragma unroll
                             for (int i = 0; i < kKeys; ++i) {
                                 const int gr = i / kTokens;
-                                if (!(factor_now[gr] > 0.f)) x[i] = 0.f;
+                                if (!(factor_now[gr] > 0.f)) x[i] *= factor_now[gr];
                                 if (i >= left_now || (GROUPS > 1 && (gone_now >> gr & 1u))) x[i] = -INFINITY;
                             }
                             if (__any_sync(0xffffffffu, move)) {
@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 return y;
             };
             if (whole) {
-                const float2 fac = none ? make_float2(0.f, 0.f) : out_factors(l, wm - kLift - m);
+                const float2 fac = out_factors(p, g.b, limit, l, wm - kLift - m);
                 for (int32_t c0 = 0; c0 < p.c.dh; c0 += 64) {
                     float o[64];
                     __syncwarp();
@@ -1054,7 +1054,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 }
             }
             __syncwarp();
-            if (!whole && have) sp.heads[at0 + lane] = PartHead{m, l, wm - kLift, 0.f};
+            if (!whole && have) sp.heads[at0 + lane] = PartHead{m, l, wm - kLift, 0};
             if (!whole && part == 1) meta = CtaMeta{g.b, g.kvh, g.rb, (int32_t) divide(g.last_unit, each)};
             tc_fence_before();
             if (kQBufs == 2) {

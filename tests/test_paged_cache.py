@@ -718,6 +718,80 @@ def test_attend_row_with_infinity_stays_alone(cuda_lib):
         assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
 
 
+def attend_softmax(q, cache, table, lens, offs, scale):
+    """softmax(scale q k^T) v of torch in 64 bits over the visible keys, NaN and infinities as they come; rows without a
+    visible key are zeros."""
+    (N, H, P, D), (T, HQ, _) = cache[0].shape, q.shape
+    y, G = torch.zeros(T, HQ, D, dtype=torch.float64), HQ // H
+    kf, vf = (cache[i].float().double() * cache[2 + i].double()[:, :, None, None] for i in range(2))
+    for b, first, n, length in sequences(offs, lens, T):
+        for i in range(n):
+            keys = [(int(table[b, j // P]), j % P) for j in range(min(length - n + i + 1, table.shape[1] * P))]
+            keys = [(p, s) for p, s in keys if 0 <= p < N]
+            if keys:
+                p, s = (torch.tensor(x) for x in zip(*keys))
+                for h in range(HQ):
+                    w = torch.softmax(scale * (kf[p, h // G, s] @ q[first + i, h].double()), 0)
+                    y[first + i, h] = w @ vf[p, h // G, s]
+    return y
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 3, 140])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P,dh", [(16, 64), (64, 128), (20, 64), (64, 256)])
+def test_attend_rows_of_nan(cuda_lib, P, dh, dtype, new):
+    """A row that holds NaN is NaN, and so is one whose scores are all minus infinity (their softmax is 0 / 0); a row
+    that sees no key is zeros whatever its query holds.  Every other row is what it is without them."""
+    H, G, lens = 2, 2, [300, 0, 40]
+    cache = make_cache(25, H, P, dh, 201)
+    cache[0][:, :, :, 3] = torch.tensor(1.0).to(CODE)           # all keys agree on the sign of element 3
+    table = make_tables(lens, P, 25, 202)
+    table[2] = -1                                             # every page of the last sequence is missing
+    offs = None if new == 1 else [0, new, new + 2, 2 * new + 2]
+    T = 3 if new == 1 else offs[-1]
+    q = new_rows(T, H * G, dh, dtype, 203)
+    bad = q.clone()
+    bad[0, 0, 5], bad[0, 1, 3], bad[0, 2] = math.nan, -math.inf, math.nan
+    bad[T - 1, 0, 5], bad[1, 0] = math.nan, math.nan
+    bad[new // 2, 3, 0], bad[new // 2, 3, 1] = math.inf, math.nan
+    want = torch.isnan(attend_softmax(bad, cache, table, lens, offs, 0.1)).any(-1)
+    assert want[0, :3].all() and not want[T - 1].any() and (~want).sum() >= want.numel() // 2
+    lens_t, offs_t = torch.tensor(lens, dtype=torch.int32), None if offs is None else torch.tensor(offs, dtype=torch.int32)
+    for room in (table, wide(table, P)):
+        clean = run_attend(cuda_lib, q, cache, room, lens_t, offs_t, 0.1, torch.full_like(q, 3.0)).cpu()
+        got = run_attend(cuda_lib, bad, cache, room, lens_t, offs_t, 0.1, torch.full_like(q, 3.0)).cpu()
+        assert got[want].isnan().all()
+        assert torch.equal(got[~want], clean[~want])
+        assert (got[T - 1] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 3, 140])
+@pytest.mark.parametrize("P,dh,span", [(16, 64, (32, 64)), (64, 128, (64, 128)), (20, 64, (64, 128)), (64, 256, (0, 200)), (32, 128, (1184, 1216)),
+                                       (64, 64, (1280, 1344)), (16, 128, (640, 1500))])
+def test_attend_keys_of_nan(cuda_lib, P, dh, span, new):
+    """NaN in the keys of one stretch of a sequence, down to a single tile that one warp or one CTA alone looks at: the
+    rows that see it are NaN, the earlier tokens' and the other sequence's are not."""
+    H, G, lens = 1, 4, [1500, 70]
+    need = sum(-(-n // P) for n in lens)
+    cache = make_cache(need, H, P, dh, 211)
+    table = make_tables(lens, P, need, 212)
+    offs = [0, new, 2 * new if new < 70 else new + 70]
+    q = new_rows(offs[-1], H * G, dh, torch.float16, 213)
+    lens_t, offs_t = torch.tensor(lens, dtype=torch.int32), torch.tensor(offs, dtype=torch.int32)
+    hurt = [x.clone() for x in cache]
+    for j in range(*span):
+        hurt[0].view(torch.uint8)[int(table[0, j // P]), 0, j % P, 7] = 0x7F
+    sees = lens[0] - new + torch.arange(new) >= span[0]
+    for room in (table, wide(table, P)):
+        clean = run_attend(cuda_lib, q, cache, room, lens_t, offs_t, 0.1, torch.full_like(q, 3.0)).cpu()
+        got = run_attend(cuda_lib, q, hurt, room, lens_t, offs_t, 0.1, torch.full_like(q, 3.0)).cpu()
+        assert got[:new][sees].isnan().all()
+        keep = torch.cat([~sees, torch.ones(offs[-1] - new, dtype=torch.bool)])
+        assert torch.equal(got[keep], clean[keep])
+
+
 @gpu
 @pytest.mark.parametrize("P", [16, 64])
 @pytest.mark.parametrize("new", [2, 150])

@@ -301,9 +301,10 @@ INFINIOP_API infiniopStatus_t infiniopDestroyAttentionDescriptor(infiniopAttenti
  * outside the pool is a page whose tokens are masked (attention) or dropped
  * (append, copy, compact), offsets outside the rows are clamped, tokens beyond
  * the table's columns are dropped, a length <= 0 is an empty sequence.
- * Pointers must be aligned to their element.  The workspace must hold the
- * reported size, else STATUS_MEMORY_NOT_ALLOCATED; calls that may overlap on
- * the GPU (two streams, two captured graphs) need a workspace each.
+ * Pointers must be aligned to their element and the workspace to 16 bytes, else
+ * STATUS_BAD_PARAM.  The workspace must hold the reported size, else
+ * STATUS_MEMORY_NOT_ALLOCATED; calls that may overlap on the GPU (two streams,
+ * two captured graphs) need a workspace each.
  * Roundings are to nearest, ties to even (there is no reference counterpart
  * whose truncation would have to be followed). */
 

@@ -801,6 +801,9 @@ INFINIOP_API infiniopStatus_t infiniopPagedAttention(infiniopPagedAttentionDescr
     if (!empty && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || block_table == nullptr)) return STATUS_BAD_PARAM;
     const uint64_t need = workspace_of_desc(*d);
     if (need > 0 && (workspace == nullptr || workspace_size < need)) return STATUS_MEMORY_NOT_ALLOCATED;
+    if ((need > 0 && !aligned16(workspace)) || !aligned_to(2, {out, q}) || !aligned_to(4, {k_scales, v_scales, block_table, seq_lens, q_offsets})) {
+        return STATUS_BAD_PARAM;
+    }
     DeviceGuard guard(d->device_id);
     AttendParams p{};
     p.out = reinterpret_cast<uint16_t *>(out), p.q = reinterpret_cast<const uint16_t *>(q);

@@ -550,6 +550,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheAppend(infiniopPagedCacheAppendD
         block_table == nullptr || seq_lens == nullptr || d->t.offsets != (q_offsets != nullptr)) {
         return STATUS_BAD_PARAM;
     }
+    if (!aligned_to(2, {k, v}) || !aligned_to(4, {k_scales, v_scales, block_table, seq_lens, q_offsets})) return STATUS_BAD_PARAM;
     DeviceGuard guard(d->device_id);
     AppendParams p{reinterpret_cast<const uint16_t *>(k), reinterpret_cast<const uint16_t *>(v), d->k_st, d->k_sh, d->v_st, d->v_sh,
                    reinterpret_cast<uint8_t *>(k_pages), reinterpret_cast<uint8_t *>(v_pages), reinterpret_cast<float *>(k_scales),
@@ -618,6 +619,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheCopy(infiniopPagedCacheCopyDescr
     auto *d = reinterpret_cast<CopyDesc *>(desc);
     if (d->count == 0 || d->c.pages == 0) return STATUS_SUCCESS;
     if (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || pairs == nullptr) return STATUS_BAD_PARAM;
+    if (!aligned_to(4, {k_scales, v_scales, pairs})) return STATUS_BAD_PARAM;
     DeviceGuard guard(d->device_id);
     MoveParams m = move_params(d->c, k_pages, v_pages, k_scales, v_scales);
     const int unit = std::min(run_unit(m.k, k_pages), run_unit(m.v, v_pages));
@@ -692,6 +694,7 @@ INFINIOP_API infiniopStatus_t infiniopPagedCacheCompact(infiniopPagedCacheCompac
     if (!no_pages && (k_pages == nullptr || v_pages == nullptr || k_scales == nullptr || v_scales == nullptr || page_map == nullptr)) return STATUS_BAD_PARAM;
     if (!no_rows && (new_table == nullptr || block_table == nullptr || seq_lens == nullptr)) return STATUS_BAD_PARAM;
     if (workspace == nullptr || workspace_size < plan_bytes((uint64_t) d->c.pages)) return STATUS_MEMORY_NOT_ALLOCATED;
+    if (!aligned16(workspace) || !aligned_to(4, {k_scales, v_scales, new_table, block_table, seq_lens, page_map, live})) return STATUS_BAD_PARAM;
     DeviceGuard guard(d->device_id);
     auto st = reinterpret_cast<cudaStream_t>(stream);
     CompactParams p{};

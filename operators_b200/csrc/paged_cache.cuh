@@ -6,6 +6,7 @@
 #include "paged_index.h"
 
 #include <algorithm>
+#include <initializer_list>
 #include <utility>
 
 namespace b200 {
@@ -96,6 +97,13 @@ static inline infiniopStatus_t check_tables(const TensorDescriptor *table, const
     t.batch = (int32_t) batch, t.cols = (int32_t) cols, t.cap = (int32_t) (cols * (uint64_t) page);
     t.stride = table->strides[0], t.offsets = offs != nullptr;
     return STATUS_SUCCESS;
+}
+
+// Every pointer is a multiple of `bytes` (a power of two): elements are read and written whole.
+static inline bool aligned_to(uintptr_t bytes, std::initializer_list<const void *> pointers) {
+    uintptr_t all = 0;
+    for (const void *p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+    return (all & (bytes - 1)) == 0;
 }
 
 // New tokens' tensors [rows, heads, dh]: fp16 or bf16.

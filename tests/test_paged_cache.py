@@ -412,6 +412,38 @@ def test_refused_sizes_and_calls(host):
             assert e.value.status == PARAM
 
 
+def test_misaligned_pointers_are_refused(host):
+    """Pointers off their element's size, and a workspace off 16 bytes, which parts are stored to in whole vectors."""
+    lib, handle = host
+    t = _small()
+    t["long_table"] = torch.zeros(3, 100000, dtype=torch.int32)
+    long_attend = (ops.PagedAttentionOp, [f.replace("block", "long") for f in OPS["attend"][1]])
+
+    class Off:
+        def __init__(self, tensor, by):
+            self.tensor, self.by = tensor, by
+
+        def data_ptr(self):
+            return self.tensor.data_ptr() + self.by
+
+    for name, (op, fields) in [*OPS.items(), ("attend", long_attend)]:
+        with op(lib, handle, *[t[f] for f in fields]) as o:
+            for f in fields:
+                for by in range(1, t[f].element_size()):
+                    with pytest.raises(InfiniopError) as e:
+                        o(*[Off(t[g], by) if f == g else t[g] for g in fields])
+                    assert e.value.status == PARAM, (name, f, by)
+            if o.workspace is not None:
+                whole = torch.empty(o.workspace_size + 32, dtype=torch.uint8)
+                start = -whole.data_ptr() % 16
+                for by in (1, 4, 8):
+                    o.workspace = whole[start + by:]
+                    with pytest.raises(InfiniopError) as e:
+                        o(*[t[f] for f in fields])
+                    assert e.value.status == PARAM, (name, by)
+    assert name == "attend" and o.workspace is not None
+
+
 def test_workspace_does_not_depend_on_what_it_holds(host):
     """Nothing is cleared ahead of a call: the wrapper hands out memory as it comes."""
     lib, handle = host

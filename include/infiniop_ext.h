@@ -39,8 +39,10 @@ INFINIOP_API infiniopStatus_t infiniopExtSelectKernel(int family, int variant);
  * infiniopExtDeviceTimeouts reports how many groups gave up on this handle's
  * device since the library was loaded (it synchronises the device): 0 means
  * every result so far is complete.  infiniopExtSetWaitLimit sets the number of
- * polls a RoPE pipeline wait may take (0 restores the default of 2^22); it
- * exists so that a test can make the limit run out.
+ * polls a RoPE pipeline wait may take (0 restores the default of 2^22), and
+ * with any other value than 0 the waits of the paged attention's prompts kernel
+ * give up after their first poll in the calls that follow; it exists so that a
+ * test can make the limit run out.
  */
 INFINIOP_API infiniopStatus_t infiniopExtDeviceTimeouts(infiniopHandle_t handle, uint64_t *count);
 INFINIOP_API infiniopStatus_t infiniopExtSetWaitLimit(infiniopHandle_t handle, uint32_t polls);

@@ -157,6 +157,7 @@ struct SplitParams {
     PartHead *heads;// [cta][2][rows]
     CtaMeta *meta;  // [cta]
     uint32_t cluster;// decoding: CTAs of a cluster that share an item (0: equal stretches)
+    bool one_poll;  // prompts: waits give up after their first poll (a test's)
 };
 static inline uint64_t split_bytes(uint64_t ctas, uint64_t rows, uint64_t dhc) {
     return ctas * (2 * rows * (sizeof(PartHead) + dhc * 4) + sizeof(CtaMeta));

@@ -37,7 +37,8 @@
 // A product's completion is waited for only where O is touched, so it has a barrier for even and one for odd tiles: a row
 // that has seen S of tile n knows that W v of tile n - 2 (issued before it) is done, not that of tile n - 1, and one
 // barrier's parity could not tell the two apart.
-// Every wait is bounded (tc_ptx.cuh).
+// Every wait is bounded: a role that gives up raises the CTA's abort flag, all roles leave, and TMEM and shared memory are
+// given back when the products and copies that were under way have ended.
 //
 // 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 152 us, 920 TFLOP/s.  Two prompts of up to 4096
 // tokens, nothing cached before them, fp16: 150 us, 700 TFLOP/s of the visible products.
@@ -56,11 +57,12 @@ using namespace tc;
 constexpr int kRows = 128, kKeys = kPrefillKeys;
 constexpr float kSlack = 13.f, kLift = 2.f;// kSlack: of the general form, w <= 2^15 there
 constexpr float kLeast = -90.f;
+constexpr long long kDrainTicks = 2000000;// about a millisecond; a tile's products take a microsecond
 constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
 constexpr float kFarGain = 0x1p64f;// what a tile may add to a row's sum: 2^25 such tiles stay below 2^90
 constexpr int kItemUnits = 6;// what the start and the end of an item cost, in tiles
 constexpr int kMinUnits = 8;
-constexpr uint32_t kSuspendNs = 20000;
+constexpr uint32_t kSuspendNs = 20000;// up to which the hardware may keep a waiting thread suspended
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
 
 __host__ __device__ constexpr int blocks_at_once(int dhc) { return dhc <= 128 ? 2 : 1; }
@@ -80,7 +82,7 @@ static_assert(split_fits(1) && split_fits(2), "the registers' split fits what th
 constexpr uint32_t kTmemCols = 512;
 
 // barriers; the second block's own follow the first's
-enum Bar { kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty1, kScFull, kBlock = kScFull + kScaleSets,
+enum Bar { kKFull, kKFull1, kKEmpty, kKEmpty1, kVFull, kVFull1, kVEmpty, kVEmpty1, kDrained, kScFull, kBlock = kScFull + kScaleSets,
            kQFull = 0, kSFull, kSFull1, kWFull, kWFull1, kPvDone, kPvDone1, kBlockBars, kBars = kBlock + 2 * kBlockBars };
 
 struct TileScales {
@@ -132,10 +134,34 @@ __device__ __forceinline__ void umma_commit_by(uint64_t *bar, uint32_t lead) {
         ::"r"(smem_u32(bar)), "r"(lead)
         : "memory");
 }
+// a poll that never suspends the thread
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // A warp waits as one: lanes leave a wait at different times, what follows (TMEM accesses, votes) is the whole warp's, and a
 // wait that runs out ends the loop for all of its lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    return __all_sync(0xffffffffu, mbar_wait<kSuspendNs>(bar, parity, abort_flag));
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, bool one_poll) {
+    bool done = one_poll ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity);
+    if (!done) {
+        const long long t0 = clock64();
+        while (one_poll || !(done = mbar_try_wait_hint(bar, parity, kSuspendNs))) {
+            if (*abort_flag) break;
+            if (one_poll || clock64() - t0 > kWaitBudget) {
+                *abort_flag = 1;
+                atomicAdd(&g_tc_gemm_timeouts, 1ull);
+                break;
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, done);
 }
 
 // 32 columns of this warp's 32 lanes
@@ -386,7 +412,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t n = 0, bn[2] = {0, 0}, bseg[2] = {0, 0};// tiles of the stretch; tiles and items of each block
         auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-            const bool done = warp_wait(bar, parity, abort_flag);
+            const bool done = warp_wait(bar, parity, abort_flag, sp.one_poll);
             tc_fence_after();
             return done;
         };
@@ -515,7 +541,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                     const uint32_t b = n & 1u;
                     const int32_t j = tile - first;
                     if (j == kChunk / 2) id_next = page_at((first + kChunk) * kGroupsOr1 + (int32_t) lane);
-                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag, sp.one_poll))) break;
                     store_tile(b);
                     mbar_arrive(&full[b]);
                     if (j == kChunk - 1) first += kChunk, base = base_of(first * kGroupsOr1 + (int32_t) lane, id_next);
@@ -566,7 +592,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 load(g.t0);
                 for (int32_t tile = g.t0; tile < t1; ++tile, ++n) {
                     const uint32_t b = n & 1u;
-                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag, sp.one_poll))) break;
                     if (!is_v) {
                         TileScales &sc = scales[n % kScaleSets];
                         const uint32_t mask = __ballot_sync(0xffffffffu, key_ok);
@@ -725,7 +751,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
             float m = -INFINITY, wm = -INFINITY, l = 0.f;
             // O so far is multiplied by a factor per row.  Every product into it must have completed.
             auto scale_o = [&](float by) -> bool {
-                if (!warp_wait(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag)) return false;
+                if (!warp_wait(&own[kPvDone + ((n & 1u) ^ 1u)], ((n - 1) >> 1) & 1u, abort_flag, sp.one_poll)) return false;
                 tc_fence_after();
                 for (int32_t c0 = 0; c0 < p.c.dh; c0 += 64) {
                     float o[64];
@@ -797,7 +823,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                         if (j == kChunk - 1) first += kChunk, id = id_next, ks = ks_next, lv_lane = log2_of(vs_next);
                         if (tile + 1 < g.t1) look_at(tile + 1);
                     };
-                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag, sp.one_poll))) break;
                     tc_fence_after();
                     uint32_t w[kKeys / 2];
                     float gain = 0.f, most = 0.f;// what the tile adds to l; the largest sum of 16 (or 8) weights
@@ -926,9 +952,9 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 for (int32_t tile = g.t0; tile < g.t1; ++tile, ++n, ++n_all) {
                     const uint32_t b = n & 1u;
                     const TileScales &sc = scales[n_all % kScaleSets];
-                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&own[kSFull + b], (n >> 1) & 1u, abort_flag, sp.one_poll))) break;
                     // (after S: a block that sat out items may be ahead by more than a parity can tell)
-                    if (!(ok = warp_wait(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag))) break;
+                    if (!(ok = warp_wait(&bars[kScFull + n_all % kScaleSets], (n_all / kScaleSets) & 1u, abort_flag, sp.one_poll))) break;
                     tc_fence_after();
                     float x[kKeys];
                     tmem_ld64(t_lane + b * kKeys, x);
@@ -975,7 +1001,7 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
                 if (kQBufs == 2) rf_next = finish_q(other);
             }
             // ---- the item's output, or its part
-            if (!(ok = warp_wait(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag))) break;
+            if (!(ok = warp_wait(&own[kPvDone + ((n - 1) & 1u)], ((n - 1) >> 1) & 1u, abort_flag, sp.one_poll))) break;
             tc_fence_after();
             if (more && GROUPS > 0) {
                 if (id >= p.c.pages) id = -1;
@@ -1070,11 +1096,24 @@ __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_ke
     tc_fence_before();
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;");
+    if (*abort_flag) {
+        // Waits ran out: q may still be on its way, and products that nobody has waited for may be reading tiles and writing
+        // TMEM.  Shared memory is the CTA's until its last warp has left, the one that issued them.
+        cp_async_wait<0>();
+        if (warp == kWarps - 1) {
+            umma_commit_by(&bars[kDrained], elect_lane());
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&bars[kDrained], 0) && clock64() - t0 < kDrainTicks) {}
+            __syncwarp();
+        }
+    }
     if (warp == kWarps - 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
 }
+
+std::atomic<uint32_t> g_wait_polls[64];// per device: 0, or a limit that a test has set
 
 template<int DHC, int GROUPS>
 cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaStream_t st) {
@@ -1093,7 +1132,8 @@ cudaError_t launch_as(const SplitParams &sp, uint32_t ctas, int device_id, cudaS
 }
 template<int DHC>
 cudaError_t launch(const AttendParams &a, void *workspace, uint32_t ctas, int device_id, cudaStream_t st) {
-    const SplitParams sp = split_params(a, workspace, ctas, (uint64_t) prefill_rows(DHC), DHC);
+    SplitParams sp = split_params(a, workspace, ctas, (uint64_t) prefill_rows(DHC), DHC);
+    sp.one_poll = g_wait_polls[device_id & 63].load(std::memory_order_relaxed) != 0;
     if (a.vec && a.c.page % kKeys == 0) return launch_as<DHC, 1>(sp, ctas, device_id, st);
     return a.vec && a.c.page % 16 == 0 ? launch_as<DHC, 4>(sp, ctas, device_id, st) : launch_as<DHC, 0>(sp, ctas, device_id, st);
 }
@@ -1106,6 +1146,8 @@ cudaError_t launch_prefill(const AttendParams &a, void *workspace, int dhc, uint
 }
 
 }// namespace paged
+
+void paged_prefill_set_wait_polls(int device_id, unsigned int polls) { paged::g_wait_polls[device_id & 63].store(polls, std::memory_order_relaxed); }
 
 unsigned long long paged_prefill_timeouts_read() {
     unsigned long long v = 0;

@@ -37,6 +37,7 @@ unsigned long long attn_fused_timeouts_read();
 unsigned long long peer_exchange_timeouts_read();
 unsigned long long random_sample_pair_timeouts_read();
 unsigned long long paged_prefill_timeouts_read();
+void paged_prefill_set_wait_polls(int device_id, unsigned int polls);
 }// namespace b200
 
 INFINIOP_API infiniopStatus_t infiniopExtDeviceTimeouts(infiniopHandle_t handle, uint64_t *count) {
@@ -58,7 +59,9 @@ INFINIOP_API infiniopStatus_t infiniopExtDeviceTimeouts(infiniopHandle_t handle,
 
 INFINIOP_API infiniopStatus_t infiniopExtSetWaitLimit(infiniopHandle_t handle, uint32_t polls) {
     if (handle == nullptr || handle->device != DevNvGpu) return STATUS_BAD_DEVICE;
-    DeviceGuard guard(reinterpret_cast<Handle *>(handle)->device_id);
+    const int device_id = reinterpret_cast<Handle *>(handle)->device_id;
+    DeviceGuard guard(device_id);
+    paged_prefill_set_wait_polls(device_id, polls);
     return rope_pipeline_set_wait_polls(polls) ? STATUS_SUCCESS : STATUS_EXECUTION_FAILED;
 }
 

@@ -148,7 +148,8 @@ def device_timeouts(lib, handle):
 
 
 def set_wait_limit(lib, handle, polls):
-    """Polls per wait of the RoPE bulk-copy pipeline (0 = default); for the test that makes a wait run out."""
+    """Polls per wait of the RoPE bulk-copy pipeline (0 = default; otherwise the paged prompts kernel's waits give up after
+    one); for the tests that make a wait run out."""
     _declare(lib)
     check_error(lib.infiniopExtSetWaitLimit(handle, int(polls)))
 

@@ -1001,6 +1001,36 @@ def test_attend_is_repeatable(cuda_lib):
 
 
 @gpu
+@pytest.mark.parametrize("P,D", [(64, 128), (16, 64), (20, 128), (64, 256)])
+def test_wait_limit_of_the_prompts_kernel_is_reported(cuda_lib, P, D):
+    """Every wait of the prompts kernel is bounded.  With waits that give up after one poll its CTAs stop somewhere on
+    their way, let products and copies end and leave; the call returns, and the timeout query reports it.  With the default
+    limit restored the same call is complete, on a GPU that is as it was."""
+    lib, handle = cuda_lib
+    n, new = 3000, 300
+    cache = [to_dev(x) for x in make_cache(-(-n // P), 1, P, D, 251)]
+    table = wide(make_tables([n], P, -(-n // P), 252), P).to(DEV)
+    q = new_rows(new, 8, D, torch.bfloat16, 253).to(DEV)
+    lens, offs = torch.tensor([n], dtype=torch.int32, device=DEV), torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    out = [torch.zeros_like(q) for _ in range(3)]
+    with ops.PagedAttentionOp(lib, handle, q, q, *cache, table, lens, offs) as op:
+        op(out[0], q, *cache, table, lens, offs)
+        before = ops.device_timeouts(lib, handle)
+        try:
+            ops.set_wait_limit(lib, handle, 1)
+            op(out[1], q, *cache, table, lens, offs)          # returns normally
+            torch.cuda.synchronize()
+            mid = ops.device_timeouts(lib, handle)
+            assert mid > before
+        finally:
+            ops.set_wait_limit(lib, handle, 0)
+        op(out[2], q, *cache, table, lens, offs)
+        torch.cuda.synchronize()
+    assert ops.device_timeouts(lib, handle) == mid
+    assert torch.equal(out[0], out[2])
+
+
+@gpu
 def test_attend_offsets_beyond_32_bits(cuda_lib):
     """Pages whose elements lie beyond 2^32 of the pool's start."""
     lib, handle = cuda_lib

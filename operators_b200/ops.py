@@ -13,7 +13,7 @@ from ctypes import POINTER, c_float, c_int, c_int64, c_uint64, c_void_p
 
 from .data_layout import U64
 from .liboperators import infiniopHandle_t, infiniopTensorDescriptor_t
-from .utils import check_error, create_scratch, create_workspace, destroy_tensor_descriptor, to_tensor
+from .utils import check_error, create_scratch, create_workspace, destroy_tensor_descriptor, to_tensor, torch_stream
 
 _desc_t = c_void_p  # operator descriptors are opaque to Python
 
@@ -282,20 +282,41 @@ def _data(tensor):
 
 
 class _PagedOp(_Op):
-    """The operators of the paged cache write every byte of their workspace that they read."""
+    """The operators of the paged cache write every byte of their workspace that they read.
 
-    def _make_workspace(self, device):
+    The workspace is made on `stream` (None: the default stream, where calls without a stream go).  The first call on any
+    other stream waits there for what was queued on the first when the workspace was made, and the memory goes back to
+    torch when those streams are done with it.  A graph that captured a call uses the workspace at each replay: keep the
+    operator as long as the graph."""
+
+    def _make_workspace(self, device, stream):
+        import torch
+
         size = c_uint64(0)
         check_error(getattr(self.lib, self._wsize)(self.desc, ctypes.byref(size)))
         self.workspace_size = size.value
-        self.workspace = create_scratch(size.value, device)
+        self._captured = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        if stream is None and self._captured:
+            stream = torch.cuda.current_stream(device)        # no other stream's memory can be had meanwhile
+        self.workspace = create_scratch(size.value, device, stream)
+        self._streams = {_stream_ptr(stream) or 0}            # those that the workspace is ordered on
+        if self.workspace is not None and device.type == "cuda":
+            self._made = torch_stream(stream, device).record_event()
 
-    def release_after(self, stream):
-        """For the one-shot forms: the workspace goes back to torch's allocator when `stream` is done with it."""
-        if self.workspace is not None and stream is not None:
-            import torch
+    def _order(self, stream):
+        """Ahead of a call: the workspace may be used on `stream`."""
+        handle = _stream_ptr(stream) or 0
+        if self.workspace is None or handle in self._streams or not self.workspace.is_cuda:
+            return
+        import torch
 
-            self.workspace.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream))
+        s = torch_stream(stream, self.workspace.device)
+        with torch.cuda.stream(s):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing == self._captured:                       # (torch waits for the whole device ahead of a capture)
+            s.wait_event(self._made)
+            self._streams.add(handle)
+        self.workspace.record_stream(s)
 
 
 class PagedCacheAppendOp(_PagedOp):
@@ -306,14 +327,16 @@ class PagedCacheAppendOp(_PagedOp):
     q_offsets int32 [batch + 1] or None for one new token per sequence."""
     _destroy, _wsize = "infiniopDestroyPagedCacheAppendDescriptor", "infiniopGetPagedCacheAppendWorkspaceSize"
 
-    def __init__(self, lib, handle, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None):
+    def __init__(self, lib, handle, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
+                 stream=None):
         super().__init__(lib, handle)
         ts = [self._t(x).descriptor for x in (k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens)]
         ts.append(None if q_offsets is None else self._t(q_offsets).descriptor)
         check_error(lib.infiniopCreatePagedCacheAppendDescriptor(handle, ctypes.byref(self.desc), *ts))
-        self._make_workspace(k.device)
+        self._make_workspace(k.device, stream)
 
     def __call__(self, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None, stream=None):
+        self._order(stream)
         check_error(self.lib.infiniopPagedCacheAppend(
             self.desc, self._ws_ptr(), self.workspace_size, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
@@ -327,15 +350,16 @@ class PagedAttentionOp(_PagedOp):
     _destroy, _wsize = "infiniopDestroyPagedAttentionDescriptor", "infiniopGetPagedAttentionWorkspaceSize"
 
     def __init__(self, lib, handle, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
-                 scale=None):
+                 scale=None, stream=None):
         super().__init__(lib, handle)
         ts = [self._t(x).descriptor for x in (out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens)]
         ts.append(None if q_offsets is None else self._t(q_offsets).descriptor)
         check_error(lib.infiniopCreatePagedAttentionDescriptor(handle, ctypes.byref(self.desc), *ts,
                                                                q.shape[-1] ** -0.5 if scale is None else scale))
-        self._make_workspace(q.device)
+        self._make_workspace(q.device, stream)
 
     def __call__(self, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None, stream=None):
+        self._order(stream)
         check_error(self.lib.infiniopPagedAttention(
             self.desc, self._ws_ptr(), self.workspace_size, out.data_ptr(), q.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
@@ -347,13 +371,14 @@ class PagedCacheCopyOp(_PagedOp):
     id outside the pool are skipped."""
     _destroy, _wsize = "infiniopDestroyPagedCacheCopyDescriptor", "infiniopGetPagedCacheCopyWorkspaceSize"
 
-    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, pairs):
+    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, pairs, stream=None):
         super().__init__(lib, handle)
         ts = [self._t(x).descriptor for x in (k_pages, v_pages, k_scales, v_scales, pairs)]
         check_error(lib.infiniopCreatePagedCacheCopyDescriptor(handle, ctypes.byref(self.desc), *ts))
-        self._make_workspace(k_pages.device)
+        self._make_workspace(k_pages.device, stream)
 
     def __call__(self, k_pages, v_pages, k_scales, v_scales, pairs, stream=None):
+        self._order(stream)
         check_error(self.lib.infiniopPagedCacheCopy(
             self.desc, self._ws_ptr(), self.workspace_size, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
             v_scales.data_ptr(), pairs.data_ptr(), _stream_ptr(stream)))
@@ -365,14 +390,16 @@ class PagedCacheCompactOp(_PagedOp):
     int32 [1] (their number).  A sequence is freed by setting its length to 0."""
     _destroy, _wsize = "infiniopDestroyPagedCacheCompactDescriptor", "infiniopGetPagedCacheCompactWorkspaceSize"
 
-    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live):
+    def __init__(self, lib, handle, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live,
+                 stream=None):
         super().__init__(lib, handle)
         ts = [self._t(x).descriptor for x in (k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens,
                                               page_map, live)]
         check_error(lib.infiniopCreatePagedCacheCompactDescriptor(handle, ctypes.byref(self.desc), *ts))
-        self._make_workspace(k_pages.device)
+        self._make_workspace(k_pages.device, stream)
 
     def __call__(self, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live, stream=None):
+        self._order(stream)
         check_error(self.lib.infiniopPagedCacheCompact(
             self.desc, self._ws_ptr(), self.workspace_size, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
             v_scales.data_ptr(), new_table.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), page_map.data_ptr(),
@@ -548,32 +575,28 @@ def attention(lib, handle, out, q, k, v, k_cache, v_cache, pos, stream=None):
 def paged_cache_append(lib, handle, k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
                        stream=None):
     args = (k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets)
-    with PagedCacheAppendOp(lib, handle, *args) as op:
+    with PagedCacheAppendOp(lib, handle, *args, stream=stream) as op:
         op(*args, stream)
-        op.release_after(stream)
 
 
 def paged_attention(lib, handle, out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets=None,
                     scale=None, stream=None):
     args = (out, q, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, q_offsets)
-    with PagedAttentionOp(lib, handle, *args, scale) as op:
+    with PagedAttentionOp(lib, handle, *args, scale, stream=stream) as op:
         op(*args, stream)
-        op.release_after(stream)
 
 
 def paged_cache_copy(lib, handle, k_pages, v_pages, k_scales, v_scales, pairs, stream=None):
     args = (k_pages, v_pages, k_scales, v_scales, pairs)
-    with PagedCacheCopyOp(lib, handle, *args) as op:
+    with PagedCacheCopyOp(lib, handle, *args, stream=stream) as op:
         op(*args, stream)
-        op.release_after(stream)
 
 
 def paged_cache_compact(lib, handle, k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map,
                         live, stream=None):
     args = (k_pages, v_pages, k_scales, v_scales, new_table, block_table, seq_lens, page_map, live)
-    with PagedCacheCompactOp(lib, handle, *args) as op:
+    with PagedCacheCompactOp(lib, handle, *args, stream=stream) as op:
         op(*args, stream)
-        op.release_after(stream)
 
 
 def matmul(lib, handle, c, a, b, alpha=1.0, beta=0.0, stream=None):

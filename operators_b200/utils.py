@@ -72,12 +72,26 @@ def create_workspace(size, torch_device):
     return torch.zeros(size=(size,), dtype=torch.uint8, device=torch_device)
 
 
-def create_scratch(size, torch_device):
-    """A workspace whose contents do not matter: no fill is queued on the current stream, so the operator may be
-    launched on another one right away."""
+def torch_stream(stream, torch_device):
+    """The torch stream that a `stream` argument means: a torch stream, a raw handle, or None for the default stream."""
     import torch
 
-    return torch.empty(size, dtype=torch.uint8, device=torch_device) if size else None
+    if stream is None or stream == 0:
+        return torch.cuda.default_stream(torch_device)
+    return stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=torch_device)
+
+
+def create_scratch(size, torch_device, stream=None):
+    """A workspace whose contents do not matter, for calls on `stream`.  torch hands out memory again while work that is
+    queued on the stream it was made on may still use it, so it has to be made on the stream that the calls go to."""
+    import torch
+
+    if not size:
+        return None
+    if torch.device(torch_device).type != "cuda":
+        return torch.empty(size, dtype=torch.uint8, device=torch_device)
+    with torch.cuda.stream(torch_stream(stream, torch_device)):
+        return torch.empty(size, dtype=torch.uint8, device=torch_device)
 
 
 def create_handle(lib, device, id=0):

@@ -1309,6 +1309,56 @@ def test_two_streams_at_once(cuda_lib):
 
 
 @gpu
+@pytest.mark.parametrize("how", ["one shot", "made before", "dropped after", "default stream"])
+@pytest.mark.parametrize("new", [1, 200])
+def test_workspace_memory_and_streams(cuda_lib, new, how):
+    """torch hands memory out again while the stream that it was made on still has work queued for it.  A workspace is never
+    such memory on another stream: neither ahead of the call (fills of a tensor that is gone are still queued), nor behind
+    it (fills of a new tensor start while the call still runs)."""
+    lib, handle = cuda_lib
+    H, P, D, n = 2, 64, 128, 30000
+    cache = [to_dev(x) for x in make_cache(-(-n // P), H, P, D, 261)]
+    table = make_tables([n], P, -(-n // P), 262).to(DEV)
+    lens, offs = torch.tensor([n], dtype=torch.int32, device=DEV), torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    q = new_rows(new, 8 * H, D, torch.bfloat16, 263).to(DEV)
+    want, out, side = torch.zeros_like(q), torch.zeros_like(q), torch.cuda.Stream()
+    args = (out, q, *cache, table, lens, offs)
+    with ops.PagedAttentionOp(lib, handle, want, q, *cache, table, lens, offs) as op:
+        op(want, *args[1:])
+        size = op.workspace_size
+    torch.cuda.synchronize()
+
+    def fills(count):
+        x = torch.empty(size, dtype=torch.uint8, device=DEV)
+        for _ in range(count):
+            x.fill_(255)                                      # (a stretch without an item, sums of NaN)
+
+    if how == "one shot":
+        fills(2000)
+        ops.paged_attention(lib, handle, *args, stream=side)
+    elif how == "made before":
+        fills(2000)
+        with ops.PagedAttentionOp(lib, handle, *args) as op:
+            op(*args, stream=side.cuda_stream)
+    elif how == "dropped after":
+        op = ops.PagedAttentionOp(lib, handle, *args)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2000000)
+        op(*args, stream=side)
+        op.destroy()
+        del op
+        fills(500)
+    else:
+        torch.cuda._sleep(2000000)
+        with torch.cuda.stream(side):                         # a call without a stream goes to the default one all the same
+            ops.paged_attention(lib, handle, *args)
+            fills(500)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+@gpu
 @pytest.mark.parametrize("new,D", [(1, 128), (3, 64), (150, 128), (150, 256)])
 def test_captured_attention_over_long_tables(cuda_lib, new, D):
     """The forms that split work over CTAs and join it in a second kernel, captured with a table in a wider tensor and

@@ -30,6 +30,7 @@
 // others (7 us), and the join (5 us).
 #include "paged_cache.cuh"
 #include "paged_attention.cuh"
+#include "tc_ptx.cuh"
 
 #include <atomic>
 #include <cmath>
@@ -101,7 +102,6 @@ __device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
 
 __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
 
-
 // Blocks of query rows and tiles of a sequence; its units are blocks x kv heads x tiles.
 template<int ROWS>
 __device__ __forceinline__ void extent_of(const AttendParams &p, const Seq &s, int32_t &blocks, int32_t &tiles) {
@@ -110,25 +110,9 @@ __device__ __forceinline__ void extent_of(const AttendParams &p, const Seq &s, i
     tiles = keys > 0 ? (keys - 1) / kTile + 1 : 1;// a sequence without keys still writes zeros
 }
 
-// log2 of a scale; exact and cheap for the powers of two that append writes.  Zero gives -inf.
-__device__ __forceinline__ float log2_of(float v) {
-    const uint32_t u = __float_as_uint(v);
-    if (__any_sync(0xffffffffu, (u & 0x807FFFFFu) != 0 || u == 0)) return log2f(v);
-    return (float) ((int32_t) (u >> 23) - 127);
-}
-
-// 16 bytes at the same place of another CTA's shared memory
-__device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t rank) {
-    uint32_t a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
-}
-
 // The state of a warp's ring while it walks tiles first, first + kWarps, .. of one item.
 struct Walk {
-    int32_t b, keys;
+    int32_t keys;
     const uint8_t *k, *v;// this kv head's pages
     const float *ks, *vs;
 };
@@ -213,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
         if (cl > 0) ++u;
 
         Walk w;
-        w.b = b, w.keys = held(s.len, p.t.cap);
+        w.keys = held(s.len, p.t.cap);
         w.k = p.kp + (int64_t) kvh * p.c.k.sh, w.v = p.vp + (int64_t) kvh * p.c.v.sh;
         w.ks = p.ks + (int64_t) kvh * p.c.k.ch, w.vs = p.vs + (int64_t) kvh * p.c.v.ch;
         const int32_t *row_table = p.table + (int64_t) b * p.t.stride;
@@ -615,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                 for (uint32_t i = 0; i < kMaxCluster; ++i) {
                     h[i] = PartHead{-INFINITY, 0.f, -INFINITY, 0};
                     if (i < cl) {
-                        const float4 v = ld_cluster4(ph_at + (uint32_t) r * 16u, i);
+                        const float4 v = tc::ld_cluster_f4(tc::mapa_u32(ph_at + (uint32_t) r * 16u, i));
                         h[i] = PartHead{v.x, v.y, v.z, __float_as_int(v.w)};
                     }
                     mr = fmaxf(mr, h[i].m), wr = fmaxf(wr, h[i].w);
@@ -632,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DHC, NT)) decode_kernel(
                     for (uint32_t i = 0; i < kMaxCluster; ++i) {
                         if (i < cl && h[i].w != -INFINITY) {
                             const float f = fast_exp2(h[i].w - wr);
-                            const float4 a = ld_cluster4(po_at + ((uint32_t) r * DHC + grp * 4) * 4u, i);
+                            const float4 a = tc::ld_cluster_f4(tc::mapa_u32(po_at + ((uint32_t) r * DHC + grp * 4) * 4u, i));
                             y.x += f * a.x, y.y += f * a.y, y.z += f * a.z, y.w += f * a.w;
                         }
                     }

@@ -296,6 +296,8 @@ INFINIOP_API infiniopStatus_t infiniopDestroyAttentionDescriptor(infiniopAttenti
  *                      positions seq_lens[b] - n .. seq_lens[b] - 1 of b.  May
  *                      be NULL where every sequence has one new token (rows ==
  *                      batch).  Rows behind the last sequence's are left alone.
+ *                      Offsets ascend: of rows that two sequences claim the
+ *                      result is undefined (no access leaves the tensors).
  * dh <= 256, page_size < 2^22, columns * page_size < 2^31.  Table entries behind a sequence's
  * last page are never read.  Values that lead nowhere do no harm: a page id
  * outside the pool is a page whose tokens are masked (attention) or dropped
@@ -338,13 +340,20 @@ INFINIOP_API infiniopStatus_t infiniopDestroyPagedCacheAppendDescriptor(infiniop
 
 /* out[t, h, :] = softmax_j(scale * q[t, h, :] . k_j) . v_j over the cached
  * tokens j <= position of t of its sequence, kv head h / (n_q_head / n_kv_head).
+ * Products are of fp16 operands, added up in fp32: codes are exact in fp16, a
+ * BF16 row of q is brought to fp16 by a power of two (exact but for elements
+ * below 2^-29 of the row's largest), and the softmax weights are rounded to fp16
+ * before the product with v (2^-11 of a weight, 2^-27 of the row's largest).
+ * Scores, sums and unfinished outputs stay in fp32; out is rounded once.
  * q, out F16 or BF16 [rows, n_q_head, dh], unit innermost stride, free positive
  * outer strides; `scale` finite; n_q_head <= 65535, and rows * n_q_head /
  * n_kv_head < 2^31.  The new tokens' own k and v are read from the pages: append
- * them first.  out may be q itself.  A token without visible keys gets zeros.  What the pages hold
- * behind a sequence's last token is not used, NaN included; a NaN among the
- * cached values of a later new token of the call may reach the outputs of the
- * sequence's earlier ones (it is multiplied by a weight of zero). */
+ * them first.  out may be q itself.  A token without visible keys gets zeros.
+ * NaN in a row of q or in a visible key gives NaN in that row and head, and so do
+ * scores that are all minus infinity.  What the pages hold behind a sequence's
+ * last token is not used, NaN included; a NaN among the cached values of a later
+ * new token of the call may reach the outputs of the sequence's earlier ones (it
+ * is multiplied by a weight of zero). */
 typedef struct PagedAttentionDescriptor {
     Device device;
 } PagedAttentionDescriptor;

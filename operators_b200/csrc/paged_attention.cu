@@ -25,8 +25,8 @@
 //    of 128 elements, 8 rows 27 us with one and 12 rows 33 us with two; more rows take further items, or the tcgen05 kernel
 //    (prefill_is_faster).  Tiles that lie in one page (page sizes that are multiples of 32) read one page id and scale per
 //    tile: 32 sequences of 2048 tokens 36 us with pages of 64, 41 us in the general form with pages of 16.
-// Measured: 32 sequences of 1024 to 8192 tokens, 32 heads on 8 of 128 elements: 65 us, 4.8 TB/s; one sequence of 131072:
-// 57.6 us, 4.65 TB/s.  The loop itself runs at 6.7 TB/s; the rest is the start (5 us), SMs that get less bandwidth than
+// Measured: 32 sequences of 1024 to 8192 tokens, 32 heads on 8 of 128 elements: 66 us, 4.75 TB/s; one sequence of 131072:
+// 58 to 59 us, 4.6 TB/s.  The loop itself runs at 6.7 TB/s; the rest is the start (5 us), SMs that get less bandwidth than
 // others (7 us), and the join (5 us).
 #include "paged_cache.cuh"
 #include "paged_attention.cuh"
@@ -44,7 +44,10 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;      // cached tokens per warp and step
 constexpr int kMinUnits = 4;   // a CTA takes at least a tile per warp
-constexpr int kItemUnits = 8;  // what the start and the end of an item cost, in tiles
+// What the start and the end of an item cost, in tiles: with 4, 8 and 12 of them 12 sequences of up to 2500 tokens and 5 new
+// ones, 40 heads on 8, take 23.1, 22.6, 22.6 us at a head size of 64, 31.9, 30.6, 30.7 at 128, 63.4, 60.2, 58.9 at 256; 32
+// sequences of one new token differ by 1 %.
+constexpr int kItemUnits = 8;
 constexpr uint32_t kMaxCluster = 8;
 constexpr int64_t kClusterRounds = 4;
 constexpr float kSlack = 1.f;  // log2 by which a score may exceed its row's reference
@@ -749,7 +752,7 @@ INFINIOP_API infiniopStatus_t infiniopCreatePagedAttentionDescriptor(
     }
     // Few items over a table of few columns: a cluster of CTAs per item, one launch.  A CTA of four warps takes up to
     // kClusterRounds tiles per warp; beyond that equal stretches over all SMs are faster although they take a second launch.
-    // (One query over 777 tokens: 8.2 us with clusters, 12.3 us with stretches.)
+    // (One query over 777 tokens: 8.3 us with clusters, 10.3 us with stretches, which a table with room for 32768 takes.)
     d.cluster = 0;
     if (!prefill) {
         const int64_t exact = d.t.offsets ? blocks : (int64_t) d.t.batch * ((group + d.block - 1) / d.block);

@@ -40,8 +40,9 @@
 // Every wait is bounded: a role that gives up raises the CTA's abort flag, all roles leave, and TMEM and shared memory are
 // given back when the products and copies that were under way have ended.
 //
-// 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 152 us, 920 TFLOP/s.  Two prompts of up to 4096
-// tokens, nothing cached before them, fp16: 150 us, 700 TFLOP/s of the visible products.
+// 512 new tokens over 16384 cached ones, 32 heads on 8 of 128 elements, bf16: 152 to 157 us on different GPUs, 920 to 890
+// TFLOP/s.  Two prompts of up to 4096 tokens, nothing cached before them, fp16: 149 to 154 us, 700 to 680 TFLOP/s of the
+// visible products.
 #include "paged_attention.cuh"
 #include "tc_ptx.cuh"
 
@@ -60,7 +61,9 @@ constexpr float kLeast = -90.f;
 constexpr long long kDrainTicks = 2000000;// about a millisecond; a tile's products take a microsecond
 constexpr float kMostWeight = 65504.f, kFarWeight = 0x1p100f;// sums of 16 weights that fp16 or fp32 may not hold
 constexpr float kFarGain = 0x1p64f;// what a tile may add to a row's sum: 2^25 such tiles stay below 2^90
-constexpr int kItemUnits = 6;// what the start and the end of an item cost, in tiles
+// What the start and the end of an item cost, in tiles: with 4, 6 and 8 of them two prompts of up to 4096 tokens (bf16) take
+// 133, 131, 134 us at a head size of 64, 169, 160, 158 at 128, 367, 333, 310 at 256; 512 new tokens over 16384 differ by 1 %.
+constexpr int kItemUnits = 6;
 constexpr int kMinUnits = 8;
 constexpr uint32_t kSuspendNs = 20000;// up to which the hardware may keep a waiting thread suspended
 constexpr int kScaleSets = 4;// a set is rewritten four tiles later, when the rows of its tile are long done
@@ -292,7 +295,7 @@ __device__ __forceinline__ float largest(const float *v) {
 
 // GROUPS of a tile's keys that each lie in one page: 1 (page sizes that are multiples of 64), 4 (of 16), 0 (any other, and
 // codes whose rows are no aligned vectors: a page, a scale and a mask bit per key).  512 new tokens over 16384 cached ones, 32
-// heads on 8 of 128 elements: 150 us with pages of 64 tokens (1), 163 us with 16 (4), where the general form takes 412 us.
+// heads on 8 of 128 elements: 152 us with pages of 64 tokens (1), 165 us with 16 and 163 us with 48 (4), 436 us with 20 (0).
 template<int DHC, int GROUPS>
 __global__ void __launch_bounds__(threads_of(blocks_at_once(DHC)), 1) prefill_kernel(const SplitParams sp) {
     constexpr int kNB = blocks_at_once(DHC), kItemRows = kNB * kRows, kThreads = threads_of(kNB), kWarps = kThreads / 32;

@@ -13,7 +13,7 @@ from ctypes import POINTER, c_float, c_int, c_int64, c_uint64, c_void_p
 
 from .data_layout import U64
 from .liboperators import infiniopHandle_t, infiniopTensorDescriptor_t
-from .utils import check_error, create_scratch, create_workspace, destroy_tensor_descriptor, to_tensor, torch_stream
+from .utils import check_error, create_scratch, create_workspace, destroy_tensor_descriptor, stream_handle, to_tensor, torch_stream
 
 _desc_t = c_void_p  # operator descriptors are opaque to Python
 
@@ -299,14 +299,16 @@ class _PagedOp(_Op):
         if stream is None and self._captured:
             stream = torch.cuda.current_stream(device)        # no other stream's memory can be had meanwhile
         self.workspace = create_scratch(size.value, device, stream)
-        self._streams = {_stream_ptr(stream) or 0}            # those that the workspace is ordered on
+        self._streams = {stream_handle(stream)}               # those that the workspace is ordered on
         if self.workspace is not None and device.type == "cuda":
             self._made = torch_stream(stream, device).record_event()
 
     def _order(self, stream):
         """Ahead of a call: the workspace may be used on `stream`."""
-        handle = _stream_ptr(stream) or 0
-        if self.workspace is None or handle in self._streams or not self.workspace.is_cuda:
+        if self.workspace is None or not self.workspace.is_cuda:
+            return
+        handle = stream_handle(stream)
+        if handle in self._streams:
             return
         import torch
 

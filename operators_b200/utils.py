@@ -72,13 +72,21 @@ def create_workspace(size, torch_device):
     return torch.zeros(size=(size,), dtype=torch.uint8, device=torch_device)
 
 
+def stream_handle(stream):
+    """The handle, as a number, that a `stream` argument means: a torch stream, a handle (a number or a ctypes pointer), or
+    None for the default stream."""
+    handle = getattr(stream, "cuda_stream", stream)
+    return getattr(handle, "value", handle) or 0
+
+
 def torch_stream(stream, torch_device):
-    """The torch stream that a `stream` argument means: a torch stream, a raw handle, or None for the default stream."""
+    """The same as a torch stream."""
     import torch
 
-    if stream is None or stream == 0:
-        return torch.cuda.default_stream(torch_device)
-    return stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=torch_device)
+    if hasattr(stream, "cuda_stream"):
+        return stream
+    handle = stream_handle(stream)
+    return torch.cuda.ExternalStream(handle, device=torch_device) if handle else torch.cuda.default_stream(torch_device)
 
 
 def create_scratch(size, torch_device, stream=None):

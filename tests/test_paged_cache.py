@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from operators_b200 import InfiniopError, ops
+from operators_b200.utils import stream_handle
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DEV = "cuda:0"
@@ -450,6 +451,14 @@ def test_workspace_does_not_depend_on_what_it_holds(host):
     t = _small()
     with ops.PagedCacheCompactOp(lib, handle, *[t[f] for f in OPS["compact"][1]]) as o:
         assert o.workspace.numel() == o.workspace_size > 0
+
+
+def test_stream_arguments():
+    class Stream:
+        cuda_stream = 7
+
+    for stream, handle in ((None, 0), (0, 0), (5, 5), (ctypes.c_void_p(5), 5), (ctypes.c_void_p(None), 0), (Stream(), 7)):
+        assert stream_handle(stream) == handle
 
 
 # ---- append ---------------------------------------------------------------------------------------------------------
@@ -1356,6 +1365,46 @@ def test_workspace_memory_and_streams(cuda_lib, new, how):
             fills(500)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@gpu
+def test_one_shot_calls_in_a_capture(cuda_lib):
+    """Calls that make their workspace inside a capture, on the captured stream and on one that forks from it, in every
+    form of a stream argument; replayed after the memory of the capture has been asked for again."""
+    lib, handle = cuda_lib
+    H, P, D, n = 2, 32, 128, 3000
+    cache = [to_dev(x) for x in make_cache(-(-n // P), H, P, D, 271)]
+    table = wide(make_tables([n], P, -(-n // P), 272), P).to(DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    s, side = torch.cuda.Stream(), torch.cuda.Stream()
+    for new in (1, 150):
+        offs = torch.tensor([0, new], dtype=torch.int32, device=DEV)
+        q = new_rows(new, 4 * H, D, torch.float16, 273).to(DEV)
+        outs = [torch.zeros_like(q) for _ in range(5)]
+        args = (q, *cache, table, lens, offs)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ops.paged_attention(lib, handle, outs[0], *args, stream=s)
+            ops.paged_attention(lib, handle, outs[1], *args, stream=s.cuda_stream)
+            ops.paged_attention(lib, handle, outs[2], *args, stream=ctypes.c_void_p(s.cuda_stream))
+            kept = ops.PagedAttentionOp(lib, handle, outs[3], *args)
+            kept(outs[3], *args, stream=s)
+            side.wait_stream(s)
+            kept(outs[4], *args, stream=side)
+            s.wait_stream(side)
+        for length in (n, 777, 40):
+            lens.fill_(max(length, new))
+            want = torch.zeros_like(q)
+            ops.paged_attention(lib, handle, want, *args)
+            for x in outs:
+                x.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            for x in outs:
+                assert torch.equal(x, want)
+        kept.destroy()
+        del g, kept
 
 
 @gpu
